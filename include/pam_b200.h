@@ -316,6 +316,52 @@ int pamk_adam_step(float* const* p, const float* const* g, float* const* m, floa
                    float beta1, float one_minus_beta1, float beta2, float one_minus_beta2,
                    float eps, float decay, float step_size, float offset, void* stream);
 
+/* ---- text generation --------------------------------------------------------------------------------
+ * No counterpart as kernels in the reference, whose fairseq fork decodes through the operators of its training graph
+ * (fairseq/modules/multihead_attention.py:618-783, fairseq/search.py:103-147, incremental state reordering in
+ * fairseq/sequence_generator.py:380-388).
+ *
+ * pamk_cached_attention: attention of single-token rows over cached keys and values.  Row (g, r), head h, with the kv_heads key heads
+ * each serving heads / kv_heads neighbouring query heads, sees the first shared_lengths[g] of the `shared` positions of its group and the first
+ * own_lengths[g][r] of its `own` ones (lengths NULL: all of them; clamped to [0, slots]; nothing beyond them is read):
+ *   s_j = sum_d pam(q_d, k_jd);  p = PAM softmax of s over these positions;  out_d = sum_j pam(p_j, v_jd)
+ * as pamk_matmul_strided, pamk_softmax_fwd and pamk_matmul_strided give, except that the softmax shift is the floor of the row's own maximum.
+ * A row without positions gives zeros.  `strides` (host array of 17, in elements; the last dimension of every tensor is contiguous):
+ *   q: group, row, head;  shared_k: group, position, head;  shared_v: the same three;
+ *   own_k: group, row, position, head;  own_v: the same four.
+ * out is contiguous [groups, rows, heads, dim]; own_lengths contiguous [groups, rows].  dim <= 256.
+ * `workspace`: pamk_cached_attention_workspace_bytes(...) bytes, 256-byte aligned. */
+size_t pamk_cached_attention_workspace_bytes(int64_t groups, int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim,
+                                             int64_t shared, int64_t own);
+int pamk_cached_attention(const float* q, float* out,
+                          const float* shared_k, const float* shared_v, const int64_t* shared_lengths,
+                          const float* own_k, const float* own_v, const int64_t* own_lengths,
+                          int64_t groups, int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim,
+                          int64_t shared, int64_t own, const int64_t* strides, float offset,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+/* pamk_beam_select: the k best candidates of every group, best first.  Candidate (r, j) of group g is beam r continued by token j; its
+ * value is scores[g][r] + (x_j - logsumexp(x)) for the logits x of that beam, with the PAM logsumexp of pamk_logsumexp_fwd taken per beam,
+ * its sum, logarithm and quotient and the value in 64 bits.  Order: larger value first, then lower beam, then larger logit, then lower
+ * token.  Logits of -1e30 or less (-inf among them) are masked: no share in the sum, value -inf.  banned[j] != 0 (NULL: none; strides
+ * 0 share a row of flags): in the sum, value -inf.  A beam whose score is -inf or NaN, or whose sum is not finite, has value -inf for every
+ * token; the logits of one with such a score are not read.  Token strides are 1; scores [groups, rows]; outputs [groups, k].
+ * rows <= 64, k <= 64, k <= rows * vocab.  `workspace`: pamk_beam_select_workspace_bytes(...) bytes, 256-byte aligned. */
+size_t pamk_beam_select_workspace_bytes(int64_t groups, int64_t rows, int64_t vocab, int64_t k);
+int pamk_beam_select(const float* logits, const float* scores, const unsigned char* banned,
+                     float* out_scores, int64_t* out_beams, int64_t* out_tokens,
+                     int64_t groups, int64_t rows, int64_t vocab, int64_t k,
+                     int64_t logits_group, int64_t logits_row, int64_t banned_group, int64_t banned_row,
+                     float offset, void* workspace, size_t workspace_bytes, void* stream);
+
+/* pamk_reorder_states: state[g][r] = state[g][parents[g][r]] in place, for `count` tensors of any type at once.  HOST arrays of `count`
+ * entries: device pointers, byte strides of groups and rows, the bytes of a row that move (contiguous) and the bytes of one position.
+ * `positions` (device, or NULL: all): only that many leading positions move, at most moved_bytes.  A parent outside [0, rows) leaves its
+ * row as it is.  No two rows, of one tensor or of two, may overlap.  rows <= 64. */
+int pamk_reorder_states(void* const* states, const int64_t* group_bytes, const int64_t* row_bytes,
+                        const int64_t* moved_bytes, const int64_t* position_bytes, int count,
+                        const int64_t* parents, const int64_t* positions, int64_t groups, int64_t rows, void* stream);
+
 /* ---- roofline measurement --------------------------------------------------------------------
  * No counterpart in the reference.  Runs register-only chains of the instructions a PAM
  * multiply-accumulate is made of and reports how many chain steps ran in how many milliseconds;

@@ -1,0 +1,253 @@
+"""Text generation on the GPU: attention over a key/value cache, the selection step of beam search, and the reordering of
+the states that belong to the beams.
+
+The reference's fairseq fork generates through the operators of its training graph: the whole chain of projections,
+products and softmax per step (fairseq/modules/multihead_attention.py:618-783), log-probabilities sorted over beams
+and vocabulary (fairseq/search.py:103-147), states gathered by beam (fairseq/sequence_generator.py:380-388).  Here each of
+the three is one call in the same PAM arithmetic, fp32 throughout.  None has a backward pass.
+"""
+import ctypes
+
+import torch
+
+from . import _lib
+from .fused import _offset
+
+MAX_HEAD_DIM = 256
+MAX_BEAMS = 64
+MAX_SELECTED = 64
+
+
+def _no_backward(what, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
+
+
+def _fp32(name, t, dims):
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32:
+        raise TypeError(f"{name} must be an fp32 tensor, got {t.dtype if isinstance(t, torch.Tensor) else type(t).__name__}")
+    if t.dim() != dims:
+        raise ValueError(f"{name} must have {dims} dimensions, got shape {tuple(t.shape)}")
+    return t
+
+
+def _cache(name, k, v, lengths, lead, heads, dim):
+    """Checks a pair of caches [*lead, slots, kv_heads, dim]; returns them with their lengths, cut where these are a number."""
+    if (k is None) != (v is None):
+        raise ValueError(f"{name} keys and values come together")
+    if k is None:
+        if lengths is not None:
+            raise ValueError(f"{name} lengths without {name} keys and values")
+        return None, None, None
+    for what, t in ((f"{name} keys", k), (f"{name} values", v)):
+        _fp32(what, t, len(lead) + 3)
+        if tuple(t.shape[:len(lead)]) != lead or t.shape[-1] != dim:
+            raise ValueError(f"{what} {tuple(t.shape)} do not go with queries of {lead} and head dimension {dim}")
+        if dim > 1 and t.stride(-1) != 1:
+            raise ValueError(f"{what}: the last dimension must be contiguous")
+    if k.shape != v.shape:
+        raise ValueError(f"{name} keys {tuple(k.shape)} and values {tuple(v.shape)} differ")
+    if k.shape[-2] < 1 or heads % k.shape[-2]:
+        raise ValueError(f"{heads} query heads cannot be shared out to {k.shape[-2]} key heads")
+    slots = k.shape[-3]
+    if isinstance(lengths, int) and not isinstance(lengths, bool):
+        if not 0 <= lengths <= slots:
+            raise ValueError(f"{name} length {lengths} outside the cache's {slots} slots")
+        return k.narrow(-3, 0, lengths), v.narrow(-3, 0, lengths), None
+    if lengths is not None:
+        if not isinstance(lengths, torch.Tensor) or lengths.dtype != torch.int64 or tuple(lengths.shape) != lead:
+            raise ValueError(f"{name} lengths must be a number or an int64 tensor of shape {lead}")
+        lengths = lengths.contiguous()
+    return k, v, lengths
+
+
+def cached_attention(q, own_k=None, own_v=None, own_lengths=None, *, shared_k=None, shared_v=None, shared_lengths=None, offset=None):
+    """PAM attention of single-token rows over cached keys and values: softmax(q k^T) v per head, as
+    `fused.attention_heads` computes it for whole sequences (queries scaled by the caller).
+
+    q           [groups, rows, heads, dim]: the new token of each row (beam, sample, sequence) of each group
+    own_k/v     [groups, rows, slots, kv_heads, dim]: what each row has to itself (its own past), or None
+    shared_k/v  [groups, positions, kv_heads, dim]: what the rows of a group have in common (the source sentence of its
+                beams, a prompt), or None; read once for all of them
+    lengths     how much of the cache is in use: a number, an int64 tensor ([groups, rows] own, [groups] shared), or None for
+                all of it.  Lengths on the device are clamped to the slots; what lies beyond them is never read.
+
+    kv_heads divides heads; key head i serves heads/kv_heads neighbouring query heads.  Caches may be any view whose last
+    dimension is contiguous.  Returns [groups, rows, heads, dim]; a row that sees no position gets zeros.  The softmax
+    shift is the floor of the row's own maximum instead of the whole tensor's, which changes nothing but the rounding
+    of the shifted scores.  Head dimensions up to 256."""
+    _fp32("queries", q, 4)
+    groups, rows, heads, dim = q.shape
+    if own_k is None and shared_k is None:
+        raise ValueError("cached_attention needs shared or own keys and values")
+    if dim > MAX_HEAD_DIM:
+        raise ValueError(f"head dimension {dim} is above {MAX_HEAD_DIM}")
+    own_k, own_v, own_lengths = _cache("own", own_k, own_v, own_lengths, (groups, rows), heads, dim)
+    shared_k, shared_v, shared_lengths = _cache("shared", shared_k, shared_v, shared_lengths, (groups,), heads, dim)
+    if own_k is not None and shared_k is not None and own_k.shape[-2] != shared_k.shape[-2]:
+        raise ValueError(f"shared keys have {shared_k.shape[-2]} heads, own keys {own_k.shape[-2]}")
+    _no_backward("cached_attention", q, own_k, own_v, shared_k, shared_v)
+    dev = _lib.require_cuda(q, own_k, own_v, own_lengths, shared_k, shared_v, shared_lengths)
+    if dim > 1 and q.stride(-1) != 1:
+        q = q.contiguous()
+    out = torch.empty(groups, rows, heads, dim, dtype=torch.float32, device=dev)
+    if out.numel() == 0:
+        return out
+    kv_heads = (shared_k if own_k is None else own_k).shape[-2]
+    shared, own = (0 if t is None else t.shape[-3] for t in (shared_k, own_k))
+    strides = (ctypes.c_int64 * 17)(*q.stride()[:3], *(shared_k.stride()[:3] + shared_v.stride()[:3] if shared else (0,) * 6),
+                                    *(own_k.stride()[:4] + own_v.stride()[:4] if own else (0,) * 8))
+    ptr = lambda t, used=True: t.data_ptr() if t is not None and used else None
+    handle = _lib.lib()
+    sizes = (groups, rows, heads, kv_heads, dim, shared, own)
+    ws_bytes = handle.pamk_cached_attention_workspace_bytes(*sizes)
+    # (a buffer of this call alone: calls captured into different graphs share none)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    with _lib.device_guard(dev):
+        status = handle.pamk_cached_attention(q.data_ptr(), out.data_ptr(), ptr(shared_k, shared), ptr(shared_v, shared), ptr(shared_lengths),
+                                              ptr(own_k, own), ptr(own_v, own), ptr(own_lengths), *sizes, strides, _offset(offset),
+                                              ptr(ws), ws_bytes, _lib.stream_ptr(dev))
+    _lib.check(status, "pamk_cached_attention")
+    return out
+
+
+def beam_select(logits, scores, k, banned=None, *, offset=None):
+    """One selection step of beam search: the k best continuations of every group over its beams and the vocabulary.
+
+    logits  [groups, beams, vocabulary]: of the next token
+    scores  [groups, beams]: the beams' scores so far; -inf (or NaN) for a beam that is not to be continued (at the first step all but
+            one), whose logits are not read
+    banned  bool, [vocabulary] or anything that broadcasts to the logits: tokens that must not be chosen (they keep their
+            share of the probability)
+
+    Returns (scores, beams, tokens), each [groups, k], best first: the new scores `scores + log_softmax(logits)` with the
+    PAM log-softmax, the beam each continues (int64) and its token (int64).  Values are formed and compared in 64 bits; equal
+    ones go to the lower beam, then to the lower token.  Logits of -1e30 or less, -inf among them, are masked: they have no
+    share in the probability.  Masked and banned tokens and the tokens of beams that are not continued have score -inf and come
+    last, also where a beam's logits hold NaN or overflow.  Up to 64 beams and k up to 64."""
+    _fp32("logits", logits, 3)
+    _fp32("scores", scores, 2)
+    groups, beams, vocab = logits.shape
+    if tuple(scores.shape) != (groups, beams):
+        raise ValueError(f"scores {tuple(scores.shape)} do not go with logits {tuple(logits.shape)}")
+    if not isinstance(k, int) or isinstance(k, bool) or not 1 <= k <= min(MAX_SELECTED, beams * vocab):
+        raise ValueError(f"k must be a number from 1 to {min(MAX_SELECTED, beams * vocab)}, got {k!r}")
+    if beams > MAX_BEAMS:
+        raise ValueError(f"{beams} beams are more than {MAX_BEAMS}")
+    _no_backward("beam_select", logits, scores)
+    dev = _lib.require_cuda(logits, scores, banned)
+    if banned is not None:
+        if not isinstance(banned, torch.Tensor) or banned.dtype != torch.bool:
+            raise TypeError("banned must be a bool tensor")
+        banned = banned.expand(groups, beams, vocab)
+        if vocab > 1 and banned.stride(-1) != 1:
+            banned = banned.contiguous()
+    if vocab > 1 and logits.stride(-1) != 1:
+        logits = logits.contiguous()
+    scores = scores.contiguous()
+    best = torch.empty(groups, k, dtype=torch.float32, device=dev)
+    which = torch.empty(2, groups, k, dtype=torch.int64, device=dev)
+    if groups:
+        handle = _lib.lib()
+        ws_bytes = handle.pamk_beam_select_workspace_bytes(groups, beams, vocab, k)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        with _lib.device_guard(dev):
+            status = handle.pamk_beam_select(logits.data_ptr(), scores.data_ptr(), None if banned is None else banned.data_ptr(), best.data_ptr(),
+                                             which[0].data_ptr(), which[1].data_ptr(), groups, beams, vocab, k, *logits.stride()[:2],
+                                             *((0, 0) if banned is None else banned.stride()[:2]), _offset(offset), ws.data_ptr(), ws_bytes,
+                                             _lib.stream_ptr(dev))
+        _lib.check(status, "pamk_beam_select")
+    return best, which[0], which[1]
+
+
+def _span(t):
+    """The bytes between a tensor's first and last element."""
+    start = t.data_ptr()
+    return start, start + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+
+
+def _refuse_overlaps(states, moved, parents):
+    """No two rows that move may share memory: neither of one tensor nor of two."""
+    spans = []
+    for t, size in zip(states, moved):
+        (groups, rows), (by_group, by_row) = t.shape[:2], (s * t.element_size() for s in t.stride()[:2])
+        nested = ((groups == 1 or by_group >= (rows - 1) * by_row + size) and (rows == 1 or by_row >= size) or
+                  (rows == 1 or by_row >= (groups - 1) * by_group + size) and (groups == 1 or by_group >= size))
+        if not nested:
+            raise ValueError(f"rows of a state of shape {tuple(t.shape)} and strides {t.stride()} overlap")
+        steps = [s for s, n in ((by_group, groups), (by_row, rows)) if n > 1]
+        spans.append((*_span(t), size, (by_group, by_row), min(steps, default=None)))
+    spans.sort(key=lambda s: s[:2])
+    start, end = _span(parents)
+    reach = []                                            # spans that may reach into the next one
+    for s in spans:
+        if s[0] < end and start < s[1]:
+            raise ValueError("the parents lie in the memory of a state")
+        reach = [r for r in reach if r[1] > s[0]]
+        for r in reach:
+            # (two parts of one buffer, interleaved row by row, are fine)
+            apart = s[0] - r[0]
+            if not (r[3] == s[3] and r[4] is not None and apart >= r[2] and apart + s[2] <= r[4]):
+                raise ValueError("two states share memory")
+        reach.append(s)
+
+
+def reorder_states(states, parents, used=None):
+    """Moves the states of beams to where the beams go on, in place: state[g, r] = state[g, parents[g, r]] for every tensor
+    [groups, beams, ...] in `states`, of any type.
+
+    parents  int64 [groups, beams], the beam that each new beam continues; one outside the beams leaves its row as it is
+    used     only the first `used` positions of the states' third dimension move (a number, or an int64 tensor of one element on the
+             device); None: whole rows
+
+    Each state's dimensions from the third on must be contiguous, and no two may share memory."""
+    states = list(states)
+    if not isinstance(parents, torch.Tensor) or parents.dtype != torch.int64 or parents.dim() != 2:
+        raise ValueError("parents must be an int64 tensor [groups, beams]")
+    groups, rows = parents.shape
+    on_device = isinstance(used, torch.Tensor)
+    if on_device:
+        if used.dtype != torch.int64 or used.numel() != 1:
+            raise ValueError("used must be a number or an int64 tensor of one element")
+    elif used is not None and (not isinstance(used, int) or isinstance(used, bool) or used < 0):
+        raise ValueError(f"used must be a number of positions, got {used!r}")
+    if rows > MAX_BEAMS:
+        raise ValueError(f"{rows} beams are more than {MAX_BEAMS}")
+    moved, positions = [], []
+    for t in states:
+        if not isinstance(t, torch.Tensor) or t.dim() < 2 or tuple(t.shape[:2]) != (groups, rows):
+            raise ValueError(f"every state must be a tensor [{groups}, {rows}, ...]")
+        if used is not None and t.dim() < 3:
+            raise ValueError("a state without positions cannot be moved in part")
+        block = 1
+        for n, s in reversed(list(zip(t.shape[2:], t.stride()[2:]))):
+            if n > 1 and s != block:
+                raise ValueError(f"a state of shape {tuple(t.shape)} and strides {t.stride()} is not contiguous within a row")
+            block *= n
+        slots = t.shape[2] if t.dim() > 2 else 1
+        unit = block // slots * t.element_size() if slots else 0
+        if used is not None and not on_device and used > slots:
+            raise ValueError(f"{used} positions of a state with {slots}")
+        positions.append(max(unit, 1))
+        moved.append(unit * (slots if used is None or on_device else used))
+    _no_backward("reorder_states", *states)
+    if not states or parents.numel() == 0:
+        return
+    dev = _lib.require_cuda(*states, parents, used)
+    parents = parents.contiguous()
+    keep = [i for i, size in enumerate(moved) if size]
+    states, moved, positions = ([x[i] for i in keep] for x in (states, moved, positions))
+    if not states:
+        return
+    _refuse_overlaps(states, moved, parents)
+    count = len(states)
+    numbers = lambda values: (ctypes.c_int64 * count)(*values)
+    with _lib.device_guard(dev):
+        status = _lib.lib().pamk_reorder_states(
+            (ctypes.c_void_p * count)(*[t.data_ptr() for t in states]), numbers(t.stride(0) * t.element_size() for t in states),
+            numbers(t.stride(1) * t.element_size() for t in states), numbers(moved), numbers(positions), count, parents.data_ptr(),
+            used.data_ptr() if on_device else None, groups, rows, _lib.stream_ptr(dev))
+    _lib.check(status, "pamk_reorder_states")
+    for t in states:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
