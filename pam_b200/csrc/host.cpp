@@ -32,6 +32,7 @@
 #include <dlfcn.h>
 #include <nvtx3/nvToolsExt.h>
 
+#include <algorithm>
 #include <array>
 #include <atomic>
 #include <map>
@@ -57,12 +58,14 @@ using torch::autograd::variable_list;
 #define PAMK_QUERIES(X)                                                                                   \
     X(pamk_status_string) X(pamk_last_cuda_error) X(pamk_matmul_auto_split) X(pamk_matmul_bwd_auto_split) \
     X(pamk_matmul_scratch_bytes) X(pamk_column_sum_workspace_bytes) X(pamk_layer_norm_max_width) X(pamk_layer_norm_stats_per_row)      \
-    X(pamk_layer_norm_bwd_workspace_bytes) X(pamk_softmax_max_len) X(pamk_softmax_workspace_bytes)
+    X(pamk_layer_norm_bwd_workspace_bytes) X(pamk_softmax_max_len) X(pamk_softmax_workspace_bytes)                                      \
+    X(pamk_cached_attention_workspace_bytes) X(pamk_beam_select_workspace_bytes)
 #define PAMK_LAUNCHES(X)                                                                                  \
     X(pamk_pam_fwd) X(pamk_pad_fwd) X(pamk_pam_grad) X(pamk_pad_grad) X(pamk_matmul_bias)                 \
     X(pamk_matmul_strided) X(pamk_matmul_bwd) X(pamk_column_sum) X(pamk_layer_norm_fwd)                   \
     X(pamk_layer_norm_fwd_save) X(pamk_layer_norm_bwd) X(pamk_layer_norm_bwd_saved) X(pamk_softmax_fwd)   \
-    X(pamk_softmax_fwd_save) X(pamk_softmax_bwd) X(pamk_softmax_bwd_saved) X(pamk_adam_step)
+    X(pamk_softmax_fwd_save) X(pamk_softmax_bwd) X(pamk_softmax_bwd_saved) X(pamk_adam_step) \
+    X(pamk_cached_attention) X(pamk_beam_select) X(pamk_reorder_states)
 
 std::atomic<bool> g_nvtx{false};         // set_nvtx
 
@@ -126,15 +129,17 @@ bool has_tangent(const Tensor& t) {
     return meta != nullptr && meta->fw_grad_ != nullptr && t._fw_grad(0).defined();
 }
 
-// fp32 CUDA data that the kernels may read in place: strided, no wrapper of other tensors (functorch, fake, functional), no
+// CUDA data that the kernels may read in place: strided, no wrapper of other tensors (functorch, fake, functional), no
 // lazy negation or zero.  A tensor with a tangent is for the Python layer, which refuses it: here the tangent
 // would be lost without a word.
-bool usable(const Tensor& t) {
+bool readable(const Tensor& t) {
     using K = c10::DispatchKey;
     constexpr c10::DispatchKeySet special({K::Python, K::PythonTLSSnapshot, K::FuncTorchBatched, K::FuncTorchGradWrapper, K::Batched,
                                            K::Functionalize, K::Conjugate, K::Negative, K::ZeroTensor, K::Sparse, K::SparseCsr, K::NestedTensor});
-    return t.defined() && t.is_cuda() && t.scalar_type() == at::kFloat && !t.key_set().has_any(special) && !has_tangent(t);
+    return t.defined() && t.is_cuda() && !t.key_set().has_any(special) && !has_tangent(t);
 }
+
+bool usable(const Tensor& t) { return readable(t) && t.scalar_type() == at::kFloat; }      // fp32
 
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
@@ -834,6 +839,147 @@ std::optional<Tensor> op_attention_heads(const Tensor& gq, const Tensor& gk, con
     return out;
 }
 
+// ---- text generation --------------------------------------------------------------------------------------------
+
+// A cache's lengths as the caller gave them: none, a number or a tensor.
+struct Lengths {
+    Tensor t;
+    int64_t n = -1;
+};
+
+// Whether a pair of caches goes with queries of `lead` and `dim`; sets the number of slots that are in use at most.
+bool cache_ok(const Tensor& k, const Tensor& v, const Lengths& lengths, at::IntArrayRef lead, int64_t heads, int64_t dim, const Tensor& q, int64_t& slots) {
+    slots = 0;
+    if (!k.defined() && !v.defined()) return !lengths.t.defined() && lengths.n < 0;
+    const int64_t nd = (int64_t)lead.size() + 3;
+    for (const Tensor* t : {&k, &v})
+        if (!usable(*t) || t->device() != q.device() || t->dim() != nd || t->sizes().slice(0, lead.size()) != lead || t->size(-1) != dim ||
+            (dim > 1 && t->stride(-1) != 1) || wants_grad(*t))
+            return false;
+    if (k.sizes() != v.sizes() || k.size(-2) < 1 || heads % k.size(-2)) return false;
+    slots = k.size(-3);
+    if (lengths.n > slots) return false;
+    if (lengths.n >= 0) slots = lengths.n;
+    const Tensor& n = lengths.t;
+    return !n.defined() || (readable(n) && n.scalar_type() == at::kLong && n.device() == q.device() && n.sizes() == lead && n.is_contiguous());
+}
+
+std::optional<Tensor> op_cached_attention(const Tensor& q, const Tensor& own_k, const Tensor& own_v, const Lengths& own_lengths, const Tensor& shared_k,
+                                          const Tensor& shared_v, const Lengths& shared_lengths, double offset) {
+    if (!usable(q) || q.dim() != 4 || q.numel() == 0 || q.stride(3) != 1 || q.size(3) > 256 || wants_grad(q)) return {};
+    if (!own_k.defined() && !shared_k.defined()) return {};
+    const int64_t G = q.size(0), R = q.size(1), H = q.size(2), D = q.size(3);
+    int64_t own, shared;
+    const int64_t lead[2] = {G, R};
+    if (!cache_ok(own_k, own_v, own_lengths, lead, H, D, q, own) ||
+        !cache_ok(shared_k, shared_v, shared_lengths, at::IntArrayRef(lead, 1), H, D, q, shared))
+        return {};
+    if (own_k.defined() && shared_k.defined() && own_k.size(3) != shared_k.size(2)) return {};
+    const int64_t K = own_k.defined() ? own_k.size(3) : shared_k.size(2);
+    c10::cuda::CUDAGuard guard(q.device());
+    int64_t strides[17] = {q.stride(0), q.stride(1), q.stride(2)};
+    for (int i = 0; i < 3 && shared; ++i) {
+        strides[3 + i] = shared_k.stride(i);
+        strides[6 + i] = shared_v.stride(i);
+    }
+    for (int i = 0; i < 4 && own; ++i) {
+        strides[9 + i] = own_k.stride(i);
+        strides[13 + i] = own_v.stride(i);
+    }
+    Tensor out = empty_on({G, R, H, D}, q), ws;
+    const size_t bytes = lib.pamk_cached_attention_workspace_bytes(G, R, H, K, D, shared, own);
+    if (bytes) ws = scratch_bytes(bytes, q);
+    const auto count = [](const Lengths& l) { return l.t.defined() ? static_cast<const int64_t*>(l.t.data_ptr()) : nullptr; };
+    check(lib.pamk_cached_attention(ptr(q), ptr(out), shared ? ptr(shared_k) : nullptr, shared ? ptr(shared_v) : nullptr, count(shared_lengths),
+                                    own ? ptr(own_k) : nullptr, own ? ptr(own_v) : nullptr, count(own_lengths), G, R, H, K, D, shared, own, strides,
+                                    (float)offset, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q)),
+          "pamk_cached_attention");
+    return out;
+}
+
+// (scores, beams, tokens)
+std::optional<std::array<Tensor, 3>> op_beam_select(const Tensor& logits, const Tensor& scores, int64_t k, const Tensor& banned, double offset) {
+    if (!usable(logits) || !usable(scores) || logits.dim() != 3 || scores.dim() != 2 || scores.device() != logits.device() || logits.numel() == 0) return {};
+    if (scores.sizes() != logits.sizes().slice(0, 2) || !scores.is_contiguous() || logits.stride(2) != 1 || wants_grad(logits) || wants_grad(scores)) return {};
+    const int64_t G = logits.size(0), R = logits.size(1), V = logits.size(2);
+    if (R > 64 || k < 1 || k > 64 || k > R * V) return {};
+    int64_t ban[2] = {0, 0};
+    if (banned.defined()) {
+        if (!readable(banned) || banned.scalar_type() != at::kBool || banned.device() != logits.device() || banned.dim() < 1 || banned.dim() > 3 ||
+            banned.size(-1) != V || banned.stride(-1) != 1)
+            return {};
+        for (int64_t d = 2; d <= banned.dim(); ++d) {
+            const int64_t n = banned.size(-d), want = logits.size(-d);
+            if (n != want && n != 1) return {};
+            ban[3 - d] = n == 1 ? 0 : banned.stride(-d);
+        }
+    }
+    c10::cuda::CUDAGuard guard(logits.device());
+    Tensor best = empty_on({G, k}, logits);
+    const auto whole = [&] { return at::detail::empty_cuda({G, k}, at::kLong, logits.device(), std::nullopt); };
+    Tensor beams = whole(), tokens = whole();
+    const size_t bytes = lib.pamk_beam_select_workspace_bytes(G, R, V, k);
+    Tensor ws = scratch_bytes(bytes, logits);
+    check(lib.pamk_beam_select(ptr(logits), ptr(scores), banned.defined() ? static_cast<const unsigned char*>(banned.data_ptr()) : nullptr, ptr(best),
+                               static_cast<int64_t*>(beams.data_ptr()), static_cast<int64_t*>(tokens.data_ptr()), G, R, V, k, logits.stride(0),
+                               logits.stride(1), ban[0], ban[1], (float)offset, ws.data_ptr(), bytes, stream_of(logits)),
+          "pamk_beam_select");
+    return std::array<Tensor, 3>{best, beams, tokens};
+}
+
+// True once the states are moved; false where the call is for the Python layer: all that it refuses, and views of one buffer
+// whose rows lie interleaved.
+bool op_reorder_states(const std::vector<Tensor>& states, const Tensor& parents, const Tensor& used, int64_t used_n) {
+    if (!readable(parents) || parents.scalar_type() != at::kLong || parents.dim() != 2 || !parents.is_contiguous() || parents.numel() == 0) return false;
+    const int64_t G = parents.size(0), R = parents.size(1);
+    if (R > 64) return false;
+    if (used.defined() && (!readable(used) || used.scalar_type() != at::kLong || used.numel() != 1 || used.device() != parents.device())) return false;
+    const bool part = used.defined() || used_n >= 0;
+    const size_t count = states.size();
+    std::vector<void*> base;
+    std::vector<int64_t> group, row, moved, position;
+    std::vector<std::pair<char*, char*>> spans;
+    for (auto* v : {&group, &row, &moved, &position}) v->reserve(count);
+    base.reserve(count);
+    spans.reserve(count + 1);
+    for (const Tensor& t : states) {
+        if (!readable(t) || t.dim() < (part ? 3 : 2) || t.size(0) != G || t.size(1) != R || t.device() != parents.device() || wants_grad(t)) return false;
+        const int64_t item = (int64_t)t.element_size();
+        int64_t block = 1;
+        for (int64_t d = t.dim() - 1; d >= 2; --d) {
+            if (t.size(d) > 1 && t.stride(d) != block) return false;
+            block *= t.size(d);
+        }
+        const int64_t slots = t.dim() > 2 ? t.size(2) : 1;
+        if (used_n > slots) return false;
+        if (block == 0) continue;
+        const int64_t unit = block / slots * item, bytes = unit * (used_n >= 0 ? used_n : slots), by_group = t.stride(0) * item, by_row = t.stride(1) * item;
+        if (bytes == 0) continue;
+        if ((G > 1 && by_group < (R - 1) * by_row + bytes) || (R > 1 && by_row < bytes)) return false;       // (rows within groups, none overlapping)
+        char* p = static_cast<char*>(t.data_ptr());
+        base.push_back(p);
+        group.push_back(by_group);
+        row.push_back(by_row);
+        moved.push_back(bytes);
+        position.push_back(unit);
+        spans.emplace_back(p, p + (G - 1) * by_group + (R - 1) * by_row + bytes);
+    }
+    char* p = static_cast<char*>(parents.data_ptr());
+    spans.emplace_back(p, p + parents.numel() * 8);
+    if (used.defined()) spans.emplace_back(static_cast<char*>(used.data_ptr()), static_cast<char*>(used.data_ptr()) + 8);
+    std::sort(spans.begin(), spans.end());
+    for (size_t i = 1; i < spans.size(); ++i)
+        if (spans[i].first < spans[i - 1].second) return false;
+    c10::cuda::CUDAGuard guard(parents.device());
+    check(lib.pamk_reorder_states(base.data(), group.data(), row.data(), moved.data(), position.data(), (int)base.size(),
+                                  static_cast<const int64_t*>(parents.data_ptr()), used.defined() ? static_cast<const int64_t*>(used.data_ptr()) : nullptr, G, R,
+                                  stream_of(parents)),
+          "pamk_reorder_states");
+    for (const Tensor& t : states)
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    return true;
+}
+
 // ---- Python entry points -----------------------------------------------------------------------------------------
 
 // Reads a tensor argument: undefined for None, false for anything that is neither (a subclass other than
@@ -1030,6 +1176,75 @@ PyObject* py_attention_heads(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
             !as_offset(a[5], off))
             return none();
         return wrapped([&] { return op_attention_heads(q, k, v, m, heads, off); });
+    });
+}
+
+// A number of positions, a tensor of them, or None.
+bool as_lengths(PyObject* o, Lengths& l) {
+    if (PyLong_CheckExact(o)) return as_int(o, l.n) && l.n >= 0;
+    return as_tensor(o, l.t);
+}
+
+// cached_attention(q, own_k, own_v, own_lengths, shared_k, shared_v, shared_lengths, offset)
+PyObject* py_cached_attention(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    PAMK_ARGS(8)
+    return operator_call([&]() -> PyObject* {
+        Tensor q, own_k, own_v, shared_k, shared_v;
+        Lengths own, shared;
+        double off;
+        if (!as_tensor(a[0], q) || !as_tensor(a[1], own_k) || !as_tensor(a[2], own_v) || !as_lengths(a[3], own) || !as_tensor(a[4], shared_k) ||
+            !as_tensor(a[5], shared_v) || !as_lengths(a[6], shared) || !as_offset(a[7], off))
+            return none();
+        return wrapped([&] { return op_cached_attention(q, own_k, own_v, own, shared_k, shared_v, shared, off); });
+    });
+}
+
+// beam_select(logits, scores, k, banned | None, offset)
+PyObject* py_beam_select(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    PAMK_ARGS(5)
+    return operator_call([&]() -> PyObject* {
+        Tensor x, scores, banned;
+        int64_t k;
+        double off;
+        if (!as_tensor(a[0], x) || !as_tensor(a[1], scores) || !PyLong_CheckExact(a[2]) || !as_int(a[2], k) || !as_tensor(a[3], banned) || !as_offset(a[4], off))
+            return none();
+        std::optional<std::array<Tensor, 3>> found;
+        {
+            const Unlocked others_may_run;
+            found = op_beam_select(x, scores, k, banned, off);
+        }
+        if (!found) return none();
+        PyObject* out = PyTuple_New(3);
+        if (out == nullptr) return nullptr;
+        for (int i = 0; i < 3; ++i) {
+            PyObject* t = THPVariable_Wrap(std::move((*found)[i]));
+            if (t == nullptr) {
+                Py_DECREF(out);
+                return nullptr;
+            }
+            PyTuple_SET_ITEM(out, i, t);
+        }
+        return out;
+    });
+}
+
+// reorder_states(list of states, parents, used: number, tensor or None): True, or None
+PyObject* py_reorder_states(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    PAMK_ARGS(3)
+    return operator_call([&]() -> PyObject* {
+        Tensor parents;
+        Lengths used;
+        if (!PyList_CheckExact(a[0]) || !as_tensor(a[1], parents) || !as_lengths(a[2], used)) return none();
+        std::vector<Tensor> states(PyList_GET_SIZE(a[0]));
+        for (size_t i = 0; i < states.size(); ++i)
+            if (!as_tensor(PyList_GET_ITEM(a[0], i), states[i])) return none();
+        bool moved;
+        {
+            const Unlocked others_may_run;
+            moved = op_reorder_states(states, parents, used.t, used.n);
+        }
+        if (!moved) return none();
+        Py_RETURN_TRUE;
     });
 }
 
@@ -1235,6 +1450,9 @@ PyMethodDef methods[] = {
     PAMK_FAST("softmax", py_softmax),
     PAMK_FAST("attention_qkv", py_attention_qkv),
     PAMK_FAST("attention_heads", py_attention_heads),
+    PAMK_FAST("cached_attention", py_cached_attention),
+    PAMK_FAST("beam_select", py_beam_select),
+    PAMK_FAST("reorder_states", py_reorder_states),
     PAMK_FAST("adam_collect", py_adam_collect),
     PAMK_FAST("adam_apply", py_adam_apply),
     {nullptr, nullptr, 0, nullptr},

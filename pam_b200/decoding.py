@@ -76,6 +76,10 @@ def cached_attention(q, own_k=None, own_v=None, own_lengths=None, *, shared_k=No
     dimension is contiguous.  Returns [groups, rows, heads, dim]; a row that sees no position gets zeros.  The softmax
     shift is the floor of the row's own maximum instead of the whole tensor's, which changes nothing but the rounding
     of the shifted scores.  Head dimensions up to 256."""
+    if (host := _lib.host()) is not None:
+        out = host.cached_attention(q, own_k, own_v, own_lengths, shared_k, shared_v, shared_lengths, offset)
+        if out is not None:
+            return out
     _fp32("queries", q, 4)
     groups, rows, heads, dim = q.shape
     if own_k is None and shared_k is None:
@@ -125,6 +129,10 @@ def beam_select(logits, scores, k, banned=None, *, offset=None):
     ones go to the lower beam, then to the lower token.  Logits of -1e30 or less, -inf among them, are masked: they have no
     share in the probability.  Masked and banned tokens and the tokens of beams that are not continued have score -inf and come
     last, also where a beam's logits hold NaN or overflow.  Up to 64 beams and k up to 64."""
+    if (host := _lib.host()) is not None:
+        out = host.beam_select(logits, scores, k, banned, offset)
+        if out is not None:
+            return out
     _fp32("logits", logits, 3)
     _fp32("scores", scores, 2)
     groups, beams, vocab = logits.shape
@@ -202,6 +210,8 @@ def reorder_states(states, parents, used=None):
 
     Each state's dimensions from the third on must be contiguous, and no two may share memory."""
     states = list(states)
+    if (host := _lib.host()) is not None and host.reorder_states(states, parents, used):
+        return
     if not isinstance(parents, torch.Tensor) or parents.dtype != torch.int64 or parents.dim() != 2:
         raise ValueError("parents must be an int64 tensor [groups, beams]")
     groups, rows = parents.shape
