@@ -9,12 +9,21 @@
 //
 // pam is not linear: pam(pad(e, S), v) summed is not pad(sum of pam(e, v), S).  A running maximum and sum with one
 // joint pass over keys and values is therefore not to be had; the sum must be known before the first value is
-// weighted.  The keys are read in a first kernel, which leaves t and each range's maximum and sum of exponentials, the values in a
-// second one; ranges of a long axis are added by a third.
+// weighted.  So there are two passes.  The keys leave t (rows times positions, a small part of what the keys are) and each CTA's maximum and sum,
+// kept as it goes: whole shifts scale exponentials exactly.  The values read them, turn t into p on the way, and leave sums
+// of products; where the positions of a row are dealt out to several CTAs, a third kernel adds these.
 //
-// Rows that share positions are worked on together, up to eight per CTA: every key and value is loaded once for all of them.  A
-// product is one integer and one floating-point add; the range rule (pam_scalar.cuh) is decided per vector of loaded
-// elements: where every exponent field of both sides lies in [66, 187], every product passes it.
+// Rows that see the same positions are worked on together, up to 8 per CTA: every key and value is loaded once for all of them, by
+// asynchronous copies into a ring that each warp has for itself, so that the warps run without barriers until their last sums.
+// Keys: a lane owns a position, 32 floats of it per stage, and reads the queries from
+// shared memory.  Values: a lane owns four columns.  A product is one integer and one floating-point add; the range rule
+// (pam_scalar.cuh) is decided per stage: where every exponent field of both sides lies in [66, 187], every product passes it.
+#include <limits.h>
+
+#include <algorithm>
+
+#include <cuda_pipeline_primitives.h>
+
 #include "common.cuh"
 #include "pam_scalar.cuh"
 
@@ -22,172 +31,40 @@ namespace pamk {
 namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr int kMaxRows = 8;                       // rows of a tile
-constexpr int kMostChunk = 512;                   // positions of a range
+constexpr int kSlice = 32, kQuads = kSlice / 4;         // floats of a key in a stage
+constexpr int kKeyBytes = 32 * kSlice * 4;              // a stage of keys: 32 positions
+constexpr int kMostRows = 8, kWarps = 4, kMostWarps = 8;
 
-// Positions that rows see together: those of a group (`per_row` 0: all its rows), or one row's own.
+// Positions that the rows of a unit see together: a group's shared ones (all its rows and a key head's query heads), or a row's own (its query heads).
 struct Segment {
     const float *k, *v;
     const int64_t* lengths;                       // one per unit, or null: all slots
     int64_t k_group, k_row, k_pos, k_head, v_group, v_row, v_pos, v_head;
-    int slots, chunk, chunks, tiles;
-    int per_row, rows;                            // rows that share it
-    int first_chunk, first_pos;                   // among the chunks and the scores of a row
+    int slots, per_row;
+    int tiles, tile_rows, ranks;                  // CTAs of a (unit, key head): tiles of rows, shares of the positions
+    int first_pos, first_part;                    // where its scores and its parts begin among a row's
 };
 
 struct Attention {
     const float* q;
     float* out;
     int64_t q_group, q_row, q_head;
-    int groups, rows, kv_heads, share, dim;       // `share` query heads on each key head
+    int rows, kv_heads, share, dim;               // `share` query heads on each key head
     int32_t off;
-    float* scores;                                // [groups, kv_heads, rows * share, width]
-    float2* stats;                                // [groups, kv_heads, rows * share, chunks]: floor of the maximum, sum
-    float* parts;                                 // [groups, kv_heads, rows * share, chunks, dim]
-    int width, chunks;
+    int has_beside, beside;                       // the next kernel runs beside this one; this one beside the one before, and ends after it
+    int split;                                    // keys: the slices of a piece are dealt out to warps too
+    float* scores;                                // t: [(group, key head, row, head of the key head)][width]
+    float2* stats;                                // [the same][parts]: floor of the maximum, sum
+    float* sums;                                  // [the same][parts][dim], or null: straight to out
+    int width, parts;
 };
 
-// Where a CTA works.
-struct Place {
-    int64_t group, base;                          // `base` + n: index of the tile's n-th row in scores, stats and parts
-    int kv_head, row, tile, chunk, begin, end;    // positions [begin, end)
-};
-
-__device__ __forceinline__ Place place_of(const Attention& a, const Segment& s, int rows_per_tile) {
-    Place p;
-    int64_t at = blockIdx.x;
-    p.chunk = (int)(at % s.chunks);
-    at /= s.chunks;
-    p.tile = (int)(at % s.tiles);
-    at /= s.tiles;
-    p.kv_head = (int)(at % a.kv_heads);
-    at /= a.kv_heads;
-    p.row = s.per_row ? (int)(at % a.rows) : 0;
-    p.group = s.per_row ? at / a.rows : at;
-    int64_t live = s.slots;
-    if (s.lengths) {
-        const int64_t n = s.lengths[at];
-        live = n < 0 ? 0 : n < s.slots ? n : s.slots;
-    }
-    p.begin = p.chunk * s.chunk;
-    p.end = (int)(live < p.begin + s.chunk ? live : p.begin + s.chunk);
-    p.base = (p.group * a.kv_heads + p.kv_head) * ((int64_t)a.rows * a.share) + p.row * a.share + p.tile * rows_per_tile;
-    return p;
-}
-
-__device__ __forceinline__ int rows_of(const Segment& s, const Place& p, int rows_per_tile) {
-    return min(rows_per_tile, s.rows - p.tile * rows_per_tile);
-}
-
-// 0 .. below 2 * (188 - 66) << 23 where the exponent field lies in [66, 187]
-__device__ __forceinline__ uint32_t beyond(float x) { return 2u * (uint32_t)f2i(x) - 2u * (66u << 23); }
+// 0 .. below kBand where the exponent field lies in [66, 187]
+__device__ __forceinline__ uint32_t beyond(int32_t x) { return 2u * (uint32_t)x - 2u * (66u << 23); }
 constexpr uint32_t kBand = 2u * ((188u - 66u) << 23);
+__device__ __forceinline__ uint32_t beyond(int4 x) { return max(max(beyond(x.x), beyond(x.y)), max(beyond(x.z), beyond(x.w))); }
 
-// Lane l of eight holds element e of slot i of a row of `dim`: with vectors 16 bytes at a time, else one float after another.
-template <bool VEC>
-__device__ __forceinline__ int element(int l, int i, int e) { return VEC ? (l + 8 * i) * 4 + e : l + 8 * (4 * i + e); }
-
-template <int SLOTS, bool VEC>
-__device__ __forceinline__ void load_row(float (&x)[SLOTS * 4], const float* p, int l, int dim, float absent) {
-#pragma unroll
-    for (int i = 0; i < SLOTS; ++i) {
-        if (VEC) {
-            float4 w = make_float4(absent, absent, absent, absent);
-            if ((l + 8 * i) * 4 < dim) w = __ldg(reinterpret_cast<const float4*>(p) + l + 8 * i);
-            x[4 * i] = w.x; x[4 * i + 1] = w.y; x[4 * i + 2] = w.z; x[4 * i + 3] = w.w;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int d = element<VEC>(l, i, e);
-                x[4 * i + e] = d < dim ? __ldg(p + d) : absent;
-            }
-        }
-    }
-}
-
-// Adds up N values over the eight lanes of a position; lane l is left with the sum of value l / (8 / P), P the power of two from N on.
-template <int N>
-__device__ __forceinline__ float sum_over_eight(float (&s)[N], int l) {
-    constexpr int P = N > 4 ? 8 : N > 2 ? 4 : N > 1 ? 2 : 1;
-    float t[P];
-#pragma unroll
-    for (int i = 0; i < P; ++i) t[i] = i < N ? s[i] : 0.0f;
-#pragma unroll
-    for (int w = P / 2, d = 4; d > 0; w >>= 1, d >>= 1) {
-        if (w > 0) {
-            const bool upper = l & d;
-#pragma unroll
-            for (int i = 0; i < P / 2; ++i)
-                if (i < w) {
-                    const float other = __shfl_xor_sync(0xffffffffu, upper ? t[i] : t[i + w], d);
-                    t[i] = fadd(upper ? t[i + w] : t[i], other);
-                }
-        } else {
-            t[0] = fadd(t[0], __shfl_xor_sync(0xffffffffu, t[0], d));
-        }
-    }
-    return t[0];
-}
-
-// t of the tile's rows for positions [begin, end), to scores[n * stride + position - begin] in shared memory.
-template <int SLOTS, int ROWS, bool VEC>
-__device__ __forceinline__ void score_range(const Attention& a, const Segment& s, const Place& p, int rows, float* scores, int stride) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const int l = lane & 7, sub = lane >> 3;
-    constexpr int kAtOnce = SLOTS >= 8 ? 1 : SLOTS == 4 ? 2 : 4;                 // positions of a lane whose loads are on their way together
-    // an absent element of the key is 1.0f and the query's biased pattern -bits(1.0f): their product's pattern is +0
-    int32_t q[ROWS][SLOTS * 4];
-    bool plain = true;
-#pragma unroll
-    for (int n = 0; n < ROWS; ++n) {
-        const int r = p.tile * ROWS + min(n, rows - 1);
-        const int row = s.per_row ? p.row : r / a.share, head = p.kv_head * a.share + (s.per_row ? r : r % a.share);
-        float x[SLOTS * 4];
-        load_row<SLOTS, VEC>(x, a.q + p.group * a.q_group + row * a.q_row + head * a.q_head, l, a.dim, 1.0f);
-#pragma unroll
-        for (int i = 0; i < SLOTS * 4; ++i) {
-            plain = plain && beyond(x[i]) < kBand;
-            q[n][i] = element<VEC>(l, i / 4, i % 4) < a.dim ? isub(f2i(x[i]), kBias - a.off) : -kBias;
-        }
-    }
-    plain = __all_sync(0xffffffffu, plain);
-    const float* keys = s.k + p.group * s.k_group + p.row * s.k_row + p.kv_head * s.k_head;
-    for (int j0 = p.begin + warp * 4 * kAtOnce; j0 < p.end; j0 += warps * 4 * kAtOnce) {
-        float k[kAtOnce][SLOTS * 4];
-#pragma unroll
-        for (int u = 0; u < kAtOnce; ++u)
-            load_row<SLOTS, VEC>(k[u], keys + (int64_t)min(j0 + u * 4 + sub, p.end - 1) * s.k_pos, l, a.dim, 1.0f);
-#pragma unroll
-        for (int u = 0; u < kAtOnce; ++u) {
-            uint32_t far = 0u;
-#pragma unroll
-            for (int i = 0; i < SLOTS * 4; ++i) far = max(far, beyond(k[u][i]));
-            float sum[ROWS];
-            if (__all_sync(0xffffffffu, plain && far < kBand)) {
-#pragma unroll
-                for (int n = 0; n < ROWS; ++n) {
-                    sum[n] = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < SLOTS * 4; ++i) sum[n] = fadd(sum[n], i2f(iadd(q[n][i], f2i(k[u][i]))));
-                }
-            } else {
-#pragma unroll
-                for (int n = 0; n < ROWS; ++n) {
-                    sum[n] = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < SLOTS * 4; ++i)
-                        if (element<VEC>(l, i / 4, i % 4) < a.dim)
-                            sum[n] = fadd(sum[n], mul(i2f(iadd(q[n][i], kBias - a.off)), k[u][i], a.off));
-                }
-            }
-            const float total = sum_over_eight<ROWS>(sum, l);
-            constexpr int kEach = ROWS > 4 ? 1 : ROWS > 2 ? 2 : ROWS > 1 ? 4 : 8;              // lanes with the same sum
-            const int n = l / kEach, j = j0 + u * 4 + sub;
-            if (n < rows && l % kEach == 0 && j < p.end)
-                scores[n * stride + j - p.begin] = total == -INFINITY ? -INFINITY : mul(total, kLog2e, a.off);
-        }
-    }
-}
+__device__ __forceinline__ void add_pair(float2& acc, int p0, int p1) { acc = __fadd2_rn(acc, make_float2(i2f(p0), i2f(p1))); }
 
 __device__ __forceinline__ float warp_max(float m) {
 #pragma unroll
@@ -200,274 +77,649 @@ __device__ __forceinline__ float warp_sum(float m) {
     return m;
 }
 
-// e of one scaled score.  (NaN scores do not reach the shift; they reach the sum.)
+// 2^e for whole e from -126 to 127: e + 127 are the low bits of the sum
+__device__ __forceinline__ float power_of(float e) { return i2f(f2i(fadd(e, 8388608.0f + 127.0f)) << 23); }
+
+// e of one scaled score, of which t - shift < 1.  What is below 2^-126 divides to 0.  (NaN scores do not reach the shift; they reach the sum.)
 __device__ __forceinline__ float exponential(float t, float shift) {
-    return t == -INFINITY ? 0.0f : exp2_compact(fadd(t, -shift));
+    const float x = fadd(t, -shift), whole = floorf(x), e = fmul(fadd(1.0f, fadd(x, -whole)), power_of(whole));
+    return whole >= -126.0f ? e : x != x && t != -INFINITY ? x : 0.0f;
 }
 
-// 2^e for whole e <= 0, also -inf and NaN
-__device__ __forceinline__ float power(float e) {
-    return e >= -126.0f ? i2f(((int32_t)e + 127) << 23) : e != e ? quiet_nan() : 0.0f;
+// A sum (y) whose shift rises from x to `top`.
+__device__ __forceinline__ float rescaled(float2 s, float top) {
+    const float down = fadd(s.x, -top);
+    return down >= -126.0f ? fmul(s.y, power_of(down)) : s.y == s.y ? 0.0f : s.y;
 }
 
-template <int SLOTS, int ROWS, bool VEC>
-__global__ void __launch_bounds__(256) score_kernel(const Attention a, const Segment s) {
-    __shared__ float tile[ROWS * kMostChunk];
-    const Place p = place_of(a, s, ROWS);
-    const int rows = rows_of(s, p, ROWS), lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-    score_range<SLOTS, ROWS, VEC>(a, s, p, rows, tile, kMostChunk);
-    __syncthreads();
-    const int count = p.end - p.begin;
-    after_previous();                              // (the scores of the other segment are on their way: both are waited for by what follows)
-    for (int n = threadIdx.x >> 5; n < rows; n += warps) {
-        float m = -INFINITY, sum = 0.0f;
-        for (int j = lane; j < count; j += 32) m = fmaxf(m, tile[n * kMostChunk + j]);
-        const float shift = floorf(warp_max(m));
-        float* to = a.scores + (p.base + n) * a.width + s.first_pos + p.begin;
-        for (int j = lane; j < count; j += 32) {
-            const float t = tile[n * kMostChunk + j];
-            to[j] = t;
-            sum = fadd(sum, exponential(t, shift));
-        }
-        sum = warp_sum(sum);
-        if (lane == 0) a.stats[(p.base + n) * a.chunks + s.first_chunk + p.chunk] = make_float2(shift, sum);
+// A maximum and a sum from those of `count` parts.
+template <class F>
+__device__ __forceinline__ float2 joined(F&& part, int count) {
+    float top = -INFINITY, sum = 0.0f;
+    for (int i = 0; i < count; ++i) top = fmaxf(top, part(i).x);
+    for (int i = 0; i < count; ++i) sum = fadd(sum, rescaled(part(i), top));
+    return make_float2(top, sum);
+}
+
+// The floor of the maximum and the sum of exponentials, as scores come.
+struct Running {
+    float top = -INFINITY, sum = 0.0f;
+    __device__ __forceinline__ void add(float t) {
+        const float most = fmaxf(top, floorf(t));
+        sum = fadd(rescaled(make_float2(top, sum), most), exponential(t, most));
+        top = most;
+    }
+};
+
+// A warp's ring of two stages: one is read while the other one arrives.  (With a third one calls of one row gain nothing, and others lose a CTA.)
+template <int BYTES>
+struct Ring {
+    char* to;                                     // where the next copies go; what has arrived, once they have been issued
+    int turn = BYTES;
+    __device__ __forceinline__ Ring(char* memory, int warp) : to(memory + warp * 2 * BYTES) {}
+    __device__ __forceinline__ char* next() {
+        char* now = to;
+        to += turn;
+        turn = -turn;
+        return now;
+    }
+};
+
+// Four neighbouring floats to shared memory, those below `dim` of them.
+template <bool VEC>
+__device__ __forceinline__ void copy_quad(char* to, const float* from, int d, int dim) {
+    if (VEC) {
+        __pipeline_memcpy_async(to, from, 16);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (d + e < dim) __pipeline_memcpy_async(to + 4 * e, from + e, 4);
     }
 }
 
-// The row's shift and sum from those of its chunks, by one warp.
-__device__ __forceinline__ float2 row_stats(const float2* stats, int chunks, int lane) {
-    float m = -INFINITY, sum = 0.0f;
-    for (int c = lane; c < chunks; c += 32) m = fmaxf(m, __ldcg(stats + c).x);
-    m = warp_max(m);
-    for (int c = lane; c < chunks; c += 32) {
-        const float2 t = __ldcg(stats + c);
-        sum = fadd(sum, t.y == 0.0f ? 0.0f : fmul(t.y, power(fadd(t.x, -m))));
+// What a CTA works on.
+struct Share {
+    int64_t group, base;                          // `base`: the tile's first row among all
+    int rank, kv_head, row, first, rows;          // the tile's rows [first, first + rows) among those that see the positions
+    int begin, count;                             // positions
+};
+
+// Every CTA of a row takes the same number of positions, a multiple of 32, until there are none left.
+__device__ __forceinline__ Share share_of(const Attention& a, const Segment& g) {
+    Share s;
+    unsigned at = blockIdx.x;
+    s.rank = (int)(at % g.ranks);
+    at /= g.ranks;
+    const int tile = (int)(at % g.tiles);
+    at /= g.tiles;
+    s.kv_head = (int)(at % a.kv_heads);
+    at /= a.kv_heads;
+    s.row = g.per_row ? (int)(at % a.rows) : 0;
+    s.group = g.per_row ? at / a.rows : at;
+    const int together = g.per_row ? a.share : a.rows * a.share;
+    s.first = tile * g.tile_rows;
+    s.rows = min(g.tile_rows, together - s.first);
+    s.base = (s.group * a.kv_heads + s.kv_head) * ((int64_t)a.rows * a.share) + s.row * a.share + s.first;
+    int live = g.slots;
+    if (g.lengths) {
+        const int64_t n = g.lengths[at];
+        live = n < 0 ? 0 : n < g.slots ? (int)n : g.slots;
     }
-    return make_float2(m, warp_sum(sum));
+    const int each = ((live + g.ranks - 1) / g.ranks + 31) / 32 * 32;
+    s.begin = min(s.rank * each, live);
+    s.count = min(each, live - s.begin);
+    return s;
 }
 
-// sum_j pam(p_j, v_jd) of the tile's rows over positions [begin, end): a warp takes four neighbouring positions (times the rows of values
-// that it holds at once), each lane four columns of each.  Leaves the sums of all warps in sums[n * 256 + d].
-template <int SLOTS, int ROWS, bool VEC>
-__device__ __forceinline__ void weigh_range(const Attention& a, const Segment& s, const Place& p, int rows, const float* probs, int stride,
-                                            const unsigned char* odd, float* sums) {
-    constexpr int kLanes = SLOTS >= 4 ? 32 : 8 * SLOTS, kCols = SLOTS == 8 ? 2 : 1, kAcross = 32 / kLanes;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const int l = lane % kLanes, sub = lane / kLanes;
-    float acc[ROWS][kCols * 4];
+// The kernels of a call are set up behind one another.  Those of the own positions run beside those of the shared ones: they need nothing of them, only what
+// these have waited for themselves before they let the next one start, and what comes after both waits for them.
+__device__ __forceinline__ void enter(const Attention& a) {
+    if (!a.beside) after_previous();
+    if (a.has_beside) next_may_start();              // (without need it costs: 128 x 5 rows over 48 positions 19 -> 23 us)
+}
+__device__ __forceinline__ void leave(const Attention& a) {
+    if (a.beside) after_previous();
+}
+
+// ---- keys --------------------------------------------------------------------------------------------------------
+
+// Quad c of position p of a stage lies where quad c ^ (p & 7) would: eight neighbouring positions' quads c are in different banks.
+__device__ __forceinline__ int swizzled(int p, int c) { return p * (kSlice * 4) + (c ^ (p & 7)) * 16; }
+
+// The copies of one warp, in order: 32 positions (every `step`-th such piece from `first` on), 32 floats of them at a time (every slice, or one alone).
+template <bool VEC>
+struct KeyCopies {
+    const float* from;                            // the lane's quad of the next copy
+    int64_t stride;
+    int left, step, slice, only, slices;          // `left`: positions from the next piece on
+    __device__ __forceinline__ KeyCopies(const Attention& a, const Segment& g, const Share& s, int first, int step_, int only_)
+        : stride(g.k_pos), left(s.count - first * 32), step(step_ * 32), slice(max(only_, 0)), only(only_), slices((a.dim + kSlice - 1) / kSlice) {
+        const int lane = threadIdx.x & 31;
+        from = g.k + s.group * g.k_group + s.row * g.k_row + s.kv_head * g.k_head + (s.begin + first * 32 + lane / kQuads) * stride + slice * kSlice +
+               lane % kQuads * 4;
+    }
+    __device__ __forceinline__ void issue(const Attention& a, Ring<kKeyBytes>& ring) {
+        constexpr int kAtOnce = 32 / kQuads;                                     // positions whose copies are one instruction
+        const int lane = threadIdx.x & 31, sub = lane / kQuads;
+        char* to = ring.next() + swizzled(sub, lane % kQuads);            // (every fourth position: the quad's place alternates)
+        if (left > 0) {
+            const int other = swizzled(sub + kAtOnce, lane % kQuads) - swizzled(sub, lane % kQuads);
+            const auto place = [&](int i) { return to + i / 2 * (2 * kAtOnce * kSlice * 4) + (i % 2 ? other : 0); };
+            const float* p = from;
+            const int64_t far = kAtOnce * stride;
+            if (VEC && left >= 32 && (slice + 1) * kSlice <= a.dim) {
 #pragma unroll
-    for (int n = 0; n < ROWS; ++n)
-#pragma unroll
-        for (int i = 0; i < kCols * 4; ++i) acc[n][i] = 0.0f;
-    const float* values = s.v + p.group * s.v_group + p.row * s.v_row + p.kv_head * s.v_head;
-    const int count = p.end - p.begin;
-    const auto column = [l](int i, int e) { return VEC ? (l + kLanes * i) * 4 + e : l + kLanes * (4 * i + e); };
-    for (int j0 = warp * 4 * kAcross; j0 < count; j0 += warps * 4 * kAcross) {
-        const int j = j0 + sub * 4;
-        float v[4][kCols * 4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const float* row = values + (int64_t)(p.begin + j + u) * s.v_pos;
-#pragma unroll
-            for (int i = 0; i < kCols; ++i) {
-                if (VEC) {
-                    float4 w = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-                    if (j + u < count && column(i, 0) < a.dim) w = __ldg(reinterpret_cast<const float4*>(row) + l + kLanes * i);
-                    v[u][4 * i] = w.x; v[u][4 * i + 1] = w.y; v[u][4 * i + 2] = w.z; v[u][4 * i + 3] = w.w;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[u][4 * i + e] = j + u < count && column(i, e) < a.dim ? __ldg(row + column(i, e)) : 1.0f;
-                }
+                for (int i = 0; i < kQuads; ++i, p += far) copy_quad<true>(place(i), p, 0, 4);
+            } else {
+                const int d = slice * kSlice + lane % kQuads * 4;
+                for (int i = 0; i < kQuads; ++i, p += far)
+                    if (i * kAtOnce + sub < left && d < a.dim) copy_quad<VEC>(place(i), p, d, a.dim);
+            }
+            from += kSlice;
+            if (only >= 0 || ++slice == slices) {
+                from += step * stride - (only >= 0 ? 1 : slices) * kSlice;
+                slice = max(only, 0);
+                left -= step;
             }
         }
+        __pipeline_commit();
+    }
+};
+
+// Sums of a stage's products: 32 floats of the lane's key against the same of each row's query.
+template <int ROWS, bool VEC>
+__device__ __forceinline__ void key_stage(const Attention& a, float2 (&sum)[ROWS], const char* stage, const int32_t* q, int pitch, int left, bool valid, bool plain) {
+    const int lane = threadIdx.x & 31;
+    const auto quad = [&](int c) { return *reinterpret_cast<const int4*>(stage + swizzled(lane, c)); };
+    if (left >= kSlice) {
+        int4 k[kQuads];
+        uint32_t far = 0u;
+#pragma unroll
+        for (int c = 0; c < kQuads; ++c) {
+            k[c] = quad(c);
+            far = max(far, beyond(k[c]));
+        }
+        if (__all_sync(0xffffffffu, plain && (far < kBand || !valid))) {
+#pragma unroll
+            for (int c = 0; c < kQuads; ++c)
+#pragma unroll
+                for (int n = 0; n < ROWS; ++n) {
+                    const int4 w = *reinterpret_cast<const int4*>(q + n * pitch + 4 * c);
+                    add_pair(sum[n], iadd(w.x, k[c].x), iadd(w.y, k[c].y));
+                    add_pair(sum[n], iadd(w.z, k[c].z), iadd(w.w, k[c].w));
+                }
+            return;
+        }
+    }
+    // a last stage of few floats, or a value for the range rule
+    const int quads = min(kQuads, (left + 3) / 4);
+#pragma unroll 1
+    for (int c = 0; c < quads; ++c) {
+        const int4 x = quad(c);
+        const int width = VEC ? 4 : min(4, left - 4 * c);
+        const bool easy = __all_sync(0xffffffffu, plain && width == 4 && (beyond(x) < kBand || !valid));
+#pragma unroll
+        for (int n = 0; n < ROWS; ++n) {
+            const int4 w = *reinterpret_cast<const int4*>(q + n * pitch + 4 * c);
+            if (easy) {
+                add_pair(sum[n], iadd(w.x, x.x), iadd(w.y, x.y));
+                add_pair(sum[n], iadd(w.z, x.z), iadd(w.w, x.w));
+            } else {
+                const int32_t bias = kBias - a.off;
+                sum[n].x = fadd(sum[n].x, mul(i2f(iadd(w.x, bias)), i2f(x.x), a.off));
+                if (width > 1) sum[n].y = fadd(sum[n].y, mul(i2f(iadd(w.y, bias)), i2f(x.y), a.off));
+                if (width > 2) sum[n].x = fadd(sum[n].x, mul(i2f(iadd(w.z, bias)), i2f(x.z), a.off));
+                if (width > 3) sum[n].y = fadd(sum[n].y, mul(i2f(iadd(w.w, bias)), i2f(x.w), a.off));
+            }
+        }
+    }
+}
+
+template <int ROWS, bool VEC>
+__global__ void __launch_bounds__(32 * kMostWarps, 2) key_kernel(const Attention a, const Segment g) {
+    extern __shared__ __align__(16) char memory[];
+    __shared__ float2 red[kMostWarps * ROWS];
+    __shared__ float dealt[kMostWarps * ROWS * 32];                              // (split: sums of each warp's slice)
+    __shared__ int odd_query;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, warps = blockDim.x >> 5, pitch = (a.dim + 31) / 32 * 32, slices = pitch / kSlice;
+    Ring<kKeyBytes> ring(memory, warp);
+    int32_t* q = reinterpret_cast<int32_t*>(memory + warps * 2 * kKeyBytes);
+    enter(a);
+    const Share s = share_of(a, g);
+    // the queries come as they are, and become patterns where each thread finds what it copied itself
+    const auto each_of_query = [&](auto&& one) {
+        for (int n = warp; n < ROWS; n += warps)
+            for (int d = lane; d < pitch; d += 32) one(n, d);
+    };
+    each_of_query([&](int n, int d) {
+        const int r = s.row * a.share + s.first + n;
+        if (n < s.rows && d < a.dim)
+            __pipeline_memcpy_async(q + n * pitch + d, a.q + s.group * a.q_group + (r / a.share) * a.q_row + (s.kv_head * a.share + r % a.share) * a.q_head + d, 4);
+    });
+    __pipeline_commit();
+    const int step = a.split ? warps / slices : warps, first = a.split ? warp / slices : warp;
+    KeyCopies<VEC> copies(a, g, s, first, step, a.split ? warp % slices : -1);
+    copies.issue(a, ring);
+    if (t == 0) odd_query = 0;
+    __syncthreads();
+    __pipeline_wait_prior(1);
+    bool plain = true;
+    each_of_query([&](int n, int d) {
+        int32_t* x = q + n * pitch + d;
+        const bool there = n < s.rows && d < a.dim;
+        plain = plain && (!there || beyond(*x) < kBand);
+        *x = there ? isub(*x, kBias - a.off) : 0;
+    });
+    if (!plain) odd_query = 1;
+    __syncthreads();
+    plain = odd_query == 0;
+
+    Running stats[ROWS];
+    float* to = a.scores + s.base * a.width + g.first_pos + s.begin + lane;
+    const auto keep = [&](int n, float x, int at) {
+        const float y = x == -INFINITY ? -INFINITY : mul(x, kLog2e, a.off);
+        to[(int64_t)n * a.width + at] = y;
+        stats[n].add(y);
+    };
+    // (split: as many pieces as warps take one; the loop runs once, for all warps)
+    for (int piece = first; piece * 32 < s.count || (a.split && piece == first); piece += step) {
+        const bool valid = piece * 32 + lane < s.count;
+        float2 sum[ROWS];
+#pragma unroll
+        for (int n = 0; n < ROWS; ++n) sum[n] = make_float2(0.0f, 0.0f);
+        for (int d = a.split ? warp % slices * kSlice : 0; d < a.dim; d += kSlice) {
+            __pipeline_wait_prior(0);
+            __syncwarp();
+            copies.issue(a, ring);
+            key_stage<ROWS, VEC>(a, sum, ring.to, q + d, pitch, a.dim - d, valid, plain);
+            if (a.split) break;
+        }
+        if (a.split) {
+#pragma unroll
+            for (int n = 0; n < ROWS; ++n) dealt[(warp * ROWS + n) * 32 + lane] = fadd(sum[n].x, sum[n].y);
+            __syncthreads();
+            if (warp % slices != 0) break;
+#pragma unroll
+            for (int n = 0; n < ROWS; ++n) {
+                float x = dealt[(warp * ROWS + n) * 32 + lane];
+                for (int w = 1; w < slices; ++w) x = fadd(x, dealt[((warp + w) * ROWS + n) * 32 + lane]);
+                if (valid && n < s.rows) keep(n, x, piece * 32);
+            }
+        } else if (valid) {
+#pragma unroll
+            for (int n = 0; n < ROWS; ++n)
+                if (n < s.rows) keep(n, fadd(sum[n].x, sum[n].y), piece * 32);
+        }
+    }
+    __pipeline_wait_prior(0);
+#pragma unroll
+    for (int n = 0; n < ROWS; ++n) {
+        const float top = warp_max(stats[n].top);
+        const float sum = warp_sum(rescaled(make_float2(stats[n].top, stats[n].sum), top));
+        if (lane == 0) red[warp * ROWS + n] = make_float2(top, sum);
+    }
+    __syncthreads();
+    if (t < s.rows) a.stats[(s.base + t) * a.parts + g.first_part + s.rank] = joined([&](int w) { return red[w * ROWS + t]; }, warps);
+    leave(a);
+}
+
+// ---- values ------------------------------------------------------------------------------------------------------
+
+// A stage: 4 KB, as eight quads of each lane, and t of its positions.  `kLanes` lanes cover a position's columns (kCols quads each), four neighbouring
+// positions at a time.
+template <int SLOTS, int ROWS>
+struct ValueShape {
+    static constexpr int kLanes = SLOTS >= 4 ? 32 : 8 * SLOTS, kCols = SLOTS == 8 ? 2 : 1, kAcross = 32 / kLanes, kTimes = 2 / kCols;
+    static constexpr int kPositions = 4 * kAcross * kTimes, kScores = 4096;      // (kScores: where t lies in a stage)
+    static constexpr int kBytes = kScores + ROWS * kPositions * 4;
+};
+
+// The copies of one warp, in order: every `step`-th piece of kPositions.  Each lane copies what it will read itself, and some of t.
+template <int SLOTS, int ROWS, bool VEC>
+struct ValueCopies {
+    using S = ValueShape<SLOTS, ROWS>;
+    const float *from, *t;                        // the lane's first quad of values, and of t, in the next piece
+    int64_t stride;
+    int left, step, rows;
+    __device__ __forceinline__ ValueCopies(const Attention& a, const Segment& g, const Share& s, int first, int step_)
+        : stride(g.v_pos), left(s.count - first * S::kPositions), step(step_ * S::kPositions), rows(s.rows) {
+        const int lane = threadIdx.x & 31, l = lane % S::kLanes, sub = lane / S::kLanes;
+        const int at = s.begin + first * S::kPositions;
+        from = g.v + s.group * g.v_group + s.row * g.v_row + s.kv_head * g.v_head + (at + sub * 4) * stride + l * 4;
+        t = a.scores + (s.base + lane / (S::kPositions / 4)) * a.width + g.first_pos + at + lane % (S::kPositions / 4) * 4;
+    }
+    __device__ __forceinline__ void issue(const Attention& a, Ring<S::kBytes>& ring) {
+        const int lane = threadIdx.x & 31, l = lane % S::kLanes, sub = lane / S::kLanes;
+        char* stage = ring.next();
+        if (left > 0) {
+            char* to = stage + lane * 16;
+            const bool whole = VEC && left >= S::kPositions && a.dim == 4 * S::kLanes * S::kCols;
+            const float* p = from;
+#pragma unroll
+            for (int m = 0; m < S::kTimes; ++m) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u, p += stride)
+#pragma unroll
+                    for (int c = 0; c < S::kCols; ++c) {
+                        const int d = (l + S::kLanes * c) * 4;
+                        if (whole || (m * 4 * S::kAcross + sub * 4 + u < left && d < a.dim))
+                            copy_quad<VEC>(to + ((m * 4 + u) * S::kCols + c) * 512, p + S::kLanes * 4 * c, d, a.dim);
+                    }
+                p += (4 * S::kAcross - 4) * stride;
+            }
+            constexpr int kRowQuads = S::kPositions / 4, kRowsAtOnce = 32 / kRowQuads;
+            const float* x = t;
+#pragma unroll
+            for (int n = 0; n < ROWS; n += kRowsAtOnce, x += (int64_t)kRowsAtOnce * a.width)
+                if (n + lane / kRowQuads < rows) __pipeline_memcpy_async(stage + S::kScores + n * S::kPositions * 4 + lane * 16, x, 16);
+            from += step * stride;
+            t += step;
+            left -= step;
+        }
+        __pipeline_commit();
+    }
+};
+
+// What a row divides by and is shifted by.
+struct __align__(16) RowStat {
+    float flush_max, pass_max;
+    int32_t sub;
+    float shift;
+};
+
+template <int SLOTS, int ROWS, bool VEC>
+__device__ __forceinline__ void value_stage(const Attention& a, int count, int rows, float2 (&acc)[ROWS][2 * ValueShape<SLOTS, ROWS>::kCols], char* slot,
+                                            const RowStat* stats) {
+    using S = ValueShape<SLOTS, ROWS>;
+    const int lane = threadIdx.x & 31, l = lane % S::kLanes, sub = lane / S::kLanes;
+    // t becomes p, as patterns for the products
+    const int32_t bias = kBias - a.off;
+    int32_t* probs = reinterpret_cast<int32_t*>(slot + S::kScores);
+    bool odd = count < S::kPositions;                                           // (a part of a stage, or a probability for the range rule)
+#pragma unroll
+    for (int i = 0; i < (ROWS * S::kPositions + 31) / 32; ++i) {
+        const int at = i * 32 + lane, n = at / S::kPositions;
+        if (n < rows) {
+            const RowStat r = stats[n];
+            const float e = exponential(i2f(probs[at]), r.shift);
+            const float p = e <= r.flush_max ? 0.0f : e <= r.pass_max ? i2f(isub(f2i(e), r.sub)) : quiet_nan();
+            probs[at] = isub(f2i(p), bias);
+            odd = odd || beyond(f2i(p)) >= kBand;
+        }
+    }
+    const bool plain = !__any_sync(0xffffffffu, odd);
+    __syncwarp();
+    probs += sub * 4;
+    slot += lane * 16;
+#pragma unroll
+    for (int m = 0; m < S::kTimes; ++m) {
+        int4 v[4][S::kCols];
         uint32_t far = 0u;
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
-            for (int i = 0; i < kCols * 4; ++i) far = max(far, beyond(v[u][i]));
-        const bool plain = far < kBand && *reinterpret_cast<const uint32_t*>(odd + j) == 0u;
-        if (__all_sync(0xffffffffu, plain)) {
-#pragma unroll
-            for (int n = 0; n < ROWS; ++n) {
-                const float4 w = *reinterpret_cast<const float4*>(probs + n * stride + j);
-                const float pr[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int32_t b = isub(f2i(pr[u]), kBias - a.off);
-#pragma unroll
-                    for (int i = 0; i < kCols * 4; ++i) acc[n][i] = fadd(acc[n][i], i2f(iadd(b, f2i(v[u][i]))));
+            for (int c = 0; c < S::kCols; ++c) {
+                int4& x = v[u][c];
+                x = *reinterpret_cast<const int4*>(slot + ((m * 4 + u) * S::kCols + c) * 512);
+                const int d = (l + S::kLanes * c) * 4;
+                if (!VEC) {                                                     // (columns past the last hold nothing)
+                    if (d >= a.dim) x.x = kBias;
+                    if (d + 1 >= a.dim) x.y = kBias;
+                    if (d + 2 >= a.dim) x.z = kBias;
+                    if (d + 3 >= a.dim) x.w = kBias;
                 }
+                far = max(far, !VEC || d < a.dim ? beyond(x) : 0u);
             }
-        } else {
+        if (__all_sync(0xffffffffu, plain && far < kBand)) {
 #pragma unroll
-            for (int n = 0; n < ROWS; ++n) {
-                const float4 w = *reinterpret_cast<const float4*>(probs + n * stride + j);
-                const float pr[4] = {w.x, w.y, w.z, w.w};
+            for (int n = 0; n < ROWS; n += 2) {
+                int4 w[2];
+#pragma unroll
+                for (int i = n; i < n + 2 && i < ROWS; ++i) w[i - n] = *reinterpret_cast<const int4*>(probs + i * S::kPositions + m * 4 * S::kAcross);
+                // (two rows at a time: four chains of adds)
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
 #pragma unroll
-                    for (int i = 0; i < kCols * 4; ++i) acc[n][i] = fadd(acc[n][i], mul(pr[u], v[u][i], a.off));
+                    for (int i = n; i < n + 2 && i < ROWS; ++i) {
+                        const int32_t b = u == 0 ? w[i - n].x : u == 1 ? w[i - n].y : u == 2 ? w[i - n].z : w[i - n].w;
+#pragma unroll
+                        for (int c = 0; c < S::kCols; ++c) {
+                            add_pair(acc[i][2 * c], iadd(b, v[u][c].x), iadd(b, v[u][c].y));
+                            add_pair(acc[i][2 * c + 1], iadd(b, v[u][c].z), iadd(b, v[u][c].w));
+                        }
+                    }
+            }
+            continue;
+        }
+#pragma unroll 1
+        for (int u = 0; u < 4; ++u) {
+            if (m * 4 * S::kAcross + sub * 4 + u >= count) break;
+#pragma unroll
+            for (int c = 0; c < S::kCols; ++c) {
+                const int4 x = *reinterpret_cast<const int4*>(slot + ((m * 4 + u) * S::kCols + c) * 512);
+#pragma unroll
+                for (int n = 0; n < ROWS; ++n) {
+                    const float p = i2f(iadd(probs[n * S::kPositions + m * 4 * S::kAcross + u], bias));
+                    acc[n][2 * c].x = fadd(acc[n][2 * c].x, mul(p, i2f(x.x), a.off));
+                    acc[n][2 * c].y = fadd(acc[n][2 * c].y, mul(p, i2f(x.y), a.off));
+                    acc[n][2 * c + 1].x = fadd(acc[n][2 * c + 1].x, mul(p, i2f(x.z), a.off));
+                    acc[n][2 * c + 1].y = fadd(acc[n][2 * c + 1].y, mul(p, i2f(x.w), a.off));
+                }
             }
         }
     }
+}
+
+__host__ __device__ constexpr int padded(int dim) { return (dim + 3) / 4 * 4; }
+
+template <int SLOTS, int ROWS, bool VEC>
+__global__ void __launch_bounds__(32 * kMostWarps, 2) value_kernel(const Attention a, const Segment g) {
+    extern __shared__ __align__(16) char memory[];
+    __shared__ RowStat stats[ROWS];
+    using V = ValueShape<SLOTS, ROWS>;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, warps = blockDim.x >> 5;
+    Ring<V::kBytes> ring(memory, warp);
+    enter(a);
+    const Share s = share_of(a, g);
+    ValueCopies<SLOTS, ROWS, VEC> copies(a, g, s, warp, warps);
+    copies.issue(a, ring);
+    // a row's shift and sum, from those of its parts
+    for (int n = warp; n < s.rows; n += warps) {
+        const float2* from = a.stats + (s.base + n) * a.parts;
+        const float2 mine = joined([&](int i) { return i * 32 + lane < a.parts ? __ldcg(from + i * 32 + lane) : make_float2(-INFINITY, 0.0f); },
+                                   (a.parts + 31) / 32);
+        const float top = warp_max(mine.x), sum = warp_sum(rescaled(mine, top));
+        const Divisor d = make_divisor(sum, a.off);
+        if (lane == 0) stats[n] = {d.flush_max, d.pass_max, d.sub, top};
+    }
+    __syncthreads();
+
+    float2 acc[ROWS][2 * V::kCols];
 #pragma unroll
     for (int n = 0; n < ROWS; ++n)
 #pragma unroll
-        for (int i = 0; i < kCols * 4; ++i)
+        for (int c = 0; c < 2 * V::kCols; ++c) acc[n][c] = make_float2(0.0f, 0.0f);
+    for (int left = s.count - warp * V::kPositions; left > 0; left -= warps * V::kPositions) {
+        __pipeline_wait_prior(0);
+        __syncwarp();
+        copies.issue(a, ring);
+        value_stage<SLOTS, ROWS, VEC>(a, left, s.rows, acc, ring.to, stats);
+    }
+    __pipeline_wait_prior(0);
+    __syncthreads();                                                             // (the rings become the warps' sums)
+    const int columns = padded(a.dim);
+    float* sums = reinterpret_cast<float*>(memory);                              // [warp][row][column]
+    {
+        const int l = lane % V::kLanes;
 #pragma unroll
-            for (int d = kLanes; d < 32; d <<= 1) acc[n][i] = fadd(acc[n][i], __shfl_xor_sync(0xffffffffu, acc[n][i], d));
-    // one warp after another adds its sums
-    for (int w = 0; w < warps; ++w) {
-        __syncthreads();
-        if (warp == w && sub == 0) {
+        for (int n = 0; n < ROWS; ++n)
 #pragma unroll
-            for (int n = 0; n < ROWS; ++n)
+            for (int c = 0; c < V::kCols; ++c) {
+                float4 x = make_float4(acc[n][2 * c].x, acc[n][2 * c].y, acc[n][2 * c + 1].x, acc[n][2 * c + 1].y);
 #pragma unroll
-                for (int i = 0; i < kCols * 4; ++i) {
-                    float* to = sums + n * 256 + column(i / 4, i % 4);
-                    *to = w == 0 ? acc[n][i] : fadd(*to, acc[n][i]);
+                for (int d = V::kLanes; d < 32; d <<= 1) {
+                    x.x = fadd(x.x, __shfl_xor_sync(0xffffffffu, x.x, d));
+                    x.y = fadd(x.y, __shfl_xor_sync(0xffffffffu, x.y, d));
+                    x.z = fadd(x.z, __shfl_xor_sync(0xffffffffu, x.z, d));
+                    x.w = fadd(x.w, __shfl_xor_sync(0xffffffffu, x.w, d));
                 }
-        }
-    }
-    __syncthreads();
-}
-
-__device__ __forceinline__ float* out_row(const Attention& a, const Segment& s, const Place& p, int r) {
-    const int row = s.per_row ? p.row : r / a.share, head = p.kv_head * a.share + (s.per_row ? r : r % a.share);
-    return a.out + ((p.group * a.rows + row) * ((int64_t)a.kv_heads * a.share) + head) * a.dim;
-}
-
-template <int SLOTS, int ROWS, bool VEC>
-__global__ void __launch_bounds__(256) weigh_kernel(const Attention a, const Segment s) {
-    __shared__ __align__(16) float probs[ROWS * kMostChunk];
-    __shared__ __align__(16) float sums[ROWS * 256];
-    __shared__ __align__(16) unsigned char odd[kMostChunk];
-    __shared__ float2 stats[ROWS];
-    const Place p = place_of(a, s, ROWS);
-    const int rows = rows_of(s, p, ROWS), lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-    const int count = p.end - p.begin;
-    after_previous();
-    for (int n = threadIdx.x >> 5; n < rows; n += warps) {
-        const float2 t = row_stats(a.stats + (p.base + n) * a.chunks, a.chunks, lane);
-        if (lane == 0) stats[n] = t;
-    }
-    __syncthreads();
-    // probabilities; positions past the end get 0, and count as beyond the band
-    for (int j = threadIdx.x; j < (count + 3) / 4 * 4 + 16 && j < kMostChunk; j += blockDim.x) {
-        bool far = j >= count;
-#pragma unroll
-        for (int n = 0; n < ROWS; ++n) {
-            float pr = 0.0f;
-            if (j < count && n < rows) {
-                const float2 t = stats[n];
-                const float e = exponential(__ldcg(a.scores + (p.base + n) * a.width + s.first_pos + p.begin + j), t.x);
-                pr = div(e, t.y, a.off);
+                const int d = (l + V::kLanes * c) * 4;
+                if (lane < V::kLanes && d < a.dim && n < s.rows) *reinterpret_cast<float4*>(sums + (warp * ROWS + n) * columns + d) = x;
             }
-            far = far || (n < rows && beyond(pr) >= kBand);
-            probs[n * kMostChunk + j] = pr;
-        }
-        odd[j] = far;
     }
     __syncthreads();
-    weigh_range<SLOTS, ROWS, VEC>(a, s, p, rows, probs, kMostChunk, odd, sums);
-    for (int i = threadIdx.x; i < rows * a.dim; i += blockDim.x) {
-        const int n = i / a.dim, d = i - n * a.dim;
-        const float x = sums[n * 256 + d];
-        if (a.chunks == 1) out_row(a, s, p, p.tile * ROWS + n)[d] = x;
-        else a.parts[((p.base + n) * a.chunks + s.first_chunk + p.chunk) * a.dim + d] = x;
+    for (int n = warp; n < s.rows; n += warps) {
+        const int r = s.row * a.share + s.first + n;
+        float* to = a.sums ? a.sums + ((s.base + n) * a.parts + g.first_part + s.rank) * a.dim
+                           : a.out + ((s.group * a.rows + r / a.share) * ((int64_t)a.kv_heads * a.share) + s.kv_head * a.share + r % a.share) * a.dim;
+        for (int d = lane; d < a.dim; d += 32) {
+            float x = sums[n * columns + d];
+            for (int w = 1; w < warps; ++w) x = fadd(x, sums[(w * ROWS + n) * columns + d]);
+            to[d] = x;
+        }
     }
+    leave(a);
 }
 
-// Adds the sums of a row's chunks.
-__global__ void __launch_bounds__(256) join_kernel(const Attention a) {
-    const int64_t row = blockIdx.x;                                              // (group, key head, row and head of the group)
-    const int per = a.rows * a.share;
-    const int n = (int)(row % per), kv_head = (int)(row / per % a.kv_heads);
-    const int64_t group = row / per / a.kv_heads;
-    float* to = a.out + ((group * a.rows + n / a.share) * ((int64_t)a.kv_heads * a.share) + kv_head * a.share + n % a.share) * a.dim;
+// Adds the parts of a row.
+__global__ void __launch_bounds__(128) join_kernel(const Attention a) {
+    const int64_t row = blockIdx.x;                                              // (group, key head, row, head of the key head)
+    const int per = a.rows * a.share, n = (int)(row % per), kv_head = (int)(row / per % a.kv_heads);
+    float* to = a.out + ((row / per / a.kv_heads * a.rows + n / a.share) * ((int64_t)a.kv_heads * a.share) + kv_head * a.share + n % a.share) * a.dim;
     after_previous();
     for (int d = threadIdx.x; d < a.dim; d += blockDim.x) {
         float sum = 0.0f;
-        for (int c = 0; c < a.chunks; ++c) sum = fadd(sum, __ldcg(a.parts + (row * a.chunks + c) * a.dim + d));
+#pragma unroll 16
+        for (int r = 0; r < a.parts; ++r) sum = fadd(sum, __ldcg(a.sums + (row * a.parts + r) * a.dim + d));
         to[d] = sum;
-    }
-}
-
-template <int SLOTS, bool VEC>
-int most_rows() { return SLOTS == 8 ? 4 : kMaxRows; }
-
-template <int SLOTS, int ROWS, bool VEC>
-int launch_pass(int pass, bool behind, const Attention& a, const Segment& s, int64_t ctas, unsigned threads, cudaStream_t st) {
-    auto* kernel = pass == 0 ? score_kernel<SLOTS, ROWS, VEC> : weigh_kernel<SLOTS, ROWS, VEC>;
-    if (behind) return launch_behind(kernel, dim3((unsigned)ctas), threads, st, a, s);
-    kernel<<<(unsigned)ctas, threads, 0, st>>>(a, s);
-    return check_launch();
-}
-
-template <int SLOTS, bool VEC>
-int launch_rows(int rows, int pass, bool behind, const Attention& a, const Segment& s, int64_t ctas, unsigned threads, cudaStream_t st) {
-    switch (rows) {
-        case 1: return launch_pass<SLOTS, 1, VEC>(pass, behind, a, s, ctas, threads, st);
-        case 2: return launch_pass<SLOTS, 2, VEC>(pass, behind, a, s, ctas, threads, st);
-        case 4: return launch_pass<SLOTS, 4, VEC>(pass, behind, a, s, ctas, threads, st);
-        default: return launch_pass<SLOTS, SLOTS == 8 ? 4 : 8, VEC>(pass, behind, a, s, ctas, threads, st);
-    }
-}
-
-int launch_slots(bool vec, int slots, int rows, int pass, bool behind, const Attention& a, const Segment& s, int64_t ctas, unsigned threads,
-                 cudaStream_t st) {
-    if (vec) {
-        switch (slots) {
-            case 1: return launch_rows<1, true>(rows, pass, behind, a, s, ctas, threads, st);
-            case 2: return launch_rows<2, true>(rows, pass, behind, a, s, ctas, threads, st);
-            case 4: return launch_rows<4, true>(rows, pass, behind, a, s, ctas, threads, st);
-            default: return launch_rows<8, true>(rows, pass, behind, a, s, ctas, threads, st);
-        }
-    }
-    switch (slots) {
-        case 1: return launch_rows<1, false>(rows, pass, behind, a, s, ctas, threads, st);
-        case 2: return launch_rows<2, false>(rows, pass, behind, a, s, ctas, threads, st);
-        case 4: return launch_rows<4, false>(rows, pass, behind, a, s, ctas, threads, st);
-        default: return launch_rows<8, false>(rows, pass, behind, a, s, ctas, threads, st);
     }
 }
 
 // ---- planning ------------------------------------------------------------------------------------------------
 
-struct Plan {
-    int slots, tile_rows[2], tiles[2], chunk[2], chunks[2];      // [shared, own]
-    int width, all_chunks;
-    int64_t rows;                                                // of scores
+struct Part {                                     // of the shared positions, or of the own ones
+    int rows, tiles, tile_rows, ranks;            // `rows`: the kernels', at least tile_rows
+    int key_warps, value_warps;
+    bool split;
+    int64_t ctas;
 };
 
-int round_rows(int rows, int most) {
-    const int tiles = (rows + most - 1) / most, each = (rows + tiles - 1) / tiles;
-    return each <= 2 ? each : each <= 4 ? 4 : 8;
+struct Plan {
+    int slots, width, own_first, parts;
+    Part part[2];
+    int64_t all_rows;
+};
+
+int rounded_rows(int n, bool vec) {
+    if (!vec) return n <= 1 ? 1 : n <= 4 ? 4 : 8;
+    return n <= 6 ? n : 8;
 }
 
-// A range of positions per CTA: the longest of 512 .. 64 that gives every SM two of them, if any does.
-Plan plan_of(int64_t groups, int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, int64_t shared, int64_t own) {
+constexpr int kPlaces = 4 * 148;                  // CTAs of four warps that the SMs hold at once
+
+Part part_of(int64_t units, int together, int64_t positions, int slots, int64_t dim, bool vec) {
+    Part p{};
+    if (positions == 0) return p;
+    p.tiles = (together + kMostRows - 1) / kMostRows;
+    p.tile_rows = (together + p.tiles - 1) / p.tiles;
+    p.tiles = (together + p.tile_rows - 1) / p.tile_rows;
+    p.rows = rounded_rows(p.tile_rows, vec);
+    const int64_t all = units * p.tiles, blocks = (positions + 31) / 32;
+    // CTAs of a row: what fills the places once, or whole times with nine tenths of them taken, with 8 blocks of 32 positions each at least
+    int64_t ranks = std::max<int64_t>(1, kPlaces / all);
+    for (int64_t times = 2; times <= 4 && ranks * all * 10 < (times - 1) * kPlaces * 9; ++times) ranks = std::max<int64_t>(1, times * kPlaces / all);
+    p.ranks = (int)std::min(ranks, std::max<int64_t>(1, blocks / 8));
+    p.ctas = all * p.ranks;
+    const int64_t each = (blocks + p.ranks - 1) / p.ranks;
+    const int slices = (int)((dim + kSlice - 1) / kSlice), at_once = slots == 1 ? 32 : slots == 2 ? 16 : slots == 4 ? 8 : 4;
+    // few positions of few rows: the slices of a key are dealt out to warps as well, one warp alone would be the time of the call
+    p.split = slices > 1 && each * slices <= kMostWarps && p.ctas <= 2 * 148;
+    p.key_warps = p.split ? (int)(each * slices) : (int)std::min<int64_t>(each, kWarps);
+    p.value_warps = (int)std::min<int64_t>((std::min<int64_t>(positions, each * 32) + at_once - 1) / at_once, p.split ? kMostWarps : kWarps);
+    return p;
+}
+
+Plan plan_of(int64_t groups, int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, int64_t shared, int64_t own, bool vec) {
     Plan p;
     p.slots = dim <= 32 ? 1 : dim <= 64 ? 2 : dim <= 128 ? 4 : 8;
-    const int most = p.slots == 8 ? 4 : kMaxRows, share = (int)(heads / kv_heads);
-    const int64_t together[2] = {rows * share, share}, units[2] = {groups * kv_heads, groups * rows * kv_heads}, slots[2] = {shared, own};
-    for (int i = 0; i < 2; ++i) {
-        p.tile_rows[i] = round_rows((int)together[i], most);
-        p.tiles[i] = (int)((together[i] + p.tile_rows[i] - 1) / p.tile_rows[i]);
-        int chunk = kMostChunk;
-        while (chunk > 64 && units[i] * p.tiles[i] * ((slots[i] + chunk - 1) / chunk) < 2 * 148) chunk /= 2;
-        p.chunk[i] = chunk;
-        p.chunks[i] = (int)((slots[i] + chunk - 1) / chunk);
-    }
-    p.width = (int)(shared + own);
-    p.all_chunks = p.chunks[0] + p.chunks[1];
-    p.rows = groups * rows * heads;
+    const int share = (int)(heads / kv_heads);
+    p.part[0] = part_of(groups * kv_heads, (int)(rows * share), shared, p.slots, dim, vec);
+    p.part[1] = part_of(groups * kv_heads * rows, share, own, p.slots, dim, vec);
+    p.own_first = (int)((shared + 31) / 32 * 32);
+    p.width = p.own_first + (int)((own + 31) / 32 * 32);
+    p.parts = p.part[0].ranks + p.part[1].ranks;
+    p.all_rows = groups * rows * heads;
     return p;
 }
 
 size_t aligned(size_t n) { return (n + 255) / 256 * 256; }
+size_t score_bytes(const Plan& p) { return aligned((size_t)p.all_rows * p.width * 4); }
+size_t stat_bytes(const Plan& p) { return aligned((size_t)p.all_rows * p.parts * 8); }
+size_t bytes_of(const Plan& p, int64_t dim) { return score_bytes(p) + stat_bytes(p) + (p.parts > 1 ? aligned((size_t)(p.all_rows * p.parts * dim) * 4) : 0); }
 
-bool sizes_ok(int64_t groups, int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, int64_t shared, int64_t own) {
+template <class K>
+int launch(K* kernel, int64_t ctas, int warps, size_t memory, const Attention& a, const Segment& g, cudaStream_t st) {
+    if (memory > 32 * 1024) {                                                    // (48 KB with what the kernels declare)
+        const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)memory);
+        if (err != cudaSuccess) return record_cuda_error(err);
+    }
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;                // (set up behind the kernel before)
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3((unsigned)ctas);
+    config.blockDim = dim3(warps * 32);
+    config.dynamicSmemBytes = memory;
+    config.stream = st;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    const cudaError_t err = cudaLaunchKernelEx(&config, kernel, a, g);
+    count_launch();
+    return err == cudaSuccess ? PAMK_OK : record_cuda_error(err);
+}
+
+template <int ROWS, bool VEC>
+int launch_keys(const Part& p, const Attention& a, const Segment& g, cudaStream_t st) {
+    return launch(key_kernel<ROWS, VEC>, p.ctas, p.key_warps, (size_t)p.key_warps * 2 * kKeyBytes + (size_t)ROWS * ((a.dim + 31) / 32 * 32) * 4, a, g, st);
+}
+
+template <int SLOTS, int ROWS, bool VEC>
+int launch_slots(const Part& p, const Attention& a, const Segment& g, cudaStream_t st) {
+    const size_t ring = (size_t)p.value_warps * 2 * ValueShape<SLOTS, ROWS>::kBytes;
+    return launch(value_kernel<SLOTS, ROWS, VEC>, p.ctas, p.value_warps, std::max(ring, (size_t)p.value_warps * ROWS * padded(a.dim) * 4), a, g, st);
+}
+
+template <int ROWS, bool VEC>
+int launch_pass(bool values, int slots, const Part& p, const Attention& a, const Segment& g, cudaStream_t st) {
+    if (!values) return launch_keys<ROWS, VEC>(p, a, g, st);
+    switch (slots) {
+        case 1: return launch_slots<1, ROWS, VEC>(p, a, g, st);
+        case 2: return launch_slots<2, ROWS, VEC>(p, a, g, st);
+        case 4: return launch_slots<4, ROWS, VEC>(p, a, g, st);
+        default: return launch_slots<8, ROWS, VEC>(p, a, g, st);
+    }
+}
+
+int launch_part(bool values, bool vec, int slots, const Part& p, const Attention& a, const Segment& g, cudaStream_t st) {
+    if (!vec) {
+        switch (p.rows) {
+            case 1: return launch_pass<1, false>(values, slots, p, a, g, st);
+            case 4: return launch_pass<4, false>(values, slots, p, a, g, st);
+            default: return launch_pass<8, false>(values, slots, p, a, g, st);
+        }
+    }
+    switch (p.rows) {
+        case 1: return launch_pass<1, true>(values, slots, p, a, g, st);
+        case 2: return launch_pass<2, true>(values, slots, p, a, g, st);
+        case 3: return launch_pass<3, true>(values, slots, p, a, g, st);
+        case 4: return launch_pass<4, true>(values, slots, p, a, g, st);
+        case 5: return launch_pass<5, true>(values, slots, p, a, g, st);
+        case 6: return launch_pass<6, true>(values, slots, p, a, g, st);
+        default: return launch_pass<8, true>(values, slots, p, a, g, st);
+    }
+}
+
+bool sizes_ok(int64_t groups, int64_t rows, int64_t heads, int64_t dim, int64_t shared, int64_t own) {
     if (dim > 256 || rows * heads > (1 << 20) || shared > (1 << 30) || own > (1 << 30) || groups > INT32_MAX) return false;
     // (CTAs of the largest grid)
     return groups * rows * heads <= INT32_MAX / (2 + (shared + own) / 64);
@@ -481,10 +733,9 @@ extern "C" {
 size_t pamk_cached_attention_workspace_bytes(int64_t groups, int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim,
                                              int64_t shared, int64_t own) {
     using namespace pamk;
-    if (groups <= 0 || rows <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || dim <= 0 || shared < 0 || own < 0) return 0;
-    if (!sizes_ok(groups, rows, heads, kv_heads, dim, shared, own)) return 0;
-    const Plan p = plan_of(groups, rows, heads, kv_heads, dim, shared, own);
-    return aligned(p.rows * p.width * 4) + aligned(p.rows * p.all_chunks * 8) + (p.all_chunks > 1 ? aligned(p.rows * p.all_chunks * dim * 4) : 0);
+    if (groups <= 0 || rows <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || dim <= 0 || shared < 0 || own < 0 || shared + own == 0) return 0;
+    if (!sizes_ok(groups, rows, heads, dim, shared, own)) return 0;
+    return bytes_of(plan_of(groups, rows, heads, kv_heads, dim, shared, own, true), dim);       // (the same whichever way rows are loaded)
 }
 
 int pamk_cached_attention(const float* q, float* out, const float* shared_k, const float* shared_v, const int64_t* shared_lengths,
@@ -495,62 +746,53 @@ int pamk_cached_attention(const float* q, float* out, const float* shared_k, con
     if (groups < 0 || rows < 0 || heads < 0 || kv_heads < 1 || dim < 0 || shared < 0 || own < 0 || heads % kv_heads || !strides) return PAMK_ERR_ARG;
     if (groups == 0 || rows == 0 || heads == 0 || dim == 0) return PAMK_OK;
     if (!q || !out || (shared && (!shared_k || !shared_v)) || (own && (!own_k || !own_v))) return PAMK_ERR_ARG;
-    if (!sizes_ok(groups, rows, heads, kv_heads, dim, shared, own)) return PAMK_ERR_SIZE;
+    if (!sizes_ok(groups, rows, heads, dim, shared, own)) return PAMK_ERR_SIZE;
     cudaStream_t st = (cudaStream_t)stream;
     if (shared + own == 0) {
         const cudaError_t err = cudaMemsetAsync(out, 0, (size_t)(groups * rows * heads * dim) * 4, st);
         return err == cudaSuccess ? PAMK_OK : record_cuda_error(err);
     }
-    const Plan p = plan_of(groups, rows, heads, kv_heads, dim, shared, own);
-    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) ||
-        workspace_bytes < pamk_cached_attention_workspace_bytes(groups, rows, heads, kv_heads, dim, shared, own))
-        return PAMK_ERR_WORKSPACE;
     Attention a{};
     a.q = q; a.out = out;
     a.q_group = strides[0]; a.q_row = strides[1]; a.q_head = strides[2];
-    a.groups = (int)groups; a.rows = (int)rows; a.kv_heads = (int)kv_heads; a.share = (int)(heads / kv_heads); a.dim = (int)dim;
+    a.rows = (int)rows; a.kv_heads = (int)kv_heads; a.share = (int)(heads / kv_heads); a.dim = (int)dim;
     a.off = offset_bits(offset);
+    Segment g[2] = {};
+    g[0].k = shared_k; g[0].v = shared_v; g[0].lengths = shared_lengths; g[0].slots = (int)shared;
+    g[0].k_group = strides[3]; g[0].k_pos = strides[4]; g[0].k_head = strides[5];
+    g[0].v_group = strides[6]; g[0].v_pos = strides[7]; g[0].v_head = strides[8];
+    g[1].k = own_k; g[1].v = own_v; g[1].lengths = own_lengths; g[1].slots = (int)own; g[1].per_row = 1;
+    g[1].k_group = strides[9]; g[1].k_row = strides[10]; g[1].k_pos = strides[11]; g[1].k_head = strides[12];
+    g[1].v_group = strides[13]; g[1].v_row = strides[14]; g[1].v_pos = strides[15]; g[1].v_head = strides[16];
+    // 16-byte copies: every address that starts a position's row of a head is a multiple of 16 bytes
+    bool vec = dim % 4 == 0;
+    for (int i = 3; i < 9 && shared; ++i) vec = vec && strides[i] % 4 == 0;
+    for (int i = 9; i < 17 && own; ++i) vec = vec && strides[i] % 4 == 0;
+    vec = vec && (!shared || (aligned16(shared_k) && aligned16(shared_v))) && (!own || (aligned16(own_k) && aligned16(own_v)));
+    const Plan p = plan_of(groups, rows, heads, kv_heads, dim, shared, own, vec);
+    if (p.part[0].ctas > INT32_MAX || p.part[1].ctas > INT32_MAX) return PAMK_ERR_SIZE;
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < bytes_of(p, dim)) return PAMK_ERR_WORKSPACE;
     char* ws = static_cast<char*>(workspace);
     a.scores = reinterpret_cast<float*>(ws);
-    ws += aligned(p.rows * p.width * 4);
-    a.stats = reinterpret_cast<float2*>(ws);
-    ws += aligned(p.rows * p.all_chunks * 8);
-    a.parts = reinterpret_cast<float*>(ws);
+    a.stats = reinterpret_cast<float2*>(ws + score_bytes(p));
+    if (p.parts > 1) a.sums = reinterpret_cast<float*>(ws + score_bytes(p) + stat_bytes(p));
     a.width = p.width;
-    a.chunks = p.all_chunks;
-    Segment seg[2] = {};
-    seg[0].k = shared_k; seg[0].v = shared_v; seg[0].lengths = shared_lengths;
-    seg[0].k_group = strides[3]; seg[0].k_pos = strides[4]; seg[0].k_head = strides[5];
-    seg[0].v_group = strides[6]; seg[0].v_pos = strides[7]; seg[0].v_head = strides[8];
-    seg[0].slots = (int)shared; seg[0].rows = a.rows * a.share;
-    seg[1].k = own_k; seg[1].v = own_v; seg[1].lengths = own_lengths;
-    seg[1].k_group = strides[9]; seg[1].k_row = strides[10]; seg[1].k_pos = strides[11]; seg[1].k_head = strides[12];
-    seg[1].v_group = strides[13]; seg[1].v_row = strides[14]; seg[1].v_pos = strides[15]; seg[1].v_head = strides[16];
-    seg[1].slots = (int)own; seg[1].rows = a.share; seg[1].per_row = 1;
-    seg[1].first_pos = (int)shared; seg[1].first_chunk = p.chunks[0];
-    // 16-byte loads: every address that starts a row of a head is a multiple of 16 bytes
-    bool vec = dim % 4 == 0 && aligned16(q);
-    for (int i = 0; i < 3; ++i) vec = vec && strides[i] % 4 == 0;
-    if (shared) {
-        vec = vec && aligned16(shared_k) && aligned16(shared_v);
-        for (int i = 3; i < 9; ++i) vec = vec && strides[i] % 4 == 0;
-    }
-    if (own) {
-        vec = vec && aligned16(own_k) && aligned16(own_v);
-        for (int i = 9; i < 17; ++i) vec = vec && strides[i] % 4 == 0;
-    }
-    bool behind = false;
+    a.parts = p.parts;
+    g[1].first_pos = p.own_first;
+    g[1].first_part = p.part[0].ranks;
     for (int pass = 0; pass < 2; ++pass)
         for (int i = 0; i < 2; ++i) {
-            if (!seg[i].slots) continue;
-            seg[i].chunk = p.chunk[i]; seg[i].chunks = p.chunks[i]; seg[i].tiles = p.tiles[i];
-            const int64_t ctas = groups * kv_heads * (i ? rows : 1) * p.tiles[i] * p.chunks[i];
-            const int status = launch_slots(vec, p.slots, p.tile_rows[i], pass, behind, a, seg[i], ctas, p.chunk[i] > 64 ? 256 : 128, st);
+            const Part& part = p.part[i];
+            if (!g[i].slots) continue;
+            g[i].tiles = part.tiles; g[i].tile_rows = part.tile_rows; g[i].ranks = part.ranks;
+            a.split = part.split;
+            a.beside = i == 1 && g[0].slots;
+            a.has_beside = i == 0 && g[1].slots;
+            const int status = launch_part(pass == 1, vec, p.slots, part, a, g[i], st);
             if (status != PAMK_OK) return status;
-            behind = true;
         }
-    if (a.chunks > 1) return launch_behind(join_kernel, dim3((unsigned)p.rows), dim <= 64 ? 64 : 128, st, a);
-    return PAMK_OK;
+    if (!a.sums) return PAMK_OK;
+    return launch_behind(join_kernel, dim3((unsigned)p.all_rows), dim <= 64 ? 64 : 128, st, a);
 }
 
 }
