@@ -8,11 +8,13 @@
 // are 64-bit ones, so that candidates of different beams are told apart where fp32 could not.  Within a beam the larger logit comes
 // first, whatever the value's rounding.
 //
-// The logits are read once.  A first kernel takes up to 4096 of a beam's logits into the registers of a CTA and leaves
-// their maximum, their sum and the best k of them: the k-th largest of a warp's 32 thread maxima bounds the k-th largest
+// The logits are read once.  A first kernel takes up to 4092 of a beam's logits into the registers of a CTA and leaves
+// their maximum, their sum and the best k of them: each thread has two maxima, the k-th largest distinct one of a warp's 64 bounds the k-th largest
 // logit from below, the largest such bound of the eight warps leaves a few dozen candidates, and each of those counts how many are
 // larger.  Keys (logit, then lower token) are all different, so a candidate's rank is its place, and no order of atomics shows.  A
 // second kernel joins the parts of each beam and picks the k best of the group from the lists in the same way.
+#include <limits.h>
+
 #include <type_traits>
 
 #include "common.cuh"
@@ -60,90 +62,191 @@ __device__ __forceinline__ double warp_sum(double s) {
     return s;
 }
 
-__global__ void __launch_bounds__(kThreads) pick_kernel(const Select a) {
+// 2^e for whole e from -127 (there 0) to 127: e + 127 are the low bits of the sum
+__device__ __forceinline__ float power_of(float e) { return i2f(f2i(fadd(e, 8388608.0f + 127.0f)) << 23); }
+
+// A term of the sum: t = pam(x, log2 e) as 1 + fraction, times a power of two.
+__device__ __forceinline__ double term(float t, float shift) {
+    const float whole = floorf(t), lin = fadd(1.0f, fadd(t, -whole));
+    return (double)fmul(lin, power_of(fmaxf(fadd(whole, -shift), -127.0f)));
+}
+
+// Below kBand where the exponent field lies in [66, 187]: the product with log2 e passes the range rule, and such a logit is not masked (|x| < 2^61, and
+// -1e30 is beyond it).
+__device__ __forceinline__ uint32_t beyond(float x) { return 2u * (uint32_t)f2i(x) - 2u * (66u << 23); }
+constexpr uint32_t kBand = 2u * ((188u - 66u) << 23);
+
+constexpr int kWarps = kThreads / 32, kQuads = kEach / 4;
+constexpr int kMany = 512;                            // so many candidates are narrowed down by their full keys first
+
+__global__ void __launch_bounds__(kThreads, 4) pick_kernel(const Select a) {
     __shared__ unsigned long long found[kMostLogits];
-    __shared__ unsigned long long warp_least[kThreads / 32];
-    __shared__ double warp_total[kThreads / 32];
-    __shared__ float warp_top[kThreads / 32];
-    __shared__ int count;
+    __shared__ double warp_total[kWarps];
+    __shared__ float warp_shift[kWarps];
+    __shared__ uint32_t warp_least[kWarps];
+    __shared__ unsigned long long warp_key[kWarps];
+    __shared__ int count, live;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int64_t beam = blockIdx.x / a.parts;
     const int part = (int)(blockIdx.x % a.parts);
-    if (dead(a.scores[beam])) return;                                             // (its logits are not looked at)
+    after_previous();
     const int64_t group = beam / a.rows, row = beam % a.rows;
     const int begin = part * a.part, end = min(begin + a.part, a.vocab);
+    const float score = a.scores[beam];
     const float* x = a.logits + group * a.x_group + row * a.x_row;
     const unsigned char* banned = a.banned ? a.banned + group * a.ban_group + row * a.ban_row : nullptr;
+    if (dead(score)) return;                                                      // (its logits are not looked at)
     // vectors start at addresses that are multiples of 16 bytes: the first one may begin before the range
     const int first = begin - (int)((reinterpret_cast<uintptr_t>(x + begin) >> 2) & 3);
-    float v[kEach];
-    uint32_t key[kEach];
+    float4 v[kQuads];
+    uint32_t flags[kQuads];                                                       // a byte for each of the four: banned
+    const auto start = [&](int i) { return first + (i * kThreads + t) * 4; };
 #pragma unroll
-    for (int i = 0; i < kEach / 4; ++i) {
-        const int j = first + (i * kThreads + t) * 4;
+    for (int i = 0; i < kQuads; ++i) {
+        const int j = start(i);
+        v[i] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);           // (masked, where there is nothing)
+        flags[i] = 0u;
         if (j >= begin && j + 4 <= end) {
-            const float4 w = __ldg(reinterpret_cast<const float4*>(x + j));
-            v[4 * i] = w.x; v[4 * i + 1] = w.y; v[4 * i + 2] = w.z; v[4 * i + 3] = w.w;
-        } else {
+            v[i] = __ldcs(reinterpret_cast<const float4*>(x + j));
+        } else if (j < end) {
+            if (j >= begin) v[i].x = x[j];
+            if (j + 1 >= begin && j + 1 < end) v[i].y = x[j + 1];
+            if (j + 2 >= begin && j + 2 < end) v[i].z = x[j + 2];
+            if (j + 3 >= begin && j + 3 < end) v[i].w = x[j + 3];
+        }
+        if (banned && j < end) {
+            if (j >= begin && j + 4 <= end && (reinterpret_cast<uintptr_t>(banned + j) & 3) == 0) {
+                flags[i] = *reinterpret_cast<const uint32_t*>(banned + j);
+            } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[4 * i + e] = j + e >= begin && j + e < end ? __ldg(x + j + e) : -INFINITY;
+                for (int e = 0; e < 4; ++e)
+                    if (j + e >= begin && j + e < end && banned[j + e]) flags[i] |= 1u << (8 * e);
+            }
         }
     }
-    if (t == 0) count = 0;
-    float top = -INFINITY;
-    unsigned long long best = 0ull;
+    if (t == 0) count = live = 0;
+    const auto value = [&](int i, int e) { return e == 0 ? v[i].x : e == 1 ? v[i].y : e == 2 ? v[i].z : v[i].w; };
+    const auto flag = [&](int i, int e) { return (flags[i] >> (8 * e) & 0xffu) != 0u; };
+    // maxima: of all (for the shift), and of what may be chosen, for each half of the thread's
+    float half[2], all[2];
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-        const int j = first + ((i / 4) * kThreads + t) * 4 + i % 4;
-        const bool inside = j >= begin && j < end, masked = !(v[i] > kMasked);    // (NaN: the beam has no finite sum, and no candidates)
-        const bool ban = banned && inside && banned[j];
-        if (!masked || v[i] != v[i]) top = fmaxf(top, v[i]);
-        key[i] = !inside ? 0u : masked || ban ? kMaskedKey : ordered(v[i]);
-        const unsigned long long full = inside ? (unsigned long long)key[i] << 32 | (uint32_t)~j : 0ull;
-        best = full > best ? full : best;
-    }
-    // the k-th largest of the warp's thread maxima (0 if there are fewer)
-    int rank = 0;
-#pragma unroll 8
-    for (int l = 0; l < 32; ++l) rank += __shfl_sync(0xffffffffu, best, l) > best;
-    const unsigned who = __ballot_sync(0xffffffffu, rank == a.k - 1 && best != 0ull);
-    const unsigned long long least = who ? __shfl_sync(0xffffffffu, best, __ffs(who) - 1) : 0ull;
+    for (int h = 0; h < 2; ++h) {
+        half[h] = all[h] = -INFINITY;
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    if (lane == 0) {
-        warp_least[warp] = least;
-        warp_top[warp] = top;
-    }
-    __syncthreads();
-    unsigned long long from = 1ull;
+        for (int i = h * (kQuads / 2); i < (h + 1) * (kQuads / 2); ++i) {
+            const float most = fmaxf(fmaxf(v[i].x, v[i].y), fmaxf(v[i].z, v[i].w));
+            all[h] = fmaxf(all[h], most);
+            if (flags[i] == 0u) half[h] = fmaxf(half[h], most);
+            else
 #pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) {
-        from = warp_least[w] > from ? warp_least[w] : from;
-        top = fmaxf(top, warp_top[w]);
+                for (int e = 0; e < 4; ++e)
+                    if (!flag(i, e)) half[h] = fmaxf(half[h], value(i, e));
+        }
     }
-    const float shift = floorf(mul(top, kLog2e, a.off));
+    const uint32_t masked = ordered(kMasked);                                     // (as low as this: nothing to choose)
+    uint32_t b0 = max(ordered(half[0]), masked), b1 = max(ordered(half[1]), masked), least = masked;
+    for (int i = 0; i < a.k; ++i) {                                               // the k-th largest distinct maximum of the warp's halves
+        least = __reduce_max_sync(0xffffffffu, max(b0, b1));
+        if (least == masked) break;
+        if (b0 == least) b0 = masked;
+        if (b1 == least) b1 = masked;
+    }
+    const float top = of_ordered(__reduce_max_sync(0xffffffffu, ordered(fmaxf(all[0], all[1]))));
+    if (lane == 0) warp_least[warp] = least;
+    // the sum, shifted by the warp's own maximum
+    const float shift = top > kMasked ? floorf(mul(top, kLog2e, a.off)) : -INFINITY;
+    const int32_t by = isub(f2i(kLog2e), kBias - a.off);
     double total = 0.0;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-        const int j = first + ((i / 4) * kThreads + t) * 4 + i % 4;
-        const unsigned long long full = (unsigned long long)key[i] << 32 | (uint32_t)~j;
-        if (key[i] && full >= from) found[atomicAdd(&count, 1)] = full;
-        if (v[i] > kMasked || v[i] != v[i]) {
-            const float s = mul(v[i], kLog2e, a.off), whole = floorf(s), lin = fadd(1.0f, fadd(s, -whole));
-            const float down = fadd(whole, -shift);
-            total += down >= -126.0f ? (double)fmul(lin, i2f(((int32_t)down + 127) << 23)) : down != down ? (double)down : 0.0;
+    for (int i = 0; i < kQuads; ++i) {
+        if (start(i) >= end) continue;
+        const uint32_t far = max(max(beyond(v[i].x), beyond(v[i].y)), max(beyond(v[i].z), beyond(v[i].w)));
+        if (far < kBand) {
+            const double s01 = term(i2f(iadd(f2i(v[i].x), by)), shift) + term(i2f(iadd(f2i(v[i].y), by)), shift);
+            total += s01 + (term(i2f(iadd(f2i(v[i].z), by)), shift) + term(i2f(iadd(f2i(v[i].w), by)), shift));
+        } else {
+#pragma unroll 1
+            for (int e = 0; e < 4; ++e) {
+                const float y = value(i, e);
+                if (!(y <= kMasked)) {
+                    const float s = mul(y, kLog2e, a.off);
+                    total += s == s && shift > -INFINITY ? term(s, shift) : (double)quiet_nan();       // (NaN, or too large)
+                }
+            }
         }
     }
     total = warp_sum(total);
-    if (lane == 0) warp_total[warp] = total;
+    if (lane == 0) {
+        warp_total[warp] = total;
+        warp_shift[warp] = shift;
+    }
     __syncthreads();
+    const auto key = [&](int i, int e) {                                          // 0 outside the range
+        const int j = start(i) + e;
+        if (j < begin || j >= end) return 0ull;
+        const float y = value(i, e);
+        return (unsigned long long)(y > kMasked && !flag(i, e) ? ordered(y) : kMaskedKey) << 32 | (uint32_t)~j;
+    };
+    const auto push = [&](unsigned long long from, int before) {                  // what is at least `from`; masked ones below a token only
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i) {
+            if (start(i) >= end) break;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const unsigned long long full = key(i, e);
+                if (full >= from && full && ((uint32_t)(full >> 32) != kMaskedKey || start(i) + e < before)) found[atomicAdd(&count, 1)] = full;
+            }
+        }
+    };
+    uint32_t bound = warp_least[0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) bound = max(bound, warp_least[w]);
+    const float most = fmaxf(half[0], half[1]);
+    if (bound != masked) {
+        if (most > kMasked && ordered(most) >= bound) push((unsigned long long)bound << 32, 0);
+    } else {
+        // too few to choose from for a bound: all of them, and masked ones from the first on, of which as many are needed at most
+        int mine = 0;
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mine += value(i, e) > kMasked && !flag(i, e);
+        mine = __reduce_add_sync(0xffffffffu, mine);
+        if (lane == 0 && mine) atomicAdd(&live, mine);
+        __syncthreads();
+        push(1ull, begin + a.k + live);
+    }
+    __syncthreads();
+    const int at_first = count;
+    __syncthreads();
+    if (at_first > kMany) {
+        // many equal ones: the k-th largest full key of a warp's threads is a bound that they do not share
+        unsigned long long best = 0ull;
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) best = max(best, key(i, e));
+        int rank = 0;
+#pragma unroll 8
+        for (int l = 0; l < 32; ++l) rank += __shfl_sync(0xffffffffu, best, l) > best;
+        const unsigned who = __ballot_sync(0xffffffffu, rank == a.k - 1 && best != 0ull);
+        const unsigned long long mine = who ? __shfl_sync(0xffffffffu, best, __ffs(who) - 1) : 1ull;
+        if (lane == 0) warp_key[warp] = mine;
+        if (t == 0) count = 0;
+        __syncthreads();
+        unsigned long long from = 1ull;
+        for (int w = 0; w < kWarps; ++w) from = max(from, warp_key[w]);
+        push(from, INT_MAX);
+        __syncthreads();
+    }
     const int64_t list = beam * a.parts + part;
     if (t == 0) {
-        double sum = warp_total[0];
-#pragma unroll
-        for (int w = 1; w < kThreads / 32; ++w) sum += warp_total[w];
+        float m = warp_shift[0];
+        for (int w = 1; w < kWarps; ++w) m = fmaxf(m, warp_shift[w]);
+        double sum = 0.0;
+        for (int w = 0; w < kWarps; ++w) sum += warp_total[w] == 0.0 ? 0.0 : warp_total[w] * exp2_int_d(fadd(warp_shift[w], -m));
         a.sums[list] = sum;
-        a.shifts[list] = shift;
+        a.shifts[list] = m;
     }
     unsigned long long* to = a.lists + list * a.k;
     const int n = count;
@@ -181,16 +284,25 @@ struct Candidate {
     }
 };
 
+// `KEPT`: the lists have been copied to shared memory.
+template <bool KEPT>
 __global__ void __launch_bounds__(kThreads) merge_kernel(const Select a) {
     extern __shared__ __align__(16) unsigned char shared[];
     __shared__ Candidate least;
     __shared__ int count;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const int lists = a.rows * a.parts;
+    const int lists = a.rows * a.parts, entries = lists * a.k;
     double* lse = reinterpret_cast<double*>(shared);                              // [rows], NaN for a beam without finite sum
-    unsigned long long* heads = reinterpret_cast<unsigned long long*>(lse + a.rows);   // [lists]
+    double* score = lse + a.rows;                                                 // [rows]
+    unsigned long long* heads = reinterpret_cast<unsigned long long*>(score + a.rows);   // [lists]
+    unsigned long long* kept = heads + lists;                                     // [lists, k]
+    Candidate* found = reinterpret_cast<Candidate*>(kept + (KEPT ? entries : 0));
     const int64_t first_beam = (int64_t)blockIdx.x * a.rows;
+    const unsigned long long* from = a.lists + first_beam * a.parts * a.k;
+    for (int r = t; r < a.rows; r += kThreads) score[r] = (double)a.scores[first_beam + r];
     after_previous();
+    if (KEPT)
+        for (int i = t; i < entries; i += kThreads) kept[i] = __ldcg(from + i);   // (of a beam that is not continued: anything)
     for (int r = warp; r < a.rows; r += kThreads / 32) {
         double value = (double)quiet_nan();
         if (!dead(a.scores[first_beam + r])) {
@@ -221,16 +333,15 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(const Select a) {
         Candidate c;
         c.beam = list / a.parts;
         const double by = lse[c.beam];
-        const float score = a.scores[first_beam + c.beam];
         if (by != by) {
             c.key = list % a.parts == 0 && i < a.vocab ? (unsigned long long)kMaskedKey << 32 | (uint32_t)~i : 0ull;
             c.value = c.key ? ordered((double)-INFINITY) : 0ull;
             return c;
         }
-        c.key = __ldcg(a.lists + (first_beam * a.parts + list) * a.k + i);
+        c.key = KEPT ? kept[list * a.k + i] : __ldcg(from + (int64_t)list * a.k + i);
         const uint32_t x = (uint32_t)(c.key >> 32);
         c.value = c.key == 0ull ? 0ull
-                                : ordered(x == kMaskedKey ? (double)-INFINITY : ((double)of_ordered(x) - by) + (double)score);
+                                : ordered(x == kMaskedKey ? (double)-INFINITY : ((double)of_ordered(x) - by) + score[c.beam]);
         return c;
     };
     // The k-th best head of a list bounds the k-th best candidate: only k lists reach it.
@@ -239,23 +350,34 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(const Select a) {
         for (int i = t; i < lists; i += kThreads) heads[i] = candidate(i, 0).value;
         __syncthreads();
         for (int i = t; i < lists; i += kThreads) {
-            const Candidate mine = candidate(i, 0);
-            int r = 0;
+            const unsigned long long mine = heads[i];
+            if (mine == 0ull) continue;
+            int r = 0, same = 0;
             for (int o = 0; o < lists; ++o) {
-                const unsigned long long other = heads[o];
-                r += other > mine.value || (other == mine.value && o != i && candidate(o, 0).before(mine));
+                r += heads[o] > mine;
+                same += heads[o] == mine;
             }
-            if (r == a.k - 1 && mine.value != 0ull) least = mine;
+            if (r >= a.k || r + same < a.k) continue;
+            const Candidate full = candidate(i, 0);
+            if (same > 1)
+                for (int o = 0; o < lists; ++o) r += heads[o] == mine && o != i && candidate(o, 0).before(full);
+            if (r == a.k - 1) least = full;
         }
         __syncthreads();
     }
-    Candidate* found = reinterpret_cast<Candidate*>(heads + (lists + 1) / 2 * 2);
-    for (int i = t; i < lists; i += kThreads)
-        for (int e = 0; e < a.k; ++e) {
-            const Candidate c = candidate(i, e);
-            if (c.value == 0ull || (bounded && least.before(c))) break;
-            found[atomicAdd(&count, 1)] = c;
+    if (KEPT) {
+        for (int i = t; i < entries; i += kThreads) {
+            const Candidate c = candidate(i / a.k, i % a.k);
+            if (c.value != 0ull && !(bounded && least.before(c))) found[atomicAdd(&count, 1)] = c;
         }
+    } else {
+        for (int i = t; i < lists; i += kThreads)
+            for (int e = 0; e < a.k; ++e) {
+                const Candidate c = candidate(i, e);
+                if (c.value == 0ull || (bounded && least.before(c))) break;
+                found[atomicAdd(&count, 1)] = c;
+            }
+    }
     __syncthreads();
     const int n = count;
     for (int i = t; i < n; i += kThreads) {
@@ -265,8 +387,7 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(const Select a) {
         if (r < a.k) {
             const int64_t to = (int64_t)blockIdx.x * a.k + r;
             const uint32_t x = (uint32_t)(mine.key >> 32);
-            const float score = a.scores[first_beam + mine.beam];
-            a.out_scores[to] = x == kMaskedKey ? -INFINITY : (float)(((double)of_ordered(x) - lse[mine.beam]) + (double)score);
+            a.out_scores[to] = x == kMaskedKey ? -INFINITY : (float)(((double)of_ordered(x) - lse[mine.beam]) + score[mine.beam]);
             a.out_beams[to] = mine.beam;
             a.out_tokens[to] = (int64_t)(uint32_t)~(uint32_t)mine.key;
         }
@@ -279,10 +400,32 @@ size_t aligned(size_t n) { return (n + 255) / 256 * 256; }
 constexpr int kMostPart = kMostLogits - 4;
 int parts_of(int64_t vocab) { return (int)((vocab + kMostPart - 1) / kMostPart); }
 
-// The shared memory of the second kernel: at most k lists of k entries reach the bound, fewer lists than k are taken whole.
+// The shared memory of the second kernel: at most k lists of k entries reach the bound, fewer lists than k are taken whole.  Lists that are kept there
+// are read at once; beyond 8192 entries (a dozen times 128 x 5 beams of 10000 words) each is read as far as the bound.
+constexpr int64_t kMostKept = 8192;
 size_t merge_bytes(int64_t rows, int64_t parts, int64_t k) {
-    const int64_t lists = rows * parts, entries = (lists < k ? lists : k) * k;
-    return (size_t)(rows * 8 + (lists + 1) / 2 * 16 + entries * sizeof(Candidate) + 16);
+    const int64_t lists = rows * parts, reach = (lists < k ? lists : k) * k;
+    return (size_t)(rows * 16 + lists * 8 + (lists * k <= kMostKept ? lists * k * 8 : 0) + reach * (int64_t)sizeof(Candidate));
+}
+
+int launch_merge(void (*kernel)(const Select), int64_t groups, size_t bytes, const Select& a, cudaStream_t st) {
+    if (bytes > 40 * 1024) {                                                      // (48 KB with what the kernel declares)
+        const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (err != cudaSuccess) return record_cuda_error(err);
+    }
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;                // (set up behind the first kernel)
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3((unsigned)groups);
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = bytes;
+    config.stream = st;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    const cudaError_t err = cudaLaunchKernelEx(&config, kernel, a);
+    count_launch();
+    return err == cudaSuccess ? PAMK_OK : record_cuda_error(err);
 }
 
 // ---- reordering ------------------------------------------------------------------------------------------------
@@ -378,16 +521,10 @@ int pamk_beam_select(const float* logits, const float* scores, const unsigned ch
     ws += aligned((size_t)(groups * lists) * 4);
     a.lists = reinterpret_cast<unsigned long long*>(ws);
     a.out_scores = out_scores; a.out_beams = out_beams; a.out_tokens = out_tokens;
-    pick_kernel<<<(unsigned)(groups * lists), kThreads, 0, st>>>(a);
-    const int status = check_launch();
+    const int status = launch_behind(pick_kernel, dim3((unsigned)(groups * lists)), kThreads, st, a);
     if (status != PAMK_OK) return status;
-    const size_t bytes = merge_bytes(rows, parts, k);
-    if (bytes > 48 * 1024) {
-        const cudaError_t err = cudaFuncSetAttribute(merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-        if (err != cudaSuccess) return record_cuda_error(err);
-    }
-    merge_kernel<<<(unsigned)groups, kThreads, bytes, st>>>(a);
-    return check_launch();
+    return lists * k <= kMostKept ? launch_merge(merge_kernel<true>, groups, merge_bytes(rows, parts, k), a, st)
+                                  : launch_merge(merge_kernel<false>, groups, merge_bytes(rows, parts, k), a, st);
 }
 
 int pamk_reorder_states(void* const* states, const int64_t* group_bytes, const int64_t* row_bytes, const int64_t* moved_bytes,
