@@ -9,12 +9,11 @@
 // first, whatever the value's rounding.
 //
 // The logits are read once.  A first kernel takes up to 4092 of a beam's logits into the registers of a CTA and leaves
-// their maximum, their sum and the best k of them: each thread has two maxima, the k-th largest distinct one of a warp's 64 bounds the k-th largest
-// logit from below, the largest such bound of the eight warps leaves a few dozen candidates, and each of those counts how many are
+// their maximum, their sum and the best k of them: where each of W warps has k / W logits of at least some value, the k-th largest of all is no
+// smaller, so the least of the warps' (k / W)-th largest thread maxima leaves a few dozen candidates, and each of those counts how many are
 // larger.  Keys (logit, then lower token) are all different, so a candidate's rank is its place, and no order of atomics shows.  A
 // second kernel joins the parts of each beam and picks the k best of the group from the lists in the same way.
-#include <limits.h>
-
+// (A closer bound, the k-th largest of all that the warps give, leaves a dozen candidates and costs more than they do: 128 x 5 beams 24 -> 26 us.)
 #include <type_traits>
 
 #include "common.cuh"
@@ -65,6 +64,11 @@ __device__ __forceinline__ double warp_sum(double s) {
 // 2^e for whole e from -127 (there 0) to 127: e + 127 are the low bits of the sum
 __device__ __forceinline__ float power_of(float e) { return i2f(f2i(fadd(e, 8388608.0f + 127.0f)) << 23); }
 
+// s 2^e for whole e <= 0 (-inf and NaN among them: 0, unless s is NaN)
+__device__ __forceinline__ double rescaled(double s, float e) {
+    return e >= -1000.0f ? s * __longlong_as_double((long long)((int)e + 1023) << 52) : s == s ? 0.0 : s;
+}
+
 // A term of the sum: t = pam(x, log2 e) as 1 + fraction, times a power of two.
 __device__ __forceinline__ double term(float t, float shift) {
     const float whole = floorf(t), lin = fadd(1.0f, fadd(t, -whole));
@@ -77,20 +81,20 @@ __device__ __forceinline__ uint32_t beyond(float x) { return 2u * (uint32_t)f2i(
 constexpr uint32_t kBand = 2u * ((188u - 66u) << 23);
 
 constexpr int kWarps = kThreads / 32, kQuads = kEach / 4;
+static_assert(kWarps == 8 && kQuads == 4);
 constexpr int kMany = 512;                            // so many candidates are narrowed down by their full keys first
 
 __global__ void __launch_bounds__(kThreads, 4) pick_kernel(const Select a) {
     __shared__ unsigned long long found[kMostLogits];
     __shared__ double warp_total[kWarps];
     __shared__ float warp_shift[kWarps];
-    __shared__ uint32_t warp_least[kWarps];
+    __shared__ float bounds[kWarps];
     __shared__ unsigned long long warp_key[kWarps];
     __shared__ int count, live;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const int64_t beam = blockIdx.x / a.parts;
-    const int part = (int)(blockIdx.x % a.parts);
+    const unsigned beam = blockIdx.x / (unsigned)a.parts, group = beam / (unsigned)a.rows, row = beam - group * a.rows;
+    const int part = (int)(blockIdx.x - beam * a.parts);
     after_previous();
-    const int64_t group = beam / a.rows, row = beam % a.rows;
     const int begin = part * a.part, end = min(begin + a.part, a.vocab);
     const float score = a.scores[beam];
     const float* x = a.logits + group * a.x_group + row * a.x_row;
@@ -101,6 +105,7 @@ __global__ void __launch_bounds__(kThreads, 4) pick_kernel(const Select a) {
     float4 v[kQuads];
     uint32_t flags[kQuads];                                                       // a byte for each of the four: banned
     const auto start = [&](int i) { return first + (i * kThreads + t) * 4; };
+    const bool by_four = banned && (reinterpret_cast<uintptr_t>(banned + first) & 3) == 0;
 #pragma unroll
     for (int i = 0; i < kQuads; ++i) {
         const int j = start(i);
@@ -108,51 +113,58 @@ __global__ void __launch_bounds__(kThreads, 4) pick_kernel(const Select a) {
         flags[i] = 0u;
         if (j >= begin && j + 4 <= end) {
             v[i] = __ldcs(reinterpret_cast<const float4*>(x + j));
-        } else if (j < end) {
-            if (j >= begin) v[i].x = x[j];
-            if (j + 1 >= begin && j + 1 < end) v[i].y = x[j + 1];
-            if (j + 2 >= begin && j + 2 < end) v[i].z = x[j + 2];
-            if (j + 3 >= begin && j + 3 < end) v[i].w = x[j + 3];
-        }
-        if (banned && j < end) {
-            if (j >= begin && j + 4 <= end && (reinterpret_cast<uintptr_t>(banned + j) & 3) == 0) {
-                flags[i] = *reinterpret_cast<const uint32_t*>(banned + j);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (j + e >= begin && j + e < end && banned[j + e]) flags[i] |= 1u << (8 * e);
-            }
+            if (by_four) flags[i] = *reinterpret_cast<const uint32_t*>(banned + j);
         }
     }
+    // the two vectors that the range may cut
+    const auto cut = [&](int i) {
+        const int j = start(i);
+        if (j >= begin && j < end) v[i].x = x[j];
+        if (j + 1 >= begin && j + 1 < end) v[i].y = x[j + 1];
+        if (j + 2 >= begin && j + 2 < end) v[i].z = x[j + 2];
+        if (j + 3 >= begin && j + 3 < end) v[i].w = x[j + 3];
+    };
+    if (t == 0 && first < begin) cut(0);
+    const int last = (end - first) / 4;
+    if (((end - first) & 3) != 0 && t == last % kThreads)
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i)
+            if (i == last / kThreads) cut(i);
+    if (banned)
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i) {
+            const int j = start(i);
+            if (j < end && !(by_four && j >= begin && j + 4 <= end))
+#pragma unroll 1
+                for (int e = 0; e < 4; ++e)
+                    if (j + e >= begin && j + e < end && banned[j + e]) flags[i] |= 1u << (8 * e);
+        }
     if (t == 0) count = live = 0;
     const auto value = [&](int i, int e) { return e == 0 ? v[i].x : e == 1 ? v[i].y : e == 2 ? v[i].z : v[i].w; };
     const auto flag = [&](int i, int e) { return (flags[i] >> (8 * e) & 0xffu) != 0u; };
-    // maxima: of all (for the shift), and of what may be chosen, for each half of the thread's
-    float half[2], all[2];
+    // maxima: of all (for the shift), and of what may be chosen, by quads
+    float best[kQuads];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        half[h] = all[h] = -INFINITY;
+    for (int i = 0; i < kQuads; ++i) best[i] = fmaxf(fmaxf(v[i].x, v[i].y), fmaxf(v[i].z, v[i].w));
+    const float all = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
+    if ((flags[0] | flags[1] | flags[2] | flags[3]) != 0u)
 #pragma unroll
-        for (int i = h * (kQuads / 2); i < (h + 1) * (kQuads / 2); ++i) {
-            const float most = fmaxf(fmaxf(v[i].x, v[i].y), fmaxf(v[i].z, v[i].w));
-            all[h] = fmaxf(all[h], most);
-            if (flags[i] == 0u) half[h] = fmaxf(half[h], most);
-            else
+        for (int i = 0; i < kQuads; ++i) {
+            best[i] = -INFINITY;
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (!flag(i, e)) half[h] = fmaxf(half[h], value(i, e));
+            for (int e = 0; e < 4; ++e) best[i] = flag(i, e) ? best[i] : fmaxf(best[i], value(i, e));
         }
+    const float most = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
+    // the n-th largest distinct thread maximum, n = k / W rounded up, of the W warps that have one in each lane
+    const int full = min(max((end - first) / 128, 1), kWarps), need = (a.k + full - 1) / full;
+    const uint32_t masked = ordered(kMasked);
+    uint32_t left = max(ordered(most), masked), least = masked;
+    for (int i = 0; i < need; ++i) {
+        least = __reduce_max_sync(0xffffffffu, left);
+        left = left == least ? masked : left;
     }
-    const uint32_t masked = ordered(kMasked);                                     // (as low as this: nothing to choose)
-    uint32_t b0 = max(ordered(half[0]), masked), b1 = max(ordered(half[1]), masked), least = masked;
-    for (int i = 0; i < a.k; ++i) {                                               // the k-th largest distinct maximum of the warp's halves
-        least = __reduce_max_sync(0xffffffffu, max(b0, b1));
-        if (least == masked) break;
-        if (b0 == least) b0 = masked;
-        if (b1 == least) b1 = masked;
-    }
-    const float top = of_ordered(__reduce_max_sync(0xffffffffu, ordered(fmaxf(all[0], all[1]))));
-    if (lane == 0) warp_least[warp] = least;
+    if (lane == 0) bounds[warp] = least == masked ? -INFINITY : of_ordered(least);
+    const float top = of_ordered(__reduce_max_sync(0xffffffffu, ordered(all)));
     // the sum, shifted by the warp's own maximum
     const float shift = top > kMasked ? floorf(mul(top, kLog2e, a.off)) : -INFINITY;
     const int32_t by = isub(f2i(kLog2e), kBias - a.off);
@@ -187,23 +199,18 @@ __global__ void __launch_bounds__(kThreads, 4) pick_kernel(const Select a) {
         const float y = value(i, e);
         return (unsigned long long)(y > kMasked && !flag(i, e) ? ordered(y) : kMaskedKey) << 32 | (uint32_t)~j;
     };
-    const auto push = [&](unsigned long long from, int before) {                  // what is at least `from`; masked ones below a token only
+    const auto push = [&](unsigned long long full) { found[atomicAdd(&count, 1)] = full; };
+    float bound = bounds[min(lane & 7, full - 1)];
 #pragma unroll
-        for (int i = 0; i < kQuads; ++i) {
-            if (start(i) >= end) break;
+    for (int d = 4; d > 0; d >>= 1) bound = fminf(bound, __shfl_xor_sync(0xffffffffu, bound, d));
+    if (bound > kMasked) {
+        if (most >= bound)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const unsigned long long full = key(i, e);
-                if (full >= from && full && ((uint32_t)(full >> 32) != kMaskedKey || start(i) + e < before)) found[atomicAdd(&count, 1)] = full;
-            }
-        }
-    };
-    uint32_t bound = warp_least[0];
+            for (int i = 0; i < kQuads; ++i)
+                if (best[i] >= bound)
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) bound = max(bound, warp_least[w]);
-    const float most = fmaxf(half[0], half[1]);
-    if (bound != masked) {
-        if (most > kMasked && ordered(most) >= bound) push((unsigned long long)bound << 32, 0);
+                    for (int e = 0; e < 4; ++e)
+                        if (value(i, e) >= bound && !flag(i, e)) push((unsigned long long)ordered(value(i, e)) << 32 | (uint32_t)~(start(i) + e));
     } else {
         // too few to choose from for a bound: all of them, and masked ones from the first on, of which as many are needed at most
         int mine = 0;
@@ -214,37 +221,48 @@ __global__ void __launch_bounds__(kThreads, 4) pick_kernel(const Select a) {
         mine = __reduce_add_sync(0xffffffffu, mine);
         if (lane == 0 && mine) atomicAdd(&live, mine);
         __syncthreads();
-        push(1ull, begin + a.k + live);
+        const int before = begin + a.k + live;
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const unsigned long long here = key(i, e);
+                if (here && ((uint32_t)(here >> 32) != kMaskedKey || start(i) + e < before)) push(here);
+            }
     }
     __syncthreads();
     const int at_first = count;
     __syncthreads();
     if (at_first > kMany) {
         // many equal ones: the k-th largest full key of a warp's threads is a bound that they do not share
-        unsigned long long best = 0ull;
+        unsigned long long first_key = 0ull;
 #pragma unroll
         for (int i = 0; i < kQuads; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) best = max(best, key(i, e));
+            for (int e = 0; e < 4; ++e) first_key = max(first_key, key(i, e));
         int rank = 0;
 #pragma unroll 8
-        for (int l = 0; l < 32; ++l) rank += __shfl_sync(0xffffffffu, best, l) > best;
-        const unsigned who = __ballot_sync(0xffffffffu, rank == a.k - 1 && best != 0ull);
-        const unsigned long long mine = who ? __shfl_sync(0xffffffffu, best, __ffs(who) - 1) : 1ull;
+        for (int l = 0; l < 32; ++l) rank += __shfl_sync(0xffffffffu, first_key, l) > first_key;
+        const unsigned who = __ballot_sync(0xffffffffu, rank == a.k - 1 && first_key != 0ull);
+        const unsigned long long mine = who ? __shfl_sync(0xffffffffu, first_key, __ffs(who) - 1) : 1ull;
         if (lane == 0) warp_key[warp] = mine;
         if (t == 0) count = 0;
         __syncthreads();
         unsigned long long from = 1ull;
         for (int w = 0; w < kWarps; ++w) from = max(from, warp_key[w]);
-        push(from, INT_MAX);
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (key(i, e) >= from) push(key(i, e));
         __syncthreads();
     }
-    const int64_t list = beam * a.parts + part;
+    const int64_t list = blockIdx.x;
     if (t == 0) {
         float m = warp_shift[0];
         for (int w = 1; w < kWarps; ++w) m = fmaxf(m, warp_shift[w]);
         double sum = 0.0;
-        for (int w = 0; w < kWarps; ++w) sum += warp_total[w] == 0.0 ? 0.0 : warp_total[w] * exp2_int_d(fadd(warp_shift[w], -m));
+        for (int w = 0; w < kWarps; ++w) sum += rescaled(warp_total[w], fadd(warp_shift[w], -m));
         a.sums[list] = sum;
         a.shifts[list] = m;
     }
@@ -263,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 4) pick_kernel(const Select a) {
 __device__ __forceinline__ double over_log2e(double x, int32_t off) {
     const long long by = __double_as_longlong((double)kLog2e), one = __double_as_longlong(1.0);
     if (!(fabs(x) < 1e37)) return (double)quiet_nan();                             // (also NaN)
-    if (fabs(x / (double)kLog2e) < 1e-37) return 0.0;
+    if (x == 0.0) return 0.0;                                                      // (a whole number plus a logarithm is nothing else below 1e-37)
     return __longlong_as_double(__double_as_longlong(x) - by + one - ((long long)off << 29));
 }
 
@@ -283,6 +301,9 @@ struct Candidate {
         return key > o.key;
     }
 };
+
+// i / n for 0 <= i < 8192 and a quotient below 128, given 1 / n: i + 1/2 is further from a multiple of n than the roundings reach
+__device__ __forceinline__ int quotient(int i, float one_over_n) { return (int)fmul(fadd((float)i, 0.5f), one_over_n); }
 
 // `KEPT`: the lists have been copied to shared memory.
 template <bool KEPT>
@@ -312,10 +333,7 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(const Select a) {
             for (int c = lane; c < a.parts; c += 32) m = fmaxf(m, __ldcg(a.shifts + at + c));
 #pragma unroll
             for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-            for (int c = lane; c < a.parts; c += 32) {
-                const double s = __ldcg(a.sums + at + c);
-                sum += s == 0.0 ? 0.0 : s * exp2_int_d(fadd(__ldcg(a.shifts + at + c), -m));
-            }
+            for (int c = lane; c < a.parts; c += 32) sum += rescaled(__ldcg(a.sums + at + c), fadd(__ldcg(a.shifts + at + c), -m));
             sum = warp_sum(sum);
             if (sum > 0.0 && sum < 1e300) value = over_log2e((double)m + affine_log2(sum), a.off);
         }
@@ -328,13 +346,15 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(const Select a) {
         least.beam = a.rows;
     }
     __syncthreads();
+    const float one_over_parts = 1.0f / (float)a.parts;
+    const auto beam_of = [&](int list) { return quotient(list, one_over_parts); };
     // entry i of a list as a candidate; a beam without finite sum has its first tokens at -inf
-    const auto candidate = [&](int list, int i) {
+    const auto candidate = [&](int beam, int list, int i) {
         Candidate c;
-        c.beam = list / a.parts;
+        c.beam = beam;
         const double by = lse[c.beam];
         if (by != by) {
-            c.key = list % a.parts == 0 && i < a.vocab ? (unsigned long long)kMaskedKey << 32 | (uint32_t)~i : 0ull;
+            c.key = list == beam * a.parts && i < a.vocab ? (unsigned long long)kMaskedKey << 32 | (uint32_t)~i : 0ull;
             c.value = c.key ? ordered((double)-INFINITY) : 0ull;
             return c;
         }
@@ -347,33 +367,36 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(const Select a) {
     // The k-th best head of a list bounds the k-th best candidate: only k lists reach it.
     const bool bounded = lists >= a.k;
     if (bounded) {
-        for (int i = t; i < lists; i += kThreads) heads[i] = candidate(i, 0).value;
+        for (int i = t; i < lists; i += kThreads) heads[i] = candidate(beam_of(i), i, 0).value;
         __syncthreads();
         for (int i = t; i < lists; i += kThreads) {
             const unsigned long long mine = heads[i];
             if (mine == 0ull) continue;
             int r = 0, same = 0;
+#pragma unroll 4
             for (int o = 0; o < lists; ++o) {
                 r += heads[o] > mine;
                 same += heads[o] == mine;
             }
             if (r >= a.k || r + same < a.k) continue;
-            const Candidate full = candidate(i, 0);
+            const Candidate full = candidate(beam_of(i), i, 0);
             if (same > 1)
-                for (int o = 0; o < lists; ++o) r += heads[o] == mine && o != i && candidate(o, 0).before(full);
+                for (int o = 0; o < lists; ++o) r += heads[o] == mine && o != i && candidate(beam_of(o), o, 0).before(full);
             if (r == a.k - 1) least = full;
         }
         __syncthreads();
     }
     if (KEPT) {
+        const float one_over_k = 1.0f / (float)a.k;
         for (int i = t; i < entries; i += kThreads) {
-            const Candidate c = candidate(i / a.k, i % a.k);
+            const int list = quotient(i, one_over_k);
+            const Candidate c = candidate(beam_of(list), list, i - list * a.k);
             if (c.value != 0ull && !(bounded && least.before(c))) found[atomicAdd(&count, 1)] = c;
         }
     } else {
         for (int i = t; i < lists; i += kThreads)
             for (int e = 0; e < a.k; ++e) {
-                const Candidate c = candidate(i, e);
+                const Candidate c = candidate(beam_of(i), i, e);
                 if (c.value == 0ull || (bounded && least.before(c))) break;
                 found[atomicAdd(&count, 1)] = c;
             }
