@@ -325,7 +325,8 @@ int pamk_adam_step(float* const* p, const float* const* g, float* const* m, floa
  * each serving heads / kv_heads neighbouring query heads, sees the first shared_lengths[g] of the `shared` positions of its group and the first
  * own_lengths[g][r] of its `own` ones (lengths NULL: all of them; clamped to [0, slots]; nothing beyond them is read):
  *   s_j = sum_d pam(q_d, k_jd);  p = PAM softmax of s over these positions;  out_d = sum_j pam(p_j, v_jd)
- * as pamk_matmul_strided, pamk_softmax_fwd and pamk_matmul_strided give, except that the softmax shift is the floor of the row's own maximum.
+ * as pamk_matmul_strided, pamk_softmax_fwd and pamk_matmul_strided give, except that the softmax shift is the floor of the row's own maximum (which is why there
+ * is no offset here: with one, the softmax would depend on the shift).
  * A row without positions gives zeros.  `strides` (host array of 17, in elements; the last dimension of every tensor is contiguous):
  *   q: group, row, head;  shared_k: group, position, head;  shared_v: the same three;
  *   own_k: group, row, position, head;  own_v: the same four.
@@ -337,7 +338,7 @@ int pamk_cached_attention(const float* q, float* out,
                           const float* shared_k, const float* shared_v, const int64_t* shared_lengths,
                           const float* own_k, const float* own_v, const int64_t* own_lengths,
                           int64_t groups, int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim,
-                          int64_t shared, int64_t own, const int64_t* strides, float offset,
+                          int64_t shared, int64_t own, const int64_t* strides,
                           void* workspace, size_t workspace_bytes, void* stream);
 
 /* pamk_beam_select: the k best candidates of every group, best first.  Candidate (r, j) of group g is beam r continued by token j; its
@@ -352,7 +353,7 @@ int pamk_beam_select(const float* logits, const float* scores, const unsigned ch
                      float* out_scores, int64_t* out_beams, int64_t* out_tokens,
                      int64_t groups, int64_t rows, int64_t vocab, int64_t k,
                      int64_t logits_group, int64_t logits_row, int64_t banned_group, int64_t banned_row,
-                     float offset, void* workspace, size_t workspace_bytes, void* stream);
+                     void* workspace, size_t workspace_bytes, void* stream);
 
 /* pamk_reorder_states: state[g][r] = state[g][parents[g][r]] in place, for `count` tensors of any type at once.  HOST arrays of `count`
  * entries: device pointers, byte strides of groups and rows, the bytes of a row that move (contiguous) and the bytes of one position.

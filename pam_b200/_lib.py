@@ -77,9 +77,9 @@ _SIGNATURES = {
     "pamk_cross_entropy_bwd": (_i, [_p, _p, _p, _p, _p, _i64, _i64, _f, _f, _f, _i, ctypes.c_longlong, _f, _p, _sz, _p]),
     "pamk_adam_step": (_i, [_p, _p, _p, _p, _p, _i] + [_f] * 8 + [_p]),
     "pamk_cached_attention_workspace_bytes": (_sz, [_i64] * 7),
-    "pamk_cached_attention": (_i, [_p] * 8 + [_i64] * 7 + [ctypes.POINTER(_i64), _f, _p, _sz, _p]),
+    "pamk_cached_attention": (_i, [_p] * 8 + [_i64] * 7 + [ctypes.POINTER(_i64), _p, _sz, _p]),
     "pamk_beam_select_workspace_bytes": (_sz, [_i64] * 4),
-    "pamk_beam_select": (_i, [_p] * 6 + [_i64] * 8 + [_f, _p, _sz, _p]),
+    "pamk_beam_select": (_i, [_p] * 6 + [_i64] * 8 + [_p, _sz, _p]),
     "pamk_reorder_states": (_i, [_p] * 5 + [_i, _p, _p, _i64, _i64, _p]),
     "pamk_issue_rate": (_i, [_i, _i, _i, _p, ctypes.POINTER(_f), ctypes.POINTER(ctypes.c_double), _p]),
 }

@@ -50,7 +50,6 @@ struct Attention {
     float* out;
     int64_t q_group, q_row, q_head;
     int rows, kv_heads, share, dim;               // `share` query heads on each key head
-    int32_t off;
     int has_beside, beside;                       // the next kernel runs beside this one; this one beside the one before, and ends after it
     int split;                                    // keys: the slices of a piece are dealt out to warps too
     float* scores;                                // t: [(group, key head, row, head of the key head)][width]
@@ -265,11 +264,10 @@ __device__ __forceinline__ void key_stage(const Attention& a, float2 (&sum)[ROWS
                 add_pair(sum[n], iadd(w.x, x.x), iadd(w.y, x.y));
                 add_pair(sum[n], iadd(w.z, x.z), iadd(w.w, x.w));
             } else {
-                const int32_t bias = kBias - a.off;
-                sum[n].x = fadd(sum[n].x, mul(i2f(iadd(w.x, bias)), i2f(x.x), a.off));
-                if (width > 1) sum[n].y = fadd(sum[n].y, mul(i2f(iadd(w.y, bias)), i2f(x.y), a.off));
-                if (width > 2) sum[n].x = fadd(sum[n].x, mul(i2f(iadd(w.z, bias)), i2f(x.z), a.off));
-                if (width > 3) sum[n].y = fadd(sum[n].y, mul(i2f(iadd(w.w, bias)), i2f(x.w), a.off));
+                sum[n].x = fadd(sum[n].x, mul(i2f(iadd(w.x, kBias)), i2f(x.x), 0));
+                if (width > 1) sum[n].y = fadd(sum[n].y, mul(i2f(iadd(w.y, kBias)), i2f(x.y), 0));
+                if (width > 2) sum[n].x = fadd(sum[n].x, mul(i2f(iadd(w.z, kBias)), i2f(x.z), 0));
+                if (width > 3) sum[n].y = fadd(sum[n].y, mul(i2f(iadd(w.w, kBias)), i2f(x.w), 0));
             }
         }
     }
@@ -308,7 +306,7 @@ __global__ void __launch_bounds__(32 * kMostWarps, 2) key_kernel(const Attention
         int32_t* x = q + n * pitch + d;
         const bool there = n < s.rows && d < a.dim;
         plain = plain && (!there || beyond(*x) < kBand);
-        *x = there ? isub(*x, kBias - a.off) : 0;
+        *x = there ? isub(*x, kBias) : 0;
     });
     if (!plain) odd_query = 1;
     __syncthreads();
@@ -317,7 +315,7 @@ __global__ void __launch_bounds__(32 * kMostWarps, 2) key_kernel(const Attention
     Running stats[ROWS];
     float* to = a.scores + s.base * a.width + g.first_pos + s.begin + lane;
     const auto keep = [&](int n, float x, int at) {
-        const float y = x == -INFINITY ? -INFINITY : mul(x, kLog2e, a.off);
+        const float y = x == -INFINITY ? -INFINITY : mul(x, kLog2e, 0);
         to[(int64_t)n * a.width + at] = y;
         stats[n].add(y);
     };
@@ -433,7 +431,6 @@ __device__ __forceinline__ void value_stage(const Attention& a, int count, int r
     using S = ValueShape<SLOTS, ROWS>;
     const int lane = threadIdx.x & 31, l = lane % S::kLanes, sub = lane / S::kLanes;
     // t becomes p, as patterns for the products
-    const int32_t bias = kBias - a.off;
     int32_t* probs = reinterpret_cast<int32_t*>(slot + S::kScores);
     bool odd = count < S::kPositions;                                           // (a part of a stage, or a probability for the range rule)
 #pragma unroll
@@ -443,7 +440,7 @@ __device__ __forceinline__ void value_stage(const Attention& a, int count, int r
             const RowStat r = stats[n];
             const float e = exponential(i2f(probs[at]), r.shift);
             const float p = e <= r.flush_max ? 0.0f : e <= r.pass_max ? i2f(isub(f2i(e), r.sub)) : quiet_nan();
-            probs[at] = isub(f2i(p), bias);
+            probs[at] = isub(f2i(p), kBias);
             odd = odd || beyond(f2i(p)) >= kBand;
         }
     }
@@ -499,11 +496,11 @@ __device__ __forceinline__ void value_stage(const Attention& a, int count, int r
                 const int4 x = *reinterpret_cast<const int4*>(slot + ((m * 4 + u) * S::kCols + c) * 512);
 #pragma unroll
                 for (int n = 0; n < ROWS; ++n) {
-                    const float p = i2f(iadd(probs[n * S::kPositions + m * 4 * S::kAcross + u], bias));
-                    acc[n][2 * c].x = fadd(acc[n][2 * c].x, mul(p, i2f(x.x), a.off));
-                    acc[n][2 * c].y = fadd(acc[n][2 * c].y, mul(p, i2f(x.y), a.off));
-                    acc[n][2 * c + 1].x = fadd(acc[n][2 * c + 1].x, mul(p, i2f(x.z), a.off));
-                    acc[n][2 * c + 1].y = fadd(acc[n][2 * c + 1].y, mul(p, i2f(x.w), a.off));
+                    const float p = i2f(iadd(probs[n * S::kPositions + m * 4 * S::kAcross + u], kBias));
+                    acc[n][2 * c].x = fadd(acc[n][2 * c].x, mul(p, i2f(x.x), 0));
+                    acc[n][2 * c].y = fadd(acc[n][2 * c].y, mul(p, i2f(x.y), 0));
+                    acc[n][2 * c + 1].x = fadd(acc[n][2 * c + 1].x, mul(p, i2f(x.z), 0));
+                    acc[n][2 * c + 1].y = fadd(acc[n][2 * c + 1].y, mul(p, i2f(x.w), 0));
                 }
             }
         }
@@ -529,7 +526,7 @@ __global__ void __launch_bounds__(32 * kMostWarps, 2) value_kernel(const Attenti
         const float2 mine = joined([&](int i) { return i * 32 + lane < a.parts ? __ldcg(from + i * 32 + lane) : make_float2(-INFINITY, 0.0f); },
                                    (a.parts + 31) / 32);
         const float top = warp_max(mine.x), sum = warp_sum(rescaled(mine, top));
-        const Divisor d = make_divisor(sum, a.off);
+        const Divisor d = make_divisor(sum, 0);
         if (lane == 0) stats[n] = {d.flush_max, d.pass_max, d.sub, top};
     }
     __syncthreads();
@@ -741,7 +738,7 @@ size_t pamk_cached_attention_workspace_bytes(int64_t groups, int64_t rows, int64
 int pamk_cached_attention(const float* q, float* out, const float* shared_k, const float* shared_v, const int64_t* shared_lengths,
                           const float* own_k, const float* own_v, const int64_t* own_lengths,
                           int64_t groups, int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, int64_t shared, int64_t own,
-                          const int64_t* strides, float offset, void* workspace, size_t workspace_bytes, void* stream) {
+                          const int64_t* strides, void* workspace, size_t workspace_bytes, void* stream) {
     using namespace pamk;
     if (groups < 0 || rows < 0 || heads < 0 || kv_heads < 1 || dim < 0 || shared < 0 || own < 0 || heads % kv_heads || !strides) return PAMK_ERR_ARG;
     if (groups == 0 || rows == 0 || heads == 0 || dim == 0) return PAMK_OK;
@@ -756,7 +753,6 @@ int pamk_cached_attention(const float* q, float* out, const float* shared_k, con
     a.q = q; a.out = out;
     a.q_group = strides[0]; a.q_row = strides[1]; a.q_head = strides[2];
     a.rows = (int)rows; a.kv_heads = (int)kv_heads; a.share = (int)(heads / kv_heads); a.dim = (int)dim;
-    a.off = offset_bits(offset);
     Segment g[2] = {};
     g[0].k = shared_k; g[0].v = shared_v; g[0].lengths = shared_lengths; g[0].slots = (int)shared;
     g[0].k_group = strides[3]; g[0].k_pos = strides[4]; g[0].k_head = strides[5];

@@ -865,7 +865,7 @@ bool cache_ok(const Tensor& k, const Tensor& v, const Lengths& lengths, at::IntA
 }
 
 std::optional<Tensor> op_cached_attention(const Tensor& q, const Tensor& own_k, const Tensor& own_v, const Lengths& own_lengths, const Tensor& shared_k,
-                                          const Tensor& shared_v, const Lengths& shared_lengths, double offset) {
+                                          const Tensor& shared_v, const Lengths& shared_lengths) {
     if (!usable(q) || q.dim() != 4 || q.numel() == 0 || q.stride(3) != 1 || q.size(3) > 256 || wants_grad(q)) return {};
     if (!own_k.defined() && !shared_k.defined()) return {};
     const int64_t G = q.size(0), R = q.size(1), H = q.size(2), D = q.size(3);
@@ -892,13 +892,13 @@ std::optional<Tensor> op_cached_attention(const Tensor& q, const Tensor& own_k, 
     const auto count = [](const Lengths& l) { return l.t.defined() ? static_cast<const int64_t*>(l.t.data_ptr()) : nullptr; };
     check(lib.pamk_cached_attention(ptr(q), ptr(out), shared ? ptr(shared_k) : nullptr, shared ? ptr(shared_v) : nullptr, count(shared_lengths),
                                     own ? ptr(own_k) : nullptr, own ? ptr(own_v) : nullptr, count(own_lengths), G, R, H, K, D, shared, own, strides,
-                                    (float)offset, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q)),
+                                    bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q)),
           "pamk_cached_attention");
     return out;
 }
 
 // (scores, beams, tokens)
-std::optional<std::array<Tensor, 3>> op_beam_select(const Tensor& logits, const Tensor& scores, int64_t k, const Tensor& banned, double offset) {
+std::optional<std::array<Tensor, 3>> op_beam_select(const Tensor& logits, const Tensor& scores, int64_t k, const Tensor& banned) {
     if (!usable(logits) || !usable(scores) || logits.dim() != 3 || scores.dim() != 2 || scores.device() != logits.device() || logits.numel() == 0) return {};
     if (scores.sizes() != logits.sizes().slice(0, 2) || !scores.is_contiguous() || logits.stride(2) != 1 || wants_grad(logits) || wants_grad(scores)) return {};
     const int64_t G = logits.size(0), R = logits.size(1), V = logits.size(2);
@@ -922,7 +922,7 @@ std::optional<std::array<Tensor, 3>> op_beam_select(const Tensor& logits, const 
     Tensor ws = scratch_bytes(bytes, logits);
     check(lib.pamk_beam_select(ptr(logits), ptr(scores), banned.defined() ? static_cast<const unsigned char*>(banned.data_ptr()) : nullptr, ptr(best),
                                static_cast<int64_t*>(beams.data_ptr()), static_cast<int64_t*>(tokens.data_ptr()), G, R, V, k, logits.stride(0),
-                               logits.stride(1), ban[0], ban[1], (float)offset, ws.data_ptr(), bytes, stream_of(logits)),
+                               logits.stride(1), ban[0], ban[1], ws.data_ptr(), bytes, stream_of(logits)),
           "pamk_beam_select");
     return std::array<Tensor, 3>{best, beams, tokens};
 }
@@ -1185,33 +1185,31 @@ bool as_lengths(PyObject* o, Lengths& l) {
     return as_tensor(o, l.t);
 }
 
-// cached_attention(q, own_k, own_v, own_lengths, shared_k, shared_v, shared_lengths, offset)
+// cached_attention(q, own_k, own_v, own_lengths, shared_k, shared_v, shared_lengths)
 PyObject* py_cached_attention(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
-    PAMK_ARGS(8)
+    PAMK_ARGS(7)
     return operator_call([&]() -> PyObject* {
         Tensor q, own_k, own_v, shared_k, shared_v;
         Lengths own, shared;
-        double off;
         if (!as_tensor(a[0], q) || !as_tensor(a[1], own_k) || !as_tensor(a[2], own_v) || !as_lengths(a[3], own) || !as_tensor(a[4], shared_k) ||
-            !as_tensor(a[5], shared_v) || !as_lengths(a[6], shared) || !as_offset(a[7], off))
+            !as_tensor(a[5], shared_v) || !as_lengths(a[6], shared))
             return none();
-        return wrapped([&] { return op_cached_attention(q, own_k, own_v, own, shared_k, shared_v, shared, off); });
+        return wrapped([&] { return op_cached_attention(q, own_k, own_v, own, shared_k, shared_v, shared); });
     });
 }
 
-// beam_select(logits, scores, k, banned | None, offset)
+// beam_select(logits, scores, k, banned | None)
 PyObject* py_beam_select(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
-    PAMK_ARGS(5)
+    PAMK_ARGS(4)
     return operator_call([&]() -> PyObject* {
         Tensor x, scores, banned;
         int64_t k;
-        double off;
-        if (!as_tensor(a[0], x) || !as_tensor(a[1], scores) || !PyLong_CheckExact(a[2]) || !as_int(a[2], k) || !as_tensor(a[3], banned) || !as_offset(a[4], off))
+        if (!as_tensor(a[0], x) || !as_tensor(a[1], scores) || !PyLong_CheckExact(a[2]) || !as_int(a[2], k) || !as_tensor(a[3], banned))
             return none();
         std::optional<std::array<Tensor, 3>> found;
         {
             const Unlocked others_may_run;
-            found = op_beam_select(x, scores, k, banned, off);
+            found = op_beam_select(x, scores, k, banned);
         }
         if (!found) return none();
         PyObject* out = PyTuple_New(3);

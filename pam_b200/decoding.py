@@ -4,14 +4,14 @@ the states that belong to the beams.
 The reference's fairseq fork generates through the operators of its training graph: the whole chain of projections,
 products and softmax per step (fairseq/modules/multihead_attention.py:618-783), log-probabilities sorted over beams
 and vocabulary (fairseq/search.py:103-147), states gathered by beam (fairseq/sequence_generator.py:380-388).  Here each of
-the three is one call in the same PAM arithmetic, fp32 throughout.  None has a backward pass.
+the three is one call in the same PAM arithmetic, fp32 throughout.  None has a backward pass, and none takes an `offset`:
+with one, the PAM softmax depends on the maximum of the whole tensor.
 """
 import ctypes
 
 import torch
 
 from . import _lib
-from .fused import _offset
 
 MAX_HEAD_DIM = 256
 MAX_BEAMS = 64
@@ -61,7 +61,7 @@ def _cache(name, k, v, lengths, lead, heads, dim):
     return k, v, lengths
 
 
-def cached_attention(q, own_k=None, own_v=None, own_lengths=None, *, shared_k=None, shared_v=None, shared_lengths=None, offset=None):
+def cached_attention(q, own_k=None, own_v=None, own_lengths=None, *, shared_k=None, shared_v=None, shared_lengths=None):
     """PAM attention of single-token rows over cached keys and values: softmax(q k^T) v per head, as
     `fused.attention_heads` computes it for whole sequences (queries scaled by the caller).
 
@@ -77,7 +77,7 @@ def cached_attention(q, own_k=None, own_v=None, own_lengths=None, *, shared_k=No
     shift is the floor of the row's own maximum instead of the whole tensor's, which changes nothing but the rounding
     of the shifted scores.  Head dimensions up to 256."""
     if (host := _lib.host()) is not None:
-        out = host.cached_attention(q, own_k, own_v, own_lengths, shared_k, shared_v, shared_lengths, offset)
+        out = host.cached_attention(q, own_k, own_v, own_lengths, shared_k, shared_v, shared_lengths)
         if out is not None:
             return out
     _fp32("queries", q, 4)
@@ -109,13 +109,13 @@ def cached_attention(q, own_k=None, own_v=None, own_lengths=None, *, shared_k=No
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
     with _lib.device_guard(dev):
         status = handle.pamk_cached_attention(q.data_ptr(), out.data_ptr(), ptr(shared_k, shared), ptr(shared_v, shared), ptr(shared_lengths),
-                                              ptr(own_k, own), ptr(own_v, own), ptr(own_lengths), *sizes, strides, _offset(offset),
+                                              ptr(own_k, own), ptr(own_v, own), ptr(own_lengths), *sizes, strides,
                                               ptr(ws), ws_bytes, _lib.stream_ptr(dev))
     _lib.check(status, "pamk_cached_attention")
     return out
 
 
-def beam_select(logits, scores, k, banned=None, *, offset=None):
+def beam_select(logits, scores, k, banned=None):
     """One selection step of beam search: the k best continuations of every group over its beams and the vocabulary.
 
     logits  [groups, beams, vocabulary]: of the next token
@@ -130,7 +130,7 @@ def beam_select(logits, scores, k, banned=None, *, offset=None):
     share in the probability.  Masked and banned tokens and the tokens of beams that are not continued have score -inf and come
     last, also where a beam's logits hold NaN or overflow.  Up to 64 beams and k up to 64."""
     if (host := _lib.host()) is not None:
-        out = host.beam_select(logits, scores, k, banned, offset)
+        out = host.beam_select(logits, scores, k, banned)
         if out is not None:
             return out
     _fp32("logits", logits, 3)
@@ -162,7 +162,7 @@ def beam_select(logits, scores, k, banned=None, *, offset=None):
         with _lib.device_guard(dev):
             status = handle.pamk_beam_select(logits.data_ptr(), scores.data_ptr(), None if banned is None else banned.data_ptr(), best.data_ptr(),
                                              which[0].data_ptr(), which[1].data_ptr(), groups, beams, vocab, k, *logits.stride()[:2],
-                                             *((0, 0) if banned is None else banned.stride()[:2]), _offset(offset), ws.data_ptr(), ws_bytes,
+                                             *((0, 0) if banned is None else banned.stride()[:2]), ws.data_ptr(), ws_bytes,
                                              _lib.stream_ptr(dev))
         _lib.check(status, "pamk_beam_select")
     return best, which[0], which[1]

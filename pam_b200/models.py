@@ -31,7 +31,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from . import factories, fused
+from . import decoding, factories, fused
 from .pam_opt import _pam_binding
 from .steps import DeitConfig, TransformerConfig, sinusoidal_positions
 
@@ -164,6 +164,42 @@ class MultiheadAttention(nn.Module):
         ctx = self.bmm_op(w, split(v, S)).reshape(B, H, T, hd).transpose(1, 2).reshape(B, T, d)
         return self.out_proj(ctx)
 
+    def cache(self, memory):
+        """The keys and values of `memory` [..., length, dim], heads apart: [..., length, heads, head_dim]."""
+        return tuple(f(memory).unflatten(-1, (self.num_heads, self.head_dim)) for f in (self.k_proj, self.v_proj))
+
+    def step(self, query, own=None, own_length=None, shared=None, shared_lengths=None):
+        """One new token of each row, [groups, rows, dim], over cached keys and values: each row's `own` ones, of which `own_length`
+        positions are in use, or those that the rows of a group have in common (`shared`, `shared_lengths` of them)."""
+        q = self.gain_op(self.q_proj(query), self.scaling).unflatten(-1, (self.num_heads, self.head_dim))
+        bound = _pam_binding(self.ops, ("bmm", "softmax"))
+        if _plain(bound, q) and self.head_dim <= decoding.MAX_HEAD_DIM:
+            kv = dict(zip(("own_k", "own_v"), own)) if shared is None else dict(zip(("shared_k", "shared_v"), shared))
+            ctx = decoding.cached_attention(q, own_lengths=own_length, shared_lengths=shared_lengths, **kv)
+            return self.out_proj(ctx.flatten(2))
+        G, R, H, hd = q.shape
+        if shared is None:                                       # rows and heads apart, one query each
+            q, k, v = q.reshape(G * R * H, 1, hd), *(t[:, :, :own_length].transpose(2, 3).reshape(G * R * H, -1, hd) for t in own)
+        else:                                                    # heads apart, a group's rows together
+            q, k, v = q.transpose(1, 2).reshape(G * H, R, hd), *(t.transpose(1, 2).reshape(G * H, -1, hd) for t in shared)
+        w = self.bmm_op(q, k.transpose(1, 2))
+        if shared_lengths is not None:
+            w = w + _beyond(shared_lengths, k.shape[1]).repeat_interleave(H, 0)
+        ctx = self.bmm_op(self.softmax_op(w, dim=-1), v)
+        ctx = ctx.view(G, R, H, hd) if shared is None else ctx.view(G, H, R, hd).transpose(1, 2)
+        return self.out_proj(ctx.reshape(G, R, H * hd))
+
+
+def _plain(bound, t):
+    """Whether the operators of `decoding` stand for the dictionary's on this tensor: PAM functions without an offset, fp32 on a GPU."""
+    return bound is not None and bound.get("offset") in (None, 1.0) and t.is_cuda and t.dtype == torch.float32
+
+
+def _beyond(lengths, slots):
+    """-inf at the positions from each length on, 0 before: [count, 1, slots]."""
+    beyond = torch.arange(slots, device=lengths.device) >= lengths[:, None]
+    return torch.zeros(beyond.shape, device=lengths.device).masked_fill_(beyond, float("-inf")).unsqueeze(1)
+
 
 class TransformerLayer(nn.Module):
     """Post-norm encoder layer, or decoder layer when `cross` is set (transformer_layer.py)."""
@@ -184,6 +220,15 @@ class TransformerLayer(nn.Module):
         x = self.self_attn_layer_norm(x + self.self_attn(x, x, self_mask))
         if self.cross:
             x = self.encoder_attn_layer_norm(x + self.encoder_attn(x, memory))
+        return self.final_layer_norm(x + self.fc2(torch.relu(self.fc1(x))))
+
+    def step(self, x, own, position, shared, shared_lengths):
+        """The decoder layer on one new token of each row, [groups, rows, dim]: its key and value go to `position` of the row's own
+        cache, the source's are those of its group."""
+        for cache, new in zip(own, self.self_attn.cache(x)):
+            cache[:, :, position] = new
+        x = self.self_attn_layer_norm(x + self.self_attn.step(x, own=own, own_length=position + 1))
+        x = self.encoder_attn_layer_norm(x + self.encoder_attn.step(x, shared=shared, shared_lengths=shared_lengths))
         return self.final_layer_norm(x + self.fc2(torch.relu(self.fc1(x))))
 
 
@@ -241,6 +286,24 @@ class _Stack(nn.Module):
         return x + self._positions(tokens.shape[1], tokens.device)
 
 
+def _select(ops, logits, scores, count, banned):
+    """The `count` best continuations: (scores, beams, tokens) as `decoding.beam_select` gives them."""
+    bound = _pam_binding(ops, ("log_softmax",))
+    if _plain(bound, logits):
+        return decoding.beam_select(logits, scores, count, banned)
+    values = ops["log_softmax"](logits, dim=-1) + scores.unsqueeze(-1)
+    values, at = values.masked_fill(banned, float("-inf")).flatten(1).topk(count, 1)
+    return values, at // logits.shape[-1], at % logits.shape[-1]
+
+
+def _reorder(states, parents, used):
+    if parents.is_cuda:
+        return decoding.reorder_states(states, parents, used)
+    group = torch.arange(parents.shape[0])[:, None]
+    for t in states:
+        t[:, :, :used] = t[group, parents, :used]
+
+
 class Transformer(nn.Module):
     def __init__(self, cfg=TransformerConfig(), linear_cfg="standard", norm_cfg="layer_norm", functional_cfg="torch",
                  loss_functional_cfg="torch"):
@@ -258,15 +321,82 @@ class Transformer(nn.Module):
         self.decoder.output_projection = linear_factory(cfg.dim, cfg.vocab, bias=False)
         self.decoder.output_projection.weight = self.decoder.embed_tokens.weight
 
-    def forward(self, src, prev_out):
+    def encode(self, src, src_lengths=None):
+        """The encoder's output.  `src_lengths` (int64 [sentences]): the tokens behind a sentence's length are padding, which no other position
+        attends to."""
+        mask = None if src_lengths is None else _beyond(src_lengths, src.shape[1]).repeat_interleave(self.cfg.heads, 0)
         x = self.encoder.embed(src)
         for layer in self.encoder.layers:
-            x = layer(x)
+            x = layer(x, self_mask=mask)
+        return x
+
+    def forward(self, src, prev_out):
+        x = self.encode(src)
         future = self.decoder._future(prev_out.shape[1], src.device)
         y = self.decoder.embed(prev_out)
         for layer in self.decoder.layers:
             y = layer(y, x, future)
         return self.decoder.output_projection(y)
+
+    @torch.no_grad()
+    def generate(self, src, beam=5, max_len=200, *, src_lengths=None, min_len=1, length_penalty=1.0, eos=2):
+        """Beam search (fairseq/sequence_generator.py:199-552, search.py:103-147): the `beam` best translations of each sentence.
+
+        src [sentences, length], padded behind `src_lengths` where these are given.  At most `max_len` tokens come out, the end of
+        sentence `eos` among them (forced at the last one, not before the `min_len`-th).  Returns (tokens [sentences, beam, n], scores
+        [sentences, beam]), best first; a hypothesis' score is its log-probability over its length to the power of
+        `length_penalty`, -inf (and padding alone) where there were fewer; tokens behind the end are padding.
+
+        The source's keys and values are kept once for the beams of a sentence, which attend to them together; each beam's own go where
+        the beam goes on."""
+        cfg, ops, device = self.cfg, self.decoder.op_dict, src.device
+        if not 1 <= min_len <= max_len or beam < 1 or 2 * beam > decoding.MAX_SELECTED:
+            raise ValueError(f"generate needs 1 <= min_len <= max_len and up to {decoding.MAX_SELECTED // 2} beams")
+        if eos == cfg.pad or not 0 <= eos < cfg.vocab or cfg.vocab < 3:
+            raise ValueError(f"end of sentence {eos} with padding {cfg.pad} in a vocabulary of {cfg.vocab}")
+        memory = self.encode(src, src_lengths)
+        shared = [layer.encoder_attn.cache(memory) for layer in self.decoder.layers]
+        G, H = src.shape[0], cfg.heads
+        own = [tuple(torch.empty(G, beam, max_len, H, cfg.dim // H, device=device) for _ in range(2)) for _ in self.decoder.layers]
+        caches = [t for pair in own for t in pair]
+        positions = self.decoder._positions(max_len, device)
+        tokens = torch.full((G, beam, max_len), cfg.pad, device=device)
+        last = torch.full((G, beam), eos, device=device)
+        scores = torch.full((G, beam), float("-inf"), device=device)
+        scores[:, 0] = 0.0
+        best, best_tokens = torch.full((G, beam), float("-inf"), device=device), tokens.clone()
+        # what may not be chosen: early, in between and at last
+        banned = torch.zeros(3, cfg.vocab, dtype=torch.bool, device=device)
+        banned[:, cfg.pad] = True
+        banned[0, eos] = True
+        banned[2] = True
+        banned[2, eos] = False
+        count = min(2 * beam, beam * cfg.vocab)
+        rank = torch.arange(count, device=device)
+        for t in range(max_len):
+            x = ops["mul"](self.decoder.embed_scale, self.decoder.embed_tokens(last)) + positions[t]
+            for layer, mine, ours in zip(self.decoder.layers, own, shared):
+                x = layer.step(x, mine, t, ours, src_lengths)
+            logits = self.decoder.output_projection(x)
+            found, parents, chosen = _select(ops, logits, scores, count, banned[2 if t == max_len - 1 else 0 if t + 1 < min_len else 1])
+            # the ends of sentences among the first `beam` are hypotheses; the best are kept
+            ends = chosen == eos
+            done = torch.where(ends & (rank < beam), found / (t + 1) ** length_penalty, float("-inf"))
+            longer = tokens.gather(1, parents.unsqueeze(-1).expand(-1, -1, max_len))
+            longer[:, :, t] = chosen
+            best, at = torch.cat([best, done], 1).topk(beam, 1)
+            best_tokens = torch.cat([best_tokens, longer], 1).gather(1, at.unsqueeze(-1).expand(-1, -1, max_len))
+            if t == max_len - 1 or bool((best > float("-inf")).all()):
+                break
+            # the first `beam` others go on
+            go = (rank + count * ends).argsort(1)[:, :beam]
+            scores, parents, last = (v.gather(1, go) for v in (found, parents, chosen))
+            scores = scores.masked_fill(ends.gather(1, go), float("-inf"))
+            _reorder(caches, parents, t + 1)
+            _reorder([tokens], parents, t)
+            tokens[:, :, t] = last
+        best_tokens = best_tokens.masked_fill((best == float("-inf")).unsqueeze(-1), cfg.pad)
+        return best_tokens[:, :, :t + 1], best
 
     def loss(self, src, prev_out, target, fused=False):
         """Label-smoothed negative log-likelihood summed over the target tokens.  `fused` takes the

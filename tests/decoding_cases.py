@@ -18,19 +18,19 @@ def _rule(true, value):
     return torch.where(true.abs() < 1e-37, 0.0, value)
 
 
-def pam(a, b, offset=0.0):
-    """Piecewise affine product of doubles; `offset`, a fraction, is what the integer offset adds to the sum of the mantissas."""
+def pam(a, b):
+    """Piecewise affine product of doubles."""
     a, b = torch.broadcast_tensors(torch.as_tensor(a, dtype=torch.float64), torch.as_tensor(b, dtype=torch.float64))
     (sa, fa, ea), (sb, fb, eb) = _split(a), _split(b)
-    f = fa + fb + offset
+    f = fa + fb
     carry = torch.floor(f)
     return _rule(a * b, torch.where((a == 0) | (b == 0), 0.0, sa * sb * torch.exp2(ea + eb + carry) * (1 + f - carry)))
 
 
-def pad(a, b, offset=0.0):
+def pad(a, b):
     a, b = torch.broadcast_tensors(torch.as_tensor(a, dtype=torch.float64), torch.as_tensor(b, dtype=torch.float64))
     (sa, fa, ea), (sb, fb, eb) = _split(a), _split(b)
-    f = fa - fb - offset
+    f = fa - fb
     carry = torch.floor(f)
     return _rule(a / b, torch.where(a == 0, 0.0, sa * sb * torch.exp2(ea - eb + carry) * (1 + f - carry)))
 
@@ -40,14 +40,7 @@ def exp2(x):
     return torch.exp2(whole) * (1 + x - whole)
 
 
-def mantissa_offset(offset):
-    if offset is None:
-        return 0.0
-    bits = int(torch.tensor(offset, dtype=torch.float32).view(torch.int32)) - 0x3F800000
-    return bits / 2.0 ** 23
-
-
-def attention(q, own_k, own_v, own_lengths, shared_k, shared_v, shared_lengths, offset=None):
+def attention(q, own_k, own_v, own_lengths, shared_k, shared_v, shared_lengths):
     """(out, bound): float64 [groups, rows, heads, dim] and what an fp32 evaluation may be off by.
 
     The bound, in units u = 2^-24, to first order: a score of `dim` products adds them with at most dim + 8 roundings, each of at most
@@ -59,7 +52,6 @@ def attention(q, own_k, own_v, own_lengths, shared_k, shared_v, shared_lengths, 
     and 2e-37 for each of the n terms, which may be flushed on one side and not on the other.
     """
     G, R, H, D = q.shape
-    off = mantissa_offset(offset)
     out, bound = torch.zeros(G, R, H, D, dtype=torch.float64), torch.zeros(G, R, H, D, dtype=torch.float64)
     for g in range(G):
         for r in range(R):
@@ -74,24 +66,23 @@ def attention(q, own_k, own_v, own_lengths, shared_k, shared_v, shared_lengths, 
             n = keys.shape[0]
             if n == 0:
                 continue
-            products = pam(q[g, r].double(), keys, off)
+            products = pam(q[g, r].double(), keys)
             s = products.sum(-1)                                                                                # [n, H]
             s = torch.where(s.abs() < 2.0 ** 128, s, torch.sign(s) * INF)                                       # (fp32 sums overflow)
-            t = torch.where(s == -INF, -INF, pam(s, LOG2E, off))
+            t = torch.where(s == -INF, -INF, pam(s, LOG2E))
             m = torch.floor(t.amax(0))
             e = torch.where(t == -INF, 0.0, exp2(t - m))
-            p = pad(e, e.sum(0), off)
-            terms = pam(p.unsqueeze(-1), values, off)
+            p = pad(e, e.sum(0))
+            terms = pam(p.unsqueeze(-1), values)
             out[g, r] = terms.sum(0)
             E = 2 * (D + 8) * U * products.abs().sum(-1).amax(0) + U * torch.where(p > 0, (t - m).abs(), 0.0).amax(0) + 2 * U
             bound[g, r] = (4 * (2 * E + n * U) + n * U).unsqueeze(-1) * terms.abs().sum(0) + 2e-37 * n
     return out, bound
 
 
-def select(logits, scores, k, banned=None, offset=None):
+def select(logits, scores, k, banned=None):
     """(scores, beams, tokens) by value, then lower beam, then larger logit, then lower token, one candidate after another."""
     G, R, V = logits.shape
-    off = mantissa_offset(offset)
     x = logits.double()
     ban = torch.zeros(G, R, V, dtype=torch.bool) if banned is None else banned.expand(G, R, V)
     best, beams, tokens = [], [], []
@@ -101,7 +92,7 @@ def select(logits, scores, k, banned=None, offset=None):
             masked = x[g, r] <= -1e30
             score = float(scores[g, r])
             # (terms as the kernels round them: 1 + fraction in fp32)
-            t = torch.where(masked, -INF, pam(x[g, r], LOG2E, off)).float()
+            t = torch.where(masked, -INF, pam(x[g, r], LOG2E)).float()
             top = torch.floor(t.max())
             whole = torch.floor(t)
             e = torch.where(masked, 0.0, (1 + (t - whole)).double() * torch.exp2((whole - top).double()))
@@ -109,7 +100,7 @@ def select(logits, scores, k, banned=None, offset=None):
             finite = bool(total > 0) and bool(total < INF) and score > -INF
             if finite:
                 mant, expo = torch.frexp(total)
-                lse = float(pad(float(top) + float(expo) - 1 + (2 * float(mant) - 1), LOG2E, off))
+                lse = float(pad(float(top) + float(expo) - 1 + (2 * float(mant) - 1), LOG2E))
                 logit = torch.where(masked | ban[g, r], -INF, x[g, r])
                 value = torch.where(logit == -INF, -INF, logit - lse + score)
             else:

@@ -89,13 +89,13 @@ def test_entry_points_check_their_arguments():
     h = _lib.lib()
     one = ctypes.addressof(ctypes.c_float(1.0))
     strides = (ctypes.c_int64 * 17)()
-    call = lambda ptr, sizes, ws=None, n=0: h.pamk_cached_attention(ptr, ptr, ptr, ptr, None, None, None, None, *sizes, strides, 1.0, ws, n, None)
+    call = lambda ptr, sizes, ws=None, n=0: h.pamk_cached_attention(ptr, ptr, ptr, ptr, None, None, None, None, *sizes, strides, ws, n, None)
     assert call(None, (1, 1, 1, 1, 4, 3, 0)) == -1 and call(one, (1, 1, 3, 2, 4, 3, 0)) == -1 and call(one, (1, 1, 1, 1, -4, 3, 0)) == -1
     assert call(one, (1, 1, 1, 1, 4, 3, 2)) == -1                                 # own positions without own keys
     assert call(one, (1, 1, 1, 1, 257, 3, 0)) == -2 and call(one, (1 << 30, 64, 1, 1, 4, 3, 0)) == -2
     assert call(one, (1, 1, 1, 1, 4, 3, 0)) == -4 and call(one, (0, 1, 1, 1, 4, 3, 0)) == 0
     assert h.pamk_cached_attention_workspace_bytes(2, 3, 4, 2, 8, 6, 5) > 0 and h.pamk_cached_attention_workspace_bytes(2, 3, 4, 3, 8, 6, 5) == 0
-    pick = lambda ptr, sizes, ws=None, n=0: h.pamk_beam_select(ptr, ptr, None, ptr, ptr, ptr, *sizes, 1, 1, 0, 0, 1.0, ws, n, None)
+    pick = lambda ptr, sizes, ws=None, n=0: h.pamk_beam_select(ptr, ptr, None, ptr, ptr, ptr, *sizes, 1, 1, 0, 0, ws, n, None)
     assert pick(None, (1, 1, 10, 2)) == -1 and pick(one, (1, 0, 10, 2)) == -1 and pick(one, (1, 65, 10, 2)) == -2 and pick(one, (1, 1, 10, 65)) == -2
     assert pick(one, (1, 1, 10, 11)) == -2 and pick(one, (1, 64, 1 << 30, 2)) == -2 and pick(one, (1, 1, 10, 2)) == -4 and pick(one, (0, 1, 10, 2)) == 0
     table = (ctypes.c_int64 * 1)(8)
@@ -110,10 +110,8 @@ def test_definitions(oracle=oracle):
     g = torch.Generator().manual_seed(0)
     a, b = torch.randn(4000, generator=g), torch.randn(4000, generator=g)
     K = pam_oracle.kernels()
-    for offset in (1.0, 1.0552, 0.97):
-        off = oracle.mantissa_offset(offset)
-        assert torch.equal(oracle.pam(a, b, off).float(), K.pam_fwd(a, b, offset))
-        assert torch.equal(oracle.pad(a, b, off).float(), K.pad_fwd(a, b, offset))
+    assert torch.equal(oracle.pam(a, b).float(), K.pam_fwd(a, b, 1.0))
+    assert torch.equal(oracle.pad(a, b).float(), K.pad_fwd(a, b, 1.0))
     # (x - floor(x) is off by half of u, one plus it by u)
     want = oracle.exp2(a.double())
     assert bool(((K.pa_exp_fwd(a, 2.0, 1.0).double() - want).abs() <= 1.5 * oracle.U * want).all())

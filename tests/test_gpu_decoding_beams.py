@@ -10,10 +10,10 @@ DEV = "cuda"
 INF = float("inf")
 
 
-def _check(logits, scores, k, banned=None, offset=None):
+def _check(logits, scores, k, banned=None):
     from pam_b200 import decoding
-    got = decoding.beam_select(logits, scores, k, banned, offset=offset)
-    want = oracle.select(logits.cpu(), scores.cpu(), k, None if banned is None else banned.cpu(), offset)
+    got = decoding.beam_select(logits, scores, k, banned)
+    want = oracle.select(logits.cpu(), scores.cpu(), k, None if banned is None else banned.cpu())
     assert [tuple(t.shape) for t in got] == [(logits.shape[0], k)] * 3
     assert torch.equal(got[1].cpu(), want[1]) and torch.equal(got[2].cpu(), want[2])
     best = got[0].double().cpu()
@@ -107,12 +107,6 @@ def test_steep_and_flat_logits():
     for scale in (1e-6, 0.01, 30.0, 1e4):
         logits, scores, _ = _inputs(8, 2, 4, 6000, scale)
         _check(logits, scores, 8)
-
-
-@pytest.mark.parametrize("offset", [1.0552, 0.97])
-def test_offset(offset):
-    logits, scores, _ = _inputs(9, 2, 3, 800)
-    _check(logits, scores, 6, offset=offset)
 
 
 def test_matches_log_softmax():
