@@ -11,7 +11,8 @@
 // joint pass over keys and values is therefore not to be had; the sum must be known before the first value is
 // weighted.  So there are two passes.  The keys leave t (rows times positions, a small part of what the keys are) and each CTA's maximum and sum,
 // kept as it goes: whole shifts scale exponentials exactly.  The values read them, turn t into p on the way, and leave sums
-// of products; where the positions of a row are dealt out to several CTAs, a third kernel adds these.
+// of products; where the positions of a row are dealt out to several CTAs, a third kernel adds these.  Where one CTA has all positions of its rows
+// and they are few, it makes both passes, with t in its shared memory.
 //
 // Rows that see the same positions are worked on together, up to 8 per CTA: every key and value is loaded once for all of them, by
 // asynchronous copies into a ring that each warp has for itself, so that the warps run without barriers until their last sums.
@@ -110,7 +111,8 @@ struct Running {
     }
 };
 
-// A warp's ring of two stages: one is read while the other one arrives.  (With a third one calls of one row gain nothing, and others lose a CTA.)
+// A warp's ring of two stages: one is read while the other one arrives.  (Four stages for warps that have no more than that in all cost more places
+// than they save: 128 x 5 rows with up to 64 own positions 41 -> 50 us.)
 template <int BYTES>
 struct Ring {
     char* to;                                     // where the next copies go; what has arrived, once they have been issued
@@ -135,6 +137,8 @@ __device__ __forceinline__ void copy_quad(char* to, const float* from, int d, in
             if (d + e < dim) __pipeline_memcpy_async(to + 4 * e, from + e, 4);
     }
 }
+
+__host__ __device__ constexpr int padded(int dim) { return (dim + 3) / 4 * 4; }
 
 // What a CTA works on.
 struct Share {
@@ -170,11 +174,12 @@ __device__ __forceinline__ Share share_of(const Attention& a, const Segment& g) 
     return s;
 }
 
-// The kernels of a call are set up behind one another.  Those of the own positions run beside those of the shared ones: they need nothing of them, only what
-// these have waited for themselves before they let the next one start, and what comes after both waits for them.
+// The kernels of a call are set up behind one another, each when the one before it has come to its last sums.  Those of the own positions run beside those
+// of the shared ones: they need nothing of them, only what these have waited for themselves before they let the next one start, and what comes after both
+// waits for them.
 __device__ __forceinline__ void enter(const Attention& a) {
     if (!a.beside) after_previous();
-    if (a.has_beside) next_may_start();              // (without need it costs: 128 x 5 rows over 48 positions 19 -> 23 us)
+    if (a.has_beside) next_may_start();
 }
 __device__ __forceinline__ void leave(const Attention& a) {
     if (a.beside) after_previous();
@@ -273,17 +278,19 @@ __device__ __forceinline__ void key_stage(const Attention& a, float2 (&sum)[ROWS
     }
 }
 
-template <int ROWS, bool VEC>
-__global__ void __launch_bounds__(32 * kMostWarps, 2) key_kernel(const Attention a, const Segment g) {
-    extern __shared__ __align__(16) char memory[];
-    __shared__ float2 red[kMostWarps * ROWS];
-    __shared__ float dealt[kMostWarps * ROWS * 32];                              // (split: sums of each warp's slice)
-    __shared__ int odd_query;
+// What the warps of a CTA share while they read keys.
+template <int ROWS>
+struct KeyMemory {
+    float2 red[kMostWarps * ROWS];
+    float dealt[kMostWarps * ROWS * 32];          // (split: sums of each warp's slice)
+    int odd_query;
+};
+
+// t of the tile's rows and the CTA's positions, each handed to keep(row, t, position) by the lane that has it, and what the sums need of them.
+template <int ROWS, bool VEC, class Keep>
+__device__ __forceinline__ void key_pass(const Attention& a, const Segment& g, const Share& s, Ring<kKeyBytes>& ring, int32_t* q, KeyMemory<ROWS>& shared,
+                                         Running (&stats)[ROWS], Keep&& keep) {
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, warps = blockDim.x >> 5, pitch = (a.dim + 31) / 32 * 32, slices = pitch / kSlice;
-    Ring<kKeyBytes> ring(memory, warp);
-    int32_t* q = reinterpret_cast<int32_t*>(memory + warps * 2 * kKeyBytes);
-    enter(a);
-    const Share s = share_of(a, g);
     // the queries come as they are, and become patterns where each thread finds what it copied itself
     const auto each_of_query = [&](auto&& one) {
         for (int n = warp; n < ROWS; n += warps)
@@ -298,7 +305,7 @@ __global__ void __launch_bounds__(32 * kMostWarps, 2) key_kernel(const Attention
     const int step = a.split ? warps / slices : warps, first = a.split ? warp / slices : warp;
     KeyCopies<VEC> copies(a, g, s, first, step, a.split ? warp % slices : -1);
     copies.issue(a, ring);
-    if (t == 0) odd_query = 0;
+    if (t == 0) shared.odd_query = 0;
     __syncthreads();
     __pipeline_wait_prior(1);
     bool plain = true;
@@ -308,15 +315,13 @@ __global__ void __launch_bounds__(32 * kMostWarps, 2) key_kernel(const Attention
         plain = plain && (!there || beyond(*x) < kBand);
         *x = there ? isub(*x, kBias) : 0;
     });
-    if (!plain) odd_query = 1;
+    if (!plain) shared.odd_query = 1;
     __syncthreads();
-    plain = odd_query == 0;
+    plain = shared.odd_query == 0;
 
-    Running stats[ROWS];
-    float* to = a.scores + s.base * a.width + g.first_pos + s.begin + lane;
-    const auto keep = [&](int n, float x, int at) {
+    const auto done = [&](int n, float x, int at) {
         const float y = x == -INFINITY ? -INFINITY : mul(x, kLog2e, 0);
-        to[(int64_t)n * a.width + at] = y;
+        keep(n, y, at);
         stats[n].add(y);
     };
     // (split: as many pieces as warps take one; the loop runs once, for all warps)
@@ -334,30 +339,55 @@ __global__ void __launch_bounds__(32 * kMostWarps, 2) key_kernel(const Attention
         }
         if (a.split) {
 #pragma unroll
-            for (int n = 0; n < ROWS; ++n) dealt[(warp * ROWS + n) * 32 + lane] = fadd(sum[n].x, sum[n].y);
+            for (int n = 0; n < ROWS; ++n) shared.dealt[(warp * ROWS + n) * 32 + lane] = fadd(sum[n].x, sum[n].y);
             __syncthreads();
             if (warp % slices != 0) break;
 #pragma unroll
             for (int n = 0; n < ROWS; ++n) {
-                float x = dealt[(warp * ROWS + n) * 32 + lane];
-                for (int w = 1; w < slices; ++w) x = fadd(x, dealt[((warp + w) * ROWS + n) * 32 + lane]);
-                if (valid && n < s.rows) keep(n, x, piece * 32);
+                float x = shared.dealt[(warp * ROWS + n) * 32 + lane];
+                for (int w = 1; w < slices; ++w) x = fadd(x, shared.dealt[((warp + w) * ROWS + n) * 32 + lane]);
+                if (valid && n < s.rows) done(n, x, piece * 32 + lane);
             }
         } else if (valid) {
 #pragma unroll
             for (int n = 0; n < ROWS; ++n)
-                if (n < s.rows) keep(n, fadd(sum[n].x, sum[n].y), piece * 32);
+                if (n < s.rows) done(n, fadd(sum[n].x, sum[n].y), piece * 32 + lane);
         }
     }
     __pipeline_wait_prior(0);
+}
+
+// The warps' maxima and sums to shared.red; what row n has in all, by joined_row after the next barrier.
+template <int ROWS>
+__device__ __forceinline__ void leave_stats(KeyMemory<ROWS>& shared, const Running (&stats)[ROWS]) {
 #pragma unroll
     for (int n = 0; n < ROWS; ++n) {
         const float top = warp_max(stats[n].top);
         const float sum = warp_sum(rescaled(make_float2(stats[n].top, stats[n].sum), top));
-        if (lane == 0) red[warp * ROWS + n] = make_float2(top, sum);
+        if ((threadIdx.x & 31) == 0) shared.red[(threadIdx.x >> 5) * ROWS + n] = make_float2(top, sum);
     }
+}
+template <int ROWS>
+__device__ __forceinline__ float2 joined_row(const KeyMemory<ROWS>& shared, int n) {
+    return joined([&](int w) { return shared.red[w * ROWS + n]; }, blockDim.x >> 5);
+}
+
+template <int ROWS, bool VEC>
+__global__ void __launch_bounds__(32 * kMostWarps, 2) key_kernel(const Attention a, const Segment g) {
+    extern __shared__ __align__(16) char memory[];
+    __shared__ KeyMemory<ROWS> shared;
+    const int t = threadIdx.x, warp = t >> 5, warps = blockDim.x >> 5;
+    Ring<kKeyBytes> ring(memory, warp);
+    enter(a);
+    const Share s = share_of(a, g);
+    Running stats[ROWS];
+    float* to = a.scores + s.base * a.width + g.first_pos + s.begin;
+    key_pass<ROWS, VEC>(a, g, s, ring, reinterpret_cast<int32_t*>(memory + warps * 2 * kKeyBytes), shared, stats,
+                        [&](int n, float y, int at) { to[(int64_t)n * a.width + at] = y; });
+    if (!a.has_beside) next_may_start();
+    leave_stats(shared, stats);
     __syncthreads();
-    if (t < s.rows) a.stats[(s.base + t) * a.parts + g.first_part + s.rank] = joined([&](int w) { return red[w * ROWS + t]; }, warps);
+    if (t < s.rows) a.stats[(s.base + t) * a.parts + g.first_part + s.rank] = joined_row(shared, t);
     leave(a);
 }
 
@@ -386,33 +416,43 @@ struct ValueCopies {
         from = g.v + s.group * g.v_group + s.row * g.v_row + s.kv_head * g.v_head + (at + sub * 4) * stride + l * 4;
         t = a.scores + (s.base + lane / (S::kPositions / 4)) * a.width + g.first_pos + at + lane % (S::kPositions / 4) * 4;
     }
-    __device__ __forceinline__ void issue(const Attention& a, Ring<S::kBytes>& ring) {
+    __device__ __forceinline__ void values(const Attention& a, char* to) const {
         const int lane = threadIdx.x & 31, l = lane % S::kLanes, sub = lane / S::kLanes;
-        char* stage = ring.next();
+        const bool whole = VEC && left >= S::kPositions && a.dim == 4 * S::kLanes * S::kCols;
+        const float* p = from;
+        to += lane * 16;
+#pragma unroll
+        for (int m = 0; m < S::kTimes; ++m) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u, p += stride)
+#pragma unroll
+                for (int c = 0; c < S::kCols; ++c) {
+                    const int d = (l + S::kLanes * c) * 4;
+                    if (whole || (m * 4 * S::kAcross + sub * 4 + u < left && d < a.dim))
+                        copy_quad<VEC>(to + ((m * 4 + u) * S::kCols + c) * 512, p + S::kLanes * 4 * c, d, a.dim);
+                }
+            p += (4 * S::kAcross - 4) * stride;
+        }
+    }
+    __device__ __forceinline__ void scores(const Attention& a, char* to) const {
+        constexpr int kRowQuads = S::kPositions / 4, kRowsAtOnce = 32 / kRowQuads;
+        const int lane = threadIdx.x & 31;
+        const float* x = t;
+#pragma unroll
+        for (int n = 0; n < ROWS; n += kRowsAtOnce, x += (int64_t)kRowsAtOnce * a.width)
+            if (n + lane / kRowQuads < rows) __pipeline_memcpy_async(to + S::kScores + n * S::kPositions * 4 + lane * 16, x, 16);
+    }
+    __device__ __forceinline__ void advance() {
+        from += step * stride;
+        t += step;
+        left -= step;
+    }
+    __device__ __forceinline__ void issue(const Attention& a, Ring<S::kBytes>& ring) {
+        char* to = ring.next();
         if (left > 0) {
-            char* to = stage + lane * 16;
-            const bool whole = VEC && left >= S::kPositions && a.dim == 4 * S::kLanes * S::kCols;
-            const float* p = from;
-#pragma unroll
-            for (int m = 0; m < S::kTimes; ++m) {
-#pragma unroll
-                for (int u = 0; u < 4; ++u, p += stride)
-#pragma unroll
-                    for (int c = 0; c < S::kCols; ++c) {
-                        const int d = (l + S::kLanes * c) * 4;
-                        if (whole || (m * 4 * S::kAcross + sub * 4 + u < left && d < a.dim))
-                            copy_quad<VEC>(to + ((m * 4 + u) * S::kCols + c) * 512, p + S::kLanes * 4 * c, d, a.dim);
-                    }
-                p += (4 * S::kAcross - 4) * stride;
-            }
-            constexpr int kRowQuads = S::kPositions / 4, kRowsAtOnce = 32 / kRowQuads;
-            const float* x = t;
-#pragma unroll
-            for (int n = 0; n < ROWS; n += kRowsAtOnce, x += (int64_t)kRowsAtOnce * a.width)
-                if (n + lane / kRowQuads < rows) __pipeline_memcpy_async(stage + S::kScores + n * S::kPositions * 4 + lane * 16, x, 16);
-            from += step * stride;
-            t += step;
-            left -= step;
+            values(a, to);
+            scores(a, to);
+            advance();
         }
         __pipeline_commit();
     }
@@ -425,9 +465,10 @@ struct __align__(16) RowStat {
     float shift;
 };
 
-template <int SLOTS, int ROWS, bool VEC>
+// `kept` (rows `pitch` apart): t of the stage's positions, where it is not in the stage.
+template <int SLOTS, int ROWS, bool VEC, bool KEPT>
 __device__ __forceinline__ void value_stage(const Attention& a, int count, int rows, float2 (&acc)[ROWS][2 * ValueShape<SLOTS, ROWS>::kCols], char* slot,
-                                            const RowStat* stats) {
+                                            const RowStat* stats, const float* kept, int pitch) {
     using S = ValueShape<SLOTS, ROWS>;
     const int lane = threadIdx.x & 31, l = lane % S::kLanes, sub = lane / S::kLanes;
     // t becomes p, as patterns for the products
@@ -438,7 +479,7 @@ __device__ __forceinline__ void value_stage(const Attention& a, int count, int r
         const int at = i * 32 + lane, n = at / S::kPositions;
         if (n < rows) {
             const RowStat r = stats[n];
-            const float e = exponential(i2f(probs[at]), r.shift);
+            const float e = exponential(KEPT ? kept[n * pitch + at % S::kPositions] : i2f(probs[at]), r.shift);
             const float p = e <= r.flush_max ? 0.0f : e <= r.pass_max ? i2f(isub(f2i(e), r.sub)) : quiet_nan();
             probs[at] = isub(f2i(p), kBias);
             odd = odd || beyond(f2i(p)) >= kBand;
@@ -507,63 +548,35 @@ __device__ __forceinline__ void value_stage(const Attention& a, int count, int r
     }
 }
 
-__host__ __device__ constexpr int padded(int dim) { return (dim + 3) / 4 * 4; }
+__device__ __forceinline__ RowStat row_stat(float top, float sum) {
+    const Divisor d = make_divisor(sum, 0);
+    return {d.flush_max, d.pass_max, d.sub, top};
+}
 
-template <int SLOTS, int ROWS, bool VEC>
-__global__ void __launch_bounds__(32 * kMostWarps, 2) value_kernel(const Attention a, const Segment g) {
-    extern __shared__ __align__(16) char memory[];
-    __shared__ RowStat stats[ROWS];
+// The sums of a CTA's warps, added and stored.
+template <int SLOTS, int ROWS>
+__device__ __forceinline__ void store_sums(const Attention& a, const Segment& g, const Share& s, const float2 (&acc)[ROWS][2 * ValueShape<SLOTS, ROWS>::kCols],
+                                           char* memory) {
     using V = ValueShape<SLOTS, ROWS>;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, warps = blockDim.x >> 5;
-    Ring<V::kBytes> ring(memory, warp);
-    enter(a);
-    const Share s = share_of(a, g);
-    ValueCopies<SLOTS, ROWS, VEC> copies(a, g, s, warp, warps);
-    copies.issue(a, ring);
-    // a row's shift and sum, from those of its parts
-    for (int n = warp; n < s.rows; n += warps) {
-        const float2* from = a.stats + (s.base + n) * a.parts;
-        const float2 mine = joined([&](int i) { return i * 32 + lane < a.parts ? __ldcg(from + i * 32 + lane) : make_float2(-INFINITY, 0.0f); },
-                                   (a.parts + 31) / 32);
-        const float top = warp_max(mine.x), sum = warp_sum(rescaled(mine, top));
-        const Divisor d = make_divisor(sum, 0);
-        if (lane == 0) stats[n] = {d.flush_max, d.pass_max, d.sub, top};
-    }
-    __syncthreads();
-
-    float2 acc[ROWS][2 * V::kCols];
+    __syncthreads();                                                             // (the rings become the warps' sums)
+    const int columns = padded(a.dim), l = lane % V::kLanes;
+    float* sums = reinterpret_cast<float*>(memory);                              // [warp][row][column]
 #pragma unroll
     for (int n = 0; n < ROWS; ++n)
 #pragma unroll
-        for (int c = 0; c < 2 * V::kCols; ++c) acc[n][c] = make_float2(0.0f, 0.0f);
-    for (int left = s.count - warp * V::kPositions; left > 0; left -= warps * V::kPositions) {
-        __pipeline_wait_prior(0);
-        __syncwarp();
-        copies.issue(a, ring);
-        value_stage<SLOTS, ROWS, VEC>(a, left, s.rows, acc, ring.to, stats);
-    }
-    __pipeline_wait_prior(0);
-    __syncthreads();                                                             // (the rings become the warps' sums)
-    const int columns = padded(a.dim);
-    float* sums = reinterpret_cast<float*>(memory);                              // [warp][row][column]
-    {
-        const int l = lane % V::kLanes;
+        for (int c = 0; c < V::kCols; ++c) {
+            float4 x = make_float4(acc[n][2 * c].x, acc[n][2 * c].y, acc[n][2 * c + 1].x, acc[n][2 * c + 1].y);
 #pragma unroll
-        for (int n = 0; n < ROWS; ++n)
-#pragma unroll
-            for (int c = 0; c < V::kCols; ++c) {
-                float4 x = make_float4(acc[n][2 * c].x, acc[n][2 * c].y, acc[n][2 * c + 1].x, acc[n][2 * c + 1].y);
-#pragma unroll
-                for (int d = V::kLanes; d < 32; d <<= 1) {
-                    x.x = fadd(x.x, __shfl_xor_sync(0xffffffffu, x.x, d));
-                    x.y = fadd(x.y, __shfl_xor_sync(0xffffffffu, x.y, d));
-                    x.z = fadd(x.z, __shfl_xor_sync(0xffffffffu, x.z, d));
-                    x.w = fadd(x.w, __shfl_xor_sync(0xffffffffu, x.w, d));
-                }
-                const int d = (l + V::kLanes * c) * 4;
-                if (lane < V::kLanes && d < a.dim && n < s.rows) *reinterpret_cast<float4*>(sums + (warp * ROWS + n) * columns + d) = x;
+            for (int d = V::kLanes; d < 32; d <<= 1) {
+                x.x = fadd(x.x, __shfl_xor_sync(0xffffffffu, x.x, d));
+                x.y = fadd(x.y, __shfl_xor_sync(0xffffffffu, x.y, d));
+                x.z = fadd(x.z, __shfl_xor_sync(0xffffffffu, x.z, d));
+                x.w = fadd(x.w, __shfl_xor_sync(0xffffffffu, x.w, d));
             }
-    }
+            const int d = (l + V::kLanes * c) * 4;
+            if (lane < V::kLanes && d < a.dim && n < s.rows) *reinterpret_cast<float4*>(sums + (warp * ROWS + n) * columns + d) = x;
+        }
     __syncthreads();
     for (int n = warp; n < s.rows; n += warps) {
         const int r = s.row * a.share + s.first + n;
@@ -575,7 +588,104 @@ __global__ void __launch_bounds__(32 * kMostWarps, 2) value_kernel(const Attenti
             to[d] = x;
         }
     }
+}
+
+template <int ROWS, int COLS>
+__device__ __forceinline__ void clear(float2 (&acc)[ROWS][COLS]) {
+#pragma unroll
+    for (int n = 0; n < ROWS; ++n)
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) acc[n][c] = make_float2(0.0f, 0.0f);
+}
+
+template <int SLOTS, int ROWS, bool VEC>
+__global__ void __launch_bounds__(32 * kMostWarps, 2) value_kernel(const Attention a, const Segment g) {
+    extern __shared__ __align__(16) char memory[];
+    __shared__ RowStat stats[ROWS];
+    using V = ValueShape<SLOTS, ROWS>;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    Ring<V::kBytes> ring(memory, warp);
+    // The first values are on their way before the scores are there: what the kernels of the keys do not write has been waited for by them.
+    const Share s = share_of(a, g);
+    ValueCopies<SLOTS, ROWS, VEC> copies(a, g, s, warp, warps);
+    char* first = ring.next();
+    if (copies.left > 0) copies.values(a, first);
+    enter(a);
+    if (copies.left > 0) copies.scores(a, first);
+    copies.advance();
+    __pipeline_commit();
+    // a row's shift and sum, from those of its parts
+    for (int n = warp; n < s.rows; n += warps) {
+        const float2* from = a.stats + (s.base + n) * a.parts;
+        const float2 mine = joined([&](int i) { return i * 32 + lane < a.parts ? __ldcg(from + i * 32 + lane) : make_float2(-INFINITY, 0.0f); },
+                                   (a.parts + 31) / 32);
+        const float top = warp_max(mine.x), sum = warp_sum(rescaled(mine, top));
+        if (lane == 0) stats[n] = row_stat(top, sum);
+    }
+    __syncthreads();
+
+    float2 acc[ROWS][2 * V::kCols];
+    clear(acc);
+    for (int left = s.count - warp * V::kPositions; left > 0; left -= warps * V::kPositions) {
+        __pipeline_wait_prior(0);
+        __syncwarp();
+        copies.issue(a, ring);
+        value_stage<SLOTS, ROWS, VEC, false>(a, left, s.rows, acc, ring.to, stats, nullptr, 0);
+    }
+    __pipeline_wait_prior(0);
+    if (!a.has_beside) next_may_start();
+    store_sums<SLOTS, ROWS>(a, g, s, acc, memory);
     leave(a);
+}
+
+// Both passes of rows all of whose positions, kMostKept at most, are this CTA's.
+constexpr int kMostKept = 256;
+
+template <int SLOTS, int ROWS>
+__host__ __device__ constexpr int whole_ring() { return 2 * (ValueShape<SLOTS, ROWS>::kBytes > kKeyBytes ? ValueShape<SLOTS, ROWS>::kBytes : kKeyBytes); }
+
+template <int SLOTS, int ROWS, bool VEC>
+__global__ void __launch_bounds__(32 * kMostWarps, 2) whole_kernel(const Attention a, const Segment g) {
+    extern __shared__ __align__(16) char memory[];
+    __shared__ KeyMemory<ROWS> shared;
+    __shared__ RowStat stats[ROWS];
+    using V = ValueShape<SLOTS, ROWS>;
+    const int t = threadIdx.x, warp = t >> 5, warps = blockDim.x >> 5;
+    char* mine = memory + warp * whole_ring<SLOTS, ROWS>();
+    float* kept = reinterpret_cast<float*>(memory + warps * whole_ring<SLOTS, ROWS>());      // t: [row][width]
+    Ring<kKeyBytes> keys(mine, 0);
+    after_previous();
+    const Share s = share_of(a, g);
+    Running running[ROWS];
+    key_pass<ROWS, VEC>(a, g, s, keys, reinterpret_cast<int32_t*>(kept + ROWS * a.width), shared, running,
+                        [&](int n, float y, int at) { kept[n * a.width + at] = y; });
+    __syncwarp();
+    Ring<V::kBytes> ring(mine, 0);
+    ValueCopies<SLOTS, ROWS, VEC> copies(a, g, s, warp, warps);
+    const auto issue = [&] {
+        char* to = ring.next();
+        if (copies.left > 0) copies.values(a, to);
+        copies.advance();
+        __pipeline_commit();
+    };
+    issue();
+    leave_stats(shared, running);
+    __syncthreads();
+    if (t < s.rows) {
+        const float2 x = joined_row(shared, t);
+        stats[t] = row_stat(x.x, x.y);
+    }
+    __syncthreads();
+    float2 acc[ROWS][2 * V::kCols];
+    clear(acc);
+    for (int at = warp * V::kPositions; at < s.count; at += warps * V::kPositions) {
+        __pipeline_wait_prior(0);
+        __syncwarp();
+        issue();
+        value_stage<SLOTS, ROWS, VEC, true>(a, s.count - at, s.rows, acc, ring.to, stats, kept + at, a.width);
+    }
+    __pipeline_wait_prior(0);
+    store_sums<SLOTS, ROWS>(a, g, s, acc, memory);
 }
 
 // Adds the parts of a row.
@@ -596,7 +706,7 @@ __global__ void __launch_bounds__(128) join_kernel(const Attention a) {
 
 struct Part {                                     // of the shared positions, or of the own ones
     int rows, tiles, tile_rows, ranks;            // `rows`: the kernels', at least tile_rows
-    int key_warps, value_warps;
+    int key_warps, value_warps, whole_warps;
     bool split;
     int64_t ctas;
 };
@@ -605,6 +715,7 @@ struct Plan {
     int slots, width, own_first, parts;
     Part part[2];
     int64_t all_rows;
+    bool whole;                                   // one kernel makes both passes
 };
 
 int rounded_rows(int n, bool vec) {
@@ -629,10 +740,13 @@ Part part_of(int64_t units, int together, int64_t positions, int slots, int64_t 
     p.ctas = all * p.ranks;
     const int64_t each = (blocks + p.ranks - 1) / p.ranks;
     const int slices = (int)((dim + kSlice - 1) / kSlice), at_once = slots == 1 ? 32 : slots == 2 ? 16 : slots == 4 ? 8 : 4;
-    // few positions of few rows: the slices of a key are dealt out to warps as well, one warp alone would be the time of the call
-    p.split = slices > 1 && each * slices <= kMostWarps && p.ctas <= 2 * 148;
+    // Warps: one for each block of positions, up to four.  Where that leaves places empty, up to as many as fill them: a row's few positions are then the time
+    // of the call, and the slices of a key are dealt out to warps as well.
+    const int most = p.ctas <= 2 * 148 ? kMostWarps : kWarps, at_least = p.ctas <= kPlaces ? 1 : 0;
+    p.split = at_least && slices > 1 && each * slices <= most;
     p.key_warps = p.split ? (int)(each * slices) : (int)std::min<int64_t>(each, kWarps);
-    p.value_warps = (int)std::min<int64_t>((std::min<int64_t>(positions, each * 32) + at_once - 1) / at_once, p.split ? kMostWarps : kWarps);
+    p.value_warps = (int)std::min<int64_t>((std::min<int64_t>(positions, each * 32) + at_once - 1) / at_once, most);
+    p.whole_warps = at_least && !p.split ? std::max(p.key_warps, p.value_warps) : p.key_warps;
     return p;
 }
 
@@ -646,13 +760,14 @@ Plan plan_of(int64_t groups, int64_t rows, int64_t heads, int64_t kv_heads, int6
     p.width = p.own_first + (int)((own + 31) / 32 * 32);
     p.parts = p.part[0].ranks + p.part[1].ranks;
     p.all_rows = groups * rows * heads;
+    p.whole = p.parts == 1 && shared + own <= kMostKept;
     return p;
 }
 
 size_t aligned(size_t n) { return (n + 255) / 256 * 256; }
 size_t score_bytes(const Plan& p) { return aligned((size_t)p.all_rows * p.width * 4); }
 size_t stat_bytes(const Plan& p) { return aligned((size_t)p.all_rows * p.parts * 8); }
-size_t bytes_of(const Plan& p, int64_t dim) { return score_bytes(p) + stat_bytes(p) + (p.parts > 1 ? aligned((size_t)(p.all_rows * p.parts * dim) * 4) : 0); }
+size_t bytes_of(const Plan& p, int64_t dim) { return p.whole ? 0 : score_bytes(p) + stat_bytes(p) + (p.parts > 1 ? aligned((size_t)(p.all_rows * p.parts * dim) * 4) : 0); }
 
 template <class K>
 int launch(K* kernel, int64_t ctas, int warps, size_t memory, const Attention& a, const Segment& g, cudaStream_t st) {
@@ -686,33 +801,42 @@ int launch_slots(const Part& p, const Attention& a, const Segment& g, cudaStream
     return launch(value_kernel<SLOTS, ROWS, VEC>, p.ctas, p.value_warps, std::max(ring, (size_t)p.value_warps * ROWS * padded(a.dim) * 4), a, g, st);
 }
 
+template <int SLOTS, int ROWS, bool VEC>
+int launch_whole(const Part& p, const Attention& a, const Segment& g, cudaStream_t st) {
+    const size_t memory = (size_t)p.whole_warps * whole_ring<SLOTS, ROWS>() + (size_t)ROWS * (a.width + (a.dim + 31) / 32 * 32) * 4;
+    return launch(whole_kernel<SLOTS, ROWS, VEC>, p.ctas, p.whole_warps, std::max(memory, (size_t)p.whole_warps * ROWS * padded(a.dim) * 4), a, g, st);
+}
+
+enum Pass { kKeys, kValues, kWhole };
+
 template <int ROWS, bool VEC>
-int launch_pass(bool values, int slots, const Part& p, const Attention& a, const Segment& g, cudaStream_t st) {
-    if (!values) return launch_keys<ROWS, VEC>(p, a, g, st);
+int launch_pass(Pass pass, int slots, const Part& p, const Attention& a, const Segment& g, cudaStream_t st) {
+    if (pass == kKeys) return launch_keys<ROWS, VEC>(p, a, g, st);
+    const bool values = pass == kValues;
     switch (slots) {
-        case 1: return launch_slots<1, ROWS, VEC>(p, a, g, st);
-        case 2: return launch_slots<2, ROWS, VEC>(p, a, g, st);
-        case 4: return launch_slots<4, ROWS, VEC>(p, a, g, st);
-        default: return launch_slots<8, ROWS, VEC>(p, a, g, st);
+        case 1: return values ? launch_slots<1, ROWS, VEC>(p, a, g, st) : launch_whole<1, ROWS, VEC>(p, a, g, st);
+        case 2: return values ? launch_slots<2, ROWS, VEC>(p, a, g, st) : launch_whole<2, ROWS, VEC>(p, a, g, st);
+        case 4: return values ? launch_slots<4, ROWS, VEC>(p, a, g, st) : launch_whole<4, ROWS, VEC>(p, a, g, st);
+        default: return values ? launch_slots<8, ROWS, VEC>(p, a, g, st) : launch_whole<8, ROWS, VEC>(p, a, g, st);
     }
 }
 
-int launch_part(bool values, bool vec, int slots, const Part& p, const Attention& a, const Segment& g, cudaStream_t st) {
+int launch_part(Pass pass, bool vec, int slots, const Part& p, const Attention& a, const Segment& g, cudaStream_t st) {
     if (!vec) {
         switch (p.rows) {
-            case 1: return launch_pass<1, false>(values, slots, p, a, g, st);
-            case 4: return launch_pass<4, false>(values, slots, p, a, g, st);
-            default: return launch_pass<8, false>(values, slots, p, a, g, st);
+            case 1: return launch_pass<1, false>(pass, slots, p, a, g, st);
+            case 4: return launch_pass<4, false>(pass, slots, p, a, g, st);
+            default: return launch_pass<8, false>(pass, slots, p, a, g, st);
         }
     }
     switch (p.rows) {
-        case 1: return launch_pass<1, true>(values, slots, p, a, g, st);
-        case 2: return launch_pass<2, true>(values, slots, p, a, g, st);
-        case 3: return launch_pass<3, true>(values, slots, p, a, g, st);
-        case 4: return launch_pass<4, true>(values, slots, p, a, g, st);
-        case 5: return launch_pass<5, true>(values, slots, p, a, g, st);
-        case 6: return launch_pass<6, true>(values, slots, p, a, g, st);
-        default: return launch_pass<8, true>(values, slots, p, a, g, st);
+        case 1: return launch_pass<1, true>(pass, slots, p, a, g, st);
+        case 2: return launch_pass<2, true>(pass, slots, p, a, g, st);
+        case 3: return launch_pass<3, true>(pass, slots, p, a, g, st);
+        case 4: return launch_pass<4, true>(pass, slots, p, a, g, st);
+        case 5: return launch_pass<5, true>(pass, slots, p, a, g, st);
+        case 6: return launch_pass<6, true>(pass, slots, p, a, g, st);
+        default: return launch_pass<8, true>(pass, slots, p, a, g, st);
     }
 }
 
@@ -767,7 +891,8 @@ int pamk_cached_attention(const float* q, float* out, const float* shared_k, con
     vec = vec && (!shared || (aligned16(shared_k) && aligned16(shared_v))) && (!own || (aligned16(own_k) && aligned16(own_v)));
     const Plan p = plan_of(groups, rows, heads, kv_heads, dim, shared, own, vec);
     if (p.part[0].ctas > INT32_MAX || p.part[1].ctas > INT32_MAX) return PAMK_ERR_SIZE;
-    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < bytes_of(p, dim)) return PAMK_ERR_WORKSPACE;
+    const size_t bytes = bytes_of(p, dim);
+    if (bytes && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < bytes)) return PAMK_ERR_WORKSPACE;
     char* ws = static_cast<char*>(workspace);
     a.scores = reinterpret_cast<float*>(ws);
     a.stats = reinterpret_cast<float2*>(ws + score_bytes(p));
@@ -776,6 +901,12 @@ int pamk_cached_attention(const float* q, float* out, const float* shared_k, con
     a.parts = p.parts;
     g[1].first_pos = p.own_first;
     g[1].first_part = p.part[0].ranks;
+    if (p.whole) {
+        const int i = shared ? 0 : 1;
+        g[i].tiles = p.part[i].tiles; g[i].tile_rows = p.part[i].tile_rows; g[i].ranks = 1;
+        a.split = p.part[i].split;
+        return launch_part(kWhole, vec, p.slots, p.part[i], a, g[i], st);
+    }
     for (int pass = 0; pass < 2; ++pass)
         for (int i = 0; i < 2; ++i) {
             const Part& part = p.part[i];
@@ -784,7 +915,7 @@ int pamk_cached_attention(const float* q, float* out, const float* shared_k, con
             a.split = part.split;
             a.beside = i == 1 && g[0].slots;
             a.has_beside = i == 0 && g[1].slots;
-            const int status = launch_part(pass == 1, vec, p.slots, part, a, g[i], st);
+            const int status = launch_part(pass == 0 ? kKeys : kValues, vec, p.slots, part, a, g[i], st);
             if (status != PAMK_OK) return status;
         }
     if (!a.sums) return PAMK_OK;

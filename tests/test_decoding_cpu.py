@@ -93,7 +93,7 @@ def test_entry_points_check_their_arguments():
     assert call(None, (1, 1, 1, 1, 4, 3, 0)) == -1 and call(one, (1, 1, 3, 2, 4, 3, 0)) == -1 and call(one, (1, 1, 1, 1, -4, 3, 0)) == -1
     assert call(one, (1, 1, 1, 1, 4, 3, 2)) == -1                                 # own positions without own keys
     assert call(one, (1, 1, 1, 1, 257, 3, 0)) == -2 and call(one, (1 << 30, 64, 1, 1, 4, 3, 0)) == -2
-    assert call(one, (1, 1, 1, 1, 4, 3, 0)) == -4 and call(one, (0, 1, 1, 1, 4, 3, 0)) == 0
+    assert call(one, (1, 1, 1, 1, 4, 3000, 0)) == -4 and call(one, (0, 1, 1, 1, 4, 3, 0)) == 0
     assert h.pamk_cached_attention_workspace_bytes(2, 3, 4, 2, 8, 6, 5) > 0 and h.pamk_cached_attention_workspace_bytes(2, 3, 4, 3, 8, 6, 5) == 0
     pick = lambda ptr, sizes, ws=None, n=0: h.pamk_beam_select(ptr, ptr, None, ptr, ptr, ptr, *sizes, 1, 1, 0, 0, ws, n, None)
     assert pick(None, (1, 1, 10, 2)) == -1 and pick(one, (1, 0, 10, 2)) == -1 and pick(one, (1, 65, 10, 2)) == -2 and pick(one, (1, 1, 10, 65)) == -2
