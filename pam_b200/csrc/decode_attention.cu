@@ -9,7 +9,7 @@
 //
 // pam is not linear: pam(pad(e, S), v) summed is not pad(sum of pam(e, v), S).  A running maximum and sum with one
 // joint pass over keys and values is therefore not to be had; the sum must be known before the first value is
-// weighted.  So there are two passes.  The keys leave t (rows times positions, a small part of what the keys are) and each CTA's maximum and sum,
+// weighted.  So there are two passes.  The keys leave t (rows times positions, a small part of what the keys are) and each CTA's sum of exponentials with its shift,
 // kept as it goes: whole shifts scale exponentials exactly.  The values read them, turn t into p on the way, and leave sums
 // of products; where the positions of a row are dealt out to several CTAs, a third kernel adds these.  Where one CTA has all positions of its rows
 // and they are few, it makes both passes, with t in its shared memory.
@@ -54,10 +54,22 @@ struct Attention {
     int has_beside, beside;                       // the next kernel runs beside this one; this one beside the one before, and ends after it
     int split;                                    // keys: the slices of a piece are dealt out to warps too
     float* scores;                                // t: [(group, key head, row, head of the key head)][width]
-    float2* stats;                                // [the same][parts]: floor of the maximum, sum
+    float2* stats;                                // [the same][parts]: a whole number near the maximum, the sum of exponentials shifted by it
     float* sums;                                  // [the same][parts][dim], or null: straight to out
     int width, parts;
+    int one, least;                               // 1 and INT32_MIN, as values that the compiler does not know (see sum_on_alu)
 };
+
+// A packed add takes both floating-point pipes of an SM partition for as long as an integer add takes the integer pipe, and a multiply-add can stand for an
+// integer add on one of the others: five of eight sums belong on the integer pipe, beside what else it does.  Left to choose, the compiler forms
+// six of ten as multiply-adds (8 rows of 64 floats 91 -> 88 us).
+__device__ __forceinline__ int sum_on_alu(int x, int y, int least) { return __viaddmax_s32(x, y, least); }
+__device__ __forceinline__ int sum_on_fma(int x, int y, int one) {
+    int d;
+    asm("mad.lo.s32 %0, %1, %2, %3;" : "=r"(d) : "r"(x), "r"(one), "r"(y));
+    return d;
+}
+
 
 // 0 .. below kBand where the exponent field lies in [66, 187]
 __device__ __forceinline__ uint32_t beyond(int32_t x) { return 2u * (uint32_t)x - 2u * (66u << 23); }
@@ -80,7 +92,7 @@ __device__ __forceinline__ float warp_sum(float m) {
 // 2^e for whole e from -126 to 127: e + 127 are the low bits of the sum
 __device__ __forceinline__ float power_of(float e) { return i2f(f2i(fadd(e, 8388608.0f + 127.0f)) << 23); }
 
-// e of one scaled score, of which t - shift < 1.  What is below 2^-126 divides to 0.  (NaN scores do not reach the shift; they reach the sum.)
+// e of one scaled score, of which t - shift is below 65.  What is below 2^-126 divides to 0.  (NaN scores do not reach the shift; they reach the sum.)
 __device__ __forceinline__ float exponential(float t, float shift) {
     const float x = fadd(t, -shift), whole = floorf(x), e = fmul(fadd(1.0f, fadd(x, -whole)), power_of(whole));
     return whole >= -126.0f ? e : x != x && t != -INFINITY ? x : 0.0f;
@@ -92,7 +104,7 @@ __device__ __forceinline__ float rescaled(float2 s, float top) {
     return down >= -126.0f ? fmul(s.y, power_of(down)) : s.y == s.y ? 0.0f : s.y;
 }
 
-// A maximum and a sum from those of `count` parts.
+// A shift and a sum from those of `count` parts.
 template <class F>
 __device__ __forceinline__ float2 joined(F&& part, int count) {
     float top = -INFINITY, sum = 0.0f;
@@ -101,13 +113,20 @@ __device__ __forceinline__ float2 joined(F&& part, int count) {
     return make_float2(top, sum);
 }
 
-// The floor of the maximum and the sum of exponentials, as scores come.
+// A whole number near the maximum, and the sum of exponentials shifted by it, as scores come.  Sums shifted by any whole number are the same but for a power
+// of two, so it is raised where exponentials would become large, not with every maximum.
 struct Running {
-    float top = -INFINITY, sum = 0.0f;
+    float shift = -INFINITY, sum = 0.0f;
     __device__ __forceinline__ void add(float t) {
-        const float most = fmaxf(top, floorf(t));
-        sum = fadd(rescaled(make_float2(top, sum), most), exponential(t, most));
-        top = most;
+        const float x = fadd(t, -shift);
+        if (x < 64.0f && x >= -126.0f) {
+            const float whole = floorf(x);
+            sum = fadd(sum, fmul(fadd(1.0f, fadd(x, -whole)), power_of(whole)));
+        } else {
+            const float most = fmaxf(shift, floorf(t));                          // (the first score among others; -inf and NaN end here)
+            sum = fadd(rescaled(make_float2(shift, sum), most), exponential(t, most));
+            shift = most;
+        }
     }
 };
 
@@ -249,8 +268,8 @@ __device__ __forceinline__ void key_stage(const Attention& a, float2 (&sum)[ROWS
 #pragma unroll
                 for (int n = 0; n < ROWS; ++n) {
                     const int4 w = *reinterpret_cast<const int4*>(q + n * pitch + 4 * c);
-                    add_pair(sum[n], iadd(w.x, k[c].x), iadd(w.y, k[c].y));
-                    add_pair(sum[n], iadd(w.z, k[c].z), iadd(w.w, k[c].w));
+                    add_pair(sum[n], sum_on_alu(w.x, k[c].x, a.least), sum_on_fma(w.y, k[c].y, a.one));
+                    add_pair(sum[n], sum_on_alu(w.z, k[c].z, a.least), c & 1 ? sum_on_fma(w.w, k[c].w, a.one) : sum_on_alu(w.w, k[c].w, a.least));
                 }
             return;
         }
@@ -362,8 +381,8 @@ template <int ROWS>
 __device__ __forceinline__ void leave_stats(KeyMemory<ROWS>& shared, const Running (&stats)[ROWS]) {
 #pragma unroll
     for (int n = 0; n < ROWS; ++n) {
-        const float top = warp_max(stats[n].top);
-        const float sum = warp_sum(rescaled(make_float2(stats[n].top, stats[n].sum), top));
+        const float top = warp_max(stats[n].shift);
+        const float sum = warp_sum(rescaled(make_float2(stats[n].shift, stats[n].sum), top));
         if ((threadIdx.x & 31) == 0) shared.red[(threadIdx.x >> 5) * ROWS + n] = make_float2(top, sum);
     }
 }
@@ -522,8 +541,8 @@ __device__ __forceinline__ void value_stage(const Attention& a, int count, int r
                         const int32_t b = u == 0 ? w[i - n].x : u == 1 ? w[i - n].y : u == 2 ? w[i - n].z : w[i - n].w;
 #pragma unroll
                         for (int c = 0; c < S::kCols; ++c) {
-                            add_pair(acc[i][2 * c], iadd(b, v[u][c].x), iadd(b, v[u][c].y));
-                            add_pair(acc[i][2 * c + 1], iadd(b, v[u][c].z), iadd(b, v[u][c].w));
+                            add_pair(acc[i][2 * c], sum_on_alu(b, v[u][c].x, a.least), sum_on_fma(b, v[u][c].y, a.one));
+                            add_pair(acc[i][2 * c + 1], sum_on_alu(b, v[u][c].z, a.least), u & 1 ? sum_on_fma(b, v[u][c].w, a.one) : sum_on_alu(b, v[u][c].w, a.least));
                         }
                     }
             }
@@ -688,16 +707,22 @@ __global__ void __launch_bounds__(32 * kMostWarps, 2) whole_kernel(const Attenti
     store_sums<SLOTS, ROWS>(a, g, s, acc, memory);
 }
 
-// Adds the parts of a row.
-__global__ void __launch_bounds__(128) join_kernel(const Attention a) {
+// Adds the parts of a row: every thread those of its column that its turn is, then one thread of a column what these have.
+__global__ void __launch_bounds__(512) join_kernel(const Attention a) {
+    __shared__ float red[512];
     const int64_t row = blockIdx.x;                                              // (group, key head, row, head of the key head)
-    const int per = a.rows * a.share, n = (int)(row % per), kv_head = (int)(row / per % a.kv_heads);
+    const int per = a.rows * a.share, n = (int)(row % per), kv_head = (int)(row / per % a.kv_heads), turns = max(1, (int)blockDim.x / a.dim);
     float* to = a.out + ((row / per / a.kv_heads * a.rows + n / a.share) * ((int64_t)a.kv_heads * a.share) + kv_head * a.share + n % a.share) * a.dim;
     after_previous();
-    for (int d = threadIdx.x; d < a.dim; d += blockDim.x) {
-        float sum = 0.0f;
+    const int turn = threadIdx.x / a.dim, d = threadIdx.x - turn * a.dim;
+    float sum = 0.0f;
+    if (turn < turns)
 #pragma unroll 16
-        for (int r = 0; r < a.parts; ++r) sum = fadd(sum, __ldcg(a.sums + (row * a.parts + r) * a.dim + d));
+        for (int r = turn; r < a.parts; r += turns) sum = fadd(sum, __ldcg(a.sums + (row * a.parts + r) * a.dim + d));
+    red[threadIdx.x] = sum;
+    __syncthreads();
+    if (turn == 0) {
+        for (int i = 1; i < turns; ++i) sum = fadd(sum, red[i * a.dim + d]);
         to[d] = sum;
     }
 }
@@ -898,6 +923,7 @@ int pamk_cached_attention(const float* q, float* out, const float* shared_k, con
     a.stats = reinterpret_cast<float2*>(ws + score_bytes(p));
     if (p.parts > 1) a.sums = reinterpret_cast<float*>(ws + score_bytes(p) + stat_bytes(p));
     a.width = p.width;
+    a.one = 1; a.least = INT32_MIN;
     a.parts = p.parts;
     g[1].first_pos = p.own_first;
     g[1].first_part = p.part[0].ranks;
@@ -919,7 +945,7 @@ int pamk_cached_attention(const float* q, float* out, const float* shared_k, con
             if (status != PAMK_OK) return status;
         }
     if (!a.sums) return PAMK_OK;
-    return launch_behind(join_kernel, dim3((unsigned)p.all_rows), dim <= 64 ? 64 : 128, st, a);
+    return launch_behind(join_kernel, dim3((unsigned)p.all_rows), p.parts > 8 || dim > 128 ? 512 : 128, st, a);
 }
 
 }
