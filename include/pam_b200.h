@@ -325,13 +325,14 @@ int pamk_adam_step(float* const* p, const float* const* g, float* const* m, floa
  * each serving heads / kv_heads neighbouring query heads, sees the first shared_lengths[g] of the `shared` positions of its group and the first
  * own_lengths[g][r] of its `own` ones (lengths NULL: all of them; clamped to [0, slots]; nothing beyond them is read):
  *   s_j = sum_d pam(q_d, k_jd);  p = PAM softmax of s over these positions;  out_d = sum_j pam(p_j, v_jd)
- * as pamk_matmul_strided, pamk_softmax_fwd and pamk_matmul_strided give, except that the softmax shift is the floor of the row's own maximum (which is why there
- * is no offset here: with one, the softmax would depend on the shift).
+ * as pamk_matmul_strided, pamk_softmax_fwd and pamk_matmul_strided give, except that the softmax shift is a whole number near the row's own maximum (which is
+ * why there is no offset here: with one, the softmax would depend on the shift).
  * A row without positions gives zeros.  `strides` (host array of 17, in elements; the last dimension of every tensor is contiguous):
  *   q: group, row, head;  shared_k: group, position, head;  shared_v: the same three;
  *   own_k: group, row, position, head;  own_v: the same four.
  * out is contiguous [groups, rows, heads, dim]; own_lengths contiguous [groups, rows].  dim <= 256.
- * `workspace`: pamk_cached_attention_workspace_bytes(...) bytes, 256-byte aligned. */
+ * shared + own <= 2^30.
+ * `workspace`: pamk_cached_attention_workspace_bytes(...) bytes, 256-byte aligned; NULL where that is 0. */
 size_t pamk_cached_attention_workspace_bytes(int64_t groups, int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim,
                                              int64_t shared, int64_t own);
 int pamk_cached_attention(const float* q, float* out,

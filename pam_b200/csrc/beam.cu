@@ -301,7 +301,7 @@ struct Candidate {
     }
 };
 
-// i / n for 0 <= i < 8192 and a quotient below 128, given 1 / n: i + 1/2 is further from a multiple of n than the roundings reach
+// i / n for 0 <= i <= 8192, given 1 / n: (i + 1/2) / n is 1 / 2n from a whole number at least, and the roundings reach less than (i + 1/2) / n 2^-22
 __device__ __forceinline__ int quotient(int i, float one_over_n) { return (int)fmul(fadd((float)i, 0.5f), one_over_n); }
 
 // `KEPT`: the lists have been copied to shared memory.
@@ -423,16 +423,20 @@ constexpr int kMostPart = kMostLogits - 4;
 int parts_of(int64_t vocab) { return (int)((vocab + kMostPart - 1) / kMostPart); }
 
 // The shared memory of the second kernel: at most k lists of k entries reach the bound, fewer lists than k are taken whole.  Lists that are kept there
-// are read at once; beyond 8192 entries (a dozen times 128 x 5 beams of 10000 words) each is read as far as the bound.
+// are read at once; beyond 8192 entries each is read as far as the bound.
 constexpr int64_t kMostKept = 8192;
 size_t merge_bytes(int64_t rows, int64_t parts, int64_t k) {
     const int64_t lists = rows * parts, reach = (lists < k ? lists : k) * k;
     return (size_t)(rows * 16 + lists * 8 + (lists * k <= kMostKept ? lists * k * 8 : 0) + reach * (int64_t)sizeof(Candidate));
 }
 
+// (what the kernel may ask for, whatever a call needs: calls of two threads set the same)
+constexpr int kMostMemory = 200 * 1024;
+static_assert(64 * 16 + kMostLists * 8 + kMostKept * 8 + kMostPicked * kMostPicked * sizeof(Candidate) <= kMostMemory);
+
 int launch_merge(void (*kernel)(const Select), int64_t groups, size_t bytes, const Select& a, cudaStream_t st) {
     if (bytes > 40 * 1024) {                                                      // (48 KB with what the kernel declares)
-        const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostMemory);
         if (err != cudaSuccess) return record_cuda_error(err);
     }
     cudaLaunchAttribute attr{};

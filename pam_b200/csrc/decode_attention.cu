@@ -1,10 +1,10 @@
 // Attention of single-token rows over a key/value cache, in PAM arithmetic.
 //
 // For one row q of a head and the positions j that it sees (those its group shares, then its own):
-//     s_j = sum_d pam(q_d, k_jd)       t_j = pam(s_j, log2 e)          m = floor(max_j t_j)
+//     s_j = sum_d pam(q_d, k_jd)       t_j = pam(s_j, log2 e)          m: a whole number near max_j t_j
 //     e_j = exp2(t_j - m)              p_j = pad(e_j, sum_j e_j)       out_d = sum_j pam(p_j, v_jd)
 // with the piecewise affine exp2 and -inf scores at probability 0, as in the chain bmm -> softmax -> bmm
-// (pam/pam_ops.py:82-101, 305-328).  The chain's shift is the floor of the maximum of the whole tensor, here it is the row's: a
+// (pam/pam_ops.py:82-101, 305-328).  The chain's shift is the floor of the maximum of the whole tensor, here it is the row's own: a
 // whole number either way, and exp2(t - m) = exp2(t) 2^-m exactly, so only the rounding of t - m differs.
 //
 // pam is not linear: pam(pad(e, S), v) summed is not pad(sum of pam(e, v), S).  A running maximum and sum with one
@@ -794,10 +794,14 @@ size_t score_bytes(const Plan& p) { return aligned((size_t)p.all_rows * p.width 
 size_t stat_bytes(const Plan& p) { return aligned((size_t)p.all_rows * p.parts * 8); }
 size_t bytes_of(const Plan& p, int64_t dim) { return p.whole ? 0 : score_bytes(p) + stat_bytes(p) + (p.parts > 1 ? aligned((size_t)(p.all_rows * p.parts * dim) * 4) : 0); }
 
+// What a kernel may ask for, whatever a call needs: calls of two threads set the same.  (Eight warps' rings of 10 KB, and t and queries of 8 rows: 96 KB.)
+constexpr int kMostMemory = 128 * 1024;
+
 template <class K>
 int launch(K* kernel, int64_t ctas, int warps, size_t memory, const Attention& a, const Segment& g, cudaStream_t st) {
+    if (memory > kMostMemory) return PAMK_ERR_SIZE;                              // (no plan comes near)
     if (memory > 32 * 1024) {                                                    // (48 KB with what the kernels declare)
-        const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)memory);
+        const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostMemory);
         if (err != cudaSuccess) return record_cuda_error(err);
     }
     cudaLaunchAttribute attr{};
@@ -866,7 +870,7 @@ int launch_part(Pass pass, bool vec, int slots, const Part& p, const Attention& 
 }
 
 bool sizes_ok(int64_t groups, int64_t rows, int64_t heads, int64_t dim, int64_t shared, int64_t own) {
-    if (dim > 256 || rows * heads > (1 << 20) || shared > (1 << 30) || own > (1 << 30) || groups > INT32_MAX) return false;
+    if (dim > 256 || rows * heads > (1 << 20) || shared > (1 << 30) || own > (1 << 30) - shared || groups > INT32_MAX) return false;
     // (CTAs of the largest grid)
     return groups * rows * heads <= INT32_MAX / (2 + (shared + own) / 64);
 }

@@ -10,6 +10,7 @@ with one, the PAM softmax depends on the maximum of the whole tensor.
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -19,8 +20,9 @@ MAX_SELECTED = 64
 
 
 def _no_backward(what, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
+    given = [t for t in tensors if t is not None]
+    if torch.is_grad_enabled() and any(t.requires_grad for t in given) or any(forward_ad.unpack_dual(t).tangent is not None for t in given):
+        raise RuntimeError(f"{what} has no derivative: call it under torch.no_grad() or on detached tensors")
 
 
 def _fp32(name, t, dims):
@@ -74,8 +76,8 @@ def cached_attention(q, own_k=None, own_v=None, own_lengths=None, *, shared_k=No
 
     kv_heads divides heads; key head i serves heads/kv_heads neighbouring query heads.  Caches may be any view whose last
     dimension is contiguous.  Returns [groups, rows, heads, dim]; a row that sees no position gets zeros.  The softmax
-    shift is the floor of the row's own maximum instead of the whole tensor's, which changes nothing but the rounding
-    of the shifted scores.  Head dimensions up to 256."""
+    shift is a whole number near the row's own maximum instead of the floor of the whole tensor's, which changes nothing
+    but the rounding of the shifted scores.  Head dimensions up to 256."""
     if (host := _lib.host()) is not None:
         out = host.cached_attention(q, own_k, own_v, own_lengths, shared_k, shared_v, shared_lengths)
         if out is not None:
@@ -174,8 +176,8 @@ def _span(t):
     return start, start + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
 
 
-def _refuse_overlaps(states, moved, parents):
-    """No two rows that move may share memory: neither of one tensor nor of two."""
+def _refuse_overlaps(states, moved, parents, used=None):
+    """No two rows that move may share memory, neither of one tensor nor of two, and what says how they move may not lie in them."""
     spans = []
     for t, size in zip(states, moved):
         (groups, rows), (by_group, by_row) = t.shape[:2], (s * t.element_size() for s in t.stride()[:2])
@@ -186,11 +188,11 @@ def _refuse_overlaps(states, moved, parents):
         steps = [s for s, n in ((by_group, groups), (by_row, rows)) if n > 1]
         spans.append((*_span(t), size, (by_group, by_row), min(steps, default=None)))
     spans.sort(key=lambda s: s[:2])
-    start, end = _span(parents)
+    read = [_span(t) for t in (parents, used) if t is not None]
     reach = []                                            # spans that may reach into the next one
     for s in spans:
-        if s[0] < end and start < s[1]:
-            raise ValueError("the parents lie in the memory of a state")
+        if any(s[0] < end and start < s[1] for start, end in read):
+            raise ValueError("the parents, or the number of positions, lie in the memory of a state")
         reach = [r for r in reach if r[1] > s[0]]
         for r in reach:
             # (two parts of one buffer, interleaved row by row, are fine)
@@ -249,7 +251,7 @@ def reorder_states(states, parents, used=None):
     states, moved, positions = ([x[i] for i in keep] for x in (states, moved, positions))
     if not states:
         return
-    _refuse_overlaps(states, moved, parents)
+    _refuse_overlaps(states, moved, parents, used if on_device else None)
     count = len(states)
     numbers = lambda values: (ctypes.c_int64 * count)(*values)
     with _lib.device_guard(dev):

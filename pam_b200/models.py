@@ -354,10 +354,12 @@ class Transformer(nn.Module):
             raise ValueError(f"generate needs 1 <= min_len <= max_len and up to {decoding.MAX_SELECTED // 2} beams")
         if eos == cfg.pad or not 0 <= eos < cfg.vocab or cfg.vocab < 3:
             raise ValueError(f"end of sentence {eos} with padding {cfg.pad} in a vocabulary of {cfg.vocab}")
+        if src_lengths is not None and not bool(((src_lengths >= 1) & (src_lengths <= src.shape[1])).all()):
+            raise ValueError(f"lengths must be from 1 to {src.shape[1]}")
         memory = self.encode(src, src_lengths)
         shared = [layer.encoder_attn.cache(memory) for layer in self.decoder.layers]
         G, H = src.shape[0], cfg.heads
-        own = [tuple(torch.empty(G, beam, max_len, H, cfg.dim // H, device=device) for _ in range(2)) for _ in self.decoder.layers]
+        own = [tuple(torch.empty(G, beam, max_len, H, cfg.dim // H, dtype=memory.dtype, device=device) for _ in range(2)) for _ in self.decoder.layers]
         caches = [t for pair in own for t in pair]
         positions = self.decoder._positions(max_len, device)
         tokens = torch.full((G, beam, max_len), cfg.pad, device=device)

@@ -115,3 +115,32 @@ def test_definitions(oracle=oracle):
     # (x - floor(x) is off by half of u, one plus it by u)
     want = oracle.exp2(a.double())
     assert bool(((K.pa_exp_fwd(a, 2.0, 1.0).double() - want).abs() <= 1.5 * oracle.U * want).all())
+
+
+def test_no_derivative_forward_either():
+    from torch.autograd import forward_ad
+    parents = torch.zeros(2, 3, dtype=torch.int64)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: _attention(q=dual(torch.zeros(2, 3, 4, 8))), lambda: _attention(shared_v=dual(torch.zeros(2, 6, 2, 8))),
+                     lambda: decoding.beam_select(torch.zeros(2, 3, 10), dual(torch.zeros(2, 3)), 4), lambda: decoding.reorder_states([dual(torch.zeros(2, 3, 4))], parents)):
+            with pytest.raises(RuntimeError, match="derivative"):
+                call()
+
+
+def test_positions_in_a_state():
+    states = [torch.zeros(2, 3, 4, dtype=torch.int64)]
+    parents = torch.zeros(2, 3, dtype=torch.int64)
+    decoding._refuse_overlaps(states, [32], parents, torch.zeros(1, dtype=torch.int64))
+    with pytest.raises(ValueError, match="positions"):
+        decoding._refuse_overlaps(states, [32], parents, states[0][1, 2, 3])
+
+
+def test_positions_beyond_32_bits():
+    h = _lib.lib()
+    one = ctypes.addressof(ctypes.c_float(1.0))
+    strides = (ctypes.c_int64 * 17)()
+    for sizes in ((1, 1, 1, 1, 4, 1 << 30, 1 << 30), (1, 1, 1, 1, 4, 0, (1 << 30) + 1), (1, 1, 1, 1, 4, 1 << 40, 0)):
+        assert h.pamk_cached_attention_workspace_bytes(*sizes) == 0
+        assert h.pamk_cached_attention(one, one, one, one, None, one, one, None, *sizes, strides, None, 0, None) == -2
+    assert h.pamk_cached_attention_workspace_bytes(1, 1, 1, 1, 4, 1 << 29, 1 << 29) > (1 << 30) * 4

@@ -32,3 +32,17 @@ def test_refusals():
     for kw in (dict(beam=0), dict(beam=33), dict(max_len=0), dict(min_len=5, max_len=4), dict(eos=1), dict(eos=40)):
         with pytest.raises(ValueError):
             net.generate(src, **kw)
+
+
+@pytest.mark.parametrize("lengths", [[0, 3], [4, 1], [-1, 2]])
+def test_refuses_lengths_outside_the_sentences(lengths):
+    with pytest.raises(ValueError, match="lengths"):
+        cases.model({}, "cpu").generate(torch.full((2, 3), 4), src_lengths=torch.tensor(lengths))
+
+
+def test_double_precision():
+    net = cases.model({}, "cpu", 2)
+    src = torch.randint(4, net.cfg.vocab, (2, 5), generator=torch.Generator().manual_seed(8))
+    want = net.generate(src, 3, 6)
+    got = net.double().generate(src, 3, 6)
+    assert torch.equal(got[0], want[0]) and bool(((got[1] - want[1]).abs() < 1e-4).all())
