@@ -43,7 +43,9 @@ struct Segment {
     int64_t k_group, k_row, k_pos, k_head, v_group, v_row, v_pos, v_head;
     int slots, per_row;
     int tiles, tile_rows, ranks;                  // CTAs of a (unit, key head): tiles of rows, shares of the positions
-    int first_pos, first_part;                    // where its scores and its parts begin among a row's
+    int first_part;                               // where its parts begin among a row's
+    float* scores;                                // t: [rows with the same positions, a tile at a time][blocks of 32 positions][the tile's rows][32]
+    int width;                                    // positions, a multiple of 32
 };
 
 struct Attention {
@@ -53,10 +55,9 @@ struct Attention {
     int rows, kv_heads, share, dim;               // `share` query heads on each key head
     int has_beside, beside;                       // the next kernel runs beside this one; this one beside the one before, and ends after it
     int split;                                    // keys: the slices of a piece are dealt out to warps too
-    float* scores;                                // t: [(group, key head, row, head of the key head)][width]
-    float2* stats;                                // [the same][parts]: a whole number near the maximum, the sum of exponentials shifted by it
+    float2* stats;                                // [(group, key head, row, head of the key head)][parts]: a whole number near the maximum, the sum of exponentials shifted by it
     float* sums;                                  // [the same][parts][dim], or null: straight to out
-    int width, parts;
+    int parts;
     int one, least;                               // 1 and INT32_MIN, as values that the compiler does not know (see sum_on_alu)
 };
 
@@ -92,10 +93,15 @@ __device__ __forceinline__ float warp_sum(float m) {
 // 2^e for whole e from -126 to 127: e + 127 are the low bits of the sum
 __device__ __forceinline__ float power_of(float e) { return i2f(f2i(fadd(e, 8388608.0f + 127.0f)) << 23); }
 
+// 2^floor(x) (1 + (x - floor(x))) for x from -126 on, below 65: the whole part is the exponent and the fraction the mantissa (rounded once) of the pattern x 2^23
+// + kBias.
+__device__ __forceinline__ int32_t exponent(float x) { return __float2int_rn(fmul(x, 8388608.0f)); }
+__device__ __forceinline__ float power(float x) { return i2f(iadd(exponent(x), kBias)); }
+
 // e of one scaled score, of which t - shift is below 65.  What is below 2^-126 divides to 0.  (NaN scores do not reach the shift; they reach the sum.)
 __device__ __forceinline__ float exponential(float t, float shift) {
-    const float x = fadd(t, -shift), whole = floorf(x), e = fmul(fadd(1.0f, fadd(x, -whole)), power_of(whole));
-    return whole >= -126.0f ? e : x != x && t != -INFINITY ? x : 0.0f;
+    const float x = fadd(t, -shift);
+    return x >= -126.0f ? power(x) : x != x && t != -INFINITY ? x : 0.0f;
 }
 
 // A sum (y) whose shift rises from x to `top`.
@@ -118,15 +124,9 @@ __device__ __forceinline__ float2 joined(F&& part, int count) {
 struct Running {
     float shift = -INFINITY, sum = 0.0f;
     __device__ __forceinline__ void add(float t) {
-        const float x = fadd(t, -shift);
-        if (x < 64.0f && x >= -126.0f) {
-            const float whole = floorf(x);
-            sum = fadd(sum, fmul(fadd(1.0f, fadd(x, -whole)), power_of(whole)));
-        } else {
-            const float most = fmaxf(shift, floorf(t));                          // (the first score among others; -inf and NaN end here)
-            sum = fadd(rescaled(make_float2(shift, sum), most), exponential(t, most));
-            shift = most;
-        }
+        const float most = fadd(t, -shift) < 64.0f ? shift : fmaxf(shift, floorf(t));         // (the first score raises it; -inf and NaN do not)
+        sum = fadd(rescaled(make_float2(shift, sum), most), exponential(t, most));
+        shift = most;
     }
 };
 
@@ -305,10 +305,10 @@ struct KeyMemory {
     int odd_query;
 };
 
-// t of the tile's rows and the CTA's positions, each handed to keep(row, t, position) by the lane that has it, and what the sums need of them.
-template <int ROWS, bool VEC, class Keep>
+// t of the tile's rows and the CTA's positions, stored by the lane that has it (row n, position p: place(p)[n * pitch]), and what the sums need of them.
+template <int ROWS, bool VEC, class Place>
 __device__ __forceinline__ void key_pass(const Attention& a, const Segment& g, const Share& s, Ring<kKeyBytes>& ring, int32_t* q, KeyMemory<ROWS>& shared,
-                                         Running (&stats)[ROWS], Keep&& keep) {
+                                         Running (&stats)[ROWS], Place&& place, int row_pitch) {
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, warps = blockDim.x >> 5, pitch = (a.dim + 31) / 32 * 32, slices = pitch / kSlice;
     // the queries come as they are, and become patterns where each thread finds what it copied itself
     const auto each_of_query = [&](auto&& one) {
@@ -338,10 +338,30 @@ __device__ __forceinline__ void key_pass(const Attention& a, const Segment& g, c
     __syncthreads();
     plain = shared.odd_query == 0;
 
-    const auto done = [&](int n, float x, int at) {
-        const float y = x == -INFINITY ? -INFINITY : mul(x, kLog2e, 0);
-        keep(n, y, at);
-        stats[n].add(y);
+    // (in most cases: products for which the range rule need not be looked at, and exponentials that the shifts are right for)
+    const auto done = [&](const float (&x)[ROWS], int at) {
+        float* to = place(at);
+        float y[ROWS], z[ROWS], least = 0.0f, most = 0.0f;
+        uint32_t far = 0u;
+#pragma unroll
+        for (int n = 0; n < ROWS; ++n) {
+            far = max(far, beyond(f2i(x[n])));
+            y[n] = i2f(iadd(f2i(x[n]), isub(f2i(kLog2e), kBias)));
+            z[n] = fadd(y[n], -stats[n].shift);
+            least = fminf(least, z[n]);
+            most = fmaxf(most, z[n]);
+        }
+        const bool easy = far < kBand && least >= -126.0f && most < 64.0f;
+#pragma unroll
+        for (int n = 0; n < ROWS; ++n) {
+            if (easy) {
+                stats[n].sum = fadd(stats[n].sum, power(z[n]));
+            } else {
+                y[n] = x[n] == -INFINITY ? -INFINITY : mul(x[n], kLog2e, 0);
+                stats[n].add(y[n]);
+            }
+            if (n < s.rows) to[n * row_pitch] = y[n];
+        }
     };
     // (split: as many pieces as warps take one; the loop runs once, for all warps)
     for (int piece = first; piece * 32 < s.count || (a.split && piece == first); piece += step) {
@@ -356,6 +376,7 @@ __device__ __forceinline__ void key_pass(const Attention& a, const Segment& g, c
             key_stage<ROWS, VEC>(a, sum, ring.to, q + d, pitch, a.dim - d, valid, plain);
             if (a.split) break;
         }
+        float x[ROWS];
         if (a.split) {
 #pragma unroll
             for (int n = 0; n < ROWS; ++n) shared.dealt[(warp * ROWS + n) * 32 + lane] = fadd(sum[n].x, sum[n].y);
@@ -363,15 +384,14 @@ __device__ __forceinline__ void key_pass(const Attention& a, const Segment& g, c
             if (warp % slices != 0) break;
 #pragma unroll
             for (int n = 0; n < ROWS; ++n) {
-                float x = shared.dealt[(warp * ROWS + n) * 32 + lane];
-                for (int w = 1; w < slices; ++w) x = fadd(x, shared.dealt[((warp + w) * ROWS + n) * 32 + lane]);
-                if (valid && n < s.rows) done(n, x, piece * 32 + lane);
+                x[n] = shared.dealt[(warp * ROWS + n) * 32 + lane];
+                for (int w = 1; w < slices; ++w) x[n] = fadd(x[n], shared.dealt[((warp + w) * ROWS + n) * 32 + lane]);
             }
-        } else if (valid) {
+        } else {
 #pragma unroll
-            for (int n = 0; n < ROWS; ++n)
-                if (n < s.rows) done(n, fadd(sum[n].x, sum[n].y), piece * 32 + lane);
+            for (int n = 0; n < ROWS; ++n) x[n] = fadd(sum[n].x, sum[n].y);
         }
+        if (valid) done(x, piece * 32 + lane);
     }
     __pipeline_wait_prior(0);
 }
@@ -400,9 +420,9 @@ __global__ void __launch_bounds__(32 * kMostWarps, 2) key_kernel(const Attention
     enter(a);
     const Share s = share_of(a, g);
     Running stats[ROWS];
-    float* to = a.scores + s.base * a.width + g.first_pos + s.begin;
+    float* to = g.scores + s.base * g.width + (int64_t)s.begin * s.rows;
     key_pass<ROWS, VEC>(a, g, s, ring, reinterpret_cast<int32_t*>(memory + warps * 2 * kKeyBytes), shared, stats,
-                        [&](int n, float y, int at) { to[(int64_t)n * a.width + at] = y; });
+                        [&](int at) { return to + (int64_t)(at / 32) * (32 * s.rows) + at % 32; }, 32);
     if (!a.has_beside) next_may_start();
     leave_stats(shared, stats);
     __syncthreads();
@@ -425,15 +445,14 @@ struct ValueShape {
 template <int SLOTS, int ROWS, bool VEC>
 struct ValueCopies {
     using S = ValueShape<SLOTS, ROWS>;
-    const float *from, *t;                        // the lane's first quad of values, and of t, in the next piece
+    const float *from, *t;                        // the lane's first quad of values in the next piece, and of t of the segment
     int64_t stride;
-    int left, step, rows;
+    int left, step, rows, at;                     // `at`: the next piece's first position
     __device__ __forceinline__ ValueCopies(const Attention& a, const Segment& g, const Share& s, int first, int step_)
-        : stride(g.v_pos), left(s.count - first * S::kPositions), step(step_ * S::kPositions), rows(s.rows) {
+        : stride(g.v_pos), left(s.count - first * S::kPositions), step(step_ * S::kPositions), rows(s.rows), at(s.begin + first * S::kPositions) {
         const int lane = threadIdx.x & 31, l = lane % S::kLanes, sub = lane / S::kLanes;
-        const int at = s.begin + first * S::kPositions;
         from = g.v + s.group * g.v_group + s.row * g.v_row + s.kv_head * g.v_head + (at + sub * 4) * stride + l * 4;
-        t = a.scores + (s.base + lane / (S::kPositions / 4)) * a.width + g.first_pos + at + lane % (S::kPositions / 4) * 4;
+        t = g.scores + s.base * g.width + lane / (S::kPositions / 4) * 32 + lane % (S::kPositions / 4) * 4;
     }
     __device__ __forceinline__ void values(const Attention& a, char* to) const {
         const int lane = threadIdx.x & 31, l = lane % S::kLanes, sub = lane / S::kLanes;
@@ -456,14 +475,14 @@ struct ValueCopies {
     __device__ __forceinline__ void scores(const Attention& a, char* to) const {
         constexpr int kRowQuads = S::kPositions / 4, kRowsAtOnce = 32 / kRowQuads;
         const int lane = threadIdx.x & 31;
-        const float* x = t;
+        const float* x = t + ((int64_t)(at / 32) * (32 * rows) + at % 32);
 #pragma unroll
-        for (int n = 0; n < ROWS; n += kRowsAtOnce, x += (int64_t)kRowsAtOnce * a.width)
+        for (int n = 0; n < ROWS; n += kRowsAtOnce, x += kRowsAtOnce * 32)
             if (n + lane / kRowQuads < rows) __pipeline_memcpy_async(to + S::kScores + n * S::kPositions * 4 + lane * 16, x, 16);
     }
     __device__ __forceinline__ void advance() {
         from += step * stride;
-        t += step;
+        at += step;
         left -= step;
     }
     __device__ __forceinline__ void issue(const Attention& a, Ring<S::kBytes>& ring) {
@@ -492,19 +511,37 @@ __device__ __forceinline__ void value_stage(const Attention& a, int count, int r
     const int lane = threadIdx.x & 31, l = lane % S::kLanes, sub = lane / S::kLanes;
     // t becomes p, as patterns for the products
     int32_t* probs = reinterpret_cast<int32_t*>(slot + S::kScores);
+    constexpr int kTurns = (ROWS * S::kPositions + 31) / 32;
+    float x[kTurns];
+    int32_t easy[kTurns];
     bool odd = count < S::kPositions;                                           // (a part of a stage, or a probability for the range rule)
 #pragma unroll
-    for (int i = 0; i < (ROWS * S::kPositions + 31) / 32; ++i) {
+    for (int i = 0; i < kTurns; ++i) {
         const int at = i * 32 + lane, n = at / S::kPositions;
+        x[i] = 0.0f;
+        easy[i] = 0;
         if (n < rows) {
             const RowStat r = stats[n];
-            const float e = exponential(KEPT ? kept[n * pitch + at % S::kPositions] : i2f(probs[at]), r.shift);
-            const float p = e <= r.flush_max ? 0.0f : e <= r.pass_max ? i2f(isub(f2i(e), r.sub)) : quiet_nan();
-            probs[at] = isub(f2i(p), kBias);
-            odd = odd || beyond(f2i(p)) >= kBand;
+            x[i] = KEPT ? kept[n * pitch + at % S::kPositions] : i2f(probs[at]);
+            const float z = fadd(x[i], -r.shift);
+            easy[i] = isub(exponent(z), r.sub);
+            // (of the pattern's whole exponent, its sign among it: sums reach 2^94)
+            odd = odd || !(z >= -126.0f) || (uint32_t)easy[i] + ((uint32_t)kBias - (66u << 23)) >= ((188u - 66u) << 23);
         }
     }
     const bool plain = !__any_sync(0xffffffffu, odd);
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+        const int at = i * 32 + lane, n = at / S::kPositions;
+        if (n >= rows) continue;
+        if (!plain) {
+            const RowStat r = stats[n];
+            const float e = exponential(x[i], r.shift);
+            const float p = e <= r.flush_max ? 0.0f : e <= r.pass_max ? i2f(isub(f2i(e), r.sub)) : quiet_nan();
+            easy[i] = isub(f2i(p), kBias);
+        }
+        probs[at] = easy[i];
+    }
     __syncwarp();
     probs += sub * 4;
     slot += lane * 16;
@@ -671,13 +708,12 @@ __global__ void __launch_bounds__(32 * kMostWarps, 2) whole_kernel(const Attenti
     using V = ValueShape<SLOTS, ROWS>;
     const int t = threadIdx.x, warp = t >> 5, warps = blockDim.x >> 5;
     char* mine = memory + warp * whole_ring<SLOTS, ROWS>();
-    float* kept = reinterpret_cast<float*>(memory + warps * whole_ring<SLOTS, ROWS>());      // t: [row][width]
+    float* kept = reinterpret_cast<float*>(memory + warps * whole_ring<SLOTS, ROWS>());      // t: [row][width of the segment]
     Ring<kKeyBytes> keys(mine, 0);
     after_previous();
     const Share s = share_of(a, g);
     Running running[ROWS];
-    key_pass<ROWS, VEC>(a, g, s, keys, reinterpret_cast<int32_t*>(kept + ROWS * a.width), shared, running,
-                        [&](int n, float y, int at) { kept[n * a.width + at] = y; });
+    key_pass<ROWS, VEC>(a, g, s, keys, reinterpret_cast<int32_t*>(kept + ROWS * g.width), shared, running, [&](int at) { return kept + at; }, g.width);
     __syncwarp();
     Ring<V::kBytes> ring(mine, 0);
     ValueCopies<SLOTS, ROWS, VEC> copies(a, g, s, warp, warps);
@@ -701,7 +737,7 @@ __global__ void __launch_bounds__(32 * kMostWarps, 2) whole_kernel(const Attenti
         __pipeline_wait_prior(0);
         __syncwarp();
         issue();
-        value_stage<SLOTS, ROWS, VEC, true>(a, s.count - at, s.rows, acc, ring.to, stats, kept + at, a.width);
+        value_stage<SLOTS, ROWS, VEC, true>(a, s.count - at, s.rows, acc, ring.to, stats, kept + at, g.width);
     }
     __pipeline_wait_prior(0);
     store_sums<SLOTS, ROWS>(a, g, s, acc, memory);
@@ -737,7 +773,7 @@ struct Part {                                     // of the shared positions, or
 };
 
 struct Plan {
-    int slots, width, own_first, parts;
+    int slots, width[2], parts;                   // `width`: positions, shared and own, in whole blocks of 32
     Part part[2];
     int64_t all_rows;
     bool whole;                                   // one kernel makes both passes
@@ -781,8 +817,8 @@ Plan plan_of(int64_t groups, int64_t rows, int64_t heads, int64_t kv_heads, int6
     const int share = (int)(heads / kv_heads);
     p.part[0] = part_of(groups * kv_heads, (int)(rows * share), shared, p.slots, dim, vec);
     p.part[1] = part_of(groups * kv_heads * rows, share, own, p.slots, dim, vec);
-    p.own_first = (int)((shared + 31) / 32 * 32);
-    p.width = p.own_first + (int)((own + 31) / 32 * 32);
+    p.width[0] = (int)((shared + 31) / 32 * 32);
+    p.width[1] = (int)((own + 31) / 32 * 32);
     p.parts = p.part[0].ranks + p.part[1].ranks;
     p.all_rows = groups * rows * heads;
     p.whole = p.parts == 1 && shared + own <= kMostKept;
@@ -790,7 +826,7 @@ Plan plan_of(int64_t groups, int64_t rows, int64_t heads, int64_t kv_heads, int6
 }
 
 size_t aligned(size_t n) { return (n + 255) / 256 * 256; }
-size_t score_bytes(const Plan& p) { return aligned((size_t)p.all_rows * p.width * 4); }
+size_t score_bytes(const Plan& p) { return aligned((size_t)p.all_rows * ((size_t)p.width[0] + p.width[1]) * 4); }
 size_t stat_bytes(const Plan& p) { return aligned((size_t)p.all_rows * p.parts * 8); }
 size_t bytes_of(const Plan& p, int64_t dim) { return p.whole ? 0 : score_bytes(p) + stat_bytes(p) + (p.parts > 1 ? aligned((size_t)(p.all_rows * p.parts * dim) * 4) : 0); }
 
@@ -832,7 +868,7 @@ int launch_slots(const Part& p, const Attention& a, const Segment& g, cudaStream
 
 template <int SLOTS, int ROWS, bool VEC>
 int launch_whole(const Part& p, const Attention& a, const Segment& g, cudaStream_t st) {
-    const size_t memory = (size_t)p.whole_warps * whole_ring<SLOTS, ROWS>() + (size_t)ROWS * (a.width + (a.dim + 31) / 32 * 32) * 4;
+    const size_t memory = (size_t)p.whole_warps * whole_ring<SLOTS, ROWS>() + (size_t)ROWS * (g.width + (a.dim + 31) / 32 * 32) * 4;
     return launch(whole_kernel<SLOTS, ROWS, VEC>, p.ctas, p.whole_warps, std::max(memory, (size_t)p.whole_warps * ROWS * padded(a.dim) * 4), a, g, st);
 }
 
@@ -923,13 +959,14 @@ int pamk_cached_attention(const float* q, float* out, const float* shared_k, con
     const size_t bytes = bytes_of(p, dim);
     if (bytes && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < bytes)) return PAMK_ERR_WORKSPACE;
     char* ws = static_cast<char*>(workspace);
-    a.scores = reinterpret_cast<float*>(ws);
+    g[0].scores = reinterpret_cast<float*>(ws);
+    g[1].scores = g[0].scores + p.all_rows * p.width[0];
+    g[0].width = p.width[0];
+    g[1].width = p.width[1];
     a.stats = reinterpret_cast<float2*>(ws + score_bytes(p));
     if (p.parts > 1) a.sums = reinterpret_cast<float*>(ws + score_bytes(p) + stat_bytes(p));
-    a.width = p.width;
     a.one = 1; a.least = INT32_MIN;
     a.parts = p.parts;
-    g[1].first_pos = p.own_first;
     g[1].first_part = p.part[0].ranks;
     if (p.whole) {
         const int i = shared ? 0 : 1;
