@@ -347,21 +347,30 @@ __device__ __forceinline__ void key_pass(const Attention& a, const Segment& g, c
         for (int n = 0; n < ROWS; ++n) {
             far = max(far, beyond(f2i(x[n])));
             y[n] = i2f(iadd(f2i(x[n]), isub(f2i(kLog2e), kBias)));
+        }
+        if (at < 32 * step && far < kBand) {                                     // (the lane's first position)
+#pragma unroll
+            for (int n = 0; n < ROWS; ++n) stats[n].shift = floorf(y[n]);
+        }
+#pragma unroll
+        for (int n = 0; n < ROWS; ++n) {
             z[n] = fadd(y[n], -stats[n].shift);
             least = fminf(least, z[n]);
             most = fmaxf(most, z[n]);
         }
-        const bool easy = far < kBand && least >= -126.0f && most < 64.0f;
+        if (far < kBand && least >= -126.0f && most < 64.0f) {
 #pragma unroll
-        for (int n = 0; n < ROWS; ++n) {
-            if (easy) {
-                stats[n].sum = fadd(stats[n].sum, power(z[n]));
-            } else {
+            for (int n = 0; n < ROWS; ++n) stats[n].sum = fadd(stats[n].sum, power(z[n]));
+        } else {
+#pragma unroll
+            for (int n = 0; n < ROWS; ++n) {
                 y[n] = x[n] == -INFINITY ? -INFINITY : mul(x[n], kLog2e, 0);
                 stats[n].add(y[n]);
             }
-            if (n < s.rows) to[n * row_pitch] = y[n];
         }
+#pragma unroll
+        for (int n = 0; n < ROWS; ++n)
+            if (n < s.rows) to[n * row_pitch] = y[n];
     };
     // (split: as many pieces as warps take one; the loop runs once, for all warps)
     for (int piece = first; piece * 32 < s.count || (a.split && piece == first); piece += step) {
@@ -456,21 +465,25 @@ struct ValueCopies {
     }
     __device__ __forceinline__ void values(const Attention& a, char* to) const {
         const int lane = threadIdx.x & 31, l = lane % S::kLanes, sub = lane / S::kLanes;
-        const bool whole = VEC && left >= S::kPositions && a.dim == 4 * S::kLanes * S::kCols;
         const float* p = from;
         to += lane * 16;
+        const auto each = [&](auto&& one) {
 #pragma unroll
-        for (int m = 0; m < S::kTimes; ++m) {
+            for (int m = 0; m < S::kTimes; ++m) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u, p += stride)
+                for (int u = 0; u < 4; ++u, p += stride)
 #pragma unroll
-                for (int c = 0; c < S::kCols; ++c) {
-                    const int d = (l + S::kLanes * c) * 4;
-                    if (whole || (m * 4 * S::kAcross + sub * 4 + u < left && d < a.dim))
-                        copy_quad<VEC>(to + ((m * 4 + u) * S::kCols + c) * 512, p + S::kLanes * 4 * c, d, a.dim);
-                }
-            p += (4 * S::kAcross - 4) * stride;
-        }
+                    for (int c = 0; c < S::kCols; ++c)
+                        one(to + ((m * 4 + u) * S::kCols + c) * 512, p + S::kLanes * 4 * c, m * 4 * S::kAcross + sub * 4 + u, (l + S::kLanes * c) * 4);
+                p += (4 * S::kAcross - 4) * stride;
+            }
+        };
+        if (VEC && left >= S::kPositions && a.dim == 4 * S::kLanes * S::kCols)
+            each([&](char* at, const float* x, int, int) { copy_quad<true>(at, x, 0, 4); });
+        else
+            each([&](char* at, const float* x, int position, int d) {
+                if (position < left && d < a.dim) copy_quad<VEC>(at, x, d, a.dim);
+            });
     }
     __device__ __forceinline__ void scores(const Attention& a, char* to) const {
         constexpr int kRowQuads = S::kPositions / 4, kRowsAtOnce = 32 / kRowQuads;
@@ -517,31 +530,28 @@ __device__ __forceinline__ void value_stage(const Attention& a, int count, int r
     bool odd = count < S::kPositions;                                           // (a part of a stage, or a probability for the range rule)
 #pragma unroll
     for (int i = 0; i < kTurns; ++i) {
-        const int at = i * 32 + lane, n = at / S::kPositions;
-        x[i] = 0.0f;
-        easy[i] = 0;
-        if (n < rows) {
-            const RowStat r = stats[n];
-            x[i] = KEPT ? kept[n * pitch + at % S::kPositions] : i2f(probs[at]);
-            const float z = fadd(x[i], -r.shift);
-            easy[i] = isub(exponent(z), r.sub);
-            // (of the pattern's whole exponent, its sign among it: sums reach 2^94)
-            odd = odd || !(z >= -126.0f) || (uint32_t)easy[i] + ((uint32_t)kBias - (66u << 23)) >= ((188u - 66u) << 23);
-        }
+        const int at = i * 32 + lane;
+        const bool there = at < rows * S::kPositions;
+        const int n = there ? at / S::kPositions : 0;
+        x[i] = KEPT ? kept[n * pitch + at % S::kPositions] : i2f(probs[there ? at : 0]);
+        const float z = fadd(x[i], -stats[n].shift);
+        easy[i] = isub(exponent(z), stats[n].sub);
+        // (of the pattern's whole exponent, its sign among it: sums reach 2^94)
+        odd = odd || (there && (!(z >= -126.0f) || (uint32_t)easy[i] + ((uint32_t)kBias - (66u << 23)) >= ((188u - 66u) << 23)));
     }
     const bool plain = !__any_sync(0xffffffffu, odd);
+    if (!plain)
 #pragma unroll
-    for (int i = 0; i < kTurns; ++i) {
-        const int at = i * 32 + lane, n = at / S::kPositions;
-        if (n >= rows) continue;
-        if (!plain) {
-            const RowStat r = stats[n];
+        for (int i = 0; i < kTurns; ++i) {
+            const int at = i * 32 + lane;
+            const RowStat r = stats[at < rows * S::kPositions ? at / S::kPositions : 0];
             const float e = exponential(x[i], r.shift);
             const float p = e <= r.flush_max ? 0.0f : e <= r.pass_max ? i2f(isub(f2i(e), r.sub)) : quiet_nan();
             easy[i] = isub(f2i(p), kBias);
         }
-        probs[at] = easy[i];
-    }
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i)
+        if (i * 32 + lane < rows * S::kPositions) probs[i * 32 + lane] = easy[i];
     __syncwarp();
     probs += sub * 4;
     slot += lane * 16;
