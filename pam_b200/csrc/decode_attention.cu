@@ -710,8 +710,10 @@ constexpr int kMostKept = 256;
 template <int SLOTS, int ROWS>
 __host__ __device__ constexpr int whole_ring() { return 2 * (ValueShape<SLOTS, ROWS>::kBytes > kKeyBytes ? ValueShape<SLOTS, ROWS>::kBytes : kKeyBytes); }
 
+// (One or two rows need few enough registers for half as many warps again on an SM, and so more copies on their way: 128 x 5 rows of 4 heads of 128 floats with up
+// to 64 own positions 32.8 -> 28.9 us.  The kernels of one pass each gain nothing from that, 60001 positions of one row 57 -> 60.)
 template <int SLOTS, int ROWS, bool VEC>
-__global__ void __launch_bounds__(32 * kMostWarps, 2) whole_kernel(const Attention a, const Segment g) {
+__global__ void __launch_bounds__(32 * kMostWarps, ROWS <= 2 ? 3 : 2) whole_kernel(const Attention a, const Segment g) {
     extern __shared__ __align__(16) char memory[];
     __shared__ KeyMemory<ROWS> shared;
     __shared__ RowStat stats[ROWS];
