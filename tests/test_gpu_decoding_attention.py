@@ -195,3 +195,24 @@ def test_captured_graphs_share_nothing():
     graphs[1].replay()
     _check(outs[0], **cases[0])
     assert torch.equal(outs[1], want[1])
+
+
+@pytest.mark.parametrize("own", [False, True])
+def test_far_above_the_first_scores(own):
+    """Sums of 2^70 and more, shifted by what came first, beside exponentials near 2^-126: those are probabilities of zero."""
+    first, high, low = 1.0, 50.25, -96.25                  # t: 1.4, 64.8 (above its floor by less than 64) and -124.6 (below it by less than 126)
+    t = [float(oracle.pam(s, oracle.LOG2E)) for s in (first, high, low)]
+    assert 1 <= t[0] < 2 and 64 <= t[1] < 65 and -125 <= t[2] < -124
+    position = torch.arange(1000)
+    s = torch.where(position // 32 % 8 < 4, first, high)
+    s[position % 32 == 5] = torch.where(position // 32 % 8 < 4, first, low)[position % 32 == 5]
+    k = torch.zeros(1000, 8)
+    k[:, 0] = s
+    v = torch.randn(1000, 8, generator=torch.Generator().manual_seed(50))
+    v[s == low] = 2.0 ** 60
+    q = torch.zeros(1, 1, 1, 8, device=DEV)
+    q[..., 0] = 1.0
+    name = "own" if own else "shared"
+    lead = (1, 1, 1000, 1, 8) if own else (1, 1000, 1, 8)
+    case = {"q": q, f"{name}_k": k.view(lead).to(DEV), f"{name}_v": v.view(lead).to(DEV)}
+    _check(_run(case), **case)
