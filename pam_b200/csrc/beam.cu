@@ -79,6 +79,9 @@ __device__ __forceinline__ double term(float t, float shift) {
 __device__ __forceinline__ uint32_t beyond(float x) { return 2u * (uint32_t)f2i(x) - 2u * (66u << 23); }
 constexpr uint32_t kBand = 2u * ((188u - 66u) << 23);
 
+// Below kNear where |x| lies in [2^-61, 64): t 2^23 and the pattern of a term are then within 32 bits.
+constexpr uint32_t kNear = 2u * ((133u - 66u) << 23);
+
 constexpr int kWarps = kThreads / 32, kQuads = kEach / 4;
 static_assert(kWarps == 8 && kQuads == 4);
 constexpr int kMany = 512;                            // so many candidates are narrowed down by their full keys first
@@ -110,11 +113,12 @@ __global__ void __launch_bounds__(kThreads, 4) pick_kernel(const Select a) {
         const int j = start(i);
         v[i] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);           // (masked, where there is nothing)
         flags[i] = 0u;
-        if (j >= begin && j + 4 <= end) {
-            v[i] = __ldcs(reinterpret_cast<const float4*>(x + j));
-            if (by_four) flags[i] = *reinterpret_cast<const uint32_t*>(banned + j);
-        }
+        if (j >= begin && j + 4 <= end) v[i] = __ldcs(reinterpret_cast<const float4*>(x + j));
     }
+    if (by_four)
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i)
+            if (start(i) >= begin && start(i) + 4 <= end) flags[i] = *reinterpret_cast<const uint32_t*>(banned + start(i));
     // the two vectors that the range may cut
     const auto cut = [&](int i) {
         const int j = start(i);
@@ -168,20 +172,30 @@ __global__ void __launch_bounds__(kThreads, 4) pick_kernel(const Select a) {
     const float shift = top > kMasked ? floorf(mul(top, kLog2e, 0)) : -INFINITY;
     const int32_t by = isub(f2i(kLog2e), kBias);
     double total = 0.0;
+    uint32_t far[kQuads];
 #pragma unroll
-    for (int i = 0; i < kQuads; ++i) {
-        if (start(i) >= end) continue;
-        const uint32_t far = max(max(beyond(v[i].x), beyond(v[i].y)), max(beyond(v[i].z), beyond(v[i].w)));
-        if (far < kBand) {
-            const double s01 = term(i2f(iadd(f2i(v[i].x), by)), shift) + term(i2f(iadd(f2i(v[i].y), by)), shift);
-            total += s01 + (term(i2f(iadd(f2i(v[i].z), by)), shift) + term(i2f(iadd(f2i(v[i].w), by)), shift));
-        } else {
+    for (int i = 0; i < kQuads; ++i) far[i] = max(max(beyond(v[i].x), beyond(v[i].y)), max(beyond(v[i].z), beyond(v[i].w)));
+    if (__all_sync(0xffffffffu, max(max(far[0], far[1]), max(far[2], far[3])) < kNear)) {
+        // (a term's exponent is the whole part of t - shift, its mantissa the fraction, rounded once; what is below 2^-126 is as good as nothing)
+        const int32_t least_exponent = isub(kBias, (int)shift << 23);
+        const auto near_term = [&](float y) { return (double)i2f(__viaddmax_s32(__float2int_rn(i2f(iadd(f2i(y), by + (23 << 23)))), least_exponent, 0)); };
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i) total += (near_term(v[i].x) + near_term(v[i].y)) + (near_term(v[i].z) + near_term(v[i].w));
+    } else {
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i) {
+            if (start(i) >= end) continue;
+            if (far[i] < kBand) {
+                const double s01 = term(i2f(iadd(f2i(v[i].x), by)), shift) + term(i2f(iadd(f2i(v[i].y), by)), shift);
+                total += s01 + (term(i2f(iadd(f2i(v[i].z), by)), shift) + term(i2f(iadd(f2i(v[i].w), by)), shift));
+            } else {
 #pragma unroll 1
-            for (int e = 0; e < 4; ++e) {
-                const float y = value(i, e);
-                if (!(y <= kMasked)) {
-                    const float s = mul(y, kLog2e, 0);
-                    total += s == s && shift > -INFINITY ? term(s, shift) : (double)quiet_nan();       // (NaN, or too large)
+                for (int e = 0; e < 4; ++e) {
+                    const float y = value(i, e);
+                    if (!(y <= kMasked)) {
+                        const float s = mul(y, kLog2e, 0);
+                        total += s == s && shift > -INFINITY ? term(s, shift) : (double)quiet_nan();       // (NaN, or too large)
+                    }
                 }
             }
         }
