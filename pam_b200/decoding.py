@@ -19,6 +19,11 @@ MAX_BEAMS = 64
 MAX_SELECTED = 64
 
 
+def _not_traced(what):
+    if torch.jit.is_tracing():
+        raise RuntimeError(f"{what} cannot be traced: its result would be recorded as a constant")
+
+
 def _no_backward(what, *tensors):
     given = [t for t in tensors if t is not None]
     if torch.is_grad_enabled() and any(t.requires_grad for t in given) or any(forward_ad.unpack_dual(t).tangent is not None for t in given):
@@ -82,6 +87,7 @@ def cached_attention(q, own_k=None, own_v=None, own_lengths=None, *, shared_k=No
         out = host.cached_attention(q, own_k, own_v, own_lengths, shared_k, shared_v, shared_lengths)
         if out is not None:
             return out
+    _not_traced("cached_attention")
     _fp32("queries", q, 4)
     groups, rows, heads, dim = q.shape
     if own_k is None and shared_k is None:
@@ -135,6 +141,7 @@ def beam_select(logits, scores, k, banned=None):
         out = host.beam_select(logits, scores, k, banned)
         if out is not None:
             return out
+    _not_traced("beam_select")
     _fp32("logits", logits, 3)
     _fp32("scores", scores, 2)
     groups, beams, vocab = logits.shape
@@ -214,6 +221,7 @@ def reorder_states(states, parents, used=None):
     states = list(states)
     if (host := _lib.host()) is not None and host.reorder_states(states, parents, used):
         return
+    _not_traced("reorder_states")
     if not isinstance(parents, torch.Tensor) or parents.dtype != torch.int64 or parents.dim() != 2:
         raise ValueError("parents must be an int64 tensor [groups, beams]")
     groups, rows = parents.shape

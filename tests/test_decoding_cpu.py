@@ -144,3 +144,12 @@ def test_positions_beyond_32_bits():
         assert h.pamk_cached_attention_workspace_bytes(*sizes) == 0
         assert h.pamk_cached_attention(one, one, one, one, None, one, one, None, *sizes, strides, None, 0, None) == -2
     assert h.pamk_cached_attention_workspace_bytes(1, 1, 1, 1, 4, 1 << 29, 1 << 29) > (1 << 30) * 4
+
+
+def test_not_traced():
+    k = torch.zeros(1, 1, 3, 1, 8)
+    parents = torch.zeros(1, 2, dtype=torch.int64)
+    for call, arg in ((lambda q: decoding.cached_attention(q, k, k), torch.zeros(1, 1, 1, 8)), (lambda x: decoding.beam_select(x, torch.zeros(1, 2), 2), torch.zeros(1, 2, 5)),
+                      (lambda x: decoding.reorder_states([x], parents), torch.zeros(1, 2, 5))):
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(call, (arg,))
