@@ -94,10 +94,9 @@ __global__ void __launch_bounds__(kThreads, 4) pick_kernel(const Select a) {
     __shared__ unsigned long long warp_key[kWarps];
     __shared__ int count, live;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const unsigned beam = blockIdx.x / (unsigned)a.parts, group = beam / (unsigned)a.rows, row = beam - group * a.rows;
-    const int part = (int)(blockIdx.x - beam * a.parts);
+    const unsigned beam = blockIdx.x, group = beam / (unsigned)a.rows, row = beam - group * a.rows;
     after_previous();
-    const int begin = part * a.part, end = min(begin + a.part, a.vocab);
+    const int begin = (int)blockIdx.y * a.part, end = min(begin + a.part, a.vocab);
     const float score = a.scores[beam];
     const float* x = a.logits + group * a.x_group + row * a.x_row;
     const unsigned char* banned = a.banned ? a.banned + group * a.ban_group + row * a.ban_row : nullptr;
@@ -107,18 +106,19 @@ __global__ void __launch_bounds__(kThreads, 4) pick_kernel(const Select a) {
     float4 v[kQuads];
     uint32_t flags[kQuads];                                                       // a byte for each of the four: banned
     const auto start = [&](int i) { return first + (i * kThreads + t) * 4; };
+    const auto whole = [&](int i) { return (i > 0 || start(i) >= begin) && start(i) <= end - 4; };
     const bool by_four = banned && (reinterpret_cast<uintptr_t>(banned + first) & 3) == 0;
 #pragma unroll
     for (int i = 0; i < kQuads; ++i) {
         const int j = start(i);
         v[i] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);           // (masked, where there is nothing)
         flags[i] = 0u;
-        if (j >= begin && j + 4 <= end) v[i] = __ldcs(reinterpret_cast<const float4*>(x + j));
+        if (whole(i)) v[i] = __ldcs(reinterpret_cast<const float4*>(x + j));
     }
     if (by_four)
 #pragma unroll
         for (int i = 0; i < kQuads; ++i)
-            if (start(i) >= begin && start(i) + 4 <= end) flags[i] = *reinterpret_cast<const uint32_t*>(banned + start(i));
+            if (whole(i)) flags[i] = *reinterpret_cast<const uint32_t*>(banned + start(i));
     // the two vectors that the range may cut
     const auto cut = [&](int i) {
         const int j = start(i);
@@ -127,17 +127,18 @@ __global__ void __launch_bounds__(kThreads, 4) pick_kernel(const Select a) {
         if (j + 2 >= begin && j + 2 < end) v[i].z = x[j + 2];
         if (j + 3 >= begin && j + 3 < end) v[i].w = x[j + 3];
     };
-    if (t == 0 && first < begin) cut(0);
     const int last = (end - first) / 4;
-    if (((end - first) & 3) != 0 && t == last % kThreads)
+    const bool cuts_first = t == 0 && first < begin, cuts_last = ((end - first) & 3) != 0 && t == last % kThreads;
+    if (cuts_first) cut(0);
+    if (cuts_last)
 #pragma unroll
         for (int i = 0; i < kQuads; ++i)
             if (i == last / kThreads) cut(i);
-    if (banned)
+    if (banned && (!by_four || cuts_first || cuts_last))
 #pragma unroll
         for (int i = 0; i < kQuads; ++i) {
             const int j = start(i);
-            if (j < end && !(by_four && j >= begin && j + 4 <= end))
+            if (j < end && !(by_four && whole(i)))
 #pragma unroll 1
                 for (int e = 0; e < 4; ++e)
                     if (j + e >= begin && j + e < end && banned[j + e]) flags[i] |= 1u << (8 * e);
@@ -270,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, 4) pick_kernel(const Select a) {
                 if (key(i, e) >= from) push(key(i, e));
         __syncthreads();
     }
-    const int64_t list = blockIdx.x;
+    const int64_t list = (int64_t)beam * a.parts + blockIdx.y;
     if (t == 0) {
         float m = warp_shift[0];
         for (int w = 1; w < kWarps; ++w) m = fmaxf(m, warp_shift[w]);
@@ -587,7 +588,7 @@ int pamk_beam_select(const float* logits, const float* scores, const unsigned ch
     ws += aligned((size_t)(groups * lists) * 4);
     a.lists = reinterpret_cast<unsigned long long*>(ws);
     a.out_scores = out_scores; a.out_beams = out_beams; a.out_tokens = out_tokens;
-    const int status = launch_behind(pick_kernel, dim3((unsigned)(groups * lists)), kThreads, st, a);
+    const int status = launch_behind(pick_kernel, dim3((unsigned)(groups * rows), (unsigned)parts), kThreads, st, a);
     if (status != PAMK_OK) return status;
     return lists * k <= kMostKept ? launch_merge(merge_kernel<true>, groups, merge_bytes(rows, parts, k), a, st)
                                   : launch_merge(merge_kernel<false>, groups, merge_bytes(rows, parts, k), a, st);
