@@ -58,7 +58,7 @@ struct Attention {
     float2* stats;                                // [(group, key head, row, head of the key head)][parts]: a whole number near the maximum, the sum of exponentials shifted by it
     float* sums;                                  // [the same][parts][dim], or null: straight to out
     int parts;
-    int one, least;                               // 1 and INT32_MIN, as values that the compiler does not know (see sum_on_alu)
+    int two, one, least;                          // 2, 1 and INT32_MIN, as values that the compiler does not know (see sum_on_alu)
 };
 
 // A packed add takes both floating-point pipes of an SM partition for as long as an integer add takes the integer pipe, and a multiply-add can stand for an
@@ -76,6 +76,14 @@ __device__ __forceinline__ int sum_on_fma(int x, int y, int one) {
 __device__ __forceinline__ uint32_t beyond(int32_t x) { return 2u * (uint32_t)x - 2u * (66u << 23); }
 constexpr uint32_t kBand = 2u * ((188u - 66u) << 23);
 __device__ __forceinline__ uint32_t beyond(int4 x) { return max(max(beyond(x.x), beyond(x.y)), max(beyond(x.z), beyond(x.w))); }
+
+// (as a multiply-add, beside the sums on the integer pipe: 1 %)
+__device__ __forceinline__ uint32_t beyond(int32_t x, int two) {
+    uint32_t d;
+    asm("mad.lo.u32 %0, %1, %2, %3;" : "=r"(d) : "r"(x), "r"(two), "r"(0u - 2u * (66u << 23)));
+    return d;
+}
+__device__ __forceinline__ uint32_t beyond(int4 x, int two) { return max(max(beyond(x.x, two), beyond(x.y, two)), max(beyond(x.z, two), beyond(x.w, two))); }
 
 __device__ __forceinline__ void add_pair(float2& acc, int p0, int p1) { acc = __fadd2_rn(acc, make_float2(i2f(p0), i2f(p1))); }
 
@@ -260,7 +268,7 @@ __device__ __forceinline__ void key_stage(const Attention& a, float2 (&sum)[ROWS
 #pragma unroll
         for (int c = 0; c < kQuads; ++c) {
             k[c] = quad(c);
-            far = max(far, beyond(k[c]));
+            far = max(far, beyond(k[c], a.two));
         }
         if (__all_sync(0xffffffffu, plain && (far < kBand || !valid))) {
 #pragma unroll
@@ -575,7 +583,7 @@ __device__ __forceinline__ void value_stage(const Attention& a, int count, int r
                     if (d + 2 >= a.dim) x.z = kBias;
                     if (d + 3 >= a.dim) x.w = kBias;
                 }
-                far = max(far, !VEC || d < a.dim ? beyond(x) : 0u);
+                far = max(far, !VEC || d < a.dim ? beyond(x, a.two) : 0u);
             }
         if (__all_sync(0xffffffffu, plain && far < kBand)) {
 #pragma unroll
@@ -982,7 +990,7 @@ int pamk_cached_attention(const float* q, float* out, const float* shared_k, con
     g[1].width = p.width[1];
     a.stats = reinterpret_cast<float2*>(ws + score_bytes(p));
     if (p.parts > 1) a.sums = reinterpret_cast<float*>(ws + score_bytes(p) + stat_bytes(p));
-    a.one = 1; a.least = INT32_MIN;
+    a.two = 2; a.one = 1; a.least = INT32_MIN;
     a.parts = p.parts;
     g[1].first_part = p.part[0].ranks;
     if (p.whole) {
