@@ -345,7 +345,8 @@ class Transformer(nn.Module):
         src [sentences, length], padded behind `src_lengths` where these are given.  At most `max_len` tokens come out, the end of
         sentence `eos` among them (forced at the last one, not before the `min_len`-th).  Returns (tokens [sentences, beam, n], scores
         [sentences, beam]), best first; a hypothesis' score is its log-probability over its length to the power of
-        `length_penalty`, -inf (and padding alone) where there were fewer; tokens behind the end are padding.
+        `length_penalty`, -inf (and padding alone) where there were fewer; tokens behind the end are padding.  A sentence that has its `beam`
+        hypotheses keeps them while others of the batch go on: in a batch it gets what it gets alone, up to rounding.
 
         The source's keys and values are kept once for the beams of a sentence, which attend to them together; each beam's own go where
         the beam goes on."""
@@ -386,14 +387,15 @@ class Transformer(nn.Module):
             done = torch.where(ends & (rank < beam), found / (t + 1) ** length_penalty, float("-inf"))
             longer = tokens.gather(1, parents.unsqueeze(-1).expand(-1, -1, max_len))
             longer[:, :, t] = chosen
-            best, at = torch.cat([best, done], 1).topk(beam, 1)
+            best, at = (x[:, :beam] for x in torch.cat([best, done], 1).sort(dim=1, descending=True, stable=True))
             best_tokens = torch.cat([best_tokens, longer], 1).gather(1, at.unsqueeze(-1).expand(-1, -1, max_len))
-            if t == max_len - 1 or bool((best > float("-inf")).all()):
+            finished = (best > float("-inf")).all(1, keepdim=True)
+            if t == max_len - 1 or bool(finished.all()):
                 break
-            # the first `beam` others go on
+            # the first `beam` others go on; none of a finished sentence, which finds no more ends then
             go = (rank + count * ends).argsort(1)[:, :beam]
             scores, parents, last = (v.gather(1, go) for v in (found, parents, chosen))
-            scores = scores.masked_fill(ends.gather(1, go), float("-inf"))
+            scores = scores.masked_fill(ends.gather(1, go) | finished, float("-inf"))
             _reorder(caches, parents, t + 1)
             _reorder([tokens], parents, t)
             tokens[:, :, t] = last
