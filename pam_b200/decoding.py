@@ -183,6 +183,21 @@ def _span(t):
     return start, start + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
 
 
+def _rows_meet(apart, size, other, by_group, by_row, groups, rows):
+    """Whether a row of `size` bytes of one state and a row of `other` bytes of another meet that lies `apart` bytes behind and has the same strides (two parts of
+    one buffer, interleaved row by row, do not): whether apart + i by_group + j by_row is between -other and size for some differences i of groups and j
+    of rows."""
+    for j in range(1 - rows, rows):
+        at = apart + j * by_row
+        if groups == 1 or by_group == 0:
+            i = 0
+        else:
+            i = max((-other - at) // by_group + 1, 1 - groups)                             # the first group that ends behind the row's start
+        if i < groups and -other < at + i * by_group < size:
+            return True
+    return False
+
+
 def _refuse_overlaps(states, moved, parents, used=None):
     """No two rows that move may share memory, neither of one tensor nor of two, and what says how they move may not lie in them."""
     spans = []
@@ -192,8 +207,7 @@ def _refuse_overlaps(states, moved, parents, used=None):
                   (rows == 1 or by_row >= (groups - 1) * by_group + size) and (groups == 1 or by_group >= size))
         if not nested:
             raise ValueError(f"rows of a state of shape {tuple(t.shape)} and strides {t.stride()} overlap")
-        steps = [s for s, n in ((by_group, groups), (by_row, rows)) if n > 1]
-        spans.append((*_span(t), size, (by_group, by_row), min(steps, default=None)))
+        spans.append((*_span(t), size, (by_group, by_row), (groups, rows)))
     spans.sort(key=lambda s: s[:2])
     read = [_span(t) for t in (parents, used) if t is not None]
     reach = []                                            # spans that may reach into the next one
@@ -202,9 +216,7 @@ def _refuse_overlaps(states, moved, parents, used=None):
             raise ValueError("the parents, or the number of positions, lie in the memory of a state")
         reach = [r for r in reach if r[1] > s[0]]
         for r in reach:
-            # (two parts of one buffer, interleaved row by row, are fine)
-            apart = s[0] - r[0]
-            if not (r[3] == s[3] and r[4] is not None and apart >= r[2] and apart + s[2] <= r[4]):
+            if r[3] != s[3] or _rows_meet(s[0] - r[0], r[2], s[2], *s[3], *s[4]):
                 raise ValueError("two states share memory")
         reach.append(s)
 
