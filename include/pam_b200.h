@@ -348,7 +348,8 @@ int pamk_cached_attention(const float* q, float* out,
  * token.  Logits of -1e30 or less (-inf among them) are masked: no share in the sum, value -inf.  banned[j] != 0 (NULL: none; strides
  * 0 share a row of flags): in the sum, value -inf.  A beam whose score is -inf or NaN, or whose sum is not finite, has value -inf for every
  * token; the logits of one with such a score are not read.  Token strides are 1; scores [groups, rows]; outputs [groups, k].
- * rows <= 64, k <= 64, k <= rows * vocab.  `workspace`: pamk_beam_select_workspace_bytes(...) bytes, 256-byte aligned. */
+ * rows <= 64, k <= 64, k <= rows * vocab; rows * ceil(vocab / 4092) <= 4096, and groups times that below 2^31.
+ * `workspace`: pamk_beam_select_workspace_bytes(...) bytes, 256-byte aligned. */
 size_t pamk_beam_select_workspace_bytes(int64_t groups, int64_t rows, int64_t vocab, int64_t k);
 int pamk_beam_select(const float* logits, const float* scores, const unsigned char* banned,
                      float* out_scores, int64_t* out_beams, int64_t* out_tokens,

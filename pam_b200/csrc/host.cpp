@@ -902,7 +902,7 @@ std::optional<std::array<Tensor, 3>> op_beam_select(const Tensor& logits, const 
     if (!usable(logits) || !usable(scores) || logits.dim() != 3 || scores.dim() != 2 || scores.device() != logits.device() || logits.numel() == 0) return {};
     if (scores.sizes() != logits.sizes().slice(0, 2) || !scores.is_contiguous() || logits.stride(2) != 1 || wants_grad(logits) || wants_grad(scores)) return {};
     const int64_t G = logits.size(0), R = logits.size(1), V = logits.size(2);
-    if (R > 64 || k < 1 || k > 64 || k > R * V) return {};
+    if (R > 64 || k < 1 || k > 64 || k > R * V || R * ((V + 4091) / 4092) > 4096) return {};
     int64_t ban[2] = {0, 0};
     if (banned.defined()) {
         if (!readable(banned) || banned.scalar_type() != at::kBool || banned.device() != logits.device() || banned.dim() < 1 || banned.dim() > 3 ||

@@ -17,6 +17,7 @@ from . import _lib
 MAX_HEAD_DIM = 256
 MAX_BEAMS = 64
 MAX_SELECTED = 64
+_RANGE, _MAX_RANGES = 4092, 4096                # a beam's logits are worked on in ranges of so many; so many ranges may a group have
 
 
 def _not_traced(what):
@@ -136,7 +137,8 @@ def beam_select(logits, scores, k, banned=None):
     PAM log-softmax, the beam each continues (int64) and its token (int64).  Values are formed and compared in 64 bits; equal
     ones go to the lower beam, then to the lower token.  Logits of -1e30 or less, -inf among them, are masked: they have no
     share in the probability.  Masked and banned tokens and the tokens of beams that are not continued have score -inf and come
-    last, also where a beam's logits hold NaN or overflow.  Up to 64 beams and k up to 64."""
+    last, also where a beam's logits hold NaN or overflow.  Up to 64 beams and k up to 64; beams times the vocabulary in ranges of 4092 tokens, the last
+    one rounded up, up to 4096 (64 beams of 261888 tokens)."""
     if (host := _lib.host()) is not None:
         out = host.beam_select(logits, scores, k, banned)
         if out is not None:
@@ -151,6 +153,8 @@ def beam_select(logits, scores, k, banned=None):
         raise ValueError(f"k must be a number from 1 to {min(MAX_SELECTED, beams * vocab)}, got {k!r}")
     if beams > MAX_BEAMS:
         raise ValueError(f"{beams} beams are more than {MAX_BEAMS}")
+    if beams * -(-vocab // _RANGE) > _MAX_RANGES:
+        raise ValueError(f"{beams} beams of {vocab} tokens are more than {_MAX_RANGES} ranges of {_RANGE}")
     _no_backward("beam_select", logits, scores)
     dev = _lib.require_cuda(logits, scores, banned)
     if banned is not None:
