@@ -331,7 +331,7 @@ int pamk_adam_step(float* const* p, const float* const* g, float* const* m, floa
  *   q: group, row, head;  shared_k: group, position, head;  shared_v: the same three;
  *   own_k: group, row, position, head;  own_v: the same four.
  * out is contiguous [groups, rows, heads, dim]; own_lengths contiguous [groups, rows].  dim <= 256.
- * shared + own <= 2^30.
+ * shared + own <= 2^30, rows * heads <= 2^20, groups * rows * heads * (2 + (shared + own) / 64) < 2^31.
  * `workspace`: pamk_cached_attention_workspace_bytes(...) bytes, 256-byte aligned; NULL where that is 0. */
 size_t pamk_cached_attention_workspace_bytes(int64_t groups, int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim,
                                              int64_t shared, int64_t own);

@@ -35,6 +35,7 @@
 #include <algorithm>
 #include <array>
 #include <atomic>
+#include <limits>
 #include <map>
 #include <mutex>
 #include <optional>
@@ -876,6 +877,7 @@ std::optional<Tensor> op_cached_attention(const Tensor& q, const Tensor& own_k, 
         return {};
     if (own_k.defined() && shared_k.defined() && own_k.size(3) != shared_k.size(2)) return {};
     const int64_t K = own_k.defined() ? own_k.size(3) : shared_k.size(2);
+    if (R * H > 1 << 20 || shared + own > 1 << 30 || G * R * H > std::numeric_limits<int32_t>::max() / (2 + (shared + own) / 64)) return {};
     c10::cuda::CUDAGuard guard(q.device());
     int64_t strides[17] = {q.stride(0), q.stride(1), q.stride(2)};
     for (int i = 0; i < 3 && shared; ++i) {

@@ -83,7 +83,8 @@ def cached_attention(q, own_k=None, own_v=None, own_lengths=None, *, shared_k=No
     kv_heads divides heads; key head i serves heads/kv_heads neighbouring query heads.  Caches may be any view whose last
     dimension is contiguous.  Returns [groups, rows, heads, dim]; a row that sees no position gets zeros.  The softmax
     shift is a whole number near the row's own maximum instead of the floor of the whole tensor's, which changes nothing
-    but the rounding of the shifted scores.  Head dimensions up to 256."""
+    but the rounding of the shifted scores.  Head dimensions up to 256, 2^20 rows times heads in a group, 2^30 positions, and groups x rows x heads x
+    (2 + positions / 64) below 2^31."""
     if (host := _lib.host()) is not None:
         out = host.cached_attention(q, own_k, own_v, own_lengths, shared_k, shared_v, shared_lengths)
         if out is not None:
@@ -99,6 +100,9 @@ def cached_attention(q, own_k=None, own_v=None, own_lengths=None, *, shared_k=No
     shared_k, shared_v, shared_lengths = _cache("shared", shared_k, shared_v, shared_lengths, (groups,), heads, dim)
     if own_k is not None and shared_k is not None and own_k.shape[-2] != shared_k.shape[-2]:
         raise ValueError(f"shared keys have {shared_k.shape[-2]} heads, own keys {own_k.shape[-2]}")
+    shared, own = (0 if t is None else t.shape[-3] for t in (shared_k, own_k))
+    if rows * heads > 1 << 20 or shared + own > 1 << 30 or groups * rows * heads > (2 ** 31 - 1) // (2 + (shared + own) // 64):
+        raise ValueError(f"{groups} groups of {rows} rows of {heads} heads over {shared + own} positions are too many for one call")
     _no_backward("cached_attention", q, own_k, own_v, shared_k, shared_v)
     dev = _lib.require_cuda(q, own_k, own_v, own_lengths, shared_k, shared_v, shared_lengths)
     if dim > 1 and q.stride(-1) != 1:
@@ -107,7 +111,6 @@ def cached_attention(q, own_k=None, own_v=None, own_lengths=None, *, shared_k=No
     if out.numel() == 0:
         return out
     kv_heads = (shared_k if own_k is None else own_k).shape[-2]
-    shared, own = (0 if t is None else t.shape[-3] for t in (shared_k, own_k))
     strides = (ctypes.c_int64 * 17)(*q.stride()[:3], *(shared_k.stride()[:3] + shared_v.stride()[:3] if shared else (0,) * 6),
                                     *(own_k.stride()[:4] + own_v.stride()[:4] if own else (0,) * 8))
     ptr = lambda t, used=True: t.data_ptr() if t is not None and used else None
