@@ -251,22 +251,28 @@ __global__ void __launch_bounds__(kThreads, 5) pick_kernel(const Select a) {
     const int at_first = count;
     __syncthreads();
     if (at_first > kMany) {
-        // many equal ones: the k-th largest full key of a warp's threads is a bound that they do not share
+        // many equal ones: the k-th largest full key of a warp's threads is a bound that they do not share, or the least of two warps' (k / 2)-th largest where k
+        // is more than a warp has (four have one in each thread where so many were found)
         unsigned long long first_key = 0ull;
 #pragma unroll
         for (int i = 0; i < kQuads; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) first_key = max(first_key, key(i, e));
+        const int of_each = a.k > 32 ? (a.k + 1) / 2 : a.k;
         int rank = 0;
 #pragma unroll 8
         for (int l = 0; l < 32; ++l) rank += __shfl_sync(0xffffffffu, first_key, l) > first_key;
-        const unsigned who = __ballot_sync(0xffffffffu, rank == a.k - 1 && first_key != 0ull);
+        const unsigned who = __ballot_sync(0xffffffffu, rank == of_each - 1 && first_key != 0ull);
         const unsigned long long mine = who ? __shfl_sync(0xffffffffu, first_key, __ffs(who) - 1) : 1ull;
         if (lane == 0) warp_key[warp] = mine;
         if (t == 0) count = 0;
         __syncthreads();
-        unsigned long long from = 1ull;
-        for (int w = 0; w < kWarps; ++w) from = max(from, warp_key[w]);
+        unsigned long long from = 1ull, second = 1ull;
+        for (int w = 0; w < kWarps; ++w) {
+            second = max(second, min(from, warp_key[w]));
+            from = max(from, warp_key[w]);
+        }
+        if (a.k > 32) from = second;
 #pragma unroll
         for (int i = 0; i < kQuads; ++i)
 #pragma unroll
