@@ -86,8 +86,8 @@ constexpr int kWarps = kThreads / 32, kQuads = kEach / 4;
 static_assert(kWarps == 8 && kQuads == 4);
 constexpr int kMany = 512;                            // so many candidates are narrowed down by their full keys first
 
-// Bound by instructions and the barriers between them: 735 per warp and 512 logits, of which the terms of the sum are 80 and the band they lie in 24, issued in 63 % of the
-// cycles; 155 MB of logits and 39 of flags in 81 us with the second kernel, 2.4 TB/s.
+// Bound by instructions and the barriers between them: 740 per warp and 512 logits, the sum's terms the smaller part of them, issued in 71 % of the cycles; 155 MB of logits and 39 of
+// flags in 78 us with a cold cache, 2.5 TB/s.
 // (Five CTAs on an SM in 48 registers: 64 x 4 beams of 151643 words 91 -> 81 us; six spill, 90.)
 __global__ void __launch_bounds__(kThreads, 5) pick_kernel(const Select a) {
     __shared__ unsigned long long found[kMostLogits];

@@ -14,8 +14,8 @@
 // of products; where the positions of a row are dealt out to several CTAs, a third kernel adds these.  Where one CTA has all positions of its rows
 // and they are few, it makes both passes, with t in its shared memory.
 //
-// Rows that see the same positions are worked on together, up to 8 per CTA: every key and value is loaded once for all of them, by
-// asynchronous copies into a ring that each warp has for itself, so that the warps run without barriers until their last sums.
+// Rows that see the same positions are worked on together, up to 8 per CTA: every key and value is loaded once for these (more rows are several such tiles, each of which
+// loads them), by asynchronous copies into a ring that each warp has for itself, so that the warps run without barriers until their last sums.
 // Keys: a lane owns a position, 32 floats of it per stage, and reads the queries from
 // shared memory.  Values: a lane owns four columns.  A product is one integer and one floating-point add; the range rule
 // (pam_scalar.cuh) is decided per stage: where every exponent field of both sides lies in [66, 187], every product passes it.
@@ -444,9 +444,10 @@ __device__ __forceinline__ float2 joined_row(const KeyMemory<ROWS>& shared, int 
     return joined([&](int w) { return shared.red[w * ROWS + n]; }, blockDim.x >> 5);
 }
 
-// 64 groups of 8 rows of 64 floats over 8192 positions: 44 us, 6.1 T products per second.  Bound by instructions: 3.1 per product, of which 1.5 are the product's two adds and 0.25
-// the load of a query; the schedulers issue in 63 % of the cycles and the packed adds take a second slot each, 73 % in all, from 16 warps per SM (128 registers; 20 warps
-// at 104 spill, 70 -> 86 us for both passes).  One row of 64 floats, 60001 positions of 8 heads: 123 MB in 31 us with a cold cache, bound by memory and the start of the kernel.
+// 64 groups of 8 rows of 64 floats over 8192 positions: 43 us with a cold cache, 6.3 T products per second.  Bound by instructions: 3.1 per product, of which 1.5 are the product's
+// two adds and 0.25 the load of a query; the schedulers issue in 65 % of the cycles and the packed adds take a second slot each, from 16 warps per SM (128 registers; 20 warps
+// at 102 spill, both passes back to back 76 -> 89 us).  One row of 64 floats, 60001 positions of 8 heads: 123 MB in 30 us with a cold cache, 4.0 TB/s, bound by memory and the start
+// of the kernel.
 template <int ROWS, bool VEC>
 __global__ void __launch_bounds__(32 * kMostWarps, 2) key_kernel(const Attention a, const Segment g) {
     extern __shared__ __align__(16) char memory[];
@@ -691,7 +692,7 @@ __device__ __forceinline__ void clear(float2 (&acc)[ROWS][COLS]) {
         for (int c = 0; c < COLS; ++c) acc[n][c] = make_float2(0.0f, 0.0f);
 }
 
-// The same 64 groups of 8 rows: 39 us, 7.0 T products per second, 2.7 instructions each; one row over 60001 positions 31 us.
+// The same 64 groups of 8 rows: 38 us, 7.0 T products per second, 2.8 instructions each; one row over 60001 positions 30 us.
 template <int SLOTS, int ROWS, bool VEC>
 __global__ void __launch_bounds__(32 * kMostWarps, 2) value_kernel(const Attention a, const Segment g) {
     extern __shared__ __align__(16) char memory[];
@@ -738,8 +739,8 @@ constexpr int kMostKept = 256;
 template <int SLOTS, int ROWS>
 __host__ __device__ constexpr int whole_ring() { return 2 * (ValueShape<SLOTS, ROWS>::kBytes > kKeyBytes ? ValueShape<SLOTS, ROWS>::kBytes : kKeyBytes); }
 
-// (One or two rows need few enough registers for half as many warps again on an SM, and so more copies on their way: 128 x 5 rows of 4 heads of 128 floats with up
-// to 64 own positions 32.8 -> 28.9 us.  The kernels of one pass each gain nothing from that, 60001 positions of one row 57 -> 60.)
+// (One or two rows need few enough registers for a third more warps on an SM, 22 in CTAs of two, whose shared memory has room for no more, and so more copies on their way: 128 x 5
+// rows of 4 heads of 128 floats with up to 64 own positions 32.8 -> 28.9 us.  The kernels of one pass each gain nothing from that, 60001 positions of one row 57 -> 60.)
 template <int SLOTS, int ROWS, bool VEC>
 __global__ void __launch_bounds__(32 * kMostWarps, ROWS <= 2 ? 3 : 2) whole_kernel(const Attention a, const Segment g) {
     extern __shared__ __align__(16) char memory[];

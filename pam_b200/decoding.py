@@ -76,7 +76,7 @@ def cached_attention(q, own_k=None, own_v=None, own_lengths=None, *, shared_k=No
     q           [groups, rows, heads, dim]: the new token of each row (beam, sample, sequence) of each group
     own_k/v     [groups, rows, slots, kv_heads, dim]: what each row has to itself (its own past), or None
     shared_k/v  [groups, positions, kv_heads, dim]: what the rows of a group have in common (the source sentence of its
-                beams, a prompt), or None; read once for all of them
+                beams, a prompt), or None; read once for every eight rows times query heads of a key head
     lengths     how much of the cache is in use: a number, an int64 tensor ([groups, rows] own, [groups] shared), or None for
                 all of it.  Lengths on the device are clamped to the slots; what lies beyond them is never read.
 
@@ -138,7 +138,7 @@ def beam_select(logits, scores, k, banned=None):
 
     Returns (scores, beams, tokens), each [groups, k], best first: the new scores `scores + log_softmax(logits)` with the
     PAM log-softmax, the beam each continues (int64) and its token (int64).  Values are formed and compared in 64 bits; equal
-    ones go to the lower beam, then to the lower token.  Logits of -1e30 or less, -inf among them, are masked: they have no
+    ones go to the lower beam, then to the larger logit, then to the lower token.  Logits of -1e30 or less, -inf among them, are masked: they have no
     share in the probability.  Masked and banned tokens and the tokens of beams that are not continued have score -inf and come
     last, also where a beam's logits hold NaN or overflow.  Up to 64 beams and k up to 64; beams times the vocabulary in ranges of 4092 tokens, the last
     one rounded up, up to 4096 (64 beams of 261888 tokens)."""
