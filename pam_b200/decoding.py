@@ -194,6 +194,9 @@ def _rows_meet(apart, size, other, by_group, by_row, groups, rows):
     """Whether a row of `size` bytes of one state and a row of `other` bytes of another meet that lies `apart` bytes behind and has the same strides (two parts of
     one buffer, interleaved row by row, do not): whether apart + i by_group + j by_row is between -other and size for some differences i of groups and j
     of rows."""
+    steps = sorted((step, n) for step, n in ((by_group, groups), (by_row, rows)) if n > 1)
+    if steps and size <= apart <= steps[0][0] - other and (len(steps) == 1 or steps[1][0] >= steps[0][0] * steps[0][1]):
+        return False                                      # (between two neighbouring rows, at the end of a group too: most often so)
     for j in range(1 - rows, rows):
         at = apart + j * by_row
         if groups == 1 or by_group == 0:
