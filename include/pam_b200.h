@@ -365,6 +365,48 @@ int pamk_reorder_states(void* const* states, const int64_t* group_bytes, const i
                         const int64_t* moved_bytes, const int64_t* position_bytes, int count,
                         const int64_t* parents, const int64_t* positions, int64_t groups, int64_t rows, void* stream);
 
+/* pamk_sample: one token of each of `rows` rows of logits ([rows, vocab], row stride logits_row, token stride 1), drawn by uniform[row] in [0, 1).
+ *   x = pad(logit, temperature);  t = pam(x, log2 e);  the weight of a token is its PAM exponential 2^floor(t) (1 + f), f = t - floor(t) rounded down to steps
+ *   of 2^-23, as a whole number of units of 2^-44 of the greatest 2^floor(t) that may be drawn.
+ * Tokens in the order of their exponentials, equal ones by number: the first top_k stay (0: all), of these the ones before which less than top_p of their
+ * weights lies (1: all), of these the ones of at least min_p times the first one's weight; the first token, by number, with which the weights that stay exceed
+ * uniform times their sum is tokens[row] (fractions rounded down to steps of 2^-24).  All sums are of whole numbers and exact.  scores[row] is x minus the PAM logsumexp of
+ * the row (pamk_logsumexp_fwd; its sum, logarithm and quotient in 64 bits).  Logits of -1e30 or less are masked: no weight and no share in the sum.  banned as in
+ * pamk_beam_select (NULL: none): in the sum, never drawn.  A row without a token to draw, with a NaN or a product beyond the PAM range, or with a
+ * temperature that is not positive and finite gets token -1 and score -inf.  temperatures, top_ks, top_ps, min_ps: [rows] on the device, or NULL: the number beside
+ * it for all rows.  vocab <= 262144; rows < 2^28. */
+int pamk_sample(const float* logits, const float* uniform, const unsigned char* banned, int64_t* tokens, float* scores, int64_t rows, int64_t vocab,
+                int64_t logits_row, int64_t banned_row, const float* temperatures, float temperature, const int64_t* top_ks, int64_t top_k, const float* top_ps,
+                float top_p, const float* min_ps, float min_p, void* stream);
+
+/* ---- embedding and dropout -----------------------------------------------------------------------------
+ * No counterpart as kernels in the reference, whose fairseq fork looks tokens up, scales, adds positions and drops out one operator after another
+ * (fairseq/models/transformer/transformer_encoder.py:177-196, fairseq/modules/fairseq_dropout.py).
+ *
+ * The mask of a dropout: element i (of the contiguous output) has the 32 bits of word i mod 4 of the Philox4x32-10 block with counter i / 4 under the 64-bit key
+ * *seed_at (on the device; NULL: `seed`), and stays where they are at least p 2^32, to the nearest whole number; s is the fp32 number next to 1 / (1 - p).
+ *   pamk_dropout       out_i = residual_i + (kept_i ? pam(x_i, s) : 0); residual NULL: none.  Also the approximate gradient, on dy.
+ *   pamk_dropout_bwd   dx_i = kept_i ? pam_bwd(x_i, s, dy_i) : 0, the exact one.
+ * 0 < p < 1. */
+int pamk_dropout(const float* x, const float* residual, float* out, int64_t n, double p, const int64_t* seed_at, int64_t seed, float offset, void* stream);
+int pamk_dropout_bwd(const float* x, const float* dy, float* dx, int64_t n, double p, const int64_t* seed_at, int64_t seed, float offset, void* stream);
+
+/* pamk_embedding: out[i] = drop(pam(table[tokens[i]], scale) + positions[i mod positions_count]) for `count` tokens, [count, dim] contiguous; has_scale 0: no
+ * product; positions NULL: none; p 0: no dropout.  table and positions have unit column strides and the given row strides; count is a multiple of
+ * positions_count.  A token outside [0, vocab) gives a row of NaN.  With dy ([count, dim]; p > 0) it gives the exact gradient of the dropout instead: dy times
+ * its slope at the sum, 0 where dropped.
+ * pamk_embedding_bwd: dtable[v] = sum over the i with tokens[i] = v, v != padding, of pam(drop'(dy[i]), scale), [vocab, dim] contiguous; with approx_bwd 0 of
+ * dy[i] slope(table[v], scale), and then p must be 0 (pamk_embedding gives the dropout's gradient).  Rows without a token get zeros.  The terms of a row are added
+ * in an order that follows from the tokens alone.  padding: -1 for none.
+ * count < 2^31, vocab <= 2^22.  `workspace`: pamk_embedding_bwd_workspace_bytes(...) bytes, 256-byte aligned; NULL where that is 0. */
+int pamk_embedding(const int64_t* tokens, const float* table, const float* positions, const float* dy, float* out, int64_t count, int64_t vocab, int64_t dim,
+                   int64_t table_row, int64_t positions_row, int64_t positions_count, int has_scale, float scale, double p, const int64_t* seed_at, int64_t seed,
+                   float offset, void* stream);
+size_t pamk_embedding_bwd_workspace_bytes(int64_t count, int64_t vocab, int64_t dim);
+int pamk_embedding_bwd(const int64_t* tokens, const float* dy, const float* table, float* dtable, int64_t count, int64_t vocab, int64_t dim, int64_t table_row,
+                       int64_t padding, int has_scale, float scale, double p, const int64_t* seed_at, int64_t seed, float offset, int approx_bwd, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
 /* ---- roofline measurement --------------------------------------------------------------------
  * No counterpart in the reference.  Runs register-only chains of the instructions a PAM
  * multiply-accumulate is made of and reports how many chain steps ran in how many milliseconds;

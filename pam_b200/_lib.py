@@ -19,6 +19,7 @@ FULL, SCALAR, ROW, COL, IMM = 0, 1, 2, 3, 4
 MUL_PAM, MUL_STANDARD = 0, 1
 
 _p, _i, _i64, _f, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
+_seeded = [ctypes.c_double, _p, _i64, _f]                  # p, seed on the device, seed, offset
 _operand = [_p, _i, _f]
 
 _SIGNATURES = {
@@ -81,6 +82,12 @@ _SIGNATURES = {
     "pamk_beam_select_workspace_bytes": (_sz, [_i64] * 4),
     "pamk_beam_select": (_i, [_p] * 6 + [_i64] * 8 + [_p, _sz, _p]),
     "pamk_reorder_states": (_i, [_p] * 5 + [_i, _p, _p, _i64, _i64, _p]),
+    "pamk_sample": (_i, [_p] * 5 + [_i64] * 4 + [_p, _f, _p, _i64, _p, _f, _p, _f, _p]),
+    "pamk_dropout": (_i, [_p] * 3 + [_i64] + _seeded + [_p]),
+    "pamk_dropout_bwd": (_i, [_p] * 3 + [_i64] + _seeded + [_p]),
+    "pamk_embedding": (_i, [_p] * 5 + [_i64] * 6 + [_i, _f] + _seeded + [_p]),
+    "pamk_embedding_bwd_workspace_bytes": (_sz, [_i64] * 3),
+    "pamk_embedding_bwd": (_i, [_p] * 4 + [_i64] * 5 + [_i, _f] + _seeded + [_i, _p, _sz, _p]),
     "pamk_issue_rate": (_i, [_i, _i, _i, _p, ctypes.POINTER(_f), ctypes.POINTER(ctypes.c_double), _p]),
 }
 

@@ -17,6 +17,7 @@ from . import _lib
 MAX_HEAD_DIM = 256
 MAX_BEAMS = 64
 MAX_SELECTED = 64
+MAX_SAMPLED = 1 << 18
 _RANGE, _MAX_RANGES = 4092, 4096                # a beam's logits are worked on in ranges of so many; so many ranges may a group have
 
 
@@ -182,6 +183,71 @@ def beam_select(logits, scores, k, banned=None):
                                              _lib.stream_ptr(dev))
         _lib.check(status, "pamk_beam_select")
     return best, which[0], which[1]
+
+
+def _setting(name, value, shape, low, high, whole=False):
+    """A number within [low, high], or a tensor of one for each row: (tensor or None, number)."""
+    if isinstance(value, torch.Tensor):
+        want = torch.int64 if whole else torch.float32
+        if value.dtype != want or value.shape != shape:
+            raise ValueError(f"{name} must be a number or a tensor {want} {tuple(shape)}, got {value.dtype} {tuple(value.shape)}")
+        return value.contiguous(), 0
+    if not isinstance(value, int if whole else (int, float)) or isinstance(value, bool) or not low <= value <= high:
+        raise ValueError(f"{name} must be a {'whole ' if whole else ''}number from {low:g} to {high:g}, got {value!r}")
+    return None, value
+
+
+def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, banned=None):
+    """Draws a token for every row of logits.
+
+    logits   [..., vocabulary]: of the next token
+    uniform  [...]: a number from [0, 1) for each row, in steps of 2^-24 as torch.rand gives them
+    banned   bool, [vocabulary] or anything that broadcasts to the logits: tokens that must not be drawn (they keep their share of the probability)
+
+    Tokens are drawn by the PAM softmax of pad(logits, temperature).  In the order of their probabilities, equal ones by number, there stay the first
+    `top_k` (0: all), of these the ones before which less than `top_p` of their probability lies, of these the ones with at least `min_p` times the first one's.
+    Each of the four is a number, or a tensor with one for each row (fp32, top_k int64; values out of range there are taken as the next one in range, a
+    temperature that is not positive and finite leaves its row without a token).  The token is the first, by number, with which the probabilities that stay reach
+    beyond `uniform`.  Probabilities are whole numbers of units of 2^-44 of the largest power of two, so that what is drawn depends on no rounding.
+
+    Returns (tokens int64 [...], scores [...]): a score is the PAM log-softmax of pad(logits, temperature) at the token, over all tokens of the row.  Logits of -1e30 or less
+    are masked.  A row that has no token to draw, or holds a NaN or a value beyond the PAM range, gets token -1 and score -inf.  Up to 262144 tokens."""
+    _not_traced("sample")
+    if not isinstance(logits, torch.Tensor) or logits.dim() < 1:
+        raise ValueError("logits must be a tensor [..., vocabulary]")
+    _fp32("logits", logits, logits.dim())
+    lead, vocab = logits.shape[:-1], logits.shape[-1]
+    _fp32("uniform", uniform, len(lead))
+    if uniform.shape != lead:
+        raise ValueError(f"uniform {tuple(uniform.shape)} does not go with logits {tuple(logits.shape)}")
+    if not 1 <= vocab <= MAX_SAMPLED:
+        raise ValueError(f"a vocabulary of {vocab} is not from 1 to {MAX_SAMPLED}")
+    temperature = _setting("temperature", temperature, lead, 2.0 ** -126, 2.0 ** 127)
+    top_k = _setting("top_k", top_k, lead, 0, 2 ** 62, whole=True)
+    top_p = _setting("top_p", top_p, lead, 2.0 ** -24, 1.0)
+    min_p = _setting("min_p", min_p, lead, 0.0, 1.0)
+    _no_backward("sample", logits, uniform)
+    if banned is not None:
+        if not isinstance(banned, torch.Tensor) or banned.dtype != torch.bool:
+            raise TypeError("banned must be a bool tensor")
+        # (one row of flags for all stays one)
+        banned = banned.expand(vocab) if banned.dim() <= 1 else banned.expand(logits.shape).reshape(-1, vocab)
+        banned = banned.contiguous()
+    dev = _lib.require_cuda(logits, uniform, banned, *(s[0] for s in (temperature, top_k, top_p, min_p)))
+    rows = uniform.numel()
+    x = logits.reshape(rows, vocab)
+    if vocab > 1 and x.stride(-1) != 1:
+        x = x.contiguous()
+    uniform = uniform.contiguous()
+    tokens = torch.empty(lead, dtype=torch.int64, device=dev)
+    scores = torch.empty(lead, dtype=torch.float32, device=dev)
+    ptr = lambda t: None if t is None else t.data_ptr()
+    with _lib.device_guard(dev):
+        status = _lib.lib().pamk_sample(x.data_ptr(), uniform.data_ptr(), ptr(banned), tokens.data_ptr(), scores.data_ptr(), rows, vocab, x.stride(0),
+                                        vocab if banned is not None and banned.dim() == 2 else 0,
+                                        *(v for t, n in (temperature, top_k, top_p, min_p) for v in (ptr(t), n)), _lib.stream_ptr(dev))
+    _lib.check(status, "pamk_sample")
+    return tokens, scores
 
 
 def _span(t):

@@ -8,6 +8,7 @@ primitives one kernel at a time (still on the GPU).
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -473,6 +474,125 @@ def cross_entropy_grad(logits, target, weight, grad_out, *, hot, cold, mean_rows
                                               dx.data_ptr(), rows, length, float(hot), float(cold), float(mean_rows),
                                               int(has_ignore), int(ignore_index or 0), _offset(offset)])
     return dx
+
+
+# ---- dropout and embedding ------------------------------------------------------------------------------
+
+def _seed_args(p, seed, offset):
+    """p, the seed on the device or by value, and the offset, as the kernels take them."""
+    on_device = isinstance(seed, torch.Tensor)
+    return float(p), seed.data_ptr() if on_device else None, 0 if on_device else int(seed), offset
+
+
+def _drop(x, residual, p, seed, offset):
+    out = torch.empty_like(x)
+    with _lib.device_guard(x.device):
+        status = _lib.lib().pamk_dropout(x.data_ptr(), _ptr(residual), out.data_ptr(), x.numel(), *_seed_args(p, seed, offset), _lib.stream_ptr(x.device))
+    _lib.check(status, "pamk_dropout")
+    return out
+
+
+class _Dropout(torch.autograd.Function):
+    """The mask is drawn again in the backward pass, which needs the seed alone (the exact gradients also the input)."""
+
+    @staticmethod
+    def forward(ctx, x, residual, p, seed, offset, approx):
+        x = x.contiguous()
+        on_device = isinstance(seed, torch.Tensor)
+        ctx.save_for_backward(seed if on_device else None, None if approx else x)
+        ctx.cfg = (p, None if on_device else seed, offset)
+        return _drop(x, None if residual is None else residual.contiguous(), p, seed, offset)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        seed, x = ctx.saved_tensors
+        p, number, offset = ctx.cfg
+        seed = number if seed is None else seed
+        dx = None
+        if ctx.needs_input_grad[0]:
+            g1 = g.float().contiguous()
+            if x is None:
+                dx = _drop(g1, None, p, seed, offset)
+            else:
+                dx = torch.empty_like(x)
+                with _lib.device_guard(x.device):
+                    status = _lib.lib().pamk_dropout_bwd(x.data_ptr(), g1.data_ptr(), dx.data_ptr(), x.numel(), *_seed_args(p, seed, offset),
+                                                         _lib.stream_ptr(x.device))
+                _lib.check(status, "pamk_dropout_bwd")
+        return dx, g if ctx.needs_input_grad[1] else None, None, None, None, None
+
+
+def dropout(x, residual, p, seed, *, offset=None, approx_bwd=False):
+    """See pam_ops.dropout, which checks the arguments; 0 < p < 1."""
+    return _Dropout.apply(x, residual, p, seed, _offset(offset), approx_bwd)
+
+
+def _rows_of(t):
+    """A matrix with unit column stride, and its row stride."""
+    if t.shape[-1] > 1 and t.stride(-1) != 1 or t.stride(0) < 0:
+        t = t.contiguous()
+    return t, t.stride(0)
+
+
+def _embed(tokens, weight, positions, dy, scale, p, seed, offset):
+    dev = weight.device
+    weight, row = _rows_of(weight.detach())
+    pos, pos_row = (None, 0) if positions is None else _rows_of(positions.detach())
+    out = torch.empty(*tokens.shape, weight.shape[1], dtype=torch.float32, device=dev)
+    with _lib.device_guard(dev):
+        status = _lib.lib().pamk_embedding(tokens.data_ptr(), weight.data_ptr(), _ptr(pos), _ptr(dy), out.data_ptr(), tokens.numel(), *weight.shape, row, pos_row,
+                                           0 if pos is None else pos.shape[0], int(scale is not None), float(scale or 0.0), *_seed_args(p, seed, offset),
+                                           _lib.stream_ptr(dev))
+    _lib.check(status, "pamk_embedding")
+    return out
+
+
+class _Embedding(torch.autograd.Function):
+    """Nothing of the output's size is kept: with the approximate gradients the tokens and the seed alone, with the exact ones also what the sums are made of."""
+
+    @staticmethod
+    def forward(ctx, tokens, weight, positions, padding, scale, p, seed, offset, approx):
+        on_device = isinstance(seed, torch.Tensor)
+        slopes = not approx and (scale is not None or p > 0)
+        ctx.save_for_backward(tokens, seed if on_device else None, weight if slopes else None, positions if slopes and p > 0 else None)
+        ctx.cfg = (padding, scale, p, None if on_device else seed, offset, approx, tuple(weight.shape), None if positions is None else positions.shape[0])
+        return _embed(tokens, weight, positions, None, scale, p, seed, offset)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        tokens, seed, weight, positions = ctx.saved_tensors
+        padding, scale, p, number, offset, approx, (vocab, dim), pos_count = ctx.cfg
+        seed = number if seed is None else seed
+        dev = g.device
+        d_weight = d_pos = None
+        g = g.float().contiguous()
+        need_pos = ctx.needs_input_grad[2] and pos_count is not None
+        if p > 0 and (need_pos or not approx):                # the gradient before the dropout, which two sums or the slopes need
+            g = _drop(g, None, p, seed, offset) if approx else _embed(tokens, weight, positions, g, scale, p, seed, offset)
+            p = 0.0
+        if ctx.needs_input_grad[1]:
+            d_weight = torch.empty(vocab, dim, dtype=torch.float32, device=dev)
+            table, row = (None, 0) if weight is None else _rows_of(weight.detach())
+            handle = _lib.lib()
+            ws_bytes = handle.pamk_embedding_bwd_workspace_bytes(tokens.numel(), vocab, dim)
+            # (a buffer of this call alone: calls captured into different graphs share none)
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+            with _lib.device_guard(dev):
+                status = handle.pamk_embedding_bwd(tokens.data_ptr(), g.data_ptr(), _ptr(table), d_weight.data_ptr(), tokens.numel(), vocab, dim, row,
+                                                   -1 if padding is None else padding, int(scale is not None), float(scale or 0.0),
+                                                   *_seed_args(p, seed, offset), int(approx), _ptr(ws), ws_bytes, _lib.stream_ptr(dev))
+            _lib.check(status, "pamk_embedding_bwd")
+        if need_pos:
+            from .cuda_bindings import _column_sum
+            d_pos = _column_sum(g.view(-1, pos_count * dim)).view(pos_count, dim) if g.numel() else torch.zeros(pos_count, dim, device=dev)
+        return None, d_weight, d_pos, None, None, None, None, None, None
+
+
+def embedding(tokens, weight, positions, padding, scale, p, seed, *, offset=None, approx_bwd=False):
+    """See pam_ops.embedding, which checks the arguments; positions [count, dim] or None."""
+    return _Embedding.apply(tokens, weight, positions, padding, scale, p, seed, _offset(offset), approx_bwd)
 
 
 # ---- linear layer with bias ----------------------------------------------------------------------------

@@ -16,6 +16,7 @@ from .utils import is_number
 __all__ = [
     "mul", "div", "exp", "exp2", "log", "log2", "pow", "matmul", "bmm", "linear", "conv2d", "conv2d_group",
     "Conv2d", "Linear", "mean", "softmax", "logsumexp", "log_softmax", "layer_norm", "LayerNorm",
+    "dropout", "Dropout", "embedding", "Embedding",
 ]
 
 
@@ -305,3 +306,118 @@ class LayerNorm(_PamModule, torch.nn.LayerNorm):
 
     def extra_repr(self):
         return self._pam_repr(torch.nn.LayerNorm.extra_repr(self), with_kernel=True)
+
+
+# ---- dropout and embedding (no counterpart in the reference's library, whose forks use the stock ones around its products) -----------
+
+def _gradient_mode(approx_bwd):
+    if not fused._uniform(approx_bwd):
+        raise ValueError(f"one gradient mode for both operands, got approx_bwd={approx_bwd}")
+    return fused._flag(approx_bwd)
+
+
+def _fp32(name, t):
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32:
+        raise TypeError(f"{name} must be an fp32 tensor, got {t.dtype if isinstance(t, torch.Tensor) else type(t).__name__}")
+    return t
+
+
+def _probability(p):
+    if not is_number(p) or not 0 <= p < 1:
+        raise ValueError(f"p must be a number from 0 to below 1, got {p!r}")
+    return float(p)
+
+
+def _seed(seed, device):
+    """The seed of a mask: the one that is given, or one from the device's default generator (which a captured graph draws anew at each replay)."""
+    if seed is None:
+        return torch.randint(-2 ** 63, 2 ** 63 - 1, (1,), device=device)
+    if isinstance(seed, torch.Tensor):
+        if seed.dtype != torch.int64 or seed.numel() != 1:
+            raise ValueError(f"seed must be a number or an int64 tensor of one element, got {seed.dtype} {tuple(seed.shape)}")
+    elif not isinstance(seed, int) or isinstance(seed, bool) or not -2 ** 63 <= seed < 2 ** 63:
+        raise ValueError(f"seed must be a whole number of 64 bits, got {seed!r}")
+    return seed
+
+
+def dropout(x, p=0.5, seed=None, residual=None, *, training=True, offset=None, approx_bwd=False, use_kernel=True):
+    """Dropout with a PAM product: x times fp32(1 / (1 - p)) where it is kept, 0 elsewhere (whatever is there), plus `residual` of the same shape.
+
+    The mask is a function of the seed and of each element's place (Philox4x32-10, csrc/philox.cuh) and is not stored: the backward pass draws it
+    again.  `seed` is a number or an int64 tensor of one element on x's device, None for one from the default generator.  The gradient of x is the PAM product
+    of the incoming one (approx_bwd) or its product with the slope (exact).  With training=False or p = 0: x itself, plus the residual."""
+    approx, p = _gradient_mode(approx_bwd), _probability(p)
+    _fp32("x", x)
+    if residual is not None:
+        _fp32("residual", residual)
+        if residual.shape != x.shape:
+            raise ValueError(f"residual {tuple(residual.shape)} does not go with x {tuple(x.shape)}")
+    if not training or p == 0:
+        return x if residual is None else residual + x
+    _lib.require_cuda(x, residual, seed)
+    return fused.dropout(x, residual, p, _seed(seed, x.device), offset=offset, approx_bwd=approx)
+
+
+class Dropout(_PamModule, torch.nn.Dropout):
+    def __init__(self, p=0.5, *, offset=None, approx_bwd=False, use_kernel=True):
+        _probability(p)
+        super().__init__(p)
+        self._init_pam(offset, approx_bwd, use_kernel)
+
+    def forward(self, input, residual=None, seed=None):
+        return dropout(input, self.p, seed, residual, training=self.training, **self._pam_kwargs())
+
+    def extra_repr(self):
+        return self._pam_repr(f"p={self.p}")
+
+
+def embedding(tokens, weight, scale=None, positions=None, padding_idx=None, *, p=0.0, seed=None, training=True, offset=None, approx_bwd=False,
+              use_kernel=True):
+    """The rows of `weight` [vocabulary, dim] for `tokens` (any shape, int64 or int32), [*tokens, dim]: times `scale` by PAM (None: as they are), plus
+    `positions` ([length, dim] with tokens [..., length], or one row [dim] or [1, dim] for all tokens), through dropout(..., p, seed).
+
+    The gradient of the table has PAM products (approx_bwd) or slopes (exact) of the incoming one, added for each row in an order that follows from
+    the tokens alone; the row `padding_idx` has none.  A token outside the vocabulary gives a row of NaN and has no gradient.  Up to 2^22 rows, fewer than
+    2^31 tokens."""
+    approx, p = _gradient_mode(approx_bwd), _probability(p)
+    if not isinstance(tokens, torch.Tensor) or tokens.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"tokens must be an int64 or int32 tensor, got {tokens.dtype if isinstance(tokens, torch.Tensor) else type(tokens).__name__}")
+    if _fp32("weight", weight).dim() != 2:
+        raise ValueError(f"weight must be [vocabulary, dim], got {tuple(weight.shape)}")
+    vocab, dim = weight.shape
+    if scale is not None and not is_number(scale):
+        raise TypeError(f"scale must be a number or None, got {type(scale).__name__}")
+    if padding_idx is not None:
+        if not isinstance(padding_idx, int) or isinstance(padding_idx, bool) or not -vocab <= padding_idx < vocab:
+            raise ValueError(f"padding_idx {padding_idx!r} outside the vocabulary of {vocab}")
+        padding_idx %= vocab
+    if positions is not None:
+        if _fp32("positions", positions).dim() == 1:
+            positions = positions.unsqueeze(0)
+        length = tokens.shape[-1] if tokens.dim() else 1
+        if positions.dim() != 2 or positions.shape[1] != dim or positions.shape[0] not in (1, length) or not positions.shape[0]:
+            raise ValueError(f"positions {tuple(positions.shape)} do not go with tokens {tuple(tokens.shape)} and rows of {dim}")
+    if not training:
+        p = 0.0
+    _lib.require_cuda(tokens, weight, positions, seed)
+    return fused.embedding(tokens.long().contiguous(), weight, positions, padding_idx, None if scale is None else float(scale), p,
+                           _seed(seed, weight.device) if p else 0, offset=offset, approx_bwd=approx)
+
+
+class Embedding(_PamModule, torch.nn.Embedding):
+    """torch.nn.Embedding with a PAM `scale` and dropout `p`; forward(tokens, positions=None, seed=None)."""
+
+    def __init__(self, num_embeddings, embedding_dim, padding_idx=None, scale=None, p=0.0, *, offset=None, approx_bwd=False, use_kernel=True, **kwargs):
+        refused = sorted(k for k in ("max_norm", "scale_grad_by_freq", "sparse") if kwargs.get(k))
+        if refused:
+            raise ValueError(f"pam.Embedding has no {', '.join(refused)}")
+        _probability(p)
+        super().__init__(num_embeddings, embedding_dim, padding_idx, **kwargs)
+        self.scale, self.p = scale, p
+        self._init_pam(offset, approx_bwd, use_kernel)
+
+    def forward(self, input, positions=None, seed=None):
+        return embedding(input, self.weight, self.scale, positions, self.padding_idx, p=self.p, seed=seed, training=self.training, **self._pam_kwargs())
+
+    def extra_repr(self):
+        return self._pam_repr(torch.nn.Embedding.extra_repr(self) + f", scale={self.scale}, p={self.p}")
