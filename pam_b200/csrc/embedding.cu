@@ -1,8 +1,14 @@
 // Embedding: rows of a table by token, scaled by a PAM product, with positions added and dropout, and the table's gradient.
 //     x_i = pam(w[token_i], scale) + pos[i mod T]        y_i = kept ? pam(x_i, s) : 0       (philox.cuh; every step but the first is left out on demand)
-//     dw[v] = sum over i with token_i = v, in order of i, of pam(drop'(g_i), scale)   (approximate gradients; exact ones: times slope(w[v], scale))
+//     dw[v] = sum over i with token_i = v of pam(drop'(g_i), scale)   (approximate gradients; exact ones: times slope(w[v], scale))
 // with drop'(g) = kept ? pam(g, s) : 0 (exact: g slope(x, s)).  The row of the padding token has no gradient.
 // A token outside the table reads nothing: its row is NaN, and it has no gradient.
+//
+// The gradient is a sort and a segmented sum, so that every row of g is read once, wherever its token occurs, and no atomics decide on an order:
+//   sort   the places of the tokens in the order (token, place), by two digits of at most 11 bits, each pass stable.  Up to 8192 tokens one CTA sorts in shared
+//          memory; more are cut into tiles, whose counts place them.  The other CTAs of these launches fill the gradient with zeros meanwhile.
+//   sums   a warp adds the rows of 16 neighbours in that order (32 where there are many), 128 columns of them, and writes the tokens that lie within;
+//   joins  a token with neighbours in several such chunks has its parts added in their order by a CTA for each 128 columns.
 #include "common.cuh"
 #include "pam_scalar.cuh"
 #include "philox.cuh"
@@ -23,15 +29,24 @@ struct Embedding {
     Dropping drop;
 };
 
+__device__ __forceinline__ int64_t token_at(const int64_t* tokens, int64_t i) { return __ldg(reinterpret_cast<const long long*>(tokens) + i); }
+
 __device__ __forceinline__ float looked_up(const Embedding& a, int64_t i, int c) {
-    const int64_t token = __ldg(reinterpret_cast<const long long*>(a.tokens) + i);
+    const int64_t token = token_at(a.tokens, i);
     if ((uint64_t)token >= (uint64_t)a.vocab) return quiet_nan();
     float x = __ldg(a.table + token * a.table_row + c);
     if (a.scaled) x = mul(x, a.scale, a.off);
     return a.pos ? fadd(x, __ldg(a.pos + (a.pos_count == 1 ? 0 : i % a.pos_count) * a.pos_row + c)) : x;
 }
 
-// SLOPES: g times the slope of the dropout at x, where it is kept; else y.  A thread takes four neighbouring elements of the output.
+// The output element of a sum x: dropped out; SLOPES: g times the slope of the dropout at x, where it is kept.
+template <bool SLOPES>
+__device__ __forceinline__ float finished(const Embedding& a, float x, uint32_t bits, float g) {
+    if (!a.drops) return x;
+    return bits < a.drop.below ? 0.0f : SLOPES ? mul_bwd(x, a.drop.scale, g, a.off) : mul(x, a.drop.scale, a.off);
+}
+
+// A thread takes four neighbouring elements of the output, which is what a block of the counter has bits for; here of any row length.
 template <bool SLOPES>
 __global__ void __launch_bounds__(kThreads) embed_kernel(const Embedding a, const float* g, float* out) {
     const int64_t e = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 4, n = a.count * a.dim;
@@ -43,12 +58,7 @@ __global__ void __launch_bounds__(kThreads) embed_kernel(const Embedding a, cons
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         if (e + k >= n) return;
-        float x = looked_up(a, i, c);
-        if (SLOPES)
-            x = bits[k] < a.drop.below ? 0.0f : mul_bwd(x, a.drop.scale, __ldg(g + e + k), a.off);
-        else if (a.drops)
-            x = bits[k] < a.drop.below ? 0.0f : mul(x, a.drop.scale, a.off);
-        out[e + k] = x;
+        out[e + k] = finished<SLOPES>(a, looked_up(a, i, c), bits[k], SLOPES ? __ldg(g + e + k) : 0.0f);
         if (++c == a.dim) {
             c = 0;
             ++i;
@@ -56,31 +66,440 @@ __global__ void __launch_bounds__(kThreads) embed_kernel(const Embedding a, cons
     }
 }
 
-// A warp takes 32 columns of one row of the table and looks through all tokens.
+// Rows of whole quads at aligned addresses, fewer than 2^31 quads.
 template <bool SLOPES>
-__global__ void __launch_bounds__(kThreads) table_grad_kernel(const Embedding a, const float* g, float* dw) {
-    const int lane = threadIdx.x & 31, c = blockIdx.y * 32 + lane;
-    const int64_t v = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-    if (v >= a.vocab) return;
+__global__ void __launch_bounds__(kThreads) embed_quads_kernel(const Embedding a, const float* g, float* out, uint32_t quads, uint32_t row_quads) {
+    const uint32_t q = blockIdx.x * kThreads + threadIdx.x;
+    if (q >= quads) return;
+    const uint32_t i = q / row_quads, c = (q - i * row_quads) * 4;
+    const int64_t token = token_at(a.tokens, i);
+    const bool known = (uint64_t)token < (uint64_t)a.vocab;
+    float4 x = make_float4(quiet_nan(), quiet_nan(), quiet_nan(), quiet_nan()), p = make_float4(0.0f, 0.0f, 0.0f, 0.0f), d = p;
+    if (known) x = __ldg(reinterpret_cast<const float4*>(a.table + token * a.table_row + c));
+    if (a.pos) p = __ldg(reinterpret_cast<const float4*>(a.pos + (int64_t)(a.pos_count == 1 ? 0u : i % (uint32_t)a.pos_count) * a.pos_row + c));
+    if (SLOPES) d = __ldg(reinterpret_cast<const float4*>(g) + q);
+    const uint4 w = a.drops ? philox(q, key_of(a.drop)) : make_uint4(0u, 0u, 0u, 0u);
+    const auto one = [&](float v, float at, uint32_t bits, float dv) {
+        if (a.scaled) v = mul(v, a.scale, a.off);
+        if (a.pos) v = fadd(v, at);
+        return finished<SLOPES>(a, v, bits, dv);
+    };
+    reinterpret_cast<float4*>(out)[q] = make_float4(one(x.x, p.x, w.x, d.x), one(x.y, p.y, w.y, d.y), one(x.z, p.z, w.z, d.z), one(x.w, p.w, w.w, d.w));
+}
+
+// ---- the order of the tokens ------------------------------------------------------------------------------------
+
+constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kMostInOne = 8192;
+constexpr int kTileThreads = 512, kTileWarps = kTileThreads / 32, kRounds = 8, kTile = kTileThreads * kRounds;
+constexpr int kMostTiles = 512;           // each reads the counts of all
+constexpr uint32_t kNone = 0xffffffffu;
+
+struct Entry { uint32_t token, place; };
+
+struct Sort {
+    const int64_t* tokens;
+    int64_t count, vocab, padding;
+    int low_bits, high_bits;
+    int tiles, tile;                      // of `tile` tokens, a multiple of kTile
+    uint32_t *counts_low, *counts_high;   // [tiles][1 << bits]
+    Entry *by_low, *sorted;
+    uint32_t* totals;                     // [0]: tokens that have a gradient; [1]: those in several chunks
+    float* zeros;                         // the gradient
+    int64_t zero_count;
+    int fillers;                          // CTAs that fill
+};
+
+// A share of the zeros: part `part` of `parts`, by the CTAs from `first` on.
+__device__ void fill(const Sort& a, int first, int part, int parts) {
+    const int64_t quads = (a.zero_count + 3) / 4, per = (quads + parts - 1) / parts, begin = per * part, end = min(begin + per, quads);
+    const bool aligned = aligned16(a.zeros);
+    for (int64_t q = begin + (int64_t)(blockIdx.x - first) * blockDim.x + threadIdx.x; q < end; q += (int64_t)a.fillers * blockDim.x) {
+        if (aligned && q * 4 + 4 <= a.zero_count)
+            reinterpret_cast<float4*>(a.zeros)[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        else
+            for (int64_t e = q * 4; e < min(q * 4 + 4, a.zero_count); ++e) a.zeros[e] = 0.0f;
+    }
+}
+
+__device__ __forceinline__ uint32_t token_of(const Sort& a, int64_t i) {
+    if (i >= a.count) return kNone;
+    const int64_t token = token_at(a.tokens, i);
+    return (uint64_t)token < (uint64_t)a.vocab && token != a.padding ? (uint32_t)token : kNone;
+}
+
+// How many of the warp's earlier elements have the same digit (kNone: no element), which its counts are left with.
+template <int ROUNDS>
+__device__ __forceinline__ void rank_in_warp(uint16_t* counts, const uint32_t (&digit)[ROUNDS], uint32_t (&rank)[ROUNDS], int rounds) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        if (r >= rounds) break;
+        const bool is = digit[r] != kNone;
+        const uint32_t peers = __match_any_sync(0xffffffffu, digit[r]);
+        const uint32_t before = is ? counts[digit[r]] : 0u;
+        rank[r] = before + __popc(peers & ((1u << lane) - 1u));
+        __syncwarp();
+        if (is && lane == __ffs(peers) - 1) counts[digit[r]] = (uint16_t)(before + __popc(peers));
+        __syncwarp();
+    }
+}
+
+// Sums before each of the n <= 2 * 1024 values in shared memory, in place; `warps` holds a value for each warp.  Ends with a barrier.
+__device__ uint32_t sums_before(uint32_t* values, int n, uint32_t* warps) {
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, threads = blockDim.x, each = (n + threads - 1) / threads;
+    uint32_t own[4], sum = 0u;
+    __syncthreads();
+    for (int k = 0; k < each; ++k) {
+        own[k] = t * each + k < n ? values[t * each + k] : 0u;
+        sum += own[k];
+    }
+    uint32_t upto = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += v;
+    }
+    if (lane == 31) warps[warp] = upto;
+    __syncthreads();
+    uint32_t before = upto - sum, total = 0u;
+    for (int w = 0; w < threads / 32; ++w) {
+        if (w < warp) before += warps[w];
+        total += warps[w];
+    }
+    for (int k = 0; k < each; ++k) {
+        if (t * each + k < n) values[t * each + k] = before;
+        before += own[k];
+    }
+    __syncthreads();
+    return total;
+}
+
+// counts [warps][bins] -> what the warps before have, in place; totals [bins]
+__device__ void sums_over_warps(uint16_t* counts, uint32_t* totals, int bins, int warps) {
+    for (int b = threadIdx.x; b < bins; b += blockDim.x) {
+        uint32_t run = 0u;
+        for (int w = 0; w < warps; ++w) {
+            const uint32_t c = counts[w * bins + b];
+            counts[w * bins + b] = (uint16_t)run;
+            run += c;
+        }
+        totals[b] = run;
+    }
+}
+
+// Up to 8192 tokens in one CTA: a warp has neighbouring tokens in both passes, which keeps them stable.
+__global__ void __launch_bounds__(kSortThreads) sort_kernel(const Sort a) {
+    extern __shared__ __align__(16) unsigned char memory[];
+    __shared__ uint32_t warp_sums[kSortWarps];
+    if (blockIdx.x > 0) {
+        fill(a, 1, 0, 1);
+        next_may_start();
+        return;
+    }
+    Entry* entries = reinterpret_cast<Entry*>(memory);
+    const int most = 1 << max(a.low_bits, a.high_bits);
+    uint32_t* totals = reinterpret_cast<uint32_t*>(entries + (a.count + 31) / 32 * 32);
+    uint16_t* counts = reinterpret_cast<uint16_t*>(totals + most);
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, rounds = (int)((a.count + kSortThreads - 1) / kSortThreads);
+    uint32_t token[kRounds], place[kRounds], digit[kRounds], rank[kRounds];
+    int live = (int)a.count;
+    for (int pass = 0; pass < 2; ++pass) {
+        const int bins = 1 << (pass ? a.high_bits : a.low_bits);
+        for (int i = t; i < bins * kSortWarps / 2; i += kSortThreads) reinterpret_cast<uint32_t*>(counts)[i] = 0u;
+#pragma unroll
+        for (int r = 0; r < kRounds; ++r) {
+            token[r] = digit[r] = kNone;
+            const int i = (warp * rounds + r) * 32 + lane;
+            if (r >= rounds || i >= live) continue;
+            token[r] = pass ? entries[i].token : token_of(a, i);
+            place[r] = pass ? entries[i].place : (uint32_t)i;
+            if (token[r] != kNone) digit[r] = pass ? token[r] >> a.low_bits : token[r] & (bins - 1);
+        }
+        __syncthreads();
+        rank_in_warp<kRounds>(counts + warp * bins, digit, rank, rounds);
+        __syncthreads();
+        sums_over_warps(counts, totals, bins, kSortWarps);
+        live = (int)sums_before(totals, bins, warp_sums);
+#pragma unroll
+        for (int r = 0; r < kRounds; ++r) {
+            if (digit[r] == kNone) continue;
+            const uint32_t to = totals[digit[r]] + counts[warp * bins + digit[r]] + rank[r];
+            (pass ? a.sorted : entries)[to] = {token[r], place[r]};
+        }
+        __syncthreads();
+    }
+    if (t == 0) {
+        a.totals[0] = (uint32_t)live;
+        a.totals[1] = 0u;
+    }
+    next_may_start();
+}
+
+// The low digits of each tile of tokens.
+__global__ void __launch_bounds__(kTileThreads) count_kernel(const Sort a) {
+    extern __shared__ __align__(16) unsigned char memory[];
+    if ((int)blockIdx.x >= a.tiles) {
+        fill(a, a.tiles, 0, 3);
+        next_may_start();
+        return;
+    }
+    uint32_t* counts = reinterpret_cast<uint32_t*>(memory);
+    const int bins = 1 << a.low_bits, high = 1 << a.high_bits;
+    for (int b = threadIdx.x; b < bins; b += kTileThreads) counts[b] = 0u;
+    for (int b = threadIdx.x; b < high; b += kTileThreads) a.counts_high[(int64_t)blockIdx.x * high + b] = 0u;
+    if (blockIdx.x == 0 && threadIdx.x < 2) a.totals[threadIdx.x] = 0u;
+    __syncthreads();
+    const int64_t begin = (int64_t)blockIdx.x * a.tile;
+    for (int i = threadIdx.x; i < a.tile; i += kTileThreads) {
+        const uint32_t token = token_of(a, begin + i);
+        if (token != kNone) atomicAdd(&counts[token & (bins - 1)], 1u);
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < bins; b += kTileThreads) a.counts_low[(int64_t)blockIdx.x * bins + b] = counts[b];
+    next_may_start();
+}
+
+// Moves the elements of a tile to their places by one digit.  The counts of all tiles say where each starts.
+template <bool HIGH>
+__global__ void __launch_bounds__(kTileThreads) scatter_kernel(const Sort a) {
+    extern __shared__ __align__(16) unsigned char memory[];
+    __shared__ uint32_t warp_sums[kTileWarps];
+    if ((int)blockIdx.x >= a.tiles) {
+        // (not before the launch in front has ended: a chain of launches ends in their order only if each waits for the one before)
+        after_previous();
+        fill(a, a.tiles, HIGH ? 2 : 1, 3);
+        next_may_start();
+        return;
+    }
+    const int bits = HIGH ? a.high_bits : a.low_bits, bins = 1 << bits, t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    uint32_t* start = reinterpret_cast<uint32_t*>(memory);                            // where the tile's next element of each digit goes
+    uint32_t* totals = start + bins;
+    uint16_t* counts = reinterpret_cast<uint16_t*>(totals + bins);
+    after_previous();
+    const uint32_t* all = HIGH ? a.counts_high : a.counts_low;
+    for (int b = t; b < bins; b += kTileThreads) {
+        uint32_t before = 0u, sum = 0u;
+        for (int k = 0; k < a.tiles; ++k) {
+            if (k == (int)blockIdx.x) before = sum;
+            sum += __ldcg(all + (int64_t)k * bins + b);
+        }
+        start[b] = sum;
+        totals[b] = before;
+    }
+    const uint32_t live = sums_before(start, bins, warp_sums);
+    for (int b = t; b < bins; b += kTileThreads) start[b] += totals[b];
+    if (!HIGH && blockIdx.x == 0 && t == 0) a.totals[0] = live;
+    const int64_t tile_begin = (int64_t)blockIdx.x * a.tile, tile_end = min(tile_begin + a.tile, HIGH ? (int64_t)live : a.count);
+    uint32_t token[kRounds], place[kRounds], digit[kRounds], rank[kRounds];
+    for (int64_t begin = tile_begin; begin < tile_end; begin += kTile) {
+        for (int i = t; i < bins * kTileWarps / 2; i += kTileThreads) reinterpret_cast<uint32_t*>(counts)[i] = 0u;
+#pragma unroll
+        for (int r = 0; r < kRounds; ++r) {
+            token[r] = digit[r] = kNone;
+            const int64_t i = begin + (warp * kRounds + r) * 32 + lane;
+            if (i >= tile_end) continue;
+            if (HIGH) {
+                const uint2 e = __ldcg(reinterpret_cast<const uint2*>(a.by_low) + i);
+                token[r] = e.x;
+                place[r] = e.y;
+            } else {
+                token[r] = token_of(a, i);
+                place[r] = (uint32_t)i;
+            }
+            if (token[r] != kNone) digit[r] = HIGH ? token[r] >> a.low_bits : token[r] & (bins - 1);
+        }
+        __syncthreads();
+        rank_in_warp<kRounds>(counts + warp * bins, digit, rank, kRounds);
+        __syncthreads();
+        sums_over_warps(counts, totals, bins, kTileWarps);
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < kRounds; ++r) {
+            if (digit[r] == kNone) continue;
+            const uint32_t to = start[digit[r]] + counts[warp * bins + digit[r]] + rank[r];
+            (HIGH ? a.sorted : a.by_low)[to] = {token[r], place[r]};
+            if (!HIGH) atomicAdd(a.counts_high + ((int64_t)(to / (uint32_t)a.tile) << a.high_bits) + (token[r] >> a.low_bits), 1u);
+        }
+        __syncthreads();
+        for (int b = t; b < bins; b += kTileThreads) start[b] += totals[b];
+        __syncthreads();
+    }
+    next_may_start();
+}
+
+// ---- sums ---------------------------------------------------------------------------------------------------------
+
+constexpr int kColumns = 128;             // of a warp: four of a lane
+
+struct Sums {
+    const float *g, *table;
+    float* dw;
+    const Entry* sorted;
+    uint32_t* totals;
+    float* parts;                         // [chunks][2][dim]: what continues from the chunk before; what the next continues
+    uint32_t* list;                       // chunks in which a token starts that the next continues
+    int64_t table_row;
+    int dim, slabs, chunk;
+    uint32_t chunks;
+    bool scaled, drops;
+    float scale;
+    int32_t off;
+    Dropping drop;
+};
+
+__device__ __forceinline__ Entry entry_at(const Entry* sorted, uint32_t i) {
+    const uint2 e = __ldcg(reinterpret_cast<const uint2*>(sorted) + i);
+    return {e.x, e.y};
+}
+
+// The columns of a lane: four neighbours (VEC), or every 32nd.
+template <bool VEC>
+__device__ __forceinline__ int column(int slab, int lane, int k) { return slab * kColumns + (VEC ? lane * 4 + k : lane + 32 * k); }
+
+template <bool VEC>
+__device__ __forceinline__ void load_columns(const float* row, int slab, int lane, int dim, float (&v)[4]) {
+    if (VEC) {
+        const int c = column<true>(slab, lane, 0);
+        const float4 x = c < dim ? __ldg(reinterpret_cast<const float4*>(row + c)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = column<false>(slab, lane, k) < dim ? __ldg(row + column<false>(slab, lane, k)) : 0.0f;
+    }
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store_columns(float* row, int slab, int lane, int dim, const float (&v)[4]) {
+    if (VEC) {
+        const int c = column<true>(slab, lane, 0);
+        if (c < dim) *reinterpret_cast<float4*>(row + c) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (column<false>(slab, lane, k) < dim) row[column<false>(slab, lane, k)] = v[k];
+    }
+}
+
+template <bool VEC, bool SLOPES>
+__global__ void __launch_bounds__(kThreads) sum_kernel(const Sums a) {
+    constexpr int kAhead = 8;             // rows on their way
+    const int lane = threadIdx.x & 31;
+    const uint32_t unit = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+    const uint32_t chunk = unit / (uint32_t)a.slabs;
+    const int slab = (int)(unit - chunk * a.slabs);
+    after_previous();
+    const uint32_t live = __ldcg(a.totals), begin = chunk * (uint32_t)a.chunk;
+    if (chunk >= a.chunks || begin >= live) return;
+    const int n = (int)min((uint32_t)a.chunk, live - begin);
     const uint2 key = a.drops ? key_of(a.drop) : make_uint2(0u, 0u);
-    const bool in = c < a.dim;
-    const float slope = SLOPES && a.scaled && in ? mul_slope(__ldg(a.table + v * a.table_row + c), a.scale, a.off) : 1.0f;
-    float sum = 0.0f;
-    if (v != a.padding) {
-        for (int64_t first = 0; first < a.count; first += 32) {
-            const int64_t j = first + lane;
-            uint32_t here = __ballot_sync(0xffffffffu, j < a.count && a.tokens[j] == v);
-            for (; here; here &= here - 1) {
-                const int64_t e = (first + __ffs(here) - 1) * a.dim + c;
-                if (!in) continue;
-                float x = __ldg(g + e);
-                if (a.drops) x = philox_word((uint64_t)e, key) < a.drop.below ? 0.0f : mul(x, a.drop.scale, a.off);
-                if (a.scaled) x = SLOPES ? fmul(x, slope) : mul(x, a.scale, a.off);
-                sum = fadd(sum, x);
+    const Entry mine = lane < n ? entry_at(a.sorted, begin + lane) : Entry{kNone, 0u};
+    const uint32_t token_before = begin > 0 ? entry_at(a.sorted, begin - 1).token : kNone;
+    const uint32_t token_after = begin + n < live ? entry_at(a.sorted, begin + n).token : kNone;
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f}, slope[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+    uint32_t now = kNone;
+    for (int first = 0; first < n; first += kAhead) {
+        float v[kAhead][4];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const uint32_t place = __shfl_sync(0xffffffffu, mine.place, (first + j) & 31);
+            if (first + j < n) load_columns<VEC>(a.g + (int64_t)place * a.dim, slab, lane, a.dim, v[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            if (first + j >= n) break;
+            const uint32_t token = __shfl_sync(0xffffffffu, mine.token, first + j), place = __shfl_sync(0xffffffffu, mine.place, first + j);
+            if (token != now) {
+                // a token ends and one starts
+                if (now != kNone) {
+                    const bool whole = now != token_before;
+                    store_columns<VEC>(whole ? a.dw + (int64_t)now * a.dim : a.parts + (int64_t)chunk * 2 * a.dim, slab, lane, a.dim, sum);
+                }
+                now = token;
+                sum[0] = sum[1] = sum[2] = sum[3] = 0.0f;
+                if (SLOPES && a.scaled) {
+                    load_columns<VEC>(a.table + (int64_t)token * a.table_row, slab, lane, a.dim, slope);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) slope[k] = mul_slope(slope[k], a.scale, a.off);
+                }
+            }
+            uint32_t bits[4] = {0u, 0u, 0u, 0u};
+            if (a.drops) {
+                const uint64_t e = (uint64_t)place * a.dim;
+                if (VEC) {
+                    const uint4 w = philox((e + column<true>(slab, lane, 0)) >> 2, key);
+                    bits[0] = w.x, bits[1] = w.y, bits[2] = w.z, bits[3] = w.w;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) bits[k] = philox_word(e + column<false>(slab, lane, k), key);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float x = v[j][k];
+                if (a.drops) x = bits[k] < a.drop.below ? 0.0f : mul(x, a.drop.scale, a.off);
+                if (a.scaled) x = SLOPES ? fmul(x, slope[k]) : mul(x, a.scale, a.off);
+                sum[k] = fadd(sum[k], x);
             }
         }
     }
-    if (in) dw[v * a.dim + c] = sum;
+    const bool from_before = now == token_before, goes_on = now == token_after;
+    if (!from_before && !goes_on) {
+        store_columns<VEC>(a.dw + (int64_t)now * a.dim, slab, lane, a.dim, sum);
+    } else {
+        store_columns<VEC>(a.parts + ((int64_t)chunk * 2 + !from_before) * a.dim, slab, lane, a.dim, sum);
+        if (!from_before && slab == 0 && lane == 0) a.list[atomicAdd(a.totals + 1, 1u)] = chunk;
+    }
+    next_may_start();
+}
+
+// The parts of a token: the end of the chunk that it starts in, the beginnings of those that it goes on in.  A warp has neighbouring ones of them.
+template <bool VEC>
+__global__ void __launch_bounds__(kThreads) join_kernel(const Sums a) {
+    constexpr int kWarps = kThreads / 32, kAhead = 8;
+    __shared__ float stage[kWarps][kColumns];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, slab = blockIdx.y;
+    after_previous();
+    const uint32_t live = __ldcg(a.totals), many = __ldcg(a.totals + 1);
+    for (uint32_t i = blockIdx.x; i < many; i += gridDim.x) {
+        const uint32_t chunk = __ldcg(a.list + i);
+        const uint32_t token = entry_at(a.sorted, (chunk + 1) * (uint32_t)a.chunk).token;
+        uint32_t more = 1;                                                            // chunks that it goes on in
+        for (;; more += 32) {
+            const uint64_t at = (uint64_t)(chunk + 1 + more + lane) * a.chunk;
+            const uint32_t other = __ballot_sync(0xffffffffu, at >= live || entry_at(a.sorted, (uint32_t)at).token != token);
+            if (other) {
+                more += __ffs(other) - 1;
+                break;
+            }
+        }
+        const uint32_t count = more + 1, each = (count + kWarps - 1) / kWarps, from = min(warp * each, count), to = min(from + each, count);
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t first = from; first < to; first += kAhead) {
+            float v[kAhead][4];
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                const uint32_t part = first + j;
+                if (part >= to) continue;
+                const float* row = a.parts + ((int64_t)(chunk + part) * 2 + (part == 0)) * a.dim;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[j][k] = column<VEC>(slab, lane, k) < a.dim ? __ldcg(row + column<VEC>(slab, lane, k)) : 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j)
+                if (first + j < to)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) sum[k] = fadd(sum[k], v[j][k]);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) stage[warp][VEC ? lane * 4 + k : lane + 32 * k] = sum[k];
+        __syncthreads();
+        if (threadIdx.x < kColumns && slab * kColumns + threadIdx.x < a.dim) {
+            float s = stage[0][threadIdx.x];
+            for (int w = 1; w < kWarps; ++w) s = fadd(s, stage[w][threadIdx.x]);
+            a.dw[(int64_t)token * a.dim + slab * kColumns + threadIdx.x] = s;
+        }
+        __syncthreads();
+    }
 }
 
 constexpr int64_t kMostTokens = 0x7fffffff, kMostRows = 1 << 22;
@@ -112,6 +531,94 @@ Embedding described(const int64_t* tokens, const float* table, const float* pos,
     return a;
 }
 
+// How the gradient of a table is worked on, and where its scratch lies.
+struct Plan {
+    int low_bits, high_bits, tiles, tile, chunk;
+    int64_t chunks;
+    size_t totals, counts_low, counts_high, by_low, sorted, list, parts, bytes;
+};
+
+Plan planned(int64_t count, int64_t vocab, int64_t dim) {
+    Plan p{};
+    int bits = 2;
+    while (((int64_t)1 << bits) < vocab) ++bits;
+    p.low_bits = (bits + 1) / 2;
+    p.high_bits = bits - p.low_bits;
+    if (count > kMostInOne) {
+        const int64_t each = (count + kMostTiles - 1) / kMostTiles;
+        p.tile = (int)((each + kTile - 1) / kTile * kTile);
+        p.tiles = (int)((count + p.tile - 1) / p.tile);
+    }
+    p.chunk = count > (1 << 18) ? 32 : 16;
+    p.chunks = (count + p.chunk - 1) / p.chunk;
+    size_t at = 0;
+    const auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += (bytes + 255) / 256 * 256;
+        return here;
+    };
+    p.totals = take(2 * sizeof(uint32_t));
+    p.counts_low = take((size_t)p.tiles << p.low_bits << 2);
+    p.counts_high = take((size_t)p.tiles << p.high_bits << 2);
+    p.by_low = take(p.tiles ? (size_t)count * sizeof(Entry) : 0);
+    p.sorted = take((size_t)count * sizeof(Entry));
+    p.list = take((size_t)p.chunks * sizeof(uint32_t));
+    p.parts = take((size_t)p.chunks * 2 * (size_t)dim * sizeof(float));
+    p.bytes = at;
+    return p;
+}
+
+// (what the kernels may ask for, whatever a call needs: calls of two threads set the same)
+constexpr int kMostBins = 1 << 11;
+constexpr size_t kSortMemory = kMostInOne * sizeof(Entry) + kMostBins * 4 + kMostBins * kSortWarps * 2;
+constexpr size_t kTileMemory = kMostBins * 8 + kMostBins * kTileWarps * 2;
+static_assert(kSortMemory <= 220 * 1024 && kTileMemory <= 100 * 1024);
+
+template <class K>
+int allow(K* kernel, size_t memory, size_t most) {
+    if (memory <= 40 * 1024) return PAMK_OK;
+    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+    return err == cudaSuccess ? PAMK_OK : record_cuda_error(err);
+}
+
+template <class... P, class... A>
+int launch_next(void (*kernel)(P...), dim3 grid, unsigned threads, size_t memory, cudaStream_t st, A... args) {
+    cudaLaunchAttribute overlap{};
+    overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    overlap.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = memory;
+    config.stream = st;
+    config.attrs = &overlap;
+    config.numAttrs = 1;
+    const cudaError_t err = cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...);
+    count_launch();
+    return err == cudaSuccess ? PAMK_OK : record_cuda_error(err);
+}
+
+int sort_tokens(const Plan& p, Sort s, cudaStream_t st) {
+    const int64_t fill_ctas = (s.zero_count + kSortThreads * 4 - 1) / (kSortThreads * 4);
+    s.fillers = (int)(fill_ctas < 2 * sm_count() ? fill_ctas : 2 * sm_count());
+    if (!p.tiles) {
+        const int most = 1 << p.low_bits;
+        const size_t memory = (size_t)(s.count + 31) / 32 * 32 * sizeof(Entry) + most * 4 + (size_t)most * kSortWarps * 2;
+        if (const int status = allow(sort_kernel, memory, kSortMemory)) return status;
+        sort_kernel<<<1 + s.fillers, kSortThreads, memory, st>>>(s);
+        return check_launch();
+    }
+    const size_t low = ((size_t)8 << p.low_bits) + ((size_t)kTileWarps * 2 << p.low_bits), high = ((size_t)8 << p.high_bits) + ((size_t)kTileWarps * 2 << p.high_bits);
+    if (const int status = allow(scatter_kernel<false>, low, kTileMemory)) return status;
+    if (const int status = allow(scatter_kernel<true>, high, kTileMemory)) return status;
+    s.fillers *= 2;
+    const unsigned ctas = (unsigned)(p.tiles + s.fillers);
+    count_kernel<<<ctas, kTileThreads, (size_t)4 << p.low_bits, st>>>(s);
+    if (const int status = check_launch()) return status;
+    if (const int status = launch_next(scatter_kernel<false>, dim3(ctas), kTileThreads, low, st, s)) return status;
+    return launch_next(scatter_kernel<true>, dim3(ctas), kTileThreads, high, st, s);
+}
+
 }  // namespace
 }  // namespace pamk
 
@@ -126,13 +633,24 @@ int pamk_embedding(const int64_t* tokens, const float* table, const float* posit
     if (const int status = check_sizes(a, p)) return status;
     if (count == 0 || dim == 0) return PAMK_OK;
     if (!tokens || !out || (vocab > 0 && !table) || (dy && !a.drops)) return PAMK_ERR_ARG;
-    const int64_t ctas = (count * dim + 4 * kThreads - 1) / (4 * kThreads);
+    const int64_t n = count * dim;
+    const auto st = (cudaStream_t)stream;
+    if (dim % 4 == 0 && n < ((int64_t)1 << 33) && aligned16(table) && table_row % 4 == 0 && aligned16(positions) && positions_row % 4 == 0 && aligned16(dy) && aligned16(out)) {
+        const uint32_t quads = (uint32_t)(n / 4), ctas = (quads + kThreads - 1) / kThreads;
+        (dy ? embed_quads_kernel<true> : embed_quads_kernel<false>)<<<ctas, kThreads, 0, st>>>(a, dy, out, quads, (uint32_t)(dim / 4));
+        return check_launch();
+    }
+    const int64_t ctas = (n + 4 * kThreads - 1) / (4 * kThreads);
     if (ctas > 0x7fffffff) return PAMK_ERR_SIZE;
-    (dy ? embed_kernel<true> : embed_kernel<false>)<<<(unsigned)ctas, kThreads, 0, (cudaStream_t)stream>>>(a, dy, out);
+    (dy ? embed_kernel<true> : embed_kernel<false>)<<<(unsigned)ctas, kThreads, 0, st>>>(a, dy, out);
     return check_launch();
 }
 
-size_t pamk_embedding_bwd_workspace_bytes(int64_t count, int64_t vocab, int64_t dim) { return 0 * (size_t)(count + vocab + dim); }
+size_t pamk_embedding_bwd_workspace_bytes(int64_t count, int64_t vocab, int64_t dim) {
+    using namespace pamk;
+    if (count < 1 || count > kMostTokens || vocab < 1 || vocab > kMostRows || dim < 1 || dim > 0x7fffffff - 4) return 0;
+    return planned(count, vocab, dim).bytes;
+}
 
 int pamk_embedding_bwd(const int64_t* tokens, const float* dy, const float* table, float* dtable, int64_t count, int64_t vocab, int64_t dim, int64_t table_row,
                        int64_t padding, int has_scale, float scale, double p, const int64_t* seed_at, int64_t seed, float offset, int approx_bwd, void* workspace,
@@ -143,10 +661,58 @@ int pamk_embedding_bwd(const int64_t* tokens, const float* dy, const float* tabl
     if (const int status = check_sizes(a, p)) return status;
     if (vocab == 0 || dim == 0) return PAMK_OK;
     if (!dtable || (count > 0 && (!tokens || !dy)) || (!approx_bwd && (a.drops || (has_scale && !table)))) return PAMK_ERR_ARG;
-    const int64_t columns = (dim + 31) / 32;
-    if (columns > 65535) return PAMK_ERR_SIZE;
-    (approx_bwd ? table_grad_kernel<false> : table_grad_kernel<true>)<<<dim3((unsigned)((vocab + 7) / 8), (unsigned)columns), kThreads, 0, (cudaStream_t)stream>>>(a, dy, dtable);
-    return check_launch();
+    const auto st = (cudaStream_t)stream;
+    if (count == 0) {
+        const cudaError_t err = cudaMemsetAsync(dtable, 0, (size_t)vocab * dim * sizeof(float), st);
+        return err == cudaSuccess ? PAMK_OK : record_cuda_error(err);
+    }
+    const Plan plan = planned(count, vocab, dim);
+    const int64_t slabs = (dim + kColumns - 1) / kColumns, ctas = (plan.chunks * slabs + kThreads / 32 - 1) / (kThreads / 32);
+    if (slabs > 65535 || ctas > (1 << 28)) return PAMK_ERR_SIZE;
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < plan.bytes) return PAMK_ERR_WORKSPACE;
+    char* ws = static_cast<char*>(workspace);
+    Sort s{};
+    s.tokens = tokens;
+    s.count = count;
+    s.vocab = vocab;
+    s.padding = padding;
+    s.low_bits = plan.low_bits;
+    s.high_bits = plan.high_bits;
+    s.tiles = plan.tiles;
+    s.tile = plan.tile;
+    s.counts_low = reinterpret_cast<uint32_t*>(ws + plan.counts_low);
+    s.counts_high = reinterpret_cast<uint32_t*>(ws + plan.counts_high);
+    s.by_low = reinterpret_cast<Entry*>(ws + plan.by_low);
+    s.sorted = reinterpret_cast<Entry*>(ws + plan.sorted);
+    s.totals = reinterpret_cast<uint32_t*>(ws + plan.totals);
+    s.zeros = dtable;
+    s.zero_count = vocab * dim;
+    if (const int status = sort_tokens(plan, s, st)) return status;
+    Sums u{};
+    u.g = dy;
+    u.table = table;
+    u.dw = dtable;
+    u.sorted = s.sorted;
+    u.totals = s.totals;
+    u.parts = reinterpret_cast<float*>(ws + plan.parts);
+    u.list = reinterpret_cast<uint32_t*>(ws + plan.list);
+    u.table_row = table_row;
+    u.dim = (int)dim;
+    u.slabs = (int)slabs;
+    u.chunk = plan.chunk;
+    u.chunks = (uint32_t)plan.chunks;
+    u.scaled = a.scaled;
+    u.drops = a.drops;
+    u.scale = scale;
+    u.off = a.off;
+    u.drop = a.drop;
+    const bool slopes = !approx_bwd && a.scaled;
+    const bool vec = dim % 4 == 0 && aligned16(dy) && aligned16(dtable) && (!slopes || (aligned16(table) && table_row % 4 == 0));
+    const auto sums = vec ? (slopes ? sum_kernel<true, true> : sum_kernel<true, false>) : (slopes ? sum_kernel<false, true> : sum_kernel<false, false>);
+    if (const int status = launch_next(sums, dim3((unsigned)ctas), kThreads, 0, st, u)) return status;
+    const int64_t wide = (4 * sm_count() + slabs - 1) / slabs;
+    const unsigned joins = (unsigned)(plan.chunks < wide ? plan.chunks : wide);
+    return launch_next(vec ? join_kernel<true> : join_kernel<false>, dim3(joins, (unsigned)slabs), kThreads, 0, st, u);
 }
 
 }
