@@ -60,13 +60,14 @@ using torch::autograd::variable_list;
     X(pamk_status_string) X(pamk_last_cuda_error) X(pamk_matmul_auto_split) X(pamk_matmul_bwd_auto_split) \
     X(pamk_matmul_scratch_bytes) X(pamk_column_sum_workspace_bytes) X(pamk_layer_norm_max_width) X(pamk_layer_norm_stats_per_row)      \
     X(pamk_layer_norm_bwd_workspace_bytes) X(pamk_softmax_max_len) X(pamk_softmax_workspace_bytes)                                      \
-    X(pamk_cached_attention_workspace_bytes) X(pamk_beam_select_workspace_bytes)
+    X(pamk_cached_attention_workspace_bytes) X(pamk_beam_select_workspace_bytes) X(pamk_embedding_bwd_workspace_bytes)
 #define PAMK_LAUNCHES(X)                                                                                  \
     X(pamk_pam_fwd) X(pamk_pad_fwd) X(pamk_pam_grad) X(pamk_pad_grad) X(pamk_matmul_bias)                 \
     X(pamk_matmul_strided) X(pamk_matmul_bwd) X(pamk_column_sum) X(pamk_layer_norm_fwd)                   \
     X(pamk_layer_norm_fwd_save) X(pamk_layer_norm_bwd) X(pamk_layer_norm_bwd_saved) X(pamk_softmax_fwd)   \
     X(pamk_softmax_fwd_save) X(pamk_softmax_bwd) X(pamk_softmax_bwd_saved) X(pamk_adam_step) \
-    X(pamk_cached_attention) X(pamk_beam_select) X(pamk_reorder_states)
+    X(pamk_cached_attention) X(pamk_beam_select) X(pamk_reorder_states) X(pamk_sample) \
+    X(pamk_dropout) X(pamk_dropout_bwd) X(pamk_embedding) X(pamk_embedding_bwd)
 
 std::atomic<bool> g_nvtx{false};         // set_nvtx
 
@@ -642,6 +643,105 @@ struct AttentionHeadsRule {
     }
 };
 
+// What a mask is drawn from: a tensor of one element, or a number.
+struct Seed {
+    Tensor t;
+    int64_t n = 0;
+    const int64_t* at() const { return t.defined() ? static_cast<const int64_t*>(t.data_ptr()) : nullptr; }
+};
+
+Tensor dropped(const Tensor& x, const Tensor& residual, double p, const Seed& seed, double offset) {
+    Tensor out = empty_on(x.sizes(), x);
+    check(lib.pamk_dropout(ptr(x), ptr(residual), ptr(out), x.numel(), p, seed.at(), seed.n, (float)offset, stream_of(x)), "pamk_dropout");
+    return out;
+}
+
+// The backward pass draws the mask again; the exact gradients also take the input.
+struct DropoutRule {
+    double p, offset;
+    bool approx, has_r, seed_kept;
+    int64_t seed;
+    std::string name() const { return "PamDropoutBackward"; }
+    std::string key() const { return bytes_of(p, offset, approx, has_r, seed_kept, seed); }
+    variable_list grads(const variable_list& kept, const Tensor& grad, const Wanted& wanted) const {
+        const Seed from{seed_kept ? kept[0] : Tensor(), seed};
+        variable_list out(1 + has_r);
+        if (wanted(0)) {
+            const Tensor g = grad.contiguous();
+            if (approx) {
+                out[0] = dropped(g, Tensor(), p, from, offset);
+            } else {
+                const Tensor& x = kept[seed_kept];
+                out[0] = empty_on(x.sizes(), x);
+                check(lib.pamk_dropout_bwd(ptr(x), ptr(g), ptr(out[0]), x.numel(), p, from.at(), from.n, (float)offset, stream_of(x)), "pamk_dropout_bwd");
+            }
+        }
+        if (has_r && wanted(1)) out[1] = grad;
+        return out;
+    }
+};
+
+// The settings of an embedding, and what its kernels take.
+struct EmbeddingCall {
+    int64_t padding, vocab, dim, pos_count;
+    bool has_scale;
+    double scale, p, offset;
+    Tensor forward(const Tensor& tokens, const Tensor& weight, const Tensor& pos, const Tensor& dy, const Seed& seed) const {
+        at::DimVector shape(tokens.sizes());
+        shape.push_back(dim);
+        Tensor out = empty_on(shape, weight);
+        check(lib.pamk_embedding(static_cast<const int64_t*>(tokens.data_ptr()), ptr(weight), ptr(pos), ptr(dy), ptr(out), tokens.numel(), vocab, dim, weight.stride(0),
+                                 pos.defined() && pos.dim() == 2 ? pos.stride(0) : 0, pos_count, has_scale, (float)scale, p, seed.at(), seed.n, (float)offset, stream_of(weight)),
+              "pamk_embedding");
+        return out;
+    }
+};
+
+// The exact gradients take the table, and with dropout the positions; the others nothing but the tokens and the seed.
+struct EmbeddingRule {
+    EmbeddingCall call;
+    bool approx, has_pos, seed_kept;
+    int64_t seed;
+    std::vector<int64_t> pos_shape;
+    std::string name() const { return "PamEmbeddingBackward"; }
+    std::string key() const {
+        return bytes_of(call.padding, call.vocab, call.dim, call.pos_count, call.has_scale, call.scale, call.p, call.offset, approx, has_pos, seed_kept, seed) +
+               bytes_of_list(pos_shape);
+    }
+    variable_list grads(const variable_list& kept, const Tensor& grad, const Wanted& wanted) const {
+        size_t k = 0;
+        const Tensor tokens = kept[k++];
+        Seed from;
+        from.n = seed;
+        if (seed_kept) from.t = kept[k++];
+        Tensor weight, pos;
+        if (!approx) {
+            weight = kept[k++];
+            if (has_pos) pos = kept[k++];
+        }
+        Tensor g = grad.contiguous();
+        double p = call.p;
+        const bool need_pos = has_pos && wanted(1);
+        if (p > 0 && (need_pos || !approx)) {             // the gradient before the dropout, which two sums or the slopes need
+            g = approx ? dropped(g, Tensor(), p, from, call.offset) : call.forward(tokens, weight, pos, g, from);
+            p = 0.0;
+        }
+        variable_list out(1 + has_pos);
+        if (wanted(0)) {
+            out[0] = empty_on({call.vocab, call.dim}, g);
+            const size_t bytes = lib.pamk_embedding_bwd_workspace_bytes(tokens.numel(), call.vocab, call.dim);
+            Tensor ws;
+            if (bytes) ws = scratch_bytes(bytes, g);
+            check(lib.pamk_embedding_bwd(static_cast<const int64_t*>(tokens.data_ptr()), ptr(g), ptr(weight), ptr(out[0]), tokens.numel(), call.vocab, call.dim,
+                                         weight.defined() ? weight.stride(0) : 0, call.padding, call.has_scale, (float)call.scale, p, from.at(), from.n,
+                                         (float)call.offset, approx, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(g)),
+                  "pamk_embedding_bwd");
+        }
+        if (need_pos) out[1] = column_sum(g, tokens.numel() / call.pos_count, call.pos_count * call.dim).view(pos_shape);
+        return out;
+    }
+};
+
 // ---- operators -----------------------------------------------------------------------------------------------
 
 std::optional<Tensor> op_linear(const Tensor& x, const Tensor& w, const Tensor& bias, double offset, bool approx_x, bool approx_w) {
@@ -840,6 +940,70 @@ std::optional<Tensor> op_attention_heads(const Tensor& gq, const Tensor& gk, con
     return out;
 }
 
+// ---- dropout and embedding --------------------------------------------------------------------------------------
+
+// A seed that was given, or one from the device's default generator.
+bool seed_ok(Seed& seed, bool drawn, const Tensor& like) {
+    if (drawn) seed.t = at::randint(std::numeric_limits<int64_t>::min(), std::numeric_limits<int64_t>::max(), {1}, like.options().dtype(at::kLong).requires_grad(false));
+    return !seed.t.defined() || (readable(seed.t) && seed.t.scalar_type() == at::kLong && seed.t.numel() == 1 && seed.t.device() == like.device());
+}
+
+std::optional<Tensor> op_dropout(const Tensor& x, double p, Seed seed, bool drawn, const Tensor& r, double offset, bool approx) {
+    if (!usable(x) || !(p > 0 && p < 1) || x.numel() == 0) return {};
+    if (r.defined() && (!usable(r) || r.device() != x.device() || r.sizes() != x.sizes())) return {};
+    c10::cuda::CUDAGuard guard(x.device());
+    Tensor xc, y;
+    {
+        at::AutoGradMode no_grad(false);
+        if (!seed_ok(seed, drawn, x)) return {};
+        xc = x.contiguous();
+        y = dropped(xc, r.defined() ? r.contiguous() : r, p, seed, offset);
+    }
+    if (recording() && (wants_grad(x) || wants_grad(r))) {
+        const DropoutRule rule{p, offset, approx, r.defined(), seed.t.defined(), seed.n};
+        auto fn = r.defined() ? node(rule, x, r) : node(rule, x);
+        if (seed.t.defined()) fn->keep({seed.t});
+        if (!approx) fn->keep({xc});
+        torch::autograd::set_history(y, fn);
+    }
+    return y;
+}
+
+std::optional<Tensor> op_embedding(const Tensor& tokens, const Tensor& weight, std::optional<double> scale, const Tensor& pos, int64_t padding, double p, Seed seed,
+                                   bool drawn, double offset, bool approx) {
+    if (!usable(weight) || weight.dim() != 2 || weight.numel() == 0 || (weight.size(1) > 1 && weight.stride(1) != 1)) return {};
+    if (!readable(tokens) || tokens.scalar_type() != at::kLong || tokens.device() != weight.device() || tokens.numel() == 0 || !tokens.is_contiguous()) return {};
+    if (!(p >= 0 && p < 1)) return {};
+    int64_t pos_count = 0;
+    if (pos.defined()) {
+        if (!usable(pos) || pos.device() != weight.device() || pos.dim() < 1 || pos.dim() > 2 || pos.size(-1) != weight.size(1) || (pos.size(-1) > 1 && pos.stride(-1) != 1))
+            return {};
+        pos_count = pos.dim() == 2 ? pos.size(0) : 1;
+        if (pos_count != 1 && (tokens.dim() == 0 || pos_count != tokens.size(-1))) return {};
+    }
+    c10::cuda::CUDAGuard guard(weight.device());
+    const EmbeddingCall call{padding, weight.size(0), weight.size(1), pos_count, scale.has_value(), scale.value_or(0.0), p, offset};
+    Tensor y;
+    {
+        at::AutoGradMode no_grad(false);
+        if (p > 0 ? !seed_ok(seed, drawn, weight) : seed.t.defined()) return {};
+        y = call.forward(tokens, weight, pos, Tensor(), seed);
+    }
+    if (recording() && (wants_grad(weight) || wants_grad(pos))) {
+        EmbeddingRule rule{call, approx || (!scale && p == 0), pos.defined(), seed.t.defined(), seed.n, {}};
+        if (pos.defined()) rule.pos_shape = pos.sizes().vec();
+        auto fn = pos.defined() ? node(rule, weight, pos) : node(rule, weight);
+        fn->keep({tokens});
+        if (seed.t.defined()) fn->keep({seed.t});
+        if (!rule.approx) {
+            fn->keep({weight});
+            if (pos.defined()) fn->keep({pos});
+        }
+        torch::autograd::set_history(y, fn);
+    }
+    return y;
+}
+
 // ---- text generation --------------------------------------------------------------------------------------------
 
 // A cache's lengths as the caller gave them: none, a number or a tensor.
@@ -927,6 +1091,50 @@ std::optional<std::array<Tensor, 3>> op_beam_select(const Tensor& logits, const 
                                logits.stride(1), ban[0], ban[1], ws.data_ptr(), bytes, stream_of(logits)),
           "pamk_beam_select");
     return std::array<Tensor, 3>{best, beams, tokens};
+}
+
+// One number for all rows, or a tensor with one for each.
+template <class T>
+struct Setting {
+    Tensor t;
+    T n{};
+    bool ok(at::ScalarType type, const Tensor& like) const {
+        return !t.defined() || (readable(t) && t.scalar_type() == type && t.device() == like.device() && t.sizes() == like.sizes() && t.is_contiguous());
+    }
+    template <class P>
+    const P* at() const { return t.defined() ? static_cast<const P*>(t.data_ptr()) : nullptr; }
+};
+
+// (tokens, scores)
+std::optional<std::array<Tensor, 2>> op_sample(const Tensor& logits, const Tensor& uniform, const Setting<double>& temperature, const Setting<int64_t>& top_k,
+                                               const Setting<double>& top_p, const Setting<double>& min_p, const Tensor& banned) {
+    if (!usable(logits) || logits.dim() < 1 || logits.numel() == 0 || wants_grad(logits) || logits.stride(-1) != 1) return {};
+    if (logits.dim() != 2 && !logits.is_contiguous()) return {};
+    if (!usable(uniform) || uniform.device() != logits.device() || wants_grad(uniform) || !uniform.is_contiguous() ||
+        uniform.sizes() != logits.sizes().slice(0, logits.dim() - 1))
+        return {};
+    const int64_t V = logits.size(-1), rows = uniform.numel();
+    if (V > 1 << 18) return {};
+    if (!temperature.ok(at::kFloat, uniform) || !top_k.ok(at::kLong, uniform) || !top_p.ok(at::kFloat, uniform) || !min_p.ok(at::kFloat, uniform)) return {};
+    if (!temperature.t.defined() && !(temperature.n >= 0x1p-126 && temperature.n <= 0x1p127)) return {};
+    if ((!top_k.t.defined() && (top_k.n < 0 || top_k.n > int64_t(1) << 62)) || (!top_p.t.defined() && !(top_p.n >= 0x1p-24 && top_p.n <= 1.0)) ||
+        (!min_p.t.defined() && !(min_p.n >= 0.0 && min_p.n <= 1.0)))
+        return {};
+    int64_t ban_row = 0;
+    if (banned.defined()) {
+        if (!readable(banned) || banned.scalar_type() != at::kBool || banned.device() != logits.device() || !banned.is_contiguous()) return {};
+        if (banned.sizes() == logits.sizes())
+            ban_row = V;
+        else if (banned.dim() != 1 || banned.size(0) != V)
+            return {};
+    }
+    c10::cuda::CUDAGuard guard(logits.device());
+    Tensor tokens = at::detail::empty_cuda(uniform.sizes(), at::kLong, logits.device(), std::nullopt), scores = empty_on(uniform.sizes(), logits);
+    check(lib.pamk_sample(ptr(logits), ptr(uniform), banned.defined() ? static_cast<const unsigned char*>(banned.data_ptr()) : nullptr,
+                          static_cast<int64_t*>(tokens.data_ptr()), ptr(scores), rows, V, logits.dim() == 2 ? logits.stride(0) : V, ban_row, temperature.at<float>(),
+                          (float)temperature.n, top_k.at<int64_t>(), top_k.n, top_p.at<float>(), (float)top_p.n, min_p.at<float>(), (float)min_p.n, stream_of(logits)),
+          "pamk_sample");
+    return std::array<Tensor, 2>{tokens, scores};
 }
 
 // True once the states are moved; false where the call is for the Python layer: all that it refuses, and views of one buffer
@@ -1228,6 +1436,88 @@ PyObject* py_beam_select(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     });
 }
 
+// A seed: a whole number, a tensor, or None for one to be drawn.
+bool as_seed(PyObject* o, Seed& seed, bool& drawn) {
+    drawn = o == Py_None;
+    if (PyLong_CheckExact(o)) return as_int(o, seed.n);
+    return as_tensor(o, seed.t);
+}
+
+// dropout(x, p, seed | None, residual | None, offset, approx_bwd)
+PyObject* py_dropout(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    PAMK_ARGS(6)
+    return operator_call([&]() -> PyObject* {
+        Tensor x, r;
+        double p, off;
+        Seed seed;
+        bool drawn, u, v;
+        if (!as_tensor(a[0], x) || PyBool_Check(a[1]) || !as_number(a[1], p) || !as_seed(a[2], seed, drawn) || !as_tensor(a[3], r) || !as_offset(a[4], off) ||
+            !as_pair(a[5], u, v) || u != v)
+            return none();
+        return wrapped([&] { return op_dropout(x, p, seed, drawn, r, off, u); });
+    });
+}
+
+// embedding(tokens, weight, scale | None, positions | None, padding or -1, p, seed | None, offset, approx_bwd)
+PyObject* py_embedding(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    PAMK_ARGS(9)
+    return operator_call([&]() -> PyObject* {
+        Tensor tokens, weight, pos;
+        std::optional<double> scale;
+        double p, off, by;
+        int64_t padding;
+        Seed seed;
+        bool drawn, u, v;
+        if (a[2] != Py_None) {
+            if (PyBool_Check(a[2]) || !as_number(a[2], by)) return none();
+            scale = by;
+        }
+        if (!as_tensor(a[0], tokens) || !as_tensor(a[1], weight) || !as_tensor(a[3], pos) || !as_int(a[4], padding) || !as_number(a[5], p) ||
+            !as_seed(a[6], seed, drawn) || !as_offset(a[7], off) || !as_pair(a[8], u, v) || u != v)
+            return none();
+        return wrapped([&] { return op_embedding(tokens, weight, scale, pos, padding, p, seed, drawn, off, u); });
+    });
+}
+
+bool as_setting(PyObject* o, Setting<double>& s) {
+    if (PyBool_Check(o)) return false;
+    return as_number(o, s.n) || (as_tensor(o, s.t) && s.t.defined());
+}
+bool as_setting(PyObject* o, Setting<int64_t>& s) {
+    if (PyLong_CheckExact(o)) return as_int(o, s.n);
+    return as_tensor(o, s.t) && s.t.defined();
+}
+
+// sample(logits, uniform, temperature, top_k, top_p, min_p, banned | None)
+PyObject* py_sample(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    PAMK_ARGS(7)
+    return operator_call([&]() -> PyObject* {
+        Tensor x, uniform, banned;
+        Setting<double> temperature, top_p, min_p;
+        Setting<int64_t> top_k;
+        if (!as_tensor(a[0], x) || !as_tensor(a[1], uniform) || !as_setting(a[2], temperature) || !as_setting(a[3], top_k) || !as_setting(a[4], top_p) ||
+            !as_setting(a[5], min_p) || !as_tensor(a[6], banned))
+            return none();
+        std::optional<std::array<Tensor, 2>> found;
+        {
+            const Unlocked others_may_run;
+            found = op_sample(x, uniform, temperature, top_k, top_p, min_p, banned);
+        }
+        if (!found) return none();
+        PyObject* out = PyTuple_New(2);
+        if (out == nullptr) return nullptr;
+        for (int i = 0; i < 2; ++i) {
+            PyObject* t = THPVariable_Wrap(std::move((*found)[i]));
+            if (t == nullptr) {
+                Py_DECREF(out);
+                return nullptr;
+            }
+            PyTuple_SET_ITEM(out, i, t);
+        }
+        return out;
+    });
+}
+
 // reorder_states(list of states, parents, used: number, tensor or None): True, or None
 PyObject* py_reorder_states(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     PAMK_ARGS(3)
@@ -1453,6 +1743,9 @@ PyMethodDef methods[] = {
     PAMK_FAST("cached_attention", py_cached_attention),
     PAMK_FAST("beam_select", py_beam_select),
     PAMK_FAST("reorder_states", py_reorder_states),
+    PAMK_FAST("dropout", py_dropout),
+    PAMK_FAST("embedding", py_embedding),
+    PAMK_FAST("sample", py_sample),
     PAMK_FAST("adam_collect", py_adam_collect),
     PAMK_FAST("adam_apply", py_adam_apply),
     {nullptr, nullptr, 0, nullptr},

@@ -212,6 +212,10 @@ def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, b
 
     Returns (tokens int64 [...], scores [...]): a score is the PAM log-softmax of pad(logits, temperature) at the token, over all tokens of the row.  Logits of -1e30 or less
     are masked.  A row that has no token to draw, or holds a NaN or a value beyond the PAM range, gets token -1 and score -inf.  Up to 262144 tokens."""
+    if (host := _lib.host()) is not None:
+        out = host.sample(logits, uniform, temperature, top_k, top_p, min_p, banned)
+        if out is not None:
+            return out
     _not_traced("sample")
     if not isinstance(logits, torch.Tensor) or logits.dim() < 1:
         raise ValueError("logits must be a tensor [..., vocabulary]")

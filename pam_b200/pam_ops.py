@@ -346,6 +346,10 @@ def dropout(x, p=0.5, seed=None, residual=None, *, training=True, offset=None, a
     The mask is a function of the seed and of each element's place (Philox4x32-10, csrc/philox.cuh) and is not stored: the backward pass draws it
     again.  `seed` is a number or an int64 tensor of one element on x's device, None for one from the default generator.  The gradient of x is the PAM product
     of the incoming one (approx_bwd) or its product with the slope (exact).  With training=False or p = 0: x itself, plus the residual."""
+    if training and cuda_bindings._on_cuda(x) and (host := _lib.host()) is not None:
+        out = host.dropout(x, p, seed, residual, offset, approx_bwd)
+        if out is not None:
+            return out
     approx, p = _gradient_mode(approx_bwd), _probability(p)
     _fp32("x", x)
     if residual is not None:
@@ -379,6 +383,12 @@ def embedding(tokens, weight, scale=None, positions=None, padding_idx=None, *, p
     The gradient of the table has PAM products (approx_bwd) or slopes (exact) of the incoming one, added for each row in an order that follows from
     the tokens alone; the row `padding_idx` has none.  A token outside the vocabulary gives a row of NaN and has no gradient.  Up to 2^22 rows, fewer than
     2^31 tokens."""
+    rate = p if training else 0.0 * _probability(p)
+    if cuda_bindings._on_cuda(weight) and weight.dim() == 2 and (padding_idx is None or type(padding_idx) is int and 0 <= padding_idx < weight.shape[0]):
+        if (host := _lib.host()) is not None:
+            out = host.embedding(tokens, weight, scale, positions, -1 if padding_idx is None else padding_idx, rate, seed if rate != 0 else 0, offset, approx_bwd)
+            if out is not None:
+                return out
     approx, p = _gradient_mode(approx_bwd), _probability(p)
     if not isinstance(tokens, torch.Tensor) or tokens.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"tokens must be an int64 or int32 tensor, got {tokens.dtype if isinstance(tokens, torch.Tensor) else type(tokens).__name__}")
