@@ -10,9 +10,16 @@
 // numbers: a PAM product would favour some tokens.)  Its score is x - pad(M + log2(S), log2 e), the PAM log-softmax over all of the row's tokens (pam/pam_ops.py:331-347),
 // from a sum S of all bits of the exponentials down to 2^-62 and a logarithm and a quotient in 64 bits.
 //
-// A row belongs to a cluster of up to eight CTAs, each of which keeps its part in shared memory as keys d 2^23 + (1 - f') 2^23 - 1, smaller for larger weights, after
-// reading the logits once.  A cut is found in three steps of 11, 9 and 9 bits of the key, each a histogram of numbers and weights that the CTAs of the cluster
-// read of one another.
+// An exponential is kept as the pattern of the float e = 2^-d (1 + f'), taken from that of the largest: a key that is smaller for larger weights, so that
+// "in order" is the order of (key, number).  Sums of weights are sums of e in doubles that start at 2^8 and are rounded down: there a unit is 2^-44, and adding e
+// adds floor(2^44 e) units, without an error, until they reach 2^8.
+//
+// A row belongs to a cluster of up to eight CTAs, each of which keeps its part in shared memory: the t of its tokens, then their keys.  A warp has neighbouring
+// tokens, of which a thread has the same four at a time from loading to drawing.  The logits are read once.  What stays is cut off at one token, found as follows:
+//   top-k   each warp's q-th best of its lanes' best tokens, where q of each of w warps are k at least, bounds the k-th best of all; the few tokens as good as the
+//           bound go to a list in the first CTA, which sorts it;
+//   top-p   passes over the keys take the weights below three borders each, until at most 512 tokens are left between two; these go to the list.
+// (A histogram of 2048 parts of 1/32 of an octave for the latter: its atomics, and its reading by all CTAs of a cluster, made it 640 us for 256 rows of 151643 tokens.)
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -28,7 +35,14 @@ constexpr float kMasked = -1e30f;                     // a logit as low as this 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kMostCtas = 8, kMostKeys = 32768;       // of a cluster; of a CTA
 constexpr uint32_t kOut = 0xffffffffu;                // the key of a token without weight
-constexpr int kBins = 2048;
+constexpr uint32_t kTop = 0x3fffffffu;                // key + pattern
+constexpr uint32_t kEnd = 45u << 23;                  // keys with a weight are below
+constexpr int kListed = kThreads;                     // a thread for each
+constexpr int kNumberBits = 18;
+static_assert(kMostCtas * kMostKeys == 1 << kNumberBits);
+// a thread's tokens: their e stay below 2^8 together
+static_assert((kMostKeys / 4 / kThreads + 2) * 4 * 2 < 256);
+typedef unsigned long long u64;
 
 struct Sample {
     const float *logits, *uniform;
@@ -43,42 +57,66 @@ struct Sample {
     float* scores;
 };
 
-struct Pair { unsigned long long weight; uint32_t count; };
+struct Found { u64 weights[3]; uint32_t counts[4]; };                     // before each border; and in all
 
 struct Shared {
-    uint32_t count[kBins], low[kBins], high[kBins];   // of each bin: keys, and the sum of their weights' digits by 12 bits
-    Pair scan[kWarps];
-    unsigned long long near[kWarps], far[kWarps], kept[kWarps];
-    float top_all[kWarps], top_ok[kWarps];
+    u64 list[kListed];
     // what the other CTAs of the cluster read
-    struct { float all, ok; int bad; unsigned long long near, far, kept; unsigned long long part[kWarps]; uint32_t ties[kWarps]; } mine;
-    // what a step of the search found
-    uint32_t bin, less_count;
-    unsigned long long less_weight;
-    unsigned long long before;                        // of the warp that has the token
-    int owner;
-    long long token;
+    float all, ok;
+    int bad;
+    double sums[kWarps], banned_sums[kWarps];
+    u64 parts[kWarps], staying[2][kWarps];            // weights of the warps: of all, of what stays
+    uint32_t live[kWarps], bounds[kWarps], ties[kWarps];
+    Found found[2];
+    uint32_t listed;
+    u64 cut, kept;
+    // within the CTA
+    float warp_all[kWarps], warp_ok[kWarps];
+    u64 every[kWarps * kMostCtas];                    // all warps' of the cluster
+    uint32_t every_bound[kWarps * kMostCtas], bound;
+    Found warps[kWarps];
+    u64 scan[kWarps];
 };
 
-__device__ __forceinline__ unsigned long long weight_of(uint32_t key) {
+// Where the threads of a cluster wait for one another.
+struct Team {
+    cg::cluster_group cluster;
+    int ctas;
+    __device__ void wait() {
+        if (ctas == 1) __syncthreads(); else cluster.sync();
+    }
+    __device__ Shared& of(Shared& sh, int c) { return ctas == 1 ? sh : *cluster.map_shared_rank(&sh, c); }
+};
+
+__device__ __forceinline__ float value_of(uint32_t key) { return i2f((int32_t)(kTop - key)); }
+
+__device__ __forceinline__ u64 weight_of(uint32_t key) {
     const uint32_t d = key >> 23, m = 0x800000u | (~key & 0x7fffffu);
-    return d <= 21u ? (unsigned long long)m << (21u - d) : (unsigned long long)(m >> min(d - 21u, 31u));
+    return d <= 21u ? (u64)m << (21u - d) : (u64)(m >> min(d - 21u, 31u));
 }
 
+// Sums of weights.
+struct Units {
+    double sum = 256.0;
+    __device__ void add(double e) { sum = __dadd_rd(sum, e); }
+    __device__ u64 get() const { return (u64)__double_as_longlong(sum) & 0xfffffffffffffull; }
+};
+
 // floor and the rest of fraction 2^-24 total
-struct Share { unsigned long long whole; bool rest; };
-__device__ __forceinline__ Share share(uint32_t fraction, unsigned long long total) {
-    const unsigned long long low = total * fraction;
+struct Share { u64 whole; bool rest; };
+__device__ __forceinline__ Share share(uint32_t fraction, u64 total) {
+    const u64 low = total * fraction;
     return {__umul64hi(total, fraction) << 40 | low >> 24, (low & 0xffffffu) != 0};
 }
-__device__ __forceinline__ unsigned long long share_up(uint32_t fraction, unsigned long long total) {
+__device__ __forceinline__ u64 share_up(uint32_t fraction, u64 total) {
     const Share s = share(fraction, total);
     return s.whole + s.rest;
 }
 // A fraction in steps of 2^-24, NaN as 0.
 __device__ __forceinline__ uint32_t steps(float f, uint32_t most) { return f > 0.0f ? min((uint32_t)fminf(f * 16777216.0f, 16777216.0f), most) : 0u; }
 
-__device__ __forceinline__ unsigned long long warp_sum(unsigned long long v) {
+template <class T>
+__device__ __forceinline__ T warp_sum(T v) {
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
     return v;
@@ -86,6 +124,15 @@ __device__ __forceinline__ unsigned long long warp_sum(unsigned long long v) {
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+    return v;
+}
+__device__ __forceinline__ u64 warp_upto(u64 v) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const u64 w = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v += w;
+    }
     return v;
 }
 
@@ -98,318 +145,524 @@ __device__ double log_sum(double shift, double total) {
     return __longlong_as_double(__double_as_longlong(log2) - __double_as_longlong(by) + 0x3ff0000000000000ll);
 }
 
-// The digits of a key's weight without its shift (which is the same for all keys of a bin).
-__device__ __forceinline__ uint32_t digits(uint32_t key) {
-    const uint32_t d = key >> 23, m = 0x800000u | (~key & 0x7fffffu);
-    return d <= 21u ? m : m >> (d - 21u);
-}
+// 2^e for whole e <= 1 (0 far below)
+__device__ __forceinline__ double power_of(float e) { return e >= -1000.0f ? __longlong_as_double((long long)((int)e + 1023) << 52) : 0.0; }
 
-// Where in the order of the keys a count or a weight is reached: the keys of bin `prefix` (of `shift + bits` low bits) in bins of 2^shift, less_* before them.
-// Sets sh.bin to the bin in which `target` is reached (by count, else by weight) and sh.less_* to what lies before it.
-__device__ void search(Shared& sh, const uint32_t* keys, int n, cg::cluster_group& cluster, uint32_t prefix, int shift, int bits, uint32_t less_count,
-                       unsigned long long less_weight, bool by_count, unsigned long long target) {
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, bins = 1 << bits;
-    for (int b = t; b < bins; b += kThreads) sh.count[b] = sh.low[b] = sh.high[b] = 0u;
-    __syncthreads();
-    for (int j = t; j < n; j += kThreads) {
-        const uint32_t key = keys[j];
-        if (key == kOut || key >> (shift + bits) != prefix) continue;
-        const uint32_t b = key >> shift & (bins - 1), m = digits(key);
-        atomicAdd(&sh.count[b], 1u);
-        atomicAdd(&sh.low[b], m & 0xfffu);
-        atomicAdd(&sh.high[b], m >> 12);
+// t = pam(pad(x, temperature), log2 e): one sum of patterns where x lies far from what the range rule cuts off, in which case no value in between does either.
+struct Scaling {
+    float temperature;
+    uint32_t low, span;                               // twice the pattern of the least such |x|, and how far the greatest is from there
+    int32_t shift;
+    __device__ explicit Scaling(float t) : temperature(t) {
+        // |x| / temperature from 2^-100 to 2^100, |x| normal and below what is masked
+        const int32_t bits = f2i(t);
+        const uint32_t least = (uint32_t)max(bits - (100 << 23), 1 << 23), most = (uint32_t)min((int64_t)bits + (100 << 23), (int64_t)f2i(-kMasked) - 1);
+        low = 2u * least;
+        span = most > least ? 2u * (most - least) : 0u;
+        shift = f2i(kLog2e) - bits;
     }
-    cluster.sync();
-    const int each = bins / kThreads;                 // 4 or 1 neighbouring bins
-    Pair own[4], sum{0ull, 0u};
-    const int ctas = (int)cluster.num_blocks();
-    for (int k = 0; k < each; ++k) {
-        const int b = t * each + k;
-        uint32_t count = 0u;
-        unsigned long long digits_sum = 0ull;
-        for (int c = 0; c < ctas; ++c) {
-            const Shared* other = cluster.map_shared_rank(&sh, c);
-            count += other->count[b];
-            digits_sum += (unsigned long long)other->low[b] + ((unsigned long long)other->high[b] << 12);
-        }
-        const uint32_t d = (prefix << bits | b) >> (23 - shift);
-        own[k] = {d <= 21u ? digits_sum << (21u - d) : digits_sum, count};
-        sum.weight += own[k].weight;
-        sum.count += own[k].count;
-    }
-    Pair upto = sum;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const unsigned long long w = __shfl_up_sync(0xffffffffu, upto.weight, d);
-        const uint32_t c = __shfl_up_sync(0xffffffffu, upto.count, d);
-        if (lane >= d) {
-            upto.weight += w;
-            upto.count += c;
-        }
-    }
-    if (lane == 31) sh.scan[warp] = upto;
-    __syncthreads();
-    Pair before{less_weight, less_count};
-    for (int w = 0; w < warp; ++w) {
-        before.weight += sh.scan[w].weight;
-        before.count += sh.scan[w].count;
-    }
-    before.weight += upto.weight - sum.weight;
-    before.count += upto.count - sum.count;
-    for (int k = 0; k < each; ++k) {
-        const unsigned long long from = by_count ? before.count : before.weight, to = from + (by_count ? own[k].count : own[k].weight);
-        if (from < target && target <= to) {
-            sh.bin = t * each + k;
-            sh.less_count = before.count;
-            sh.less_weight = before.weight;
-        }
-        before.weight += own[k].weight;
-        before.count += own[k].count;
-    }
-    cluster.sync();                                   // (the histograms may be written anew)
-}
-
-struct Cut {
-    uint32_t key;                                     // the last one that stays
-    uint32_t less_count, ties;                        // so many smaller ones; so many equal ones stay
-    unsigned long long less_weight;
-    __device__ unsigned long long weight() const { return less_weight + ties * weight_of(key); }
+    __device__ __forceinline__ bool plain(float x) const { return 2u * (uint32_t)f2i(x) - low < span; }
+    __device__ __forceinline__ float plainly(float x) const { return i2f(iadd(f2i(x), shift)); }
+    __device__ __noinline__ float any(float x) const { return x <= kMasked ? -INFINITY : mul(div(x, temperature, 0), kLog2e, 0); }
 };
 
-__device__ Cut find_cut(Shared& sh, const uint32_t* keys, int n, cg::cluster_group& cluster, bool by_count, unsigned long long target) {
-    uint32_t prefix = 0u, less_count = 0u;
-    unsigned long long less_weight = 0ull;
-    constexpr int kBits[3] = {11, 9, 9}, kShift[3] = {18, 9, 0};
-    for (int step = 0; step < 3; ++step) {
-        search(sh, keys, n, cluster, prefix, kShift[step], kBits[step], less_count, less_weight, by_count, target);
-        prefix = prefix << kBits[step] | sh.bin;
-        less_count = sh.less_count;
-        less_weight = sh.less_weight;
-        __syncthreads();
+// A search for the token at which a count or a weight is reached, in the order of (key, number).
+struct Search {
+    Shared& sh;
+    Team& team;
+    const uint32_t* keys;                             // of the CTA's slots
+    int first, last, lane, warp;                      // the warp's quads; the lane's are every 32nd
+    int begin, rank;                                  // the number of slot 0 (it may be before the part); the CTA's rank
+
+    __device__ __forceinline__ uint4 quad(int q) const { return q < last ? reinterpret_cast<const uint4*>(keys)[q] : make_uint4(kOut, kOut, kOut, kOut); }
+
+    template <class F>
+    __device__ __forceinline__ void each(F&& f) const {               // f(key, number) for all; warps stay together
+        for (int q = first + lane; q - lane < last; q += 32) {
+            const uint4 k = quad(q);
+            const int number = begin + q * 4;
+            f(k.x, number);
+            f(k.y, number + 1);
+            f(k.z, number + 2);
+            f(k.w, number + 3);
+        }
     }
-    Cut cut{prefix, less_count, 0u, less_weight};
-    const unsigned long long each = weight_of(prefix);
-    cut.ties = (uint32_t)(by_count ? target - less_count : (target - less_weight + each - 1) / each);
-    return cut;
+
+    // The weight of all tokens up to `cut` of at least least_e; `own` is this warp's and `before` that of the warps before.  `turn` alternates from call to call.
+    __device__ u64 weigh(u64 cut, double least_e, int turn, u64* own, u64* before) {
+        const uint32_t cut_key = (uint32_t)(cut >> kNumberBits);
+        Units stay;
+        each([&](uint32_t key, int number) {
+            if (key > cut_key || key == kOut || ((u64)key << kNumberBits | (uint32_t)number) > cut) return;
+            const double e = (double)value_of(key);
+            if (e >= least_e) stay.add(e);
+        });
+        *own = warp_sum(stay.get());
+        if (lane == 0) sh.staying[turn][warp] = *own;
+        team.wait();
+        return total_of([&](int c, int w) { return team.of(sh, c).staying[turn][w]; }, before);
+    }
+
+    // The sum of a value of all warps of the cluster, and of those before this one.  There is a barrier within.
+    template <class F>
+    __device__ u64 total_of(F&& of, u64* before) {
+        const int warps = team.ctas * kWarps, t = threadIdx.x;
+        if (t < warps) sh.every[t] = of(t / kWarps, t % kWarps);
+        __syncthreads();
+        u64 total = 0ull, less = 0ull;
+        for (int w = lane; w < warps; w += 32) {
+            total += sh.every[w];
+            if (w < rank * kWarps + warp) less += sh.every[w];
+        }
+        *before = warp_sum(less);
+        return warp_sum(total);
+    }
+
+    // What lies in [low, low + border_j) for three borders, and how many keys in [low, low + all).
+    template <bool WEIGHTS>
+    __device__ Found below(uint32_t low, const uint32_t (&border)[3], uint32_t all, int turn) {
+        Units units[3];
+        uint32_t counts[4] = {0u, 0u, 0u, 0u};
+        each([&](uint32_t key, int) {
+            const uint32_t at = key - low;
+            if (WEIGHTS) {
+                const double e = (double)value_of(key);
+#pragma unroll
+                for (int j = 0; j < 3; ++j)
+                    if (at < border[j]) {
+                        units[j].add(e);
+                        ++counts[j];
+                    }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 3; ++j) counts[j] += at < border[j];
+            }
+            counts[3] += at < all;
+        });
+        Found f;
+#pragma unroll
+        for (int j = 0; j < 3; ++j) f.weights[j] = WEIGHTS ? warp_sum(units[j].get()) : 0ull;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f.counts[j] = __reduce_add_sync(0xffffffffu, counts[j]);
+        if (lane == 0) sh.warps[warp] = f;
+        __syncthreads();
+        const auto joined = [&](int n, auto&& of) {                   // (n <= 16; the same in all lanes)
+            Found g{};
+            if (lane < n) g = of(lane);
+#pragma unroll
+            for (int j = 0; j < 3; ++j) g.weights[j] = WEIGHTS ? warp_sum(g.weights[j]) : 0ull;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) g.counts[j] = __reduce_add_sync(0xffffffffu, g.counts[j]);
+            return g;
+        };
+        f = joined(kWarps, [&](int w) { return sh.warps[w]; });
+        if (team.ctas > 1) {
+            if (threadIdx.x == 0) sh.found[turn] = f;
+            team.wait();
+            f = joined(team.ctas, [&](int c) { return team.of(sh, c).found[turn]; });
+        } else {
+            __syncthreads();                          // (the warps' are written anew)
+        }
+        return f;
+    }
+
+    // The tokens with keys from `low` to `high` to the first CTA's list; false where there are too many.  sh.listed is 0 before.
+    __device__ bool gather(uint32_t low, uint32_t high) {
+        Shared& head = team.of(sh, 0);
+        each([&](uint32_t key, int number) {
+            const bool in = key - low <= high - low;
+            const uint32_t all = __ballot_sync(0xffffffffu, in);
+            if (all == 0u) return;
+            uint32_t at = 0u;
+            if (lane == 0) at = atomicAdd(&head.listed, (uint32_t)__popc(all));
+            at = __shfl_sync(0xffffffffu, at, 0) + __popc(all & ((1u << lane) - 1u));
+            if (in && at < kListed) head.list[at] = (u64)key << kNumberBits | (uint32_t)number;
+        });
+        team.wait();
+        return head.listed <= kListed;
+    }
+
+    // In the first CTA: the list's token at which the target is reached, less_* before the list.  With a count, and top_p < 1 (the list then starts with the first token
+    // of all), the one at which that share of the weights up to there is.  sh.cut and sh.kept, the weight up to it, are set.
+    __device__ void pick(bool by_count, u64 target, float top_p, uint32_t less_count, u64 less_weight) {
+        const int t = threadIdx.x, n = (int)sh.listed;
+        u64 own = t < n ? sh.list[t] : ~0ull;
+        int size = 32;                                // sorted by pairs at distances 2^j, within a warp from 16 down
+        while (size < n) size *= 2;
+        for (int run = 2; run <= size; run *= 2)
+            for (int apart = run / 2; apart > 0; apart /= 2) {
+                u64 other;
+                if (apart >= 32) {
+                    __syncthreads();
+                    sh.list[t] = own;
+                    __syncthreads();
+                    other = sh.list[t ^ apart];
+                } else {
+                    other = __shfl_xor_sync(0xffffffffu, own, apart);
+                }
+                const bool up = (t & run) == 0 || run == size, lower = (t & apart) == 0;
+                own = (own < other) == (up == lower) ? own : other;
+            }
+        const u64 weight = t < n ? weight_of((uint32_t)(own >> kNumberBits)) : 0ull, upto_warp = warp_upto(weight);
+        if (lane == 31) sh.scan[warp] = upto_warp;
+        __syncthreads();
+        u64 upto = less_weight + upto_warp;
+        for (int w = 0; w < warp; ++w) upto += sh.scan[w];
+        if (t < n && (by_count ? less_count + t + 1 == target : upto - weight < target && target <= upto)) {
+            sh.cut = own;
+            sh.kept = upto;
+        }
+        __syncthreads();
+        if (!by_count || !(top_p < 1.0f)) return;
+        const u64 share_of = max(share_up(steps(top_p, 0xffffffu), sh.kept), 1ull);
+        __syncthreads();
+        if (t < n && upto - weight < share_of && share_of <= upto) sh.cut = own;
+    }
+
+    // gather and pick; false where there are too many.
+    __device__ bool listed(uint32_t low, uint32_t high, bool by_count, u64 target, float top_p, uint32_t less_count, u64 less_weight, u64* cut) {
+        const bool few = gather(low, high);
+        if (few && rank == 0) pick(by_count, target, top_p, less_count, less_weight);
+        team.wait();
+        *cut = team.of(sh, 0).cut;
+        if (rank == 0 && threadIdx.x == 0) sh.listed = 0u;
+        team.wait();
+        return few;
+    }
+
+    // The r-th token, by number, of those with this key.
+    __device__ u64 equal_one(uint32_t key, u64 r) {
+        uint32_t own = 0u;
+        each([&](uint32_t k, int) { own += k == key; });
+        own = __reduce_add_sync(0xffffffffu, own);
+        if (lane == 0) sh.ties[warp] = own;
+        team.wait();
+        u64 before;
+        total_of([&](int c, int w) { return (u64)team.of(sh, c).ties[w]; }, &before);
+        if (before < r && r <= before + own) {
+            uint32_t need = (uint32_t)(r - before);
+            for (int q = first + lane; q - lane < last; q += 32) {
+                const uint4 k = quad(q);
+                const uint32_t is = (k.x == key) | (k.y == key) << 1 | (k.z == key) << 2 | (k.w == key) << 3;
+                uint32_t upto = __popc(is);
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const uint32_t v = __shfl_up_sync(0xffffffffu, upto, d);
+                    if (lane >= d) upto += v;
+                }
+                const uint32_t reached = __ballot_sync(0xffffffffu, upto >= need);
+                if (reached) {
+                    if (lane == __ffs(reached) - 1) {
+                        uint32_t left = is;
+                        for (uint32_t i = upto - __popc(is) + 1; i < need; ++i) left &= left - 1;
+                        team.of(sh, 0).cut = (u64)key << kNumberBits | (uint32_t)(begin + q * 4 + __ffs(left) - 1);
+                    }
+                    break;
+                }
+                need -= __shfl_sync(0xffffffffu, upto, 31);
+            }
+        }
+        team.wait();
+        const u64 cut = team.of(sh, 0).cut;
+        team.wait();
+        return cut;
+    }
+
+    // The cut, which is among the keys up to `high`.
+    template <bool BY_COUNT>
+    __device__ u64 find(u64 target, uint32_t high) {
+        uint32_t low = 0u, less_count = 0u;
+        u64 less_weight = 0ull;
+        for (int turn = 0;; turn ^= 1) {
+            const uint32_t span = high - low;         // (below 2^29)
+            const uint32_t border[3] = {(span + 1) / 4, (span + 1) / 2, (uint32_t)((u64)(span + 1) * 3 / 4)};
+            const Found f = below<!BY_COUNT>(low, border, span + 1, turn);
+            int j = 0;                                // the last part with less than the target before it
+            while (j < 3 && (BY_COUNT ? less_count + f.counts[j] : less_weight + f.weights[j]) < target) ++j;
+            const uint32_t end = j < 3 ? border[j] : span + 1, start = j > 0 ? border[j - 1] : 0u, few = f.counts[j] - (j > 0 ? f.counts[j - 1] : 0u);
+            high = low + end - 1;
+            low += start;
+            if (j > 0) {
+                less_count += f.counts[j - 1];
+                less_weight += f.weights[j - 1];
+            }
+            u64 cut;
+            if (few <= kListed && listed(low, high, BY_COUNT, target, 1.0f, less_count, less_weight, &cut)) return cut;
+            if (low == high) {
+                const u64 each_weight = weight_of(low);
+                return equal_one(low, BY_COUNT ? target - less_count : (target - less_weight + each_weight - 1) / each_weight);
+            }
+        }
+    }
+};
+
+// What a thread's tokens add up to.
+struct Sums {
+    Units units;                                      // of the weights
+    double sum = 0.0;                                 // of the e
+    float rest = 0.0f;                                // of what f' leaves of f, where t has bits below 2^-23, times 2^floor t
+    double banned = 0.0;                              // of banned tokens' exponentials
+    uint32_t best = kOut, live = 0u;
+};
+
+// t -> key.  A t far below the largest becomes an e below 2^-125, which is no weight and adds nothing.
+template <bool BANNED, bool COUNT>
+__device__ __forceinline__ uint32_t key_of(Sums& s, float t, float shift, float shift_all, bool out) {
+    const float v = fmaxf(t, -3e38f), whole = floorf(v), lin = __fadd_rd(1.0f, __fadd_rd(v, -whole));      // lin = 1 + f'
+    // (f - f' = t - ((1 + f') + (floor t - 1)), to a part in 2^24 of itself; 0 where |t| >= 1)
+    const float rest = fabsf(v) < 1.0f ? fadd(v, -fadd(lin, fadd(whole, -1.0f))) : 0.0f;
+    if (BANNED && out) {
+        if (t > -INFINITY) s.banned += ((double)lin + (double)rest) * power_of(whole - shift_all);
+        return kOut;
+    }
+    s.rest = __fmaf_rn(rest, v < 0.0f ? 0.5f : 1.0f, s.rest);
+    const uint32_t bits = (uint32_t)f2i(lin) - ((uint32_t)min((int)(shift - whole), 126) << 23);
+    const double e = (double)i2f((int32_t)bits);
+    s.sum += e;
+    s.units.add(e);
+    const uint32_t key = kTop - bits < kEnd ? kTop - bits : kOut;
+    if (COUNT) {
+        s.best = min(s.best, key);
+        s.live += key != kOut;
+    }
+    return key;
 }
 
-__global__ void __launch_bounds__(kThreads) sample_kernel(const Sample a) {
+template <bool BANNED, bool COUNT>
+__device__ __forceinline__ void make_keys(Sums& sums, uint32_t* keys, const unsigned char* flags, int first, int last, float shift, float shift_all) {
+#pragma unroll 2
+    for (int q = first; q < last; q += 32) {
+        const float4 v = reinterpret_cast<const float4*>(keys)[q];
+        const uint32_t out = BANNED ? flags[q] : 0u;
+        const auto key = [&](float t, uint32_t bit) { return key_of<BANNED, COUNT>(sums, t, shift, shift_all, out & bit); };
+        reinterpret_cast<uint4*>(keys)[q] = make_uint4(key(v.x, 1u), key(v.y, 2u), key(v.z, 4u), key(v.w, 8u));
+    }
+}
+
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Sample a) {
     extern __shared__ __align__(16) unsigned char memory[];
     Shared& sh = *reinterpret_cast<Shared*>(memory);
-    uint32_t* keys = reinterpret_cast<uint32_t*>(memory + sizeof(Shared));
-    uint32_t* flags = keys + (a.part + 31) / 32 * 32;                                 // a bit for each token: banned
-    cg::cluster_group cluster = cg::this_cluster();
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
-    const int64_t row = blockIdx.x / ctas;
+    uint32_t* keys = reinterpret_cast<uint32_t*>(memory + (sizeof(Shared) + 15) / 16 * 16);
+    unsigned char* flags = reinterpret_cast<unsigned char*>(keys + a.part + 4);       // four bits for each quad: banned
+    Team team{cg::this_cluster(), 0};
+    team.ctas = (int)team.cluster.num_blocks();
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, rank = team.ctas == 1 ? 0 : (int)team.cluster.block_rank();
+    const int64_t row = blockIdx.x / team.ctas;
     const int begin = min(rank * a.part, a.vocab), n = min(a.part, a.vocab - begin);
-    const float* x = a.logits + row * a.x_row;
-    const unsigned char* banned = a.banned ? a.banned + row * a.ban_row : nullptr;
+    const unsigned char* banned = a.banned ? a.banned + row * a.ban_row + begin : nullptr;
     const float temperature = a.temperatures ? __ldg(a.temperatures + row) : a.temperature;
     const float top_p = a.top_ps ? __ldg(a.top_ps + row) : a.top_p, min_p = a.min_ps ? __ldg(a.min_ps + row) : a.min_p;
     const int64_t top_k = a.top_ks ? __ldg(reinterpret_cast<const long long*>(a.top_ks) + row) : a.top_k;
-    const Divisor by_temperature = make_divisor(temperature, 0);
+    const uint32_t fraction = steps(__ldg(a.uniform + row), 0xffffffu);
+    const bool cut_by_k = top_k > 0 && top_k < a.vocab;
+    const Scaling scaled(temperature);
+
+    // slots of four at aligned addresses: the first one may begin before the part, the last one end behind it
+    const float* part = a.logits + row * a.x_row + begin;
+    const int phase = (int)((reinterpret_cast<uintptr_t>(part) >> 2) & 3);
+    const float* slots = part - phase;
+    const int quads = n > 0 ? (n + phase + 3) / 4 : 0, each = (quads + kWarps - 1) / kWarps, first = min(warp * each, quads), last = min(first + each, quads);
+    if (t == 0) sh.listed = 0u;
 
     // the row's t, and the largest of all and of those that may be drawn
     float top_all = -INFINITY, top_ok = -INFINITY;
     bool bad = !(temperature > 0.0f && temperature <= i2f(0x7f7fffff));
-    for (int j = t; j < (n + 31) / 32 * 32; j += kThreads) {
-        const float raw = j < n ? __ldg(x + begin + j) : -INFINITY;
-        const float v = raw <= kMasked ? -INFINITY : mul(div_by(raw, by_temperature), kLog2e, 0);
-        const bool out = j < n && banned && banned[begin + j];
-        const uint32_t word = __ballot_sync(0xffffffffu, out);
-        if (lane == 0) flags[j >> 5] = word;
-        bad = bad || v != v;
-        if (j < n) keys[j] = (uint32_t)f2i(v);
-        top_all = fmaxf(top_all, v);
-        if (!out) top_ok = fmaxf(top_ok, v);
+    constexpr int kAhead = 4;
+    const int full_from = phase ? 1 : 0, full = (n + phase) / 4 - full_from;           // quads that are all the part's
+    for (int q0 = first + lane; q0 < last; q0 += 32 * kAhead) {
+        float4 x[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int q = q0 + k * 32;
+            x[k] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            if (q < last && (unsigned)(q - full_from) < (unsigned)max(full, 0)) x[k] = __ldcs(reinterpret_cast<const float4*>(slots) + q);
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int q = q0 + k * 32, s = q * 4 - phase;
+            if (q >= last) break;
+            if ((unsigned)(q - full_from) >= (unsigned)max(full, 0)) {
+                if (s >= 0 && s < n) x[k].x = __ldcs(part + s);
+                if (s + 1 >= 0 && s + 1 < n) x[k].y = __ldcs(part + s + 1);
+                if (s + 2 >= 0 && s + 2 < n) x[k].z = __ldcs(part + s + 2);
+                if (s + 3 >= 0 && s + 3 < n) x[k].w = __ldcs(part + s + 3);
+            }
+            float4 v;
+            if (scaled.plain(x[k].x) && scaled.plain(x[k].y) && scaled.plain(x[k].z) && scaled.plain(x[k].w)) {
+                v = make_float4(scaled.plainly(x[k].x), scaled.plainly(x[k].y), scaled.plainly(x[k].z), scaled.plainly(x[k].w));
+            } else {
+                v = make_float4(scaled.any(x[k].x), scaled.any(x[k].y), scaled.any(x[k].z), scaled.any(x[k].w));
+                bad = bad || v.x != v.x || v.y != v.y || v.z != v.z || v.w != v.w;
+            }
+            const float most = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
+            top_all = fmaxf(top_all, most);
+            if (banned) {
+                uint32_t out = 0u;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (s + j >= 0 && s + j < n && banned[s + j]) out |= 1u << j;
+                flags[q] = (unsigned char)out;
+                top_ok = fmaxf(top_ok, fmaxf(fmaxf(out & 1u ? -INFINITY : v.x, out & 2u ? -INFINITY : v.y), fmaxf(out & 4u ? -INFINITY : v.z, out & 8u ? -INFINITY : v.w)));
+            }
+            reinterpret_cast<float4*>(keys)[q] = v;
+        }
     }
     top_all = warp_max(top_all);
-    top_ok = warp_max(top_ok);
+    top_ok = banned ? warp_max(top_ok) : top_all;
     if (lane == 0) {
-        sh.top_all[warp] = top_all;
-        sh.top_ok[warp] = top_ok;
+        sh.warp_all[warp] = top_all;
+        sh.warp_ok[warp] = top_ok;
     }
     const int any_bad = __syncthreads_or(bad);
-    if (t == 0) {
-        float all = -INFINITY, ok = -INFINITY;
-        for (int w = 0; w < kWarps; ++w) {
-            all = fmaxf(all, sh.top_all[w]);
-            ok = fmaxf(ok, sh.top_ok[w]);
+    top_all = warp_max(lane < kWarps ? sh.warp_all[lane] : -INFINITY);
+    top_ok = warp_max(lane < kWarps ? sh.warp_ok[lane] : -INFINITY);
+    int no_token = any_bad;
+    if (team.ctas > 1) {
+        if (t == 0) {
+            sh.all = top_all;
+            sh.ok = top_ok;
+            sh.bad = any_bad;
         }
-        sh.mine.all = all;
-        sh.mine.ok = ok;
-        sh.mine.bad = any_bad;
-    }
-    cluster.sync();
-    int no_token = 0;
-    for (int c = 0; c < ctas; ++c) {
-        const Shared* other = cluster.map_shared_rank(&sh, c);
-        top_all = fmaxf(top_all, other->mine.all);
-        top_ok = fmaxf(top_ok, other->mine.ok);
-        no_token |= other->mine.bad;
+        team.wait();
+        for (int c = 0; c < team.ctas; ++c) {
+            const Shared& other = team.of(sh, c);
+            top_all = fmaxf(top_all, other.all);
+            top_ok = fmaxf(top_ok, other.ok);
+            no_token |= other.bad;
+        }
     }
     if (no_token || !(top_ok > -INFINITY)) {                                          // (all CTAs of the cluster alike)
         if (rank == 0 && t == 0) {
             a.tokens[row] = -1;
             a.scores[row] = -INFINITY;
         }
-        cluster.sync();
+        team.wait();
         return;
     }
-    const float shift_all = floorf(top_all), shift_ok = floorf(top_ok);
-    const uint32_t top_key = ~f2i(__fadd_rd(1.0f, __fadd_rd(top_ok, -shift_ok))) & 0x7fffffu;
+    const float shift_all = floorf(top_all), shift = floorf(top_ok);
+    const float lin_top = __fadd_rd(1.0f, __fadd_rd(top_ok, -shift));
+    const uint32_t top_key = kTop - (uint32_t)f2i(lin_top);
 
     // keys in place of the t, and the sums
-    unsigned long long near = 0ull, far = 0ull, kept = 0ull;
-    for (int j = t; j < n; j += kThreads) {
-        const float v = i2f((int32_t)keys[j]);
-        const float whole = floorf(v);
-        uint32_t key = kOut;
-        if (v > -INFINITY) {
-            const float lin = __fadd_rd(1.0f, __fadd_rd(v, -whole));                  // 1 + f'
-            const uint32_t m = 0x800000u | (f2i(lin) & 0x7fffff);
-            const int d = (int)fminf(shift_all - whole, 63.0f);
-            // (what f' leaves of f, where t has bits below 2^-23: f - f' = t - ((1 + f') + (floor t - 1)), to a part in 2^24 of itself)
-            if (fabsf(v) < 1.0f) far += (unsigned long long)(uint32_t)fmul(fadd(v, -fadd(lin, fadd(whole, -1.0f))), 0x1p44f) << 18 >> d;
-            if (d <= 21)
-                near += (unsigned long long)m << (21 - d);
-            else if (d < 63)
-                far += d <= 39 ? (unsigned long long)m << (39 - d) : (unsigned long long)(m >> (d - 39));
-            const float below = shift_ok - whole;
-            if (below <= 44.0f && !(flags[j >> 5] >> (j & 31) & 1u)) {
-                key = (uint32_t)below << 23 | (~m & 0x7fffffu);
-                kept += weight_of(key);
-            }
-        }
-        keys[j] = key;
-    }
-    near = warp_sum(near);
-    far = warp_sum(far);
-    kept = warp_sum(kept);
+    Sums sums;
+    if (banned)
+        cut_by_k ? make_keys<true, true>(sums, keys, flags, first + lane, last, shift, shift_all) : make_keys<true, false>(sums, keys, flags, first + lane, last, shift, shift_all);
+    else
+        cut_by_k ? make_keys<false, true>(sums, keys, flags, first + lane, last, shift, shift_all) : make_keys<false, false>(sums, keys, flags, first + lane, last, shift, shift_all);
+    u64 weight = warp_sum(sums.units.get());
+    const double sum = warp_sum(sums.sum + (shift >= -1.0f ? (double)sums.rest * power_of(-shift) : 0.0));     // (|t| < 1 only above)
+    const double banned_sum = banned ? warp_sum(sums.banned) : 0.0;
     if (lane == 0) {
-        sh.near[warp] = near;
-        sh.far[warp] = far;
-        sh.kept[warp] = kept;
+        sh.parts[warp] = weight;
+        sh.sums[warp] = sum;
+        sh.banned_sums[warp] = banned_sum;
     }
-    __syncthreads();
-    if (t == 0) {
-        near = far = kept = 0ull;
-        for (int w = 0; w < kWarps; ++w) {
-            near += sh.near[w];
-            far += sh.far[w];
-            kept += sh.kept[w];
+    // of the lanes' best the q-th best, where q of each warp are k at least
+    const int warps = team.ctas * kWarps, q = cut_by_k ? (int)((min(top_k, (int64_t)kListed) + warps - 1) / warps) : 0;
+    const bool bounded = cut_by_k && top_k <= kListed / 2 && q <= 32;
+    if (cut_by_k) {
+        const uint32_t live = __reduce_add_sync(0xffffffffu, sums.live);
+        if (lane == 0) sh.live[warp] = live;
+        if (bounded) {
+            int before = 0;
+#pragma unroll
+            for (int d = 0; d < 32; ++d) {
+                const uint32_t other = __shfl_sync(0xffffffffu, sums.best, d);
+                before += other < sums.best || (other == sums.best && d < lane);
+            }
+            if (before == q - 1) sh.bounds[warp] = sums.best;
         }
-        sh.mine.near = near;
-        sh.mine.far = far;
-        sh.mine.kept = kept;
     }
-    cluster.sync();
-    near = far = kept = 0ull;
-    for (int c = 0; c < ctas; ++c) {
-        const Shared* other = cluster.map_shared_rank(&sh, c);
-        near += other->mine.near;
-        far += other->mine.far;
-        kept += other->mine.kept;
-    }
+    team.wait();
+    Search search{sh, team, keys, first, last, lane, warp, begin - phase, rank};
+    u64 upto, total = search.total_of([&](int c, int w) { return team.of(sh, c).parts[w]; }, &upto);
 
     // what stays
-    Cut cut{kOut - 1u, 0u, 0u, kept};
-    if (top_k > 0 && top_k < a.vocab) {
-        // (fewer than k may have a weight)
-        uint32_t mine = 0u;
-        for (int j = t; j < n; j += kThreads) mine += keys[j] != kOut;
-        const uint32_t warps = __reduce_add_sync(0xffffffffu, mine);
-        if (lane == 0) sh.mine.ties[warp] = warps;
-        cluster.sync();
-        uint32_t all = 0u;
-        for (int c = 0; c < ctas; ++c)
-            for (int w = 0; w < kWarps; ++w) all += cluster.map_shared_rank(&sh, c)->mine.ties[w];
-        if (top_k < all) {
-            cut = find_cut(sh, keys, n, cluster, true, (unsigned long long)top_k);
-            kept = cut.weight();
-        }
-        cluster.sync();
-    }
-    if (top_p < 1.0f) {
-        const unsigned long long target = max(share_up(steps(top_p, 0xffffffu), kept), 1ull);
-        cut = find_cut(sh, keys, n, cluster, false, target);
-    }
-    const unsigned long long least = share_up(steps(min_p, 1u << 24), weight_of(top_key));
-    const unsigned long long tie = weight_of(cut.key);
-    const bool ties_stay = tie >= least;
-
-    // the sums of what stays, by warps in the order of the vocabulary
-    const int each = ((n + kWarps - 1) / kWarps + 31) / 32 * 32, from = min(warp * each, n), to = min(from + each, n);
-    unsigned long long sum = 0ull;
-    uint32_t ties = 0u;
-    for (int j = from + lane; j < to; j += 32) {
-        const uint32_t key = keys[j];
-        if (key < cut.key) {
-            const unsigned long long w = weight_of(key);
-            if (w >= least) sum += w;
-        } else if (key == cut.key) {
-            ++ties;
-        }
-    }
-    sum = warp_sum(sum);
-    ties = __reduce_add_sync(0xffffffffu, ties);
-    if (lane == 0) {
-        sh.mine.part[warp] = sum;
-        sh.mine.ties[warp] = ties;
-    }
-    if (t == 0) sh.owner = -1;
-    cluster.sync();
-    unsigned long long total = 0ull, upto = 0ull;
-    uint32_t ties_before = 0u;
-    {
-        uint32_t seen = 0u;
-        for (int c = 0; c < ctas; ++c)
-            for (int w = 0; w < kWarps; ++w) {
-                const Shared* other = cluster.map_shared_rank(&sh, c);
-                if (c == rank && w == warp) {
-                    upto = total;
-                    ties_before = seen;
+    u64 cut = ~0ull;
+    bool cut_by_p = top_p < 1.0f;
+    int turn = 0;
+    if (cut_by_k) {
+        // (fewer than k may have a weight: then all of these stay)
+        uint32_t live = 0u;
+        for (int w = lane; w < warps; w += 32) live += team.of(sh, w / kWarps).live[w % kWarps];
+        live = __reduce_add_sync(0xffffffffu, live);
+        if (top_k < live) {
+            bool done = false;
+            if (bounded) {
+                // of the warps' the one that as many reach as make k
+                const int enough = (int)((top_k + q - 1) / q);
+                if (t < warps) sh.every_bound[t] = team.of(sh, t / kWarps).bounds[t % kWarps];
+                __syncthreads();
+                if (t < warps) {
+                    const uint32_t own = sh.every_bound[t];
+                    int before = 0;
+                    for (int w = 0; w < warps; ++w) before += sh.every_bound[w] < own || (sh.every_bound[w] == own && w < t);
+                    if (before == enough - 1) sh.bound = own;
                 }
-                const uint32_t here = other->mine.ties[w], stay = ties_stay ? min(here, cut.ties - min(seen, cut.ties)) : 0u;
-                total += other->mine.part[w] + stay * tie;
-                seen += here;
+                __syncthreads();
+                if (sh.bound != kOut) done = search.listed(0u, sh.bound, true, (u64)top_k, top_p, 0u, 0ull, &cut);
             }
+            if (done) {
+                cut_by_p = false;                     // (the list has that cut too)
+            } else {
+                cut = search.find<true>((u64)top_k, kEnd - 1u);
+                if (cut_by_p) {
+                    u64 own, before;
+                    total = search.weigh(cut, 0.0, turn, &own, &before);
+                    turn ^= 1;
+                }
+            }
+        }
     }
-    const unsigned long long drawn = share(steps(__ldg(a.uniform + row), 0xffffffu), total).whole;
-    const uint32_t stay = ties_stay ? min(ties, cut.ties - min(ties_before, cut.ties)) : 0u;
-    if (upto <= drawn && drawn < upto + sum + stay * tie) {
+    if (cut_by_p) {
+        const u64 target = max(share_up(steps(top_p, 0xffffffu), total), 1ull);
+        // tokens so light that all of the vocabulary would not make up what is left out: 2^(45 - d) vocab <= total - target
+        uint32_t most = kEnd - 1u;
+        const u64 each_less = (total - target) / (u64)a.vocab;
+        if (each_less > 0) most = min(most, ((uint32_t)max(45 - (63 - __clzll((long long)each_less)), 1) << 23) - 1u);
+        if (cut != ~0ull) most = min(most, (uint32_t)(cut >> kNumberBits));
+        cut = search.find<false>(target, most);
+    }
+    const u64 least = share_up(steps(min_p, 1u << 24), weight_of(top_key));
+    if (cut != ~0ull || least > 0) total = search.weigh(cut, (double)least * 0x1p-44, turn, &weight, &upto);
+    const u64 drawn = share(fraction, total).whole;
+    if (upto <= drawn && drawn < upto + weight) {
         // this warp has the token
-        for (int first = from; first < to; first += 32) {
-            const int j = first + lane;
-            const uint32_t key = j < to ? keys[j] : kOut;
-            const uint32_t equal = __ballot_sync(0xffffffffu, key == cut.key);
-            unsigned long long w = 0ull;
-            if (key < cut.key)
-                w = weight_of(key);
-            else if (key == cut.key && ties_before + __popc(equal & ((1u << lane) - 1u)) < cut.ties)
-                w = tie;
-            if (w < least) w = 0ull;
-            ties_before += __popc(equal);
-            unsigned long long run = w;
+        double all = 0.0;
+        for (int w = lane; w < warps; w += 32) {
+            const Shared& other = team.of(sh, w / kWarps);
+            all += other.sums[w % kWarps] * power_of(shift - shift_all) + (banned ? other.banned_sums[w % kWarps] : 0.0);
+        }
+        all = warp_sum(all);
+        for (int q = first; q < last; q += 32) {
+            const uint4 k = q + lane < last ? reinterpret_cast<const uint4*>(keys)[q + lane] : make_uint4(kOut, kOut, kOut, kOut);
+            const uint32_t key[4] = {k.x, k.y, k.z, k.w};
+            const int number = search.begin + (q + lane) * 4;
+            u64 w[4], own = 0ull;
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const unsigned long long v = __shfl_up_sync(0xffffffffu, run, d);
-                if (lane >= d) run += v;
+            for (int j = 0; j < 4; ++j) {
+                const bool in = key[j] != kOut && ((u64)key[j] << kNumberBits | (uint32_t)(number + j)) <= cut;
+                w[j] = in ? weight_of(key[j]) : 0ull;
+                if (w[j] < least) w[j] = 0ull;
+                own += w[j];
             }
-            const uint32_t reached = __ballot_sync(0xffffffffu, upto + run > drawn);
+            const u64 run = upto + warp_upto(own);
+            const uint32_t reached = __ballot_sync(0xffffffffu, run > drawn);
             if (reached) {
                 if (lane == __ffs(reached) - 1) {
-                    const int token = begin + j;
-                    const float chosen = div_by(__ldg(x + token), by_temperature);
-                    a.tokens[row] = token;
-                    a.scores[row] = (float)((double)chosen - log_sum((double)shift_all, (double)near * 0x1p-44 + (double)far * 0x1p-62));
+                    u64 at = run - own;
+                    int j = 0;
+                    while (j < 3 && at + w[j] <= drawn) at += w[j++];
+                    const float chosen = div(__ldg(part + (number + j - begin)), temperature, 0);
+                    a.tokens[row] = number + j;
+                    a.scores[row] = (float)((double)chosen - log_sum((double)shift_all, all));
                 }
                 break;
             }
-            upto += __shfl_sync(0xffffffffu, run, 31);
+            upto = __shfl_sync(0xffffffffu, run, 31);
         }
     }
-    cluster.sync();                                                                   // (no CTA leaves while others read its memory)
+    team.wait();                                                                      // (no CTA leaves while others read its memory)
 }
 
 // CTAs of a row: as many as its keys need, and more where rows are few.
@@ -421,7 +674,8 @@ int ctas_of(int64_t rows, int64_t vocab) {
 }
 
 // (what the kernel may ask for, whatever a call needs: calls of two threads set the same)
-constexpr size_t kMostMemory = sizeof(Shared) + kMostKeys * 4 + kMostKeys / 8;
+constexpr size_t kFixed = (sizeof(Shared) + 15) / 16 * 16;
+constexpr size_t kMostMemory = kFixed + (kMostKeys + 4) * 4 + kMostKeys / 4 + 4;
 static_assert(kMostMemory <= 220 * 1024);
 
 }  // namespace
@@ -455,7 +709,7 @@ int pamk_sample(const float* logits, const float* uniform, const unsigned char* 
     a.part = (int)((vocab + ctas - 1) / ctas + 31) / 32 * 32;
     a.tokens = tokens;
     a.scores = scores;
-    const size_t memory = sizeof(Shared) + (size_t)a.part * 4 + (size_t)a.part / 8;
+    const size_t memory = kFixed + (size_t)(a.part + 4) * 4 + (banned ? a.part / 4 + 4 : 0);
     if (memory > 40 * 1024) {
         const cudaError_t err = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostMemory);
         if (err != cudaSuccess) return record_cuda_error(err);

@@ -46,7 +46,7 @@ def test_against_definition(sample, rows, vocab, settings):
     check(sample, *data(rows, vocab, seed=vocab), **settings)
 
 
-@pytest.mark.parametrize("spread", [0.0, 1e-30, 1e-6, 0.1, 20.0, 300.0, 1e6])
+@pytest.mark.parametrize("spread", [0.0, 1e-30, 1e-6, 0.1, 20.0, 300.0, 1e6, 1e12, 1e29])
 def test_spreads(sample, spread):
     for settings in SETTINGS:
         check(sample, *data(3, 700, seed=3, spread=spread), **settings)
