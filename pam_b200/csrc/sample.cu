@@ -38,6 +38,7 @@ constexpr uint32_t kOut = 0xffffffffu;                // the key of a token with
 constexpr uint32_t kTop = 0x3fffffffu;                // key + pattern
 constexpr uint32_t kEnd = 45u << 23;                  // keys with a weight are below
 constexpr int kListed = kThreads;                     // a thread for each
+constexpr int kFew = 256;
 constexpr int kNumberBits = 18;
 static_assert(kMostCtas * kMostKeys == 1 << kNumberBits);
 // a thread's tokens: their e stay below 2^8 together
@@ -61,6 +62,7 @@ struct Found { u64 weights[3]; uint32_t counts[4]; };                     // bef
 
 struct Shared {
     u64 list[kListed];
+    uint32_t few[kWarps][kFew];                       // a warp's keys in the range of a search
     // what the other CTAs of the cluster read
     float all, ok;
     int bad;
@@ -73,6 +75,7 @@ struct Shared {
     // within the CTA
     float warp_all[kWarps], warp_ok[kWarps];
     u64 every[kWarps * kMostCtas];                    // all warps' of the cluster
+    double every_sum[kWarps * kMostCtas];
     uint32_t every_bound[kWarps * kMostCtas], bound;
     Found warps[kWarps];
     u64 scan[kWarps];
@@ -85,10 +88,19 @@ struct Team {
     __device__ void wait() {
         if (ctas == 1) __syncthreads(); else cluster.sync();
     }
+    // In two halves: this CTA reads no more of the others; none reads of this one.
+    __device__ void done() {
+        if (ctas > 1) asm volatile("barrier.cluster.arrive;" ::: "memory");
+    }
+    __device__ void all_done() {
+        if (ctas > 1) asm volatile("barrier.cluster.wait;" ::: "memory");
+    }
     __device__ Shared& of(Shared& sh, int c) { return ctas == 1 ? sh : *cluster.map_shared_rank(&sh, c); }
 };
 
-__device__ __forceinline__ float value_of(uint32_t key) { return i2f((int32_t)(kTop - key)); }
+// A normal float >= 0 of this pattern as a double (the conversion instruction has a quarter of the rate).
+__device__ __forceinline__ double widened(uint32_t bits) { return __hiloint2double((int)((bits >> 3) + (896u << 20)), (int)(bits << 29)); }
+__device__ __forceinline__ double value_of(uint32_t key) { return widened(kTop - key); }
 
 __device__ __forceinline__ u64 weight_of(uint32_t key) {
     const uint32_t d = key >> 23, m = 0x800000u | (~key & 0x7fffffu);
@@ -161,7 +173,7 @@ struct Scaling {
         span = most > least ? 2u * (most - least) : 0u;
         shift = f2i(kLog2e) - bits;
     }
-    __device__ __forceinline__ bool plain(float x) const { return 2u * (uint32_t)f2i(x) - low < span; }
+    __device__ __forceinline__ uint32_t beyond(float x) const { return 2u * (uint32_t)f2i(x) - low; }              // below `span` there
     __device__ __forceinline__ float plainly(float x) const { return i2f(iadd(f2i(x), shift)); }
     __device__ __noinline__ float any(float x) const { return x <= kMasked ? -INFINITY : mul(div(x, temperature, 0), kLog2e, 0); }
 };
@@ -188,14 +200,12 @@ struct Search {
         }
     }
 
-    // The weight of all tokens up to `cut` of at least least_e; `own` is this warp's and `before` that of the warps before.  `turn` alternates from call to call.
-    __device__ u64 weigh(u64 cut, double least_e, int turn, u64* own, u64* before) {
-        const uint32_t cut_key = (uint32_t)(cut >> kNumberBits);
+    // The weight of all tokens up to `cut`; `own` is this warp's and `before` that of the warps before.  `turn` alternates from call to call.
+    __device__ u64 weigh(u64 cut, int turn, u64* own, u64* before) {
+        const uint32_t cut_key = (uint32_t)(cut >> kNumberBits), cut_number = (uint32_t)cut & ((1u << kNumberBits) - 1u);
         Units stay;
         each([&](uint32_t key, int number) {
-            if (key > cut_key || key == kOut || ((u64)key << kNumberBits | (uint32_t)number) > cut) return;
-            const double e = (double)value_of(key);
-            if (e >= least_e) stay.add(e);
+            if (key < cut_key || (key == cut_key && number <= (int)cut_number)) stay.add(value_of(key));
         });
         *own = warp_sum(stay.get());
         if (lane == 0) sh.staying[turn][warp] = *own;
@@ -218,27 +228,38 @@ struct Search {
         return warp_sum(total);
     }
 
-    // What lies in [low, low + border_j) for three borders, and how many keys in [low, low + all).
+    // What lies in [low, low + border_j) for three borders, and how many keys in [low, low + all).  A warp that has few of these keeps them for the calls to
+    // come, whose ranges lie within.
     template <bool WEIGHTS>
-    __device__ Found below(uint32_t low, const uint32_t (&border)[3], uint32_t all, int turn) {
+    __device__ Found below(uint32_t low, const uint32_t (&border)[3], uint32_t all, int turn, int& few) {
         Units units[3];
         uint32_t counts[4] = {0u, 0u, 0u, 0u};
-        each([&](uint32_t key, int) {
+        const auto look = [&](uint32_t key) {
             const uint32_t at = key - low;
-            if (WEIGHTS) {
-                const double e = (double)value_of(key);
+            const double e = WEIGHTS ? value_of(key) : 0.0;
 #pragma unroll
-                for (int j = 0; j < 3; ++j)
-                    if (at < border[j]) {
-                        units[j].add(e);
-                        ++counts[j];
-                    }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 3; ++j) counts[j] += at < border[j];
+            for (int j = 0; j < 3; ++j) {
+                const bool in = at < border[j];
+                if (WEIGHTS) units[j].sum = in ? __dadd_rd(units[j].sum, e) : units[j].sum;
+                counts[j] += in;
             }
             counts[3] += at < all;
-        });
+            return at < all;
+        };
+        if (few >= 0) {
+            for (int i = lane; i < few; i += 32) look(sh.few[warp][i]);
+        } else {
+            int found = 0;
+            each([&](uint32_t key, int) {
+                const bool in = look(key);
+                const uint32_t those = __ballot_sync(0xffffffffu, in);
+                const int place = found + __popc(those & ((1u << lane) - 1u));
+                if (in && place < kFew) sh.few[warp][place] = key;
+                found += __popc(those);
+            });
+            if (found <= kFew) few = found;
+            __syncwarp();
+        }
         Found f;
 #pragma unroll
         for (int j = 0; j < 3; ++j) f.weights[j] = WEIGHTS ? warp_sum(units[j].get()) : 0ull;
@@ -269,15 +290,22 @@ struct Search {
     // The tokens with keys from `low` to `high` to the first CTA's list; false where there are too many.  sh.listed is 0 before.
     __device__ bool gather(uint32_t low, uint32_t high) {
         Shared& head = team.of(sh, 0);
-        each([&](uint32_t key, int number) {
-            const bool in = key - low <= high - low;
-            const uint32_t all = __ballot_sync(0xffffffffu, in);
-            if (all == 0u) return;
-            uint32_t at = 0u;
-            if (lane == 0) at = atomicAdd(&head.listed, (uint32_t)__popc(all));
-            at = __shfl_sync(0xffffffffu, at, 0) + __popc(all & ((1u << lane) - 1u));
-            if (in && at < kListed) head.list[at] = (u64)key << kNumberBits | (uint32_t)number;
-        });
+        for (int q = first + lane; q - lane < last; q += 32) {
+            const uint4 k = quad(q);
+            const uint32_t span = high - low;
+            if (!__any_sync(0xffffffffu, min(min(k.x - low, k.y - low), min(k.z - low, k.w - low)) <= span)) continue;
+            const uint32_t key[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bool in = key[j] - low <= span;
+                const uint32_t all = __ballot_sync(0xffffffffu, in);
+                if (all == 0u) continue;
+                uint32_t at = 0u;
+                if (lane == 0) at = atomicAdd(&head.listed, (uint32_t)__popc(all));
+                at = __shfl_sync(0xffffffffu, at, 0) + __popc(all & ((1u << lane) - 1u));
+                if (in && at < kListed) head.list[at] = (u64)key[j] << kNumberBits | (uint32_t)(begin + q * 4 + j);
+            }
+        }
         team.wait();
         return head.listed <= kListed;
     }
@@ -373,13 +401,20 @@ struct Search {
     __device__ u64 find(u64 target, uint32_t high) {
         uint32_t low = 0u, less_count = 0u;
         u64 less_weight = 0ull;
-        for (int turn = 0;; turn ^= 1) {
+        int few = -1;
+        for (int turn = -2;; turn = turn < 0 ? turn + 3 : turn ^ 1) {                  // (-2: the first)
             const uint32_t span = high - low;         // (below 2^29)
-            const uint32_t border[3] = {(span + 1) / 4, (span + 1) / 2, (uint32_t)((u64)(span + 1) * 3 / 4)};
-            const Found f = below<!BY_COUNT>(low, border, span + 1, turn);
+            uint32_t border[3] = {(span + 1) / 4, (span + 1) / 2, (uint32_t)((u64)(span + 1) * 3 / 4)};
+            if (!BY_COUNT && turn < 0 && span > 8u << 23) {
+                // (what is left out weighs as much as the whole vocabulary at `high`: most often its heaviest are a few octaves above)
+                border[0] = span - (5u << 23);
+                border[1] = span - (7u << 22);
+                border[2] = span - (2u << 23);
+            }
+            const Found f = below<!BY_COUNT>(low, border, span + 1, turn & 1, few);
             int j = 0;                                // the last part with less than the target before it
             while (j < 3 && (BY_COUNT ? less_count + f.counts[j] : less_weight + f.weights[j]) < target) ++j;
-            const uint32_t end = j < 3 ? border[j] : span + 1, start = j > 0 ? border[j - 1] : 0u, few = f.counts[j] - (j > 0 ? f.counts[j - 1] : 0u);
+            const uint32_t end = j < 3 ? border[j] : span + 1, start = j > 0 ? border[j - 1] : 0u, left = f.counts[j] - (j > 0 ? f.counts[j - 1] : 0u);
             high = low + end - 1;
             low += start;
             if (j > 0) {
@@ -387,7 +422,7 @@ struct Search {
                 less_weight += f.weights[j - 1];
             }
             u64 cut;
-            if (few <= kListed && listed(low, high, BY_COUNT, target, 1.0f, less_count, less_weight, &cut)) return cut;
+            if (left <= kListed && listed(low, high, BY_COUNT, target, 1.0f, less_count, less_weight, &cut)) return cut;
             if (low == high) {
                 const u64 each_weight = weight_of(low);
                 return equal_one(low, BY_COUNT ? target - less_count : (target - less_weight + each_weight - 1) / each_weight);
@@ -405,19 +440,23 @@ struct Sums {
     uint32_t best = kOut, live = 0u;
 };
 
-// t -> key.  A t far below the largest becomes an e below 2^-125, which is no weight and adds nothing.
-template <bool BANNED, bool COUNT>
+// t -> key.  A t far below the largest becomes an e below 2^-125, which is no weight and adds nothing.  NEAR: both shifts within 2^20, where a whole part is the low bits of a sum
+// (the conversion instructions have a quarter of the rate of sums).
+template <bool NEAR, bool BANNED, bool COUNT>
 __device__ __forceinline__ uint32_t key_of(Sums& s, float t, float shift, float shift_all, bool out) {
-    const float v = fmaxf(t, -3e38f), whole = floorf(v), lin = __fadd_rd(1.0f, __fadd_rd(v, -whole));      // lin = 1 + f'
+    constexpr float kMagic = 12582912.0f;             // 3 2^22: its pattern's low nine bits are zeros
+    const float v = NEAR ? fmaxf(t, shift - 126.0f) : fmaxf(t, -3e38f), placed = __fadd_rd(v, kMagic);
+    const float whole = NEAR ? fadd(placed, -kMagic) : floorf(v), lin = __fadd_rd(1.0f, __fadd_rd(v, -whole));      // lin = 1 + f'
     // (f - f' = t - ((1 + f') + (floor t - 1)), to a part in 2^24 of itself; 0 where |t| >= 1)
-    const float rest = fabsf(v) < 1.0f ? fadd(v, -fadd(lin, fadd(whole, -1.0f))) : 0.0f;
+    const float rest = NEAR || fabsf(v) < 1.0f ? fadd(v, -fadd(lin, fadd(whole, -1.0f))) : 0.0f;
     if (BANNED && out) {
         if (t > -INFINITY) s.banned += ((double)lin + (double)rest) * power_of(whole - shift_all);
         return kOut;
     }
-    s.rest = __fmaf_rn(rest, v < 0.0f ? 0.5f : 1.0f, s.rest);
-    const uint32_t bits = (uint32_t)f2i(lin) - ((uint32_t)min((int)(shift - whole), 126) << 23);
-    const double e = (double)i2f((int32_t)bits);
+    s.rest = __fmaf_rn(rest, __fmaf_rn(whole, 0.5f, 1.0f), s.rest);                  // (2^whole for 0 and -1)
+    const uint32_t bits = NEAR ? (uint32_t)f2i(lin) + ((uint32_t)f2i(placed) << 23) - ((uint32_t)f2i(fadd(shift, kMagic)) << 23)
+                               : (uint32_t)f2i(lin) - ((uint32_t)min((int)(shift - whole), 126) << 23);
+    const double e = widened(bits);
     s.sum += e;
     s.units.add(e);
     const uint32_t key = kTop - bits < kEnd ? kTop - bits : kOut;
@@ -428,13 +467,13 @@ __device__ __forceinline__ uint32_t key_of(Sums& s, float t, float shift, float 
     return key;
 }
 
-template <bool BANNED, bool COUNT>
+template <bool NEAR, bool BANNED, bool COUNT>
 __device__ __forceinline__ void make_keys(Sums& sums, uint32_t* keys, const unsigned char* flags, int first, int last, float shift, float shift_all) {
 #pragma unroll 2
     for (int q = first; q < last; q += 32) {
         const float4 v = reinterpret_cast<const float4*>(keys)[q];
-        const uint32_t out = BANNED ? flags[q] : 0u;
-        const auto key = [&](float t, uint32_t bit) { return key_of<BANNED, COUNT>(sums, t, shift, shift_all, out & bit); };
+        const uint32_t out = BANNED && flags ? flags[q] : 0u;
+        const auto key = [&](float t, uint32_t bit) { return key_of<NEAR, BANNED, COUNT>(sums, t, shift, shift_all, out & bit); };
         reinterpret_cast<uint4*>(keys)[q] = make_uint4(key(v.x, 1u), key(v.y, 2u), key(v.z, 4u), key(v.w, 8u));
     }
 }
@@ -468,44 +507,55 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Sample a) {
     float top_all = -INFINITY, top_ok = -INFINITY;
     bool bad = !(temperature > 0.0f && temperature <= i2f(0x7f7fffff));
     constexpr int kAhead = 4;
-    const int full_from = phase ? 1 : 0, full = (n + phase) / 4 - full_from;           // quads that are all the part's
-    for (int q0 = first + lane; q0 < last; q0 += 32 * kAhead) {
-        float4 x[kAhead];
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-            const int q = q0 + k * 32;
-            x[k] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-            if (q < last && (unsigned)(q - full_from) < (unsigned)max(full, 0)) x[k] = __ldcs(reinterpret_cast<const float4*>(slots) + q);
+    const int full_from = phase ? 1 : 0, full_to = max((n + phase) / 4, full_from);    // quads that are all the part's
+    const auto scale = [&](int q, const float4& x) {
+        float4 v;
+        if (max(max(scaled.beyond(x.x), scaled.beyond(x.y)), max(scaled.beyond(x.z), scaled.beyond(x.w))) < scaled.span) {
+            v = make_float4(scaled.plainly(x.x), scaled.plainly(x.y), scaled.plainly(x.z), scaled.plainly(x.w));
+        } else {
+            v = make_float4(scaled.any(x.x), scaled.any(x.y), scaled.any(x.z), scaled.any(x.w));
+            bad = bad || v.x != v.x || v.y != v.y || v.z != v.z || v.w != v.w;
         }
+        top_all = fmaxf(top_all, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+        if (banned) {
+            const int s = q * 4 - phase;
+            uint32_t out = 0u;
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-            const int q = q0 + k * 32, s = q * 4 - phase;
-            if (q >= last) break;
-            if ((unsigned)(q - full_from) >= (unsigned)max(full, 0)) {
-                if (s >= 0 && s < n) x[k].x = __ldcs(part + s);
-                if (s + 1 >= 0 && s + 1 < n) x[k].y = __ldcs(part + s + 1);
-                if (s + 2 >= 0 && s + 2 < n) x[k].z = __ldcs(part + s + 2);
-                if (s + 3 >= 0 && s + 3 < n) x[k].w = __ldcs(part + s + 3);
-            }
-            float4 v;
-            if (scaled.plain(x[k].x) && scaled.plain(x[k].y) && scaled.plain(x[k].z) && scaled.plain(x[k].w)) {
-                v = make_float4(scaled.plainly(x[k].x), scaled.plainly(x[k].y), scaled.plainly(x[k].z), scaled.plainly(x[k].w));
-            } else {
-                v = make_float4(scaled.any(x[k].x), scaled.any(x[k].y), scaled.any(x[k].z), scaled.any(x[k].w));
-                bad = bad || v.x != v.x || v.y != v.y || v.z != v.z || v.w != v.w;
-            }
-            const float most = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
-            top_all = fmaxf(top_all, most);
-            if (banned) {
-                uint32_t out = 0u;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (s + j >= 0 && s + j < n && banned[s + j]) out |= 1u << j;
-                flags[q] = (unsigned char)out;
-                top_ok = fmaxf(top_ok, fmaxf(fmaxf(out & 1u ? -INFINITY : v.x, out & 2u ? -INFINITY : v.y), fmaxf(out & 4u ? -INFINITY : v.z, out & 8u ? -INFINITY : v.w)));
-            }
-            reinterpret_cast<float4*>(keys)[q] = v;
+            for (int j = 0; j < 4; ++j)
+                if (s + j >= 0 && s + j < n && banned[s + j]) out |= 1u << j;
+            flags[q] = (unsigned char)out;
+            top_ok = fmaxf(top_ok, fmaxf(fmaxf(out & 1u ? -INFINITY : v.x, out & 2u ? -INFINITY : v.y), fmaxf(out & 4u ? -INFINITY : v.z, out & 8u ? -INFINITY : v.w)));
         }
+        reinterpret_cast<float4*>(keys)[q] = v;
+    };
+    const auto edge = [&](int q) {
+        const int s = q * 4 - phase;
+        const auto at = [&](int i) { return i >= 0 && i < n ? __ldcs(part + i) : -INFINITY; };
+        scale(q, make_float4(at(s), at(s + 1), at(s + 2), at(s + 3)));
+    };
+    {
+        int q = first + lane;
+        if (q < full_from && q < last) {
+            edge(q);
+            q += 32;
+        }
+        const int stop = min(last, full_to);
+        const float4* from = reinterpret_cast<const float4*>(slots);
+        for (; q + 32 * (kAhead - 1) < stop; q += 32 * kAhead) {
+            float4 x[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) x[k] = __ldcs(from + q + 32 * k);
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) scale(q + 32 * k, x[k]);
+        }
+        float4 x[kAhead - 1];
+#pragma unroll
+        for (int k = 0; k < kAhead - 1; ++k)
+            if (q + 32 * k < stop) x[k] = __ldcs(from + q + 32 * k);
+#pragma unroll
+        for (int k = 0; k < kAhead - 1; ++k)
+            if (q + 32 * k < stop) scale(q + 32 * k, x[k]);
+        if (full_to >= first && full_to < last && (full_to - first) % 32 == lane) edge(full_to);
     }
     top_all = warp_max(top_all);
     top_ok = banned ? warp_max(top_ok) : top_all;
@@ -545,10 +595,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Sample a) {
 
     // keys in place of the t, and the sums
     Sums sums;
-    if (banned)
-        cut_by_k ? make_keys<true, true>(sums, keys, flags, first + lane, last, shift, shift_all) : make_keys<true, false>(sums, keys, flags, first + lane, last, shift, shift_all);
-    else
-        cut_by_k ? make_keys<false, true>(sums, keys, flags, first + lane, last, shift, shift_all) : make_keys<false, false>(sums, keys, flags, first + lane, last, shift, shift_all);
+    if (!banned) flags = nullptr;
+    if (fmaxf(fabsf(shift), fabsf(shift_all)) < 1048576.0f) {
+        if (banned)
+            cut_by_k ? make_keys<true, true, true>(sums, keys, flags, first + lane, last, shift, shift_all) : make_keys<true, true, false>(sums, keys, flags, first + lane, last, shift, shift_all);
+        else
+            cut_by_k ? make_keys<true, false, true>(sums, keys, flags, first + lane, last, shift, shift_all) : make_keys<true, false, false>(sums, keys, flags, first + lane, last, shift, shift_all);
+    } else {
+        make_keys<false, true, true>(sums, keys, flags, first + lane, last, shift, shift_all);
+    }
     u64 weight = warp_sum(sums.units.get());
     const double sum = warp_sum(sums.sum + (shift >= -1.0f ? (double)sums.rest * power_of(-shift) : 0.0));     // (|t| < 1 only above)
     const double banned_sum = banned ? warp_sum(sums.banned) : 0.0;
@@ -575,6 +630,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Sample a) {
     }
     team.wait();
     Search search{sh, team, keys, first, last, lane, warp, begin - phase, rank};
+    if (t < warps) {
+        const Shared& other = team.of(sh, t / kWarps);
+        sh.every_sum[t] = other.sums[t % kWarps] * power_of(shift - shift_all) + (banned ? other.banned_sums[t % kWarps] : 0.0);
+    }
     u64 upto, total = search.total_of([&](int c, int w) { return team.of(sh, c).parts[w]; }, &upto);
 
     // what stays
@@ -608,7 +667,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Sample a) {
                 cut = search.find<true>((u64)top_k, kEnd - 1u);
                 if (cut_by_p) {
                     u64 own, before;
-                    total = search.weigh(cut, 0.0, turn, &own, &before);
+                    total = search.weigh(cut, turn, &own, &before);
                     turn ^= 1;
                 }
             }
@@ -623,16 +682,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Sample a) {
         if (cut != ~0ull) most = min(most, (uint32_t)(cut >> kNumberBits));
         cut = search.find<false>(target, most);
     }
-    const u64 least = share_up(steps(min_p, 1u << 24), weight_of(top_key));
-    if (cut != ~0ull || least > 0) total = search.weigh(cut, (double)least * 0x1p-44, turn, &weight, &upto);
+    if (min_p > 0.0f) {
+        // the key of the least e with floor(2^44 e) as large as that share
+        const u64 least = share_up(steps(min_p, 1u << 24), weight_of(top_key));
+        cut = min(cut, (u64)(kTop - (uint32_t)f2i(__double2float_ru((double)least * 0x1p-44))) << kNumberBits | ((1u << kNumberBits) - 1u));
+    }
+    if (cut != ~0ull) total = search.weigh(cut, turn, &weight, &upto);
+    team.done();
     const u64 drawn = share(fraction, total).whole;
     if (upto <= drawn && drawn < upto + weight) {
         // this warp has the token
         double all = 0.0;
-        for (int w = lane; w < warps; w += 32) {
-            const Shared& other = team.of(sh, w / kWarps);
-            all += other.sums[w % kWarps] * power_of(shift - shift_all) + (banned ? other.banned_sums[w % kWarps] : 0.0);
-        }
+        for (int w = lane; w < warps; w += 32) all += sh.every_sum[w];
         all = warp_sum(all);
         for (int q = first; q < last; q += 32) {
             const uint4 k = q + lane < last ? reinterpret_cast<const uint4*>(keys)[q + lane] : make_uint4(kOut, kOut, kOut, kOut);
@@ -643,7 +704,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Sample a) {
             for (int j = 0; j < 4; ++j) {
                 const bool in = key[j] != kOut && ((u64)key[j] << kNumberBits | (uint32_t)(number + j)) <= cut;
                 w[j] = in ? weight_of(key[j]) : 0ull;
-                if (w[j] < least) w[j] = 0ull;
                 own += w[j];
             }
             const u64 run = upto + warp_upto(own);
@@ -662,7 +722,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Sample a) {
             upto = __shfl_sync(0xffffffffu, run, 31);
         }
     }
-    team.wait();                                                                      // (no CTA leaves while others read its memory)
+    team.all_done();                                                                  // (no CTA leaves while others read its memory)
 }
 
 // CTAs of a row: as many as its keys need, and more where rows are few.

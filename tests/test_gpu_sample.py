@@ -92,6 +92,14 @@ def test_masked_banned_and_spoilt_rows(sample):
             assert tokens[[1, 3, 4, 5]].eq(-1).all() and scores[[1, 3, 4, 5]].eq(-INF).all()
 
 
+def test_banned_tokens_far_above(sample):
+    """What may be drawn lies octaves, or a whole range of numbers, below what may not."""
+    x, u = data(7, 400, seed=14)
+    x[:, 3] = torch.tensor([20.0, 40.0, 90.0, 1e3, 1e6, 1e9, 1e30])
+    for settings in (dict(), dict(top_k=4), dict(top_p=0.6)):
+        check(sample, x, u, banned=torch.arange(400) == 3, **settings)
+
+
 def test_settings_of_each_row(sample):
     x, u = data(24, 900, seed=6)
     g = torch.Generator().manual_seed(8)
