@@ -17,8 +17,9 @@
 // A row belongs to a cluster of up to eight CTAs, each of which keeps its part in shared memory: the t of its tokens, then their keys.  A warp has neighbouring
 // tokens, of which a thread has the same four at a time from loading to drawing.  The logits are read once.  What stays is cut off at one token, found as follows:
 //   top-k   each warp's q-th best of its lanes' best tokens, where q of each of w warps are k at least, bounds the k-th best of all; the few tokens as good as the
-//           bound go to a list in the first CTA, which sorts it;
-//   top-p   passes over the keys take the weights below three borders each, until at most 512 tokens are left between two; these go to the list.
+//           bound go to a list in the first CTA, which sorts it and draws from it;
+//   top-p   passes over the keys take the weights below some borders each, until few tokens are left between two; these go to the list.  After the first pass
+//           a warp most often has few enough keys in the range to set them aside for the others.
 // (A histogram of 2048 parts of 1/32 of an octave for the latter: its atomics, and its reading by all CTAs of a cluster, made it 640 us for 256 rows of 151643 tokens.)
 #include <cooperative_groups.h>
 
@@ -32,17 +33,12 @@ namespace cg = cooperative_groups;
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kMasked = -1e30f;                     // a logit as low as this is masked
-constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kMostCtas = 8, kMostKeys = 32768;       // of a cluster; of a CTA
 constexpr uint32_t kOut = 0xffffffffu;                // the key of a token without weight
 constexpr uint32_t kTop = 0x3fffffffu;                // key + pattern
 constexpr uint32_t kEnd = 45u << 23;                  // keys with a weight are below
-constexpr int kListed = kThreads;                     // a thread for each
-constexpr int kFew = 256;
 constexpr int kNumberBits = 18;
 static_assert(kMostCtas * kMostKeys == 1 << kNumberBits);
-// a thread's tokens: their e stay below 2^8 together
-static_assert((kMostKeys / 4 / kThreads + 2) * 4 * 2 < 256);
 typedef unsigned long long u64;
 
 struct Sample {
@@ -58,11 +54,15 @@ struct Sample {
     float* scores;
 };
 
-struct Found { u64 weights[3]; uint32_t counts[4]; };                     // before each border; and in all
+constexpr int kMostBorders = 7;
+struct Found { u64 weights[kMostBorders]; uint32_t counts[kMostBorders + 1]; };        // before each border; and in all
 
+template <int THREADS>
 struct Shared {
-    u64 list[kListed];
-    uint32_t few[kWarps][kFew];                       // a warp's keys in the range of a search
+    static constexpr int kWarps = THREADS / 32, kFew = THREADS / 2;
+    u64 list[THREADS];                                // as many as there are threads
+    uint32_t few[kWarps][kFew];                       // a warp's keys in the range of a search, and their slots
+    uint16_t few_slots[kWarps][kFew];
     // what the other CTAs of the cluster read
     float all, ok;
     int bad;
@@ -95,7 +95,8 @@ struct Team {
     __device__ void all_done() {
         if (ctas > 1) asm volatile("barrier.cluster.wait;" ::: "memory");
     }
-    __device__ Shared& of(Shared& sh, int c) { return ctas == 1 ? sh : *cluster.map_shared_rank(&sh, c); }
+    template <class S>
+    __device__ S& of(S& sh, int c) { return ctas == 1 ? sh : *cluster.map_shared_rank(&sh, c); }
 };
 
 // A normal float >= 0 of this pattern as a double (the conversion instruction has a quarter of the rate).
@@ -127,11 +128,14 @@ __device__ __forceinline__ u64 share_up(uint32_t fraction, u64 total) {
 // A fraction in steps of 2^-24, NaN as 0.
 __device__ __forceinline__ uint32_t steps(float f, uint32_t most) { return f > 0.0f ? min((uint32_t)fminf(f * 16777216.0f, 16777216.0f), most) : 0u; }
 
-template <class T>
-__device__ __forceinline__ T warp_sum(T v) {
+__device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
     return v;
+}
+__device__ __forceinline__ u64 warp_sum(u64 v) {      // by 22 bits, whose sums have 27
+    const u64 low = __reduce_add_sync(0xffffffffu, (uint32_t)v & 0x3fffffu), mid = __reduce_add_sync(0xffffffffu, (uint32_t)(v >> 22) & 0x3fffffu);
+    return low + (mid << 22) + ((u64)__reduce_add_sync(0xffffffffu, (uint32_t)(v >> 44)) << 44);
 }
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
@@ -178,40 +182,58 @@ struct Scaling {
     __device__ __noinline__ float any(float x) const { return x <= kMasked ? -INFINITY : mul(div(x, temperature, 0), kLog2e, 0); }
 };
 
+// Sorts the threads' values, the first `size` (a power of two of at least 32) of them, through shared memory where pairs are in different warps.
+__device__ __forceinline__ void sort(u64& own, int size, u64* memory) {
+    const int t = threadIdx.x;
+    for (int run = 2; run <= size; run *= 2)
+        for (int apart = run / 2; apart > 0; apart /= 2) {
+            u64 other;
+            if (apart >= 32) {
+                __syncthreads();
+                memory[t] = own;
+                __syncthreads();
+                other = memory[t ^ apart];
+            } else {
+                other = __shfl_xor_sync(0xffffffffu, own, apart);
+            }
+            const bool up = (t & run) == 0 || run == size, lower = (t & apart) == 0;
+            own = (own < other) == (up == lower) ? own : other;
+        }
+}
+
+// What is asked of a row.
+struct Wanted { float top_p; uint32_t min_p, uniform; };
+
 // A search for the token at which a count or a weight is reached, in the order of (key, number).
+template <int THREADS>
 struct Search {
-    Shared& sh;
+    static constexpr int kWarps = THREADS / 32, kListed = THREADS;
+    typedef Shared<THREADS> Sh;
+    Sh& sh;
     Team& team;
     const uint32_t* keys;                             // of the CTA's slots
     int first, last, lane, warp;                      // the warp's quads; the lane's are every 32nd
     int begin, rank;                                  // the number of slot 0 (it may be before the part); the CTA's rank
+    int few = -1;                                     // how many of its keys the warp has set aside
+    u64 own_less = 0ull;                              // the warp's weights before them
 
     __device__ __forceinline__ uint4 quad(int q) const { return q < last ? reinterpret_cast<const uint4*>(keys)[q] : make_uint4(kOut, kOut, kOut, kOut); }
 
     template <class F>
-    __device__ __forceinline__ void each(F&& f) const {               // f(key, number) for all; warps stay together
+    __device__ __forceinline__ void each(F&& f) const {               // f(key, slot) for all; warps stay together
         for (int q = first + lane; q - lane < last; q += 32) {
             const uint4 k = quad(q);
-            const int number = begin + q * 4;
-            f(k.x, number);
-            f(k.y, number + 1);
-            f(k.z, number + 2);
-            f(k.w, number + 3);
+            f(k.x, q * 4);
+            f(k.y, q * 4 + 1);
+            f(k.z, q * 4 + 2);
+            f(k.w, q * 4 + 3);
         }
     }
-
-    // The weight of all tokens up to `cut`; `own` is this warp's and `before` that of the warps before.  `turn` alternates from call to call.
-    __device__ u64 weigh(u64 cut, int turn, u64* own, u64* before) {
-        const uint32_t cut_key = (uint32_t)(cut >> kNumberBits), cut_number = (uint32_t)cut & ((1u << kNumberBits) - 1u);
-        Units stay;
-        each([&](uint32_t key, int number) {
-            if (key < cut_key || (key == cut_key && number <= (int)cut_number)) stay.add(value_of(key));
-        });
-        *own = warp_sum(stay.get());
-        if (lane == 0) sh.staying[turn][warp] = *own;
-        team.wait();
-        return total_of([&](int c, int w) { return team.of(sh, c).staying[turn][w]; }, before);
+    template <class F>
+    __device__ __forceinline__ void each_aside(F&& f) const {
+        for (int i = lane; i - lane < few; i += 32) i < few ? f(sh.few[warp][i], (int)sh.few_slots[warp][i]) : f(kOut, 0);
     }
+    __device__ __forceinline__ u64 composite(uint32_t key, int slot) const { return (u64)key << kNumberBits | (uint32_t)(begin + slot); }
 
     // The sum of a value of all warps of the cluster, and of those before this one.  There is a barrier within.
     template <class F>
@@ -228,134 +250,181 @@ struct Search {
         return warp_sum(total);
     }
 
-    // What lies in [low, low + border_j) for three borders, and how many keys in [low, low + all).  A warp that has few of these keeps them for the calls to
-    // come, whose ranges lie within.
-    template <bool WEIGHTS>
-    __device__ Found below(uint32_t low, const uint32_t (&border)[3], uint32_t all, int turn, int& few) {
-        Units units[3];
-        uint32_t counts[4] = {0u, 0u, 0u, 0u};
+    // The weight of all tokens up to `cut`; `own` is this warp's and `before` that of the warps before.  `turn` alternates from call to call.
+    __device__ u64 weigh(u64 cut, int turn, u64* own, u64* before) {
+        Units stay;
+        u64 less = 0ull;
+        if (few >= 0) {                               // (the search's cut: what is before its last range is known)
+            less = own_less;
+            each_aside([&](uint32_t key, int slot) {
+                if (composite(key, slot) <= cut) stay.add(value_of(key));
+            });
+        } else {
+            const uint32_t cut_key = (uint32_t)(cut >> kNumberBits);
+            const int cut_slot = (int)((uint32_t)cut & ((1u << kNumberBits) - 1u)) - begin;
+            each([&](uint32_t key, int slot) {
+                if (key < cut_key || (key == cut_key && slot <= cut_slot)) stay.add(value_of(key));
+            });
+        }
+        *own = less + warp_sum(stay.get());
+        if (lane == 0) sh.staying[turn][warp] = *own;
+        team.wait();
+        return total_of([&](int c, int w) { return team.of(sh, c).staying[turn][w]; }, before);
+    }
+
+    // What lies in [low, low + border_j) for some borders, and how many keys in [low, low + all): of the warp, then (in *joint) of the cluster.  A warp that
+    // has few of these sets them aside for the calls to come, whose ranges lie within.
+    template <bool WEIGHTS, int BORDERS>
+    __device__ Found below(uint32_t low, const uint32_t (&border)[BORDERS], uint32_t all, int turn, Found* joint) {
+        Units units[BORDERS];
+        uint32_t counts[BORDERS + 1];
+#pragma unroll
+        for (int j = 0; j <= BORDERS; ++j) counts[j] = 0u;
         const auto look = [&](uint32_t key) {
             const uint32_t at = key - low;
             const double e = WEIGHTS ? value_of(key) : 0.0;
 #pragma unroll
-            for (int j = 0; j < 3; ++j) {
+            for (int j = 0; j < BORDERS; ++j) {
                 const bool in = at < border[j];
                 if (WEIGHTS) units[j].sum = in ? __dadd_rd(units[j].sum, e) : units[j].sum;
                 counts[j] += in;
             }
-            counts[3] += at < all;
+            counts[BORDERS] += at < all;
             return at < all;
         };
         if (few >= 0) {
-            for (int i = lane; i < few; i += 32) look(sh.few[warp][i]);
+            each_aside([&](uint32_t key, int) { look(key); });
         } else {
             int found = 0;
-            each([&](uint32_t key, int) {
+            each([&](uint32_t key, int slot) {
                 const bool in = look(key);
                 const uint32_t those = __ballot_sync(0xffffffffu, in);
                 const int place = found + __popc(those & ((1u << lane) - 1u));
-                if (in && place < kFew) sh.few[warp][place] = key;
+                if (in && place < Sh::kFew) {
+                    sh.few[warp][place] = key;
+                    sh.few_slots[warp][place] = (uint16_t)slot;
+                }
                 found += __popc(those);
             });
-            if (found <= kFew) few = found;
+            if (found <= Sh::kFew) few = found;
             __syncwarp();
         }
-        Found f;
+        Found own{};
 #pragma unroll
-        for (int j = 0; j < 3; ++j) f.weights[j] = WEIGHTS ? warp_sum(units[j].get()) : 0ull;
+        for (int j = 0; j < BORDERS; ++j) own.weights[j] = WEIGHTS ? warp_sum(units[j].get()) : 0ull;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f.counts[j] = __reduce_add_sync(0xffffffffu, counts[j]);
-        if (lane == 0) sh.warps[warp] = f;
+        for (int j = 0; j <= BORDERS; ++j) own.counts[j] = __reduce_add_sync(0xffffffffu, counts[j]);
+        if (lane == 0) sh.warps[warp] = own;
         __syncthreads();
-        const auto joined = [&](int n, auto&& of) {                   // (n <= 16; the same in all lanes)
-            Found g{};
-            if (lane < n) g = of(lane);
+        const auto joined = [&](int n, auto&& of) {                   // (n <= 32; the same in all lanes)
+            Found g{}, here{};
+            if (lane < n) here = of(lane);
 #pragma unroll
-            for (int j = 0; j < 3; ++j) g.weights[j] = WEIGHTS ? warp_sum(g.weights[j]) : 0ull;
+            for (int j = 0; j < BORDERS; ++j) g.weights[j] = WEIGHTS ? warp_sum(here.weights[j]) : 0ull;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) g.counts[j] = __reduce_add_sync(0xffffffffu, g.counts[j]);
+            for (int j = 0; j <= BORDERS; ++j) g.counts[j] = __reduce_add_sync(0xffffffffu, here.counts[j]);
             return g;
         };
-        f = joined(kWarps, [&](int w) { return sh.warps[w]; });
+        *joint = joined(kWarps, [&](int w) { return sh.warps[w]; });
         if (team.ctas > 1) {
-            if (threadIdx.x == 0) sh.found[turn] = f;
+            if (threadIdx.x == 0) sh.found[turn] = *joint;
             team.wait();
-            f = joined(team.ctas, [&](int c) { return team.of(sh, c).found[turn]; });
+            *joint = joined(team.ctas, [&](int c) { return team.of(sh, c).found[turn]; });
         } else {
             __syncthreads();                          // (the warps' are written anew)
         }
-        return f;
+        return own;
     }
 
-    // The tokens with keys from `low` to `high` to the first CTA's list; false where there are too many.  sh.listed is 0 before.
-    __device__ bool gather(uint32_t low, uint32_t high) {
-        Shared& head = team.of(sh, 0);
-        for (int q = first + lane; q - lane < last; q += 32) {
-            const uint4 k = quad(q);
-            const uint32_t span = high - low;
-            if (!__any_sync(0xffffffffu, min(min(k.x - low, k.y - low), min(k.z - low, k.w - low)) <= span)) continue;
-            const uint32_t key[4] = {k.x, k.y, k.z, k.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const bool in = key[j] - low <= span;
-                const uint32_t all = __ballot_sync(0xffffffffu, in);
-                if (all == 0u) continue;
-                uint32_t at = 0u;
-                if (lane == 0) at = atomicAdd(&head.listed, (uint32_t)__popc(all));
-                at = __shfl_sync(0xffffffffu, at, 0) + __popc(all & ((1u << lane) - 1u));
-                if (in && at < kListed) head.list[at] = (u64)key[j] << kNumberBits | (uint32_t)(begin + q * 4 + j);
+    // The tokens with keys from `low` to `high` to the first CTA's list; false where there are too many.  sh.listed is 0 before.  (best: no key of the lane is smaller.)
+    __device__ bool gather(uint32_t low, uint32_t high, uint32_t best) {
+        Sh& head = team.of(sh, 0);
+        const auto put = [&](uint32_t key, int slot) {
+            const bool in = key - low <= high - low;
+            const uint32_t those = __ballot_sync(0xffffffffu, in);
+            if (those == 0u) return;
+            uint32_t at = 0u;
+            if (lane == 0) at = atomicAdd(&head.listed, (uint32_t)__popc(those));
+            at = __shfl_sync(0xffffffffu, at, 0) + __popc(those & ((1u << lane) - 1u));
+            if (in && at < kListed) head.list[at] = composite(key, slot);
+        };
+        if (few >= 0) {
+            each_aside(put);
+        } else if (__any_sync(0xffffffffu, best <= high)) {
+            for (int q = first + lane; q - lane < last; q += 32) {
+                const uint4 k = quad(q);
+                if (!__any_sync(0xffffffffu, min(min(k.x - low, k.y - low), min(k.z - low, k.w - low)) <= high - low)) continue;
+                put(k.x, q * 4);
+                put(k.y, q * 4 + 1);
+                put(k.z, q * 4 + 2);
+                put(k.w, q * 4 + 3);
             }
         }
         team.wait();
         return head.listed <= kListed;
     }
 
-    // In the first CTA: the list's token at which the target is reached, less_* before the list.  With a count, and top_p < 1 (the list then starts with the first token
-    // of all), the one at which that share of the weights up to there is.  sh.cut and sh.kept, the weight up to it, are set.
-    __device__ void pick(bool by_count, u64 target, float top_p, uint32_t less_count, u64 less_weight) {
-        const int t = threadIdx.x, n = (int)sh.listed;
-        u64 own = t < n ? sh.list[t] : ~0ull;
-        int size = 32;                                // sorted by pairs at distances 2^j, within a warp from 16 down
-        while (size < n) size *= 2;
-        for (int run = 2; run <= size; run *= 2)
-            for (int apart = run / 2; apart > 0; apart /= 2) {
-                u64 other;
-                if (apart >= 32) {
-                    __syncthreads();
-                    sh.list[t] = own;
-                    __syncthreads();
-                    other = sh.list[t ^ apart];
-                } else {
-                    other = __shfl_xor_sync(0xffffffffu, own, apart);
-                }
-                const bool up = (t & run) == 0 || run == size, lower = (t & apart) == 0;
-                own = (own < other) == (up == lower) ? own : other;
-            }
-        const u64 weight = t < n ? weight_of((uint32_t)(own >> kNumberBits)) : 0ull, upto_warp = warp_upto(weight);
+    // Sums of weights up to each thread's, which are in order.
+    __device__ u64 upto_of(u64 weight) {
+        const u64 upto_warp = warp_upto(weight);
+        __syncthreads();
         if (lane == 31) sh.scan[warp] = upto_warp;
         __syncthreads();
-        u64 upto = less_weight + upto_warp;
+        u64 upto = upto_warp;
         for (int w = 0; w < warp; ++w) upto += sh.scan[w];
-        if (t < n && (by_count ? less_count + t + 1 == target : upto - weight < target && target <= upto)) {
-            sh.cut = own;
-            sh.kept = upto;
-        }
-        __syncthreads();
-        if (!by_count || !(top_p < 1.0f)) return;
-        const u64 share_of = max(share_up(steps(top_p, 0xffffffu), sh.kept), 1ull);
-        __syncthreads();
-        if (t < n && upto - weight < share_of && share_of <= upto) sh.cut = own;
+        return upto;
+    }
+    __device__ static int room_for(int n) {
+        int size = 32;
+        while (size < n) size *= 2;
+        return size;
     }
 
-    // gather and pick; false where there are too many.
-    __device__ bool listed(uint32_t low, uint32_t high, bool by_count, u64 target, float top_p, uint32_t less_count, u64 less_weight, u64* cut) {
-        const bool few = gather(low, high);
-        if (few && rank == 0) pick(by_count, target, top_p, less_count, less_weight);
+    // In the first CTA: sets sh.cut to the list's token at which the weight `target` is reached, less_weight before the list (by_count: the target-th, less_count before).
+    __device__ void pick(bool by_count, u64 target, uint32_t less_count, u64 less_weight) {
+        const int t = threadIdx.x, n = (int)sh.listed;
+        u64 own = t < n ? sh.list[t] : ~0ull;
+        sort(own, room_for(n), sh.list);
+        const u64 weight = t < n ? weight_of((uint32_t)(own >> kNumberBits)) : 0ull, upto = less_weight + upto_of(weight);
+        if (t < n && (by_count ? less_count + t + 1 == target : upto - weight < target && target <= upto)) sh.cut = own;
+    }
+
+    // In the first CTA: draws from the list, which holds the k best tokens and maybe others.  The token's number is then in sh.cut.
+    __device__ void draw(int k, const Wanted& wanted, u64 top_weight) {
+        const int t = threadIdx.x, n = (int)sh.listed;
+        u64 own = t < n ? sh.list[t] : ~0ull;
+        sort(own, room_for(n), sh.list);
+        u64 weight = t < k ? weight_of((uint32_t)(own >> kNumberBits)) : 0ull;
+        const u64 upto = upto_of(weight);
+        if (t == k - 1) sh.kept = upto;
+        __syncthreads();
+        const u64 limit = wanted.top_p < 1.0f ? max(share_up(steps(wanted.top_p, 0xffffffu), sh.kept), 1ull) : ~0ull;
+        if (upto - weight >= limit || weight < share_up(wanted.min_p, top_weight)) weight = 0ull;
+        // in order of their numbers
+        u64 by_number = weight ? (own & ((1u << kNumberBits) - 1u)) << 32 | (uint32_t)t : ~0ull;
+        __syncthreads();
+        sort(by_number, room_for(k), sh.list);
+        __syncthreads();
+        sh.list[t] = weight;
+        __syncthreads();
+        weight = by_number != ~0ull ? sh.list[(uint32_t)by_number] : 0ull;
+        const u64 before = upto_of(weight) - weight;
+        if (t == THREADS - 1) sh.kept = before + weight;
+        __syncthreads();
+        const u64 drawn = share(wanted.uniform, sh.kept).whole;
+        if (weight && before <= drawn && drawn < before + weight) sh.cut = by_number >> 32;
+        __syncthreads();
+    }
+
+    // The cut, of which is known that it is one of the tokens with these keys; false where there are too many.
+    __device__ bool listed(uint32_t low, uint32_t high, bool by_count, u64 target, uint32_t less_count, u64 less_weight, u64* cut) {
+        const bool fits = gather(low, high, low);
+        if (fits && rank == 0) pick(by_count, target, less_count, less_weight);
         team.wait();
         *cut = team.of(sh, 0).cut;
         if (rank == 0 && threadIdx.x == 0) sh.listed = 0u;
         team.wait();
-        return few;
+        return fits;
     }
 
     // The r-th token, by number, of those with this key.
@@ -383,7 +452,7 @@ struct Search {
                     if (lane == __ffs(reached) - 1) {
                         uint32_t left = is;
                         for (uint32_t i = upto - __popc(is) + 1; i < need; ++i) left &= left - 1;
-                        team.of(sh, 0).cut = (u64)key << kNumberBits | (uint32_t)(begin + q * 4 + __ffs(left) - 1);
+                        team.of(sh, 0).cut = composite(key, q * 4 + __ffs(left) - 1);
                     }
                     break;
                 }
@@ -396,33 +465,63 @@ struct Search {
         return cut;
     }
 
+    // One step of a search: [low, high] becomes the last of the parts between borders with less than the target before it.  How many keys it has.
+    template <bool BY_COUNT, int BORDERS>
+    __device__ uint32_t narrow(const uint32_t (&border)[BORDERS], u64 target, uint32_t& low, uint32_t& high, uint32_t& less_count, u64& less_weight, int turn) {
+        const uint32_t span = high - low;             // (below 2^29)
+        Found f;
+        const Found own = below<!BY_COUNT>(low, border, span + 1, turn, &f);
+        uint32_t start = 0u, end = span + 1, before = 0u, upto = f.counts[BORDERS];
+        u64 weight_before = 0ull, own_before = 0ull;
+        bool on = true;
+#pragma unroll
+        for (int j = 0; j < BORDERS; ++j) {
+            on = on && (BY_COUNT ? less_count + f.counts[j] : less_weight + f.weights[j]) < target;
+            if (on) {
+                start = border[j];
+                before = f.counts[j];
+                weight_before = f.weights[j];
+                own_before = own.weights[j];
+            }
+        }
+#pragma unroll
+        for (int j = BORDERS - 1; j >= 0; --j)
+            if ((BY_COUNT ? less_count + f.counts[j] : less_weight + f.weights[j]) >= target) {
+                end = border[j];
+                upto = f.counts[j];
+            }
+        high = low + end - 1;
+        low += start;
+        less_count += before;
+        less_weight += weight_before;
+        if (few < 0) own_less += own_before;          // (what was set aside counts for itself)
+        return upto - before;
+    }
+
     // The cut, which is among the keys up to `high`.
     template <bool BY_COUNT>
     __device__ u64 find(u64 target, uint32_t high) {
         uint32_t low = 0u, less_count = 0u;
         u64 less_weight = 0ull;
-        int few = -1;
-        for (int turn = -2;; turn = turn < 0 ? turn + 3 : turn ^ 1) {                  // (-2: the first)
-            const uint32_t span = high - low;         // (below 2^29)
-            uint32_t border[3] = {(span + 1) / 4, (span + 1) / 2, (uint32_t)((u64)(span + 1) * 3 / 4)};
-            if (!BY_COUNT && turn < 0 && span > 8u << 23) {
-                // (what is left out weighs as much as the whole vocabulary at `high`: most often its heaviest are a few octaves above)
-                border[0] = span - (5u << 23);
-                border[1] = span - (7u << 22);
-                border[2] = span - (2u << 23);
-            }
-            const Found f = below<!BY_COUNT>(low, border, span + 1, turn & 1, few);
-            int j = 0;                                // the last part with less than the target before it
-            while (j < 3 && (BY_COUNT ? less_count + f.counts[j] : less_weight + f.weights[j]) < target) ++j;
-            const uint32_t end = j < 3 ? border[j] : span + 1, start = j > 0 ? border[j - 1] : 0u, left = f.counts[j] - (j > 0 ? f.counts[j - 1] : 0u);
-            high = low + end - 1;
-            low += start;
-            if (j > 0) {
-                less_count += f.counts[j - 1];
-                less_weight += f.weights[j - 1];
+        few = -1;
+        own_less = 0ull;
+        for (int turn = 0, step = 0;; turn ^= 1, ++step) {
+            const uint32_t span = high - low;
+            uint32_t left;
+            if (step == 0) {
+                // (by weight, what is left out weighs as much as the whole vocabulary at `high`: most often its heaviest are a few octaves above)
+                const bool guess = !BY_COUNT && span > 8u << 23;
+                const uint32_t border[3] = {guess ? span - (5u << 23) : (span + 1) / 4, guess ? span - (7u << 22) : (span + 1) / 2,
+                                            guess ? span - (2u << 23) : (uint32_t)((u64)(span + 1) * 3 / 4)};
+                left = narrow<BY_COUNT>(border, target, low, high, less_count, less_weight, turn);
+            } else {
+                uint32_t border[kMostBorders];
+#pragma unroll
+                for (int j = 0; j < kMostBorders; ++j) border[j] = (uint32_t)((u64)(span + 1) * (j + 1) / (kMostBorders + 1));
+                left = narrow<BY_COUNT>(border, target, low, high, less_count, less_weight, turn);
             }
             u64 cut;
-            if (left <= kListed && listed(low, high, BY_COUNT, target, 1.0f, less_count, less_weight, &cut)) return cut;
+            if (left <= kListed && listed(low, high, BY_COUNT, target, less_count, less_weight, &cut)) return cut;
             if (low == high) {
                 const u64 each_weight = weight_of(low);
                 return equal_one(low, BY_COUNT ? target - less_count : (target - less_weight + each_weight - 1) / each_weight);
@@ -478,10 +577,14 @@ __device__ __forceinline__ void make_keys(Sums& sums, uint32_t* keys, const unsi
     }
 }
 
-__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Sample a) {
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const Sample a) {
+    constexpr int kWarps = THREADS / 32;
+    // (the e of a thread's tokens stay below 2^8 together)
+    static_assert((kMostKeys / 512 * THREADS / 4 / THREADS + 2) * 4 * 2 < 256);
     extern __shared__ __align__(16) unsigned char memory[];
-    Shared& sh = *reinterpret_cast<Shared*>(memory);
-    uint32_t* keys = reinterpret_cast<uint32_t*>(memory + (sizeof(Shared) + 15) / 16 * 16);
+    Shared<THREADS>& sh = *reinterpret_cast<Shared<THREADS>*>(memory);
+    uint32_t* keys = reinterpret_cast<uint32_t*>(memory + (sizeof(sh) + 15) / 16 * 16);
     unsigned char* flags = reinterpret_cast<unsigned char*>(keys + a.part + 4);       // four bits for each quad: banned
     Team team{cg::this_cluster(), 0};
     team.ctas = (int)team.cluster.num_blocks();
@@ -492,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Sample a) {
     const float temperature = a.temperatures ? __ldg(a.temperatures + row) : a.temperature;
     const float top_p = a.top_ps ? __ldg(a.top_ps + row) : a.top_p, min_p = a.min_ps ? __ldg(a.min_ps + row) : a.min_p;
     const int64_t top_k = a.top_ks ? __ldg(reinterpret_cast<const long long*>(a.top_ks) + row) : a.top_k;
-    const uint32_t fraction = steps(__ldg(a.uniform + row), 0xffffffu);
+    const Wanted wanted{top_p, steps(min_p, 1u << 24), steps(__ldg(a.uniform + row), 0xffffffu)};
     const bool cut_by_k = top_k > 0 && top_k < a.vocab;
     const Scaling scaled(temperature);
 
@@ -575,7 +678,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Sample a) {
         }
         team.wait();
         for (int c = 0; c < team.ctas; ++c) {
-            const Shared& other = team.of(sh, c);
+            const Shared<THREADS>& other = team.of(sh, c);
             top_all = fmaxf(top_all, other.all);
             top_ok = fmaxf(top_ok, other.ok);
             no_token |= other.bad;
@@ -613,8 +716,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Sample a) {
         sh.banned_sums[warp] = banned_sum;
     }
     // of the lanes' best the q-th best, where q of each warp are k at least
-    const int warps = team.ctas * kWarps, q = cut_by_k ? (int)((min(top_k, (int64_t)kListed) + warps - 1) / warps) : 0;
-    const bool bounded = cut_by_k && top_k <= kListed / 2 && q <= 32;
+    const int warps = team.ctas * kWarps, q = cut_by_k ? (int)((min(top_k, (int64_t)THREADS) + warps - 1) / warps) : 0;
+    const bool bounded = cut_by_k && top_k <= THREADS / 2 && q <= 32;
     if (cut_by_k) {
         const uint32_t live = __reduce_add_sync(0xffffffffu, sums.live);
         if (lane == 0) sh.live[warp] = live;
@@ -629,16 +732,27 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Sample a) {
         }
     }
     team.wait();
-    Search search{sh, team, keys, first, last, lane, warp, begin - phase, rank};
+    Search<THREADS> search{sh, team, keys, first, last, lane, warp, begin - phase, rank};
     if (t < warps) {
-        const Shared& other = team.of(sh, t / kWarps);
+        const Shared<THREADS>& other = team.of(sh, t / kWarps);
         sh.every_sum[t] = other.sums[t % kWarps] * power_of(shift - shift_all) + (banned ? other.banned_sums[t % kWarps] : 0.0);
+        if (bounded) sh.every_bound[t] = other.bounds[t % kWarps];
     }
     u64 upto, total = search.total_of([&](int c, int w) { return team.of(sh, c).parts[w]; }, &upto);
+    const auto all_sums = [&] {                       // (of a whole warp)
+        double all = 0.0;
+        for (int w = lane; w < warps; w += 32) all += sh.every_sum[w];
+        return warp_sum(all);
+    };
+    const auto answer = [&](int token, double all) {
+        const float chosen = div(__ldg(part + (token - begin)), temperature, 0);
+        a.tokens[row] = token;
+        a.scores[row] = (float)((double)chosen - log_sum((double)shift_all, all));
+    };
 
     // what stays
     u64 cut = ~0ull;
-    bool cut_by_p = top_p < 1.0f;
+    bool weighed = true;                              // `total`, `weight` and `upto` are of what stays
     int turn = 0;
     if (cut_by_k) {
         // (fewer than k may have a weight: then all of these stay)
@@ -646,12 +760,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Sample a) {
         for (int w = lane; w < warps; w += 32) live += team.of(sh, w / kWarps).live[w % kWarps];
         live = __reduce_add_sync(0xffffffffu, live);
         if (top_k < live) {
-            bool done = false;
             if (bounded) {
                 // of the warps' the one that as many reach as make k
                 const int enough = (int)((top_k + q - 1) / q);
-                if (t < warps) sh.every_bound[t] = team.of(sh, t / kWarps).bounds[t % kWarps];
-                __syncthreads();
                 if (t < warps) {
                     const uint32_t own = sh.every_bound[t];
                     int before = 0;
@@ -659,50 +770,66 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Sample a) {
                     if (before == enough - 1) sh.bound = own;
                 }
                 __syncthreads();
-                if (sh.bound != kOut) done = search.listed(0u, sh.bound, true, (u64)top_k, top_p, 0u, 0ull, &cut);
-            }
-            if (done) {
-                cut_by_p = false;                     // (the list has that cut too)
-            } else {
-                cut = search.find<true>((u64)top_k, kEnd - 1u);
-                if (cut_by_p) {
-                    u64 own, before;
-                    total = search.weigh(cut, turn, &own, &before);
-                    turn ^= 1;
+                if (sh.bound != kOut) {
+                    const bool fits = search.gather(0u, sh.bound, sums.best);
+                    if (fits) {
+                        team.done();
+                        if (rank == 0) {
+                            search.draw((int)top_k, wanted, weight_of(top_key));
+                            if (warp == 0) {
+                                const double all = all_sums();
+                                if (lane == 0) answer((int)sh.cut, all);
+                            }
+                        }
+                        team.all_done();
+                        return;
+                    }
+                    team.wait();
+                    if (rank == 0 && t == 0) sh.listed = 0u;          // (there are waits before the next list)
                 }
+            }
+            cut = search.template find<true>((u64)top_k, kEnd - 1u);
+            search.few = -1;                          // (the weights before those set aside are not known)
+            weighed = false;
+            if (top_p < 1.0f) {
+                total = search.weigh(cut, turn, &weight, &upto);
+                turn ^= 1;
             }
         }
     }
-    if (cut_by_p) {
+    if (top_p < 1.0f) {
         const u64 target = max(share_up(steps(top_p, 0xffffffu), total), 1ull);
         // tokens so light that all of the vocabulary would not make up what is left out: 2^(45 - d) vocab <= total - target
         uint32_t most = kEnd - 1u;
         const u64 each_less = (total - target) / (u64)a.vocab;
         if (each_less > 0) most = min(most, ((uint32_t)max(45 - (63 - __clzll((long long)each_less)), 1) << 23) - 1u);
         if (cut != ~0ull) most = min(most, (uint32_t)(cut >> kNumberBits));
-        cut = search.find<false>(target, most);
+        cut = search.template find<false>(target, most);
+        weighed = false;
     }
-    if (min_p > 0.0f) {
+    if (wanted.min_p > 0u) {
         // the key of the least e with floor(2^44 e) as large as that share
-        const u64 least = share_up(steps(min_p, 1u << 24), weight_of(top_key));
-        cut = min(cut, (u64)(kTop - (uint32_t)f2i(__double2float_ru((double)least * 0x1p-44))) << kNumberBits | ((1u << kNumberBits) - 1u));
+        const u64 least = share_up(wanted.min_p, weight_of(top_key));
+        const u64 by_share = (u64)(kTop - (uint32_t)f2i(__double2float_ru((double)least * 0x1p-44))) << kNumberBits | ((1u << kNumberBits) - 1u);
+        if (by_share < cut) {
+            cut = by_share;
+            weighed = false;
+            search.few = -1;
+        }
     }
-    if (cut != ~0ull) total = search.weigh(cut, turn, &weight, &upto);
+    if (!weighed) total = search.weigh(cut, turn, &weight, &upto);
     team.done();
-    const u64 drawn = share(fraction, total).whole;
+    const u64 drawn = share(wanted.uniform, total).whole;
     if (upto <= drawn && drawn < upto + weight) {
         // this warp has the token
-        double all = 0.0;
-        for (int w = lane; w < warps; w += 32) all += sh.every_sum[w];
-        all = warp_sum(all);
+        const double all = all_sums();
         for (int q = first; q < last; q += 32) {
-            const uint4 k = q + lane < last ? reinterpret_cast<const uint4*>(keys)[q + lane] : make_uint4(kOut, kOut, kOut, kOut);
+            const uint4 k = search.quad(q + lane);
             const uint32_t key[4] = {k.x, k.y, k.z, k.w};
-            const int number = search.begin + (q + lane) * 4;
             u64 w[4], own = 0ull;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const bool in = key[j] != kOut && ((u64)key[j] << kNumberBits | (uint32_t)(number + j)) <= cut;
+                const bool in = key[j] != kOut && search.composite(key[j], (q + lane) * 4 + j) <= cut;
                 w[j] = in ? weight_of(key[j]) : 0ull;
                 own += w[j];
             }
@@ -713,9 +840,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Sample a) {
                     u64 at = run - own;
                     int j = 0;
                     while (j < 3 && at + w[j] <= drawn) at += w[j++];
-                    const float chosen = div(__ldg(part + (number + j - begin)), temperature, 0);
-                    a.tokens[row] = number + j;
-                    a.scores[row] = (float)((double)chosen - log_sum((double)shift_all, all));
+                    answer(search.begin + (q + lane) * 4 + j, all);
                 }
                 break;
             }
@@ -733,10 +858,35 @@ int ctas_of(int64_t rows, int64_t vocab) {
     return c;
 }
 
-// (what the kernel may ask for, whatever a call needs: calls of two threads set the same)
-constexpr size_t kFixed = (sizeof(Shared) + 15) / 16 * 16;
-constexpr size_t kMostMemory = kFixed + (kMostKeys + 4) * 4 + kMostKeys / 4 + 4;
-static_assert(kMostMemory <= 220 * 1024);
+// (what the kernels may ask for, whatever a call needs: calls of two threads set the same)
+template <int THREADS>
+constexpr size_t kFixed = (sizeof(Shared<THREADS>) + 15) / 16 * 16;
+template <int THREADS>
+constexpr size_t kMostMemory = kFixed<THREADS> + (kMostKeys / 512 * THREADS + 4) * 4 + kMostKeys / 512 * THREADS / 4 + 4;
+static_assert(kMostMemory<512> <= 220 * 1024);
+
+template <int THREADS>
+int launch(const Sample& a, int64_t rows, int ctas, cudaStream_t st) {
+    const size_t memory = kFixed<THREADS> + (size_t)(a.part + 4) * 4 + (a.banned ? a.part / 4 + 4 : 0);
+    if (memory > kMostMemory<THREADS>) return PAMK_ERR_SIZE;                          // (no plan comes near)
+    if (memory > 40 * 1024) {
+        const cudaError_t err = cudaFuncSetAttribute(sample_kernel<THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostMemory<THREADS>);
+        if (err != cudaSuccess) return record_cuda_error(err);
+    }
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim = {(unsigned)ctas, 1u, 1u};
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3((unsigned)(rows * ctas));
+    config.blockDim = dim3(THREADS);
+    config.dynamicSmemBytes = memory;
+    config.stream = st;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    const cudaError_t err = cudaLaunchKernelEx(&config, sample_kernel<THREADS>, a);
+    count_launch();
+    return err == cudaSuccess ? PAMK_OK : record_cuda_error(err);
+}
 
 }  // namespace
 }  // namespace pamk
@@ -769,24 +919,7 @@ int pamk_sample(const float* logits, const float* uniform, const unsigned char* 
     a.part = (int)((vocab + ctas - 1) / ctas + 31) / 32 * 32;
     a.tokens = tokens;
     a.scores = scores;
-    const size_t memory = kFixed + (size_t)(a.part + 4) * 4 + (banned ? a.part / 4 + 4 : 0);
-    if (memory > 40 * 1024) {
-        const cudaError_t err = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostMemory);
-        if (err != cudaSuccess) return record_cuda_error(err);
-    }
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim = {(unsigned)ctas, 1u, 1u};
-    cudaLaunchConfig_t config{};
-    config.gridDim = dim3((unsigned)(rows * ctas));
-    config.blockDim = dim3(kThreads);
-    config.dynamicSmemBytes = memory;
-    config.stream = (cudaStream_t)stream;
-    config.attrs = &attr;
-    config.numAttrs = 1;
-    const cudaError_t err = cudaLaunchKernelEx(&config, sample_kernel, a);
-    count_launch();
-    return err == cudaSuccess ? PAMK_OK : record_cuda_error(err);
+    return a.part <= kMostKeys / 2 ? launch<256>(a, rows, ctas, (cudaStream_t)stream) : launch<512>(a, rows, ctas, (cudaStream_t)stream);
 }
 
 }
