@@ -18,9 +18,8 @@
 // tokens, of which a thread has the same four at a time from loading to drawing.  The logits are read once.  What stays is cut off at one token, found as follows:
 //   top-k   each warp's q-th best of its lanes' best tokens, where q of each of w warps are k at least, bounds the k-th best of all; the few tokens as good as the
 //           bound go to a list in the first CTA, which sorts it and draws from it;
-//   top-p   passes over the keys take the weights below some borders each, until few tokens are left between two; these go to the list.  After the first pass
-//           a warp most often has few enough keys in the range to set them aside for the others.
-// (A histogram of 2048 parts of 1/32 of an octave for the latter: its atomics, and its reading by all CTAs of a cluster, made it 640 us for 256 rows of 151643 tokens.)
+//   top-p   each warp sets aside its tokens that are not too light to matter (most often few), whose weights go into a histogram of as many parts as a CTA has
+//           threads; the few tokens of the part that holds the cut go to the list.  (More than a list holds: the part is divided again.)
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -54,13 +53,13 @@ struct Sample {
     float* scores;
 };
 
-constexpr int kMostBorders = 7;
-struct Found { u64 weights[kMostBorders]; uint32_t counts[kMostBorders + 1]; };        // before each border; and in all
-
 template <int THREADS>
 struct Shared {
     static constexpr int kWarps = THREADS / 32, kFew = THREADS / 2;
-    u64 list[THREADS];                                // as many as there are threads
+    union {
+        u64 list[THREADS];                            // as many as there are threads
+        struct { uint32_t count[THREADS], low[THREADS], high[THREADS]; };             // of each part: keys, and the sum of their weights' digits by 12 bits
+    };
     uint32_t few[kWarps][kFew];                       // a warp's keys in the range of a search, and their slots
     uint16_t few_slots[kWarps][kFew];
     // what the other CTAs of the cluster read
@@ -69,7 +68,6 @@ struct Shared {
     double sums[kWarps], banned_sums[kWarps];
     u64 parts[kWarps], staying[2][kWarps];            // weights of the warps: of all, of what stays
     uint32_t live[kWarps], bounds[kWarps], ties[kWarps];
-    Found found[2];
     uint32_t listed;
     u64 cut, kept;
     // within the CTA
@@ -77,8 +75,10 @@ struct Shared {
     u64 every[kWarps * kMostCtas];                    // all warps' of the cluster
     double every_sum[kWarps * kMostCtas];
     uint32_t every_bound[kWarps * kMostCtas], bound;
-    Found warps[kWarps];
     u64 scan[kWarps];
+    uint32_t scan_count[kWarps];
+    uint32_t part, part_count, less_count;            // what a histogram gave
+    u64 less_weight;
 };
 
 // Where the threads of a cluster wait for one another.
@@ -106,6 +106,12 @@ __device__ __forceinline__ double value_of(uint32_t key) { return widened(kTop -
 __device__ __forceinline__ u64 weight_of(uint32_t key) {
     const uint32_t d = key >> 23, m = 0x800000u | (~key & 0x7fffffu);
     return d <= 21u ? (u64)m << (21u - d) : (u64)(m >> min(d - 21u, 31u));
+}
+
+// The digits of a key's weight without its shift, which is the same for all keys of an octave.
+__device__ __forceinline__ uint32_t digits(uint32_t key) {
+    const uint32_t d = key >> 23, m = 0x800000u | (~key & 0x7fffffu);
+    return d <= 21u ? m : m >> (d - 21u);
 }
 
 // Sums of weights.
@@ -215,7 +221,6 @@ struct Search {
     int first, last, lane, warp;                      // the warp's quads; the lane's are every 32nd
     int begin, rank;                                  // the number of slot 0 (it may be before the part); the CTA's rank
     int few = -1;                                     // how many of its keys the warp has set aside
-    u64 own_less = 0ull;                              // the warp's weights before them
 
     __device__ __forceinline__ uint4 quad(int q) const { return q < last ? reinterpret_cast<const uint4*>(keys)[q] : make_uint4(kOut, kOut, kOut, kOut); }
 
@@ -253,9 +258,7 @@ struct Search {
     // The weight of all tokens up to `cut`; `own` is this warp's and `before` that of the warps before.  `turn` alternates from call to call.
     __device__ u64 weigh(u64 cut, int turn, u64* own, u64* before) {
         Units stay;
-        u64 less = 0ull;
-        if (few >= 0) {                               // (the search's cut: what is before its last range is known)
-            less = own_less;
+        if (few >= 0) {                               // (all up to a cut by weight)
             each_aside([&](uint32_t key, int slot) {
                 if (composite(key, slot) <= cut) stay.add(value_of(key));
             });
@@ -266,99 +269,109 @@ struct Search {
                 if (key < cut_key || (key == cut_key && slot <= cut_slot)) stay.add(value_of(key));
             });
         }
-        *own = less + warp_sum(stay.get());
+        *own = warp_sum(stay.get());
         if (lane == 0) sh.staying[turn][warp] = *own;
         team.wait();
         return total_of([&](int c, int w) { return team.of(sh, c).staying[turn][w]; }, before);
     }
 
-    // What lies in [low, low + border_j) for some borders, and how many keys in [low, low + all): of the warp, then (in *joint) of the cluster.  A warp that
-    // has few of these sets them aside for the calls to come, whose ranges lie within.
-    template <bool WEIGHTS, int BORDERS>
-    __device__ Found below(uint32_t low, const uint32_t (&border)[BORDERS], uint32_t all, int turn, Found* joint) {
-        Units units[BORDERS];
-        uint32_t counts[BORDERS + 1];
+    // Sets aside the warp's keys up to `most`, if they are few.
+    __device__ void set_aside(uint32_t most) {
+        int found = 0;
+        for (int q = first + lane; q - lane < last; q += 32) {
+            const uint4 k = quad(q);
+            const uint32_t key[4] = {k.x, k.y, k.z, k.w};
 #pragma unroll
-        for (int j = 0; j <= BORDERS; ++j) counts[j] = 0u;
-        const auto look = [&](uint32_t key) {
-            const uint32_t at = key - low;
-            const double e = WEIGHTS ? value_of(key) : 0.0;
-#pragma unroll
-            for (int j = 0; j < BORDERS; ++j) {
-                const bool in = at < border[j];
-                if (WEIGHTS) units[j].sum = in ? __dadd_rd(units[j].sum, e) : units[j].sum;
-                counts[j] += in;
-            }
-            counts[BORDERS] += at < all;
-            return at < all;
-        };
-        if (few >= 0) {
-            each_aside([&](uint32_t key, int) { look(key); });
-        } else {
-            int found = 0;
-            each([&](uint32_t key, int slot) {
-                const bool in = look(key);
-                const uint32_t those = __ballot_sync(0xffffffffu, in);
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t those = __ballot_sync(0xffffffffu, key[j] <= most);
                 const int place = found + __popc(those & ((1u << lane) - 1u));
-                if (in && place < Sh::kFew) {
-                    sh.few[warp][place] = key;
-                    sh.few_slots[warp][place] = (uint16_t)slot;
+                if (key[j] <= most && place < Sh::kFew) {
+                    sh.few[warp][place] = key[j];
+                    sh.few_slots[warp][place] = (uint16_t)(q * 4 + j);
                 }
                 found += __popc(those);
-            });
-            if (found <= Sh::kFew) few = found;
-            __syncwarp();
+            }
         }
-        Found own{};
-#pragma unroll
-        for (int j = 0; j < BORDERS; ++j) own.weights[j] = WEIGHTS ? warp_sum(units[j].get()) : 0ull;
-#pragma unroll
-        for (int j = 0; j <= BORDERS; ++j) own.counts[j] = __reduce_add_sync(0xffffffffu, counts[j]);
-        if (lane == 0) sh.warps[warp] = own;
+        few = found <= Sh::kFew ? found : -1;
+        __syncwarp();
+    }
+
+    // The keys in [low, low + THREADS 2^shift) in THREADS parts: sh.part is the one in which `target` is reached (by count, or by weight), sh.part_count has that many
+    // keys, and sh.less_* lies before it.  Parts are within an octave.
+    __device__ void divide(uint32_t low, int shift, bool by_count, u64 target, uint32_t less_count, u64 less_weight) {
+        const int t = threadIdx.x;
+        sh.count[t] = sh.low[t] = sh.high[t] = 0u;
         __syncthreads();
-        const auto joined = [&](int n, auto&& of) {                   // (n <= 32; the same in all lanes)
-            Found g{}, here{};
-            if (lane < n) here = of(lane);
-#pragma unroll
-            for (int j = 0; j < BORDERS; ++j) g.weights[j] = WEIGHTS ? warp_sum(here.weights[j]) : 0ull;
-#pragma unroll
-            for (int j = 0; j <= BORDERS; ++j) g.counts[j] = __reduce_add_sync(0xffffffffu, here.counts[j]);
-            return g;
+        const auto look = [&](uint32_t key, int) {
+            const uint32_t part = (key - low) >> shift;
+            if (part >= (uint32_t)THREADS) return;
+            atomicAdd(&sh.count[part], 1u);
+            if (!by_count) {
+                const uint32_t m = digits(key);
+                atomicAdd(&sh.low[part], m & 0xfffu);
+                atomicAdd(&sh.high[part], m >> 12);
+            }
         };
-        *joint = joined(kWarps, [&](int w) { return sh.warps[w]; });
-        if (team.ctas > 1) {
-            if (threadIdx.x == 0) sh.found[turn] = *joint;
-            team.wait();
-            *joint = joined(team.ctas, [&](int c) { return team.of(sh, c).found[turn]; });
-        } else {
-            __syncthreads();                          // (the warps' are written anew)
+        few >= 0 ? each_aside(look) : each(look);
+        team.wait();
+        uint32_t count = 0u;
+        u64 weight = 0ull;
+#pragma unroll
+        for (int c = 0; c < kMostCtas; ++c) {
+            if (c >= team.ctas) break;
+            const Sh& other = team.of(sh, c);
+            count += other.count[t];
+            if (!by_count) weight += (u64)other.low[t] + ((u64)other.high[t] << 12);
         }
-        return own;
+        const uint32_t d = (low + ((uint32_t)t << shift)) >> 23;
+        if (d <= 21u) weight <<= 21u - d;
+        const u64 weight_upto = by_count ? 0ull : warp_upto(weight);
+        uint32_t count_upto = count;
+#pragma unroll
+        for (int apart = 1; apart < 32; apart <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, count_upto, apart);
+            if (lane >= apart) count_upto += v;
+        }
+        if (lane == 31) {
+            sh.scan[warp] = weight_upto;
+            sh.scan_count[warp] = count_upto;
+        }
+        __syncthreads();
+        u64 before = less_weight + weight_upto - weight;
+        uint32_t count_before = less_count + count_upto - count;
+        for (int w = 0; w < warp; ++w) {
+            before += sh.scan[w];
+            count_before += sh.scan_count[w];
+        }
+        const u64 from = by_count ? count_before : before, to = from + (by_count ? count : weight);
+        if (from < target && target <= to) {
+            sh.part = t;
+            sh.part_count = count;
+            sh.less_count = count_before;
+            sh.less_weight = before;
+        }
+        team.wait();                                  // (the histogram may be written anew)
     }
 
     // The tokens with keys from `low` to `high` to the first CTA's list; false where there are too many.  sh.listed is 0 before.  (best: no key of the lane is smaller.)
     __device__ bool gather(uint32_t low, uint32_t high, uint32_t best) {
         Sh& head = team.of(sh, 0);
-        const auto put = [&](uint32_t key, int slot) {
-            const bool in = key - low <= high - low;
-            const uint32_t those = __ballot_sync(0xffffffffu, in);
-            if (those == 0u) return;
+        const bool aside = few >= 0;
+        if (aside || __any_sync(0xffffffffu, best <= high)) {
+            int mine = 0;
+            const auto count = [&](uint32_t key, int) { mine += key - low <= high - low; };
+            aside ? each_aside(count) : each(count);
+            const int found = (int)__reduce_add_sync(0xffffffffu, (uint32_t)mine);
             uint32_t at = 0u;
-            if (lane == 0) at = atomicAdd(&head.listed, (uint32_t)__popc(those));
-            at = __shfl_sync(0xffffffffu, at, 0) + __popc(those & ((1u << lane) - 1u));
-            if (in && at < kListed) head.list[at] = composite(key, slot);
-        };
-        if (few >= 0) {
-            each_aside(put);
-        } else if (__any_sync(0xffffffffu, best <= high)) {
-            for (int q = first + lane; q - lane < last; q += 32) {
-                const uint4 k = quad(q);
-                if (!__any_sync(0xffffffffu, min(min(k.x - low, k.y - low), min(k.z - low, k.w - low)) <= high - low)) continue;
-                put(k.x, q * 4);
-                put(k.y, q * 4 + 1);
-                put(k.z, q * 4 + 2);
-                put(k.w, q * 4 + 3);
-            }
+            if (found > 0 && lane == 0) at = atomicAdd(&head.listed, (uint32_t)found);
+            at = __shfl_sync(0xffffffffu, at, 0);
+            const auto put = [&](uint32_t key, int slot) {
+                const bool in = key - low <= high - low;
+                const uint32_t those = __ballot_sync(0xffffffffu, in), place = at + __popc(those & ((1u << lane) - 1u));
+                if (in && place < kListed) head.list[place] = composite(key, slot);
+                at += __popc(those);
+            };
+            if (found > 0) aside ? each_aside(put) : each(put);
         }
         team.wait();
         return head.listed <= kListed;
@@ -465,66 +478,29 @@ struct Search {
         return cut;
     }
 
-    // One step of a search: [low, high] becomes the last of the parts between borders with less than the target before it.  How many keys it has.
-    template <bool BY_COUNT, int BORDERS>
-    __device__ uint32_t narrow(const uint32_t (&border)[BORDERS], u64 target, uint32_t& low, uint32_t& high, uint32_t& less_count, u64& less_weight, int turn) {
-        const uint32_t span = high - low;             // (below 2^29)
-        Found f;
-        const Found own = below<!BY_COUNT>(low, border, span + 1, turn, &f);
-        uint32_t start = 0u, end = span + 1, before = 0u, upto = f.counts[BORDERS];
-        u64 weight_before = 0ull, own_before = 0ull;
-        bool on = true;
-#pragma unroll
-        for (int j = 0; j < BORDERS; ++j) {
-            on = on && (BY_COUNT ? less_count + f.counts[j] : less_weight + f.weights[j]) < target;
-            if (on) {
-                start = border[j];
-                before = f.counts[j];
-                weight_before = f.weights[j];
-                own_before = own.weights[j];
-            }
-        }
-#pragma unroll
-        for (int j = BORDERS - 1; j >= 0; --j)
-            if ((BY_COUNT ? less_count + f.counts[j] : less_weight + f.weights[j]) >= target) {
-                end = border[j];
-                upto = f.counts[j];
-            }
-        high = low + end - 1;
-        low += start;
-        less_count += before;
-        less_weight += weight_before;
-        if (few < 0) own_less += own_before;          // (what was set aside counts for itself)
-        return upto - before;
-    }
-
-    // The cut, which is among the keys up to `high`.
-    template <bool BY_COUNT>
-    __device__ u64 find(u64 target, uint32_t high) {
+    // The cut, which is among the keys up to `most`.
+    __device__ u64 find(bool by_count, u64 target, uint32_t most) {
+        constexpr int kBits = THREADS == 512 ? 9 : 8;
+        static_assert(1 << kBits == THREADS);
+        int shift = 0;
+        while (most >> shift >= (uint32_t)THREADS) ++shift;           // (at most 21: parts of a quarter of an octave)
+        few = -1;
+        if (!by_count) set_aside(most);
         uint32_t low = 0u, less_count = 0u;
         u64 less_weight = 0ull;
-        few = -1;
-        own_less = 0ull;
-        for (int turn = 0, step = 0;; turn ^= 1, ++step) {
-            const uint32_t span = high - low;
-            uint32_t left;
-            if (step == 0) {
-                // (by weight, what is left out weighs as much as the whole vocabulary at `high`: most often its heaviest are a few octaves above)
-                const bool guess = !BY_COUNT && span > 8u << 23;
-                const uint32_t border[3] = {guess ? span - (5u << 23) : (span + 1) / 4, guess ? span - (7u << 22) : (span + 1) / 2,
-                                            guess ? span - (2u << 23) : (uint32_t)((u64)(span + 1) * 3 / 4)};
-                left = narrow<BY_COUNT>(border, target, low, high, less_count, less_weight, turn);
-            } else {
-                uint32_t border[kMostBorders];
-#pragma unroll
-                for (int j = 0; j < kMostBorders; ++j) border[j] = (uint32_t)((u64)(span + 1) * (j + 1) / (kMostBorders + 1));
-                left = narrow<BY_COUNT>(border, target, low, high, less_count, less_weight, turn);
-            }
+        for (;; shift -= kBits) {
+            const int by = max(shift, 0);
+            divide(low, by, by_count, target, less_count, less_weight);
+            low += sh.part << by;
+            less_count = sh.less_count;
+            less_weight = sh.less_weight;
+            const uint32_t left = sh.part_count;
+            __syncthreads();
             u64 cut;
-            if (left <= kListed && listed(low, high, BY_COUNT, target, less_count, less_weight, &cut)) return cut;
-            if (low == high) {
+            if (left <= kListed && listed(low, low + (1u << by) - 1u, by_count, target, less_count, less_weight, &cut)) return cut;
+            if (by == 0) {
                 const u64 each_weight = weight_of(low);
-                return equal_one(low, BY_COUNT ? target - less_count : (target - less_weight + each_weight - 1) / each_weight);
+                return equal_one(low, by_count ? target - less_count : (target - less_weight + each_weight - 1) / each_weight);
             }
         }
     }
@@ -677,12 +653,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
             sh.bad = any_bad;
         }
         team.wait();
-        for (int c = 0; c < team.ctas; ++c) {
-            const Shared<THREADS>& other = team.of(sh, c);
-            top_all = fmaxf(top_all, other.all);
-            top_ok = fmaxf(top_ok, other.ok);
-            no_token |= other.bad;
-        }
+        const Shared<THREADS>& other = team.of(sh, lane < team.ctas ? lane : 0);
+        top_all = warp_max(other.all);
+        top_ok = warp_max(other.ok);
+        no_token = __any_sync(0xffffffffu, other.bad);
     }
     if (no_token || !(top_ok > -INFINITY)) {                                          // (all CTAs of the cluster alike)
         if (rank == 0 && t == 0) {
@@ -788,8 +762,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
                     if (rank == 0 && t == 0) sh.listed = 0u;          // (there are waits before the next list)
                 }
             }
-            cut = search.template find<true>((u64)top_k, kEnd - 1u);
-            search.few = -1;                          // (the weights before those set aside are not known)
+            cut = search.find(true, (u64)top_k, kEnd - 1u);
             weighed = false;
             if (top_p < 1.0f) {
                 total = search.weigh(cut, turn, &weight, &upto);
@@ -804,7 +777,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
         const u64 each_less = (total - target) / (u64)a.vocab;
         if (each_less > 0) most = min(most, ((uint32_t)max(45 - (63 - __clzll((long long)each_less)), 1) << 23) - 1u);
         if (cut != ~0ull) most = min(most, (uint32_t)(cut >> kNumberBits));
-        cut = search.template find<false>(target, most);
+        cut = search.find(false, target, most);
         weighed = false;
     }
     if (wanted.min_p > 0u) {
@@ -814,7 +787,6 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
         if (by_share < cut) {
             cut = by_share;
             weighed = false;
-            search.few = -1;
         }
     }
     if (!weighed) total = search.weigh(cut, turn, &weight, &upto);
