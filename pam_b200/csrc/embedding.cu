@@ -66,25 +66,56 @@ __global__ void __launch_bounds__(kThreads) embed_kernel(const Embedding a, cons
     }
 }
 
-// Rows of whole quads at aligned addresses, fewer than 2^31 quads.
+// n / d for n < 2^31 (Granlund and Montgomery, "Division by invariant integers using multiplication", 1994): with 2^s the power of two next to d from above,
+// floor(n (2^32 + m) / 2^(32 + s)) for m = floor(2^32 (2^s - d) / d) + 1.
+struct Divide {
+    uint32_t d, m, s;
+    explicit Divide(uint32_t by) : d(by), s(0) {
+        while (((uint64_t)1 << s) < by) ++s;
+        m = (uint32_t)(((((uint64_t)1 << s) - by) << 32) / by + 1);
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (__umulhi(n, m) + n) >> s; }
+};
+
+// Rows of whole quads at aligned addresses, fewer than 2^31 quads.  A thread has a few, as far apart as a CTA is wide, with all of its loads on their way before the
+// first product; HBM-bound where the table is small, by the 4 bytes per element that are written.
+constexpr int kQuads = 4;
 template <bool SLOPES>
-__global__ void __launch_bounds__(kThreads) embed_quads_kernel(const Embedding a, const float* g, float* out, uint32_t quads, uint32_t row_quads) {
-    const uint32_t q = blockIdx.x * kThreads + threadIdx.x;
-    if (q >= quads) return;
-    const uint32_t i = q / row_quads, c = (q - i * row_quads) * 4;
-    const int64_t token = token_at(a.tokens, i);
-    const bool known = (uint64_t)token < (uint64_t)a.vocab;
-    float4 x = make_float4(quiet_nan(), quiet_nan(), quiet_nan(), quiet_nan()), p = make_float4(0.0f, 0.0f, 0.0f, 0.0f), d = p;
-    if (known) x = __ldg(reinterpret_cast<const float4*>(a.table + token * a.table_row + c));
-    if (a.pos) p = __ldg(reinterpret_cast<const float4*>(a.pos + (int64_t)(a.pos_count == 1 ? 0u : i % (uint32_t)a.pos_count) * a.pos_row + c));
-    if (SLOPES) d = __ldg(reinterpret_cast<const float4*>(g) + q);
-    const uint4 w = a.drops ? philox(q, key_of(a.drop)) : make_uint4(0u, 0u, 0u, 0u);
-    const auto one = [&](float v, float at, uint32_t bits, float dv) {
-        if (a.scaled) v = mul(v, a.scale, a.off);
-        if (a.pos) v = fadd(v, at);
-        return finished<SLOPES>(a, v, bits, dv);
-    };
-    reinterpret_cast<float4*>(out)[q] = make_float4(one(x.x, p.x, w.x, d.x), one(x.y, p.y, w.y, d.y), one(x.z, p.z, w.z, d.z), one(x.w, p.w, w.w, d.w));
+__global__ void __launch_bounds__(kThreads) embed_quads_kernel(const Embedding a, const float* g, float* out, uint32_t quads, Divide by_row, Divide by_pos) {
+    const uint32_t first = blockIdx.x * (kThreads * kQuads) + threadIdx.x;
+    const uint2 key = a.drops ? key_of(a.drop) : make_uint2(0u, 0u);
+    uint32_t row[kQuads];
+    int64_t token[kQuads];
+    float4 x[kQuads], p[kQuads], d[kQuads];
+#pragma unroll
+    for (int k = 0; k < kQuads; ++k) {
+        const uint32_t q = first + k * kThreads;
+        row[k] = by_row(q);
+        token[k] = q < quads ? token_at(a.tokens, row[k]) : -1;
+    }
+#pragma unroll
+    for (int k = 0; k < kQuads; ++k) {
+        const uint32_t q = first + k * kThreads, c = (q - row[k] * by_row.d) * 4;
+        x[k] = make_float4(quiet_nan(), quiet_nan(), quiet_nan(), quiet_nan());
+        p[k] = d[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if ((uint64_t)token[k] < (uint64_t)a.vocab) x[k] = __ldg(reinterpret_cast<const float4*>(a.table + token[k] * a.table_row + c));
+        if (q >= quads) continue;
+        if (a.pos) p[k] = __ldg(reinterpret_cast<const float4*>(a.pos + (int64_t)(row[k] - by_pos(row[k]) * by_pos.d) * a.pos_row + c));
+        if (SLOPES) d[k] = __ldg(reinterpret_cast<const float4*>(g) + q);
+    }
+#pragma unroll
+    for (int k = 0; k < kQuads; ++k) {
+        const uint32_t q = first + k * kThreads;
+        if (q >= quads) return;
+        const uint4 w = a.drops ? philox(q, key) : make_uint4(0u, 0u, 0u, 0u);
+        const auto one = [&](float v, float at, uint32_t bits, float dv) {
+            if (a.scaled) v = mul(v, a.scale, a.off);
+            if (a.pos) v = fadd(v, at);
+            return finished<SLOPES>(a, v, bits, dv);
+        };
+        reinterpret_cast<float4*>(out)[q] =
+            make_float4(one(x[k].x, p[k].x, w.x, d[k].x), one(x[k].y, p[k].y, w.y, d[k].y), one(x[k].z, p[k].z, w.z, d[k].z), one(x[k].w, p[k].w, w.w, d[k].w));
+    }
 }
 
 // ---- the order of the tokens ------------------------------------------------------------------------------------
@@ -636,8 +667,9 @@ int pamk_embedding(const int64_t* tokens, const float* table, const float* posit
     const int64_t n = count * dim;
     const auto st = (cudaStream_t)stream;
     if (dim % 4 == 0 && n < ((int64_t)1 << 33) && aligned16(table) && table_row % 4 == 0 && aligned16(positions) && positions_row % 4 == 0 && aligned16(dy) && aligned16(out)) {
-        const uint32_t quads = (uint32_t)(n / 4), ctas = (quads + kThreads - 1) / kThreads;
-        (dy ? embed_quads_kernel<true> : embed_quads_kernel<false>)<<<ctas, kThreads, 0, st>>>(a, dy, out, quads, (uint32_t)(dim / 4));
+        const uint32_t quads = (uint32_t)(n / 4), ctas = (quads + kThreads * kQuads - 1) / (kThreads * kQuads);
+        (dy ? embed_quads_kernel<true> : embed_quads_kernel<false>)<<<ctas, kThreads, 0, st>>>(a, dy, out, quads, Divide((uint32_t)(dim / 4)),
+                                                                                              Divide(positions ? (uint32_t)positions_count : 1u));
         return check_launch();
     }
     const int64_t ctas = (n + 4 * kThreads - 1) / (4 * kThreads);
