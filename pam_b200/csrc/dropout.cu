@@ -7,6 +7,7 @@
 #include "common.cuh"
 #include "pam_scalar.cuh"
 #include "philox.cuh"
+#include "times.cuh"
 
 namespace pamk {
 namespace {
@@ -38,7 +39,7 @@ __device__ __forceinline__ void store_quad(float* p, int64_t i, int64_t n, float
 
 // SLOPES: x is the gradient and `other` the forward pass's input; else `other` is the residual, or null.
 template <bool SLOPES, bool VEC>
-__global__ void __launch_bounds__(kThreads) dropout_kernel(const float* x, const float* other, float* out, int64_t n, Dropping drop, int32_t off) {
+__global__ void __launch_bounds__(kThreads) dropout_kernel(const float* x, const float* other, float* out, int64_t n, Dropping drop, Times by) {
     const uint2 key = key_of(drop);
     const int64_t first = ((int64_t)blockIdx.x * kQuads * kThreads + threadIdx.x) * 4;
     float4 v[kQuads], o[kQuads];
@@ -53,11 +54,12 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const float* x, const
         const int64_t i = first + k * kThreads * 4;
         if (i >= n) return;
         const uint4 w = philox((uint64_t)i >> 2, key);
-        const auto one = [&](float a, float b, uint32_t bits) {
-            const float y = bits < drop.below ? 0.0f : SLOPES ? mul_bwd(b, drop.scale, a, off) : mul(a, drop.scale, off);
-            return SLOPES || !other ? y : fadd(y, b);
-        };
-        store_quad<VEC>(out, i, n, make_float4(one(v[k].x, o[k].x, w.x), one(v[k].y, o[k].y, w.y), one(v[k].z, o[k].z, w.z), one(v[k].w, o[k].w, w.w)));
+        float4 y = SLOPES ? make_float4(mul_bwd(o[k].x, by.s, v[k].x, by.off), mul_bwd(o[k].y, by.s, v[k].y, by.off), mul_bwd(o[k].z, by.s, v[k].z, by.off),
+                                        mul_bwd(o[k].w, by.s, v[k].w, by.off))
+                          : by.of(v[k]);
+        y = make_float4(w.x < drop.below ? 0.0f : y.x, w.y < drop.below ? 0.0f : y.y, w.z < drop.below ? 0.0f : y.z, w.w < drop.below ? 0.0f : y.w);
+        if (!SLOPES && other) y = make_float4(fadd(y.x, o[k].x), fadd(y.y, o[k].y), fadd(y.z, o[k].z), fadd(y.w, o[k].w));
+        store_quad<VEC>(out, i, n, y);
     }
 }
 
@@ -68,7 +70,7 @@ int launch(const float* x, const float* other, float* out, int64_t n, double p, 
     const Dropping drop = dropping(p, seed_at, seed);
     const bool vec = aligned16(x) && aligned16(out) && aligned16(other);
     const auto kernel = vec ? dropout_kernel<SLOPES, true> : dropout_kernel<SLOPES, false>;
-    kernel<<<(unsigned)ctas, kThreads, 0, st>>>(x, other, out, n, drop, offset_bits(offset));
+    kernel<<<(unsigned)ctas, kThreads, 0, st>>>(x, other, out, n, drop, Times(drop.scale, offset_bits(offset)));
     return check_launch();
 }
 

@@ -5,13 +5,15 @@
 // A token outside the table reads nothing: its row is NaN, and it has no gradient.
 //
 // The gradient is a sort and a segmented sum, so that every row of g is read once, wherever its token occurs, and no atomics decide on an order:
-//   sort   the places of the tokens in the order (token, place), by two digits of at most 11 bits, each pass stable.  Up to 8192 tokens one CTA sorts in shared
-//          memory; more are cut into tiles, whose counts place them.  The other CTAs of these launches fill the gradient with zeros meanwhile.
+//   sort   the places of the tokens in the order (token, place).  Up to 8192 tokens each counts those before it, which all SMs share (4096 tokens: 17 million comparisons);
+//          more are cut into tiles and moved by two digits of at most 11 bits, each pass stable.  The other CTAs of these launches fill the gradient with zeros
+//          meanwhile.  (One CTA that moves up to 8192 tokens by digits in its shared memory: 14 us for 4096.)
 //   sums   a warp adds the rows of 16 neighbours in that order (32 where there are many), 128 columns of them, and writes the tokens that lie within;
-//   joins  a token with neighbours in several such chunks has its parts added in their order by a CTA for each 128 columns.
+//   joins  a token with neighbours in several such chunks has its parts added in their order, by a warp for each 128 columns, or by a CTA where they are many.
 #include "common.cuh"
 #include "pam_scalar.cuh"
 #include "philox.cuh"
+#include "times.cuh"
 
 namespace pamk {
 namespace {
@@ -24,8 +26,7 @@ struct Embedding {
     int64_t count, table_row, pos_row, pos_count, vocab, padding;
     int dim;
     bool scaled, drops;
-    float scale;
-    int32_t off;
+    Times scale, keep;                    // pam(x, scale); pam(x, s)
     Dropping drop;
 };
 
@@ -35,7 +36,7 @@ __device__ __forceinline__ float looked_up(const Embedding& a, int64_t i, int c)
     const int64_t token = token_at(a.tokens, i);
     if ((uint64_t)token >= (uint64_t)a.vocab) return quiet_nan();
     float x = __ldg(a.table + token * a.table_row + c);
-    if (a.scaled) x = mul(x, a.scale, a.off);
+    if (a.scaled) x = a.scale.one(x);
     return a.pos ? fadd(x, __ldg(a.pos + (a.pos_count == 1 ? 0 : i % a.pos_count) * a.pos_row + c)) : x;
 }
 
@@ -43,7 +44,7 @@ __device__ __forceinline__ float looked_up(const Embedding& a, int64_t i, int c)
 template <bool SLOPES>
 __device__ __forceinline__ float finished(const Embedding& a, float x, uint32_t bits, float g) {
     if (!a.drops) return x;
-    return bits < a.drop.below ? 0.0f : SLOPES ? mul_bwd(x, a.drop.scale, g, a.off) : mul(x, a.drop.scale, a.off);
+    return bits < a.drop.below ? 0.0f : SLOPES ? mul_bwd(x, a.keep.s, g, a.keep.off) : a.keep.one(x);
 }
 
 // A thread takes four neighbouring elements of the output, which is what a block of the counter has bits for; here of any row length.
@@ -107,20 +108,22 @@ __global__ void __launch_bounds__(kThreads) embed_quads_kernel(const Embedding a
     for (int k = 0; k < kQuads; ++k) {
         const uint32_t q = first + k * kThreads;
         if (q >= quads) return;
-        const uint4 w = a.drops ? philox(q, key) : make_uint4(0u, 0u, 0u, 0u);
-        const auto one = [&](float v, float at, uint32_t bits, float dv) {
-            if (a.scaled) v = mul(v, a.scale, a.off);
-            if (a.pos) v = fadd(v, at);
-            return finished<SLOPES>(a, v, bits, dv);
-        };
-        reinterpret_cast<float4*>(out)[q] =
-            make_float4(one(x[k].x, p[k].x, w.x, d[k].x), one(x[k].y, p[k].y, w.y, d[k].y), one(x[k].z, p[k].z, w.z, d[k].z), one(x[k].w, p[k].w, w.w, d[k].w));
+        float4 y = a.scaled ? a.scale.of(x[k]) : x[k];
+        if (a.pos) y = make_float4(fadd(y.x, p[k].x), fadd(y.y, p[k].y), fadd(y.z, p[k].z), fadd(y.w, p[k].w));
+        if (a.drops) {
+            const uint4 w = philox(q, key);
+            y = SLOPES ? make_float4(mul_bwd(y.x, a.keep.s, d[k].x, a.keep.off), mul_bwd(y.y, a.keep.s, d[k].y, a.keep.off), mul_bwd(y.z, a.keep.s, d[k].z, a.keep.off),
+                                     mul_bwd(y.w, a.keep.s, d[k].w, a.keep.off))
+                       : a.keep.of(y);
+            y = make_float4(w.x < a.drop.below ? 0.0f : y.x, w.y < a.drop.below ? 0.0f : y.y, w.z < a.drop.below ? 0.0f : y.z, w.w < a.drop.below ? 0.0f : y.w);
+        }
+        reinterpret_cast<float4*>(out)[q] = y;
     }
 }
 
 // ---- the order of the tokens ------------------------------------------------------------------------------------
 
-constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kMostInOne = 8192;
+constexpr int kMostCounted = 8192, kRanked = 32;          // tokens that count each other; of a CTA, one of a lane
 constexpr int kTileThreads = 512, kTileWarps = kTileThreads / 32, kRounds = 8, kTile = kTileThreads * kRounds;
 constexpr int kMostTiles = 512;           // each reads the counts of all
 constexpr uint32_t kNone = 0xffffffffu;
@@ -134,7 +137,7 @@ struct Sort {
     int tiles, tile;                      // of `tile` tokens, a multiple of kTile
     uint32_t *counts_low, *counts_high;   // [tiles][1 << bits]
     Entry *by_low, *sorted;
-    uint32_t* totals;                     // [0]: tokens that have a gradient; [1]: those in several chunks
+    uint32_t* totals;                     // [0]: tokens that have a gradient; [1], [2]: those in several chunks, in many
     float* zeros;                         // the gradient
     int64_t zero_count;
     int fillers;                          // CTAs that fill
@@ -218,50 +221,54 @@ __device__ void sums_over_warps(uint16_t* counts, uint32_t* totals, int bins, in
     }
 }
 
-// Up to 8192 tokens in one CTA: a warp has neighbouring tokens in both passes, which keeps them stable.
-__global__ void __launch_bounds__(kSortThreads) sort_kernel(const Sort a) {
-    extern __shared__ __align__(16) unsigned char memory[];
-    __shared__ uint32_t warp_sums[kSortWarps];
-    if (blockIdx.x > 0) {
-        fill(a, 1, 0, 1);
+// A lane has a token and each warp of the CTA a part of the others: those before it in the order are its place there.
+__global__ void __launch_bounds__(kThreads) rank_kernel(const Sort a, int rankers) {
+    __shared__ __align__(16) uint32_t tokens[kMostCounted];
+    __shared__ uint32_t before[kThreads / 32][kRanked];
+    __shared__ uint32_t live[kThreads / 32];
+    if ((int)blockIdx.x >= rankers) {
+        fill(a, rankers, 0, 1);
         next_may_start();
         return;
     }
-    Entry* entries = reinterpret_cast<Entry*>(memory);
-    const int most = 1 << max(a.low_bits, a.high_bits);
-    uint32_t* totals = reinterpret_cast<uint32_t*>(entries + (a.count + 31) / 32 * 32);
-    uint16_t* counts = reinterpret_cast<uint16_t*>(totals + most);
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, rounds = (int)((a.count + kSortThreads - 1) / kSortThreads);
-    uint32_t token[kRounds], place[kRounds], digit[kRounds], rank[kRounds];
-    int live = (int)a.count;
-    for (int pass = 0; pass < 2; ++pass) {
-        const int bins = 1 << (pass ? a.high_bits : a.low_bits);
-        for (int i = t; i < bins * kSortWarps / 2; i += kSortThreads) reinterpret_cast<uint32_t*>(counts)[i] = 0u;
-#pragma unroll
-        for (int r = 0; r < kRounds; ++r) {
-            token[r] = digit[r] = kNone;
-            const int i = (warp * rounds + r) * 32 + lane;
-            if (r >= rounds || i >= live) continue;
-            token[r] = pass ? entries[i].token : token_of(a, i);
-            place[r] = pass ? entries[i].place : (uint32_t)i;
-            if (token[r] != kNone) digit[r] = pass ? token[r] >> a.low_bits : token[r] & (bins - 1);
-        }
-        __syncthreads();
-        rank_in_warp<kRounds>(counts + warp * bins, digit, rank, rounds);
-        __syncthreads();
-        sums_over_warps(counts, totals, bins, kSortWarps);
-        live = (int)sums_before(totals, bins, warp_sums);
-#pragma unroll
-        for (int r = 0; r < kRounds; ++r) {
-            if (digit[r] == kNone) continue;
-            const uint32_t to = totals[digit[r]] + counts[warp * bins + digit[r]] + rank[r];
-            (pass ? a.sorted : entries)[to] = {token[r], place[r]};
-        }
-        __syncthreads();
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, count = (int)a.count, padded = (count + 3) / 4 * 4;
+    uint32_t mine = 0u;
+#pragma unroll 8
+    for (int i = t; i < padded; i += kThreads) {
+        tokens[i] = token_of(a, i);
+        mine += tokens[i] != kNone;
     }
-    if (t == 0) {
-        a.totals[0] = (uint32_t)live;
-        a.totals[1] = 0u;
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    if (lane == 0) live[warp] = mine;
+    __syncthreads();
+    const int first = blockIdx.x * kRanked, i = first + lane;
+    const uint32_t own = i < count ? tokens[i] : kNone;
+    // (whole quads before the CTA's tokens, around them, behind them)
+    const int quads = padded / 4, each = (quads + kThreads / 32 - 1) / (kThreads / 32), from = min(warp * each, quads), to = min(from + each, quads);
+    const int around = min(max(first / 4, from), to), behind = min(max((first + kRanked) / 4, from), to);
+    uint32_t less = 0u;
+    const uint4* quad = reinterpret_cast<const uint4*>(tokens);
+#pragma unroll 4
+    for (int q = from; q < around; ++q) {
+        const uint4 v = quad[q];
+        less += (v.x <= own) + (v.y <= own) + (v.z <= own) + (v.w <= own);
+    }
+    for (int j = around * 4; j < behind * 4; ++j) less += tokens[j] < own || (tokens[j] == own && j < i);
+#pragma unroll 4
+    for (int q = behind; q < to; ++q) {
+        const uint4 v = quad[q];
+        less += (v.x < own) + (v.y < own) + (v.z < own) + (v.w < own);
+    }
+    before[warp][lane] = less;
+    __syncthreads();
+    if (t < kRanked && own != kNone) {
+        for (int w = 1; w < kThreads / 32; ++w) less += before[w][lane];
+        a.sorted[less] = {own, (uint32_t)i};
+    }
+    if (blockIdx.x == 0 && t == 0) {
+        for (int w = 1; w < kThreads / 32; ++w) mine += live[w];
+        a.totals[0] = mine;
+        a.totals[1] = a.totals[2] = 0u;
     }
     next_may_start();
 }
@@ -278,7 +285,7 @@ __global__ void __launch_bounds__(kTileThreads) count_kernel(const Sort a) {
     const int bins = 1 << a.low_bits, high = 1 << a.high_bits;
     for (int b = threadIdx.x; b < bins; b += kTileThreads) counts[b] = 0u;
     for (int b = threadIdx.x; b < high; b += kTileThreads) a.counts_high[(int64_t)blockIdx.x * high + b] = 0u;
-    if (blockIdx.x == 0 && threadIdx.x < 2) a.totals[threadIdx.x] = 0u;
+    if (blockIdx.x == 0 && threadIdx.x < 3) a.totals[threadIdx.x] = 0u;
     __syncthreads();
     const int64_t begin = (int64_t)blockIdx.x * a.tile;
     for (int i = threadIdx.x; i < a.tile; i += kTileThreads) {
@@ -368,15 +375,16 @@ struct Sums {
     const Entry* sorted;
     uint32_t* totals;
     float* parts;                         // [chunks][2][dim]: what continues from the chunk before; what the next continues
-    uint32_t* list;                       // chunks in which a token starts that the next continues
+    uint32_t* list;                       // chunks in which a token starts that the next continues, from the back those of the tokens that go on in many
     int64_t table_row;
     int dim, slabs, chunk;
     uint32_t chunks;
     bool scaled, drops;
-    float scale;
-    int32_t off;
+    Times scale, keep;
     Dropping drop;
 };
+
+constexpr uint32_t kMany = 24;            // chunks of a token that a warp adds alone (its loads wait three times; of 8192 tokens there are 512)
 
 __device__ __forceinline__ Entry entry_at(const Entry* sorted, uint32_t i) {
     const uint2 e = __ldcg(reinterpret_cast<const uint2*>(sorted) + i);
@@ -450,27 +458,26 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const Sums a) {
                 if (SLOPES && a.scaled) {
                     load_columns<VEC>(a.table + (int64_t)token * a.table_row, slab, lane, a.dim, slope);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) slope[k] = mul_slope(slope[k], a.scale, a.off);
+                    for (int k = 0; k < 4; ++k) slope[k] = mul_slope(slope[k], a.scale.s, a.scale.off);
                 }
             }
-            uint32_t bits[4] = {0u, 0u, 0u, 0u};
+            float4 x = make_float4(v[j][0], v[j][1], v[j][2], v[j][3]);
             if (a.drops) {
                 const uint64_t e = (uint64_t)place * a.dim;
-                if (VEC) {
-                    const uint4 w = philox((e + column<true>(slab, lane, 0)) >> 2, key);
-                    bits[0] = w.x, bits[1] = w.y, bits[2] = w.z, bits[3] = w.w;
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) bits[k] = philox_word(e + column<false>(slab, lane, k), key);
-                }
+                uint4 w;
+                if (VEC)
+                    w = philox((e + column<true>(slab, lane, 0)) >> 2, key);
+                else
+                    w = make_uint4(philox_word(e + column<false>(slab, lane, 0), key), philox_word(e + column<false>(slab, lane, 1), key),
+                                   philox_word(e + column<false>(slab, lane, 2), key), philox_word(e + column<false>(slab, lane, 3), key));
+                x = a.keep.of(x);
+                x = make_float4(w.x < a.drop.below ? 0.0f : x.x, w.y < a.drop.below ? 0.0f : x.y, w.z < a.drop.below ? 0.0f : x.z, w.w < a.drop.below ? 0.0f : x.w);
             }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                float x = v[j][k];
-                if (a.drops) x = bits[k] < a.drop.below ? 0.0f : mul(x, a.drop.scale, a.off);
-                if (a.scaled) x = SLOPES ? fmul(x, slope[k]) : mul(x, a.scale, a.off);
-                sum[k] = fadd(sum[k], x);
-            }
+            if (a.scaled) x = SLOPES ? make_float4(fmul(x.x, slope[0]), fmul(x.y, slope[1]), fmul(x.z, slope[2]), fmul(x.w, slope[3])) : a.scale.of(x);
+            sum[0] = fadd(sum[0], x.x);
+            sum[1] = fadd(sum[1], x.y);
+            sum[2] = fadd(sum[2], x.z);
+            sum[3] = fadd(sum[3], x.w);
         }
     }
     const bool from_before = now == token_before, goes_on = now == token_after;
@@ -478,49 +485,63 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const Sums a) {
         store_columns<VEC>(a.dw + (int64_t)now * a.dim, slab, lane, a.dim, sum);
     } else {
         store_columns<VEC>(a.parts + ((int64_t)chunk * 2 + !from_before) * a.dim, slab, lane, a.dim, sum);
-        if (!from_before && slab == 0 && lane == 0) a.list[atomicAdd(a.totals + 1, 1u)] = chunk;
+        if (!from_before && slab == 0 && lane == 0) {
+            const uint64_t far = (uint64_t)(chunk + kMany) * a.chunk;
+            if (far < live && entry_at(a.sorted, (uint32_t)far).token == now)
+                a.list[a.chunks - 1 - atomicAdd(a.totals + 2, 1u)] = chunk;
+            else
+                a.list[atomicAdd(a.totals + 1, 1u)] = chunk;
+        }
     }
     next_may_start();
 }
 
-// The parts of a token: the end of the chunk that it starts in, the beginnings of those that it goes on in.  A warp has neighbouring ones of them.
+// A token's parts from..to - 1: the end of the chunk that it starts in, the beginnings of those that it goes on in.
+template <bool VEC>
+__device__ __forceinline__ void add_parts(const Sums& a, uint32_t chunk, uint32_t from, uint32_t to, int slab, int lane, float (&sum)[4]) {
+    constexpr int kAhead = 8;
+    for (uint32_t first = from; first < to; first += kAhead) {
+        float v[kAhead][4];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const uint32_t part = first + j;
+            if (part >= to) continue;
+            const float* row = a.parts + ((int64_t)(chunk + part) * 2 + (part == 0)) * a.dim;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[j][k] = column<VEC>(slab, lane, k) < a.dim ? __ldcg(row + column<VEC>(slab, lane, k)) : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+            if (first + j < to)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) sum[k] = fadd(sum[k], v[j][k]);
+    }
+}
+
+// How many parts the token has that starts in this chunk.
+__device__ __forceinline__ uint32_t parts_of(const Sums& a, uint32_t chunk, uint32_t live, int lane, uint32_t* token) {
+    *token = entry_at(a.sorted, (chunk + 1) * (uint32_t)a.chunk).token;
+    for (uint32_t more = 1;; more += 32) {
+        const uint64_t at = (uint64_t)(chunk + 1 + more + lane) * a.chunk;
+        const uint32_t other = __ballot_sync(0xffffffffu, at >= live || entry_at(a.sorted, (uint32_t)at).token != *token);
+        if (other) return more + __ffs(other);
+    }
+}
+
 template <bool VEC>
 __global__ void __launch_bounds__(kThreads) join_kernel(const Sums a) {
-    constexpr int kWarps = kThreads / 32, kAhead = 8;
+    constexpr int kWarps = kThreads / 32;
     __shared__ float stage[kWarps][kColumns];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, slab = blockIdx.y;
     after_previous();
-    const uint32_t live = __ldcg(a.totals), many = __ldcg(a.totals + 1);
+    const uint32_t live = __ldcg(a.totals), some = __ldcg(a.totals + 1), many = __ldcg(a.totals + 2);
+    uint32_t token;
     for (uint32_t i = blockIdx.x; i < many; i += gridDim.x) {
-        const uint32_t chunk = __ldcg(a.list + i);
-        const uint32_t token = entry_at(a.sorted, (chunk + 1) * (uint32_t)a.chunk).token;
-        uint32_t more = 1;                                                            // chunks that it goes on in
-        for (;; more += 32) {
-            const uint64_t at = (uint64_t)(chunk + 1 + more + lane) * a.chunk;
-            const uint32_t other = __ballot_sync(0xffffffffu, at >= live || entry_at(a.sorted, (uint32_t)at).token != token);
-            if (other) {
-                more += __ffs(other) - 1;
-                break;
-            }
-        }
-        const uint32_t count = more + 1, each = (count + kWarps - 1) / kWarps, from = min(warp * each, count), to = min(from + each, count);
+        // a warp has neighbouring parts
+        const uint32_t chunk = __ldcg(a.list + a.chunks - 1 - i), count = parts_of(a, chunk, live, lane, &token);
+        const uint32_t each = (count + kWarps - 1) / kWarps, from = min(warp * each, count), to = min(from + each, count);
         float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (uint32_t first = from; first < to; first += kAhead) {
-            float v[kAhead][4];
-#pragma unroll
-            for (int j = 0; j < kAhead; ++j) {
-                const uint32_t part = first + j;
-                if (part >= to) continue;
-                const float* row = a.parts + ((int64_t)(chunk + part) * 2 + (part == 0)) * a.dim;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v[j][k] = column<VEC>(slab, lane, k) < a.dim ? __ldcg(row + column<VEC>(slab, lane, k)) : 0.0f;
-            }
-#pragma unroll
-            for (int j = 0; j < kAhead; ++j)
-                if (first + j < to)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) sum[k] = fadd(sum[k], v[j][k]);
-        }
+        add_parts<VEC>(a, chunk, from, to, slab, lane, sum);
 #pragma unroll
         for (int k = 0; k < 4; ++k) stage[warp][VEC ? lane * 4 + k : lane + 32 * k] = sum[k];
         __syncthreads();
@@ -530,6 +551,12 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Sums a) {
             a.dw[(int64_t)token * a.dim + slab * kColumns + threadIdx.x] = s;
         }
         __syncthreads();
+    }
+    for (uint32_t i = blockIdx.x * kWarps + warp; i < some; i += gridDim.x * kWarps) {
+        const uint32_t chunk = __ldcg(a.list + i), count = parts_of(a, chunk, live, lane, &token);
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        add_parts<VEC>(a, chunk, 0u, count, slab, lane, sum);
+        store_columns<VEC>(a.dw + (int64_t)token * a.dim, slab, lane, a.dim, sum);
     }
 }
 
@@ -555,10 +582,12 @@ Embedding described(const int64_t* tokens, const float* table, const float* pos,
     a.padding = padding;
     a.dim = (int)dim;
     a.scaled = scaled != 0;
-    a.scale = scale;
-    a.off = offset_bits(offset);
+    a.scale = Times(scale, offset_bits(offset));
     a.drops = p > 0.0;
-    if (a.drops) a.drop = dropping(p, seed_at, seed);
+    if (a.drops) {
+        a.drop = dropping(p, seed_at, seed);
+        a.keep = Times(a.drop.scale, offset_bits(offset));
+    }
     return a;
 }
 
@@ -575,7 +604,7 @@ Plan planned(int64_t count, int64_t vocab, int64_t dim) {
     while (((int64_t)1 << bits) < vocab) ++bits;
     p.low_bits = (bits + 1) / 2;
     p.high_bits = bits - p.low_bits;
-    if (count > kMostInOne) {
+    if (count > kMostCounted) {
         const int64_t each = (count + kMostTiles - 1) / kMostTiles;
         p.tile = (int)((each + kTile - 1) / kTile * kTile);
         p.tiles = (int)((count + p.tile - 1) / p.tile);
@@ -588,7 +617,7 @@ Plan planned(int64_t count, int64_t vocab, int64_t dim) {
         at += (bytes + 255) / 256 * 256;
         return here;
     };
-    p.totals = take(2 * sizeof(uint32_t));
+    p.totals = take(3 * sizeof(uint32_t));
     p.counts_low = take((size_t)p.tiles << p.low_bits << 2);
     p.counts_high = take((size_t)p.tiles << p.high_bits << 2);
     p.by_low = take(p.tiles ? (size_t)count * sizeof(Entry) : 0);
@@ -601,9 +630,8 @@ Plan planned(int64_t count, int64_t vocab, int64_t dim) {
 
 // (what the kernels may ask for, whatever a call needs: calls of two threads set the same)
 constexpr int kMostBins = 1 << 11;
-constexpr size_t kSortMemory = kMostInOne * sizeof(Entry) + kMostBins * 4 + kMostBins * kSortWarps * 2;
 constexpr size_t kTileMemory = kMostBins * 8 + kMostBins * kTileWarps * 2;
-static_assert(kSortMemory <= 220 * 1024 && kTileMemory <= 100 * 1024);
+static_assert(kTileMemory <= 100 * 1024);
 
 template <class K>
 int allow(K* kernel, size_t memory, size_t most) {
@@ -630,19 +658,17 @@ int launch_next(void (*kernel)(P...), dim3 grid, unsigned threads, size_t memory
 }
 
 int sort_tokens(const Plan& p, Sort s, cudaStream_t st) {
-    const int64_t fill_ctas = (s.zero_count + kSortThreads * 4 - 1) / (kSortThreads * 4);
-    s.fillers = (int)(fill_ctas < 2 * sm_count() ? fill_ctas : 2 * sm_count());
+    const int64_t fill_ctas = (s.zero_count + kThreads * 16 - 1) / (kThreads * 16);
     if (!p.tiles) {
-        const int most = 1 << p.low_bits;
-        const size_t memory = (size_t)(s.count + 31) / 32 * 32 * sizeof(Entry) + most * 4 + (size_t)most * kSortWarps * 2;
-        if (const int status = allow(sort_kernel, memory, kSortMemory)) return status;
-        sort_kernel<<<1 + s.fillers, kSortThreads, memory, st>>>(s);
+        const int rankers = (int)((s.count + kRanked - 1) / kRanked);
+        s.fillers = (int)(fill_ctas < 8 * sm_count() ? fill_ctas : 8 * sm_count());
+        rank_kernel<<<rankers + s.fillers, kThreads, 0, st>>>(s, rankers);
         return check_launch();
     }
+    s.fillers = (int)(fill_ctas < 4 * sm_count() ? fill_ctas : 4 * sm_count());
     const size_t low = ((size_t)8 << p.low_bits) + ((size_t)kTileWarps * 2 << p.low_bits), high = ((size_t)8 << p.high_bits) + ((size_t)kTileWarps * 2 << p.high_bits);
     if (const int status = allow(scatter_kernel<false>, low, kTileMemory)) return status;
     if (const int status = allow(scatter_kernel<true>, high, kTileMemory)) return status;
-    s.fillers *= 2;
     const unsigned ctas = (unsigned)(p.tiles + s.fillers);
     count_kernel<<<ctas, kTileThreads, (size_t)4 << p.low_bits, st>>>(s);
     if (const int status = check_launch()) return status;
@@ -735,14 +761,14 @@ int pamk_embedding_bwd(const int64_t* tokens, const float* dy, const float* tabl
     u.chunks = (uint32_t)plan.chunks;
     u.scaled = a.scaled;
     u.drops = a.drops;
-    u.scale = scale;
-    u.off = a.off;
+    u.scale = a.scale;
+    u.keep = a.keep;
     u.drop = a.drop;
     const bool slopes = !approx_bwd && a.scaled;
     const bool vec = dim % 4 == 0 && aligned16(dy) && aligned16(dtable) && (!slopes || (aligned16(table) && table_row % 4 == 0));
     const auto sums = vec ? (slopes ? sum_kernel<true, true> : sum_kernel<true, false>) : (slopes ? sum_kernel<false, true> : sum_kernel<false, false>);
     if (const int status = launch_next(sums, dim3((unsigned)ctas), kThreads, 0, st, u)) return status;
-    const int64_t wide = (4 * sm_count() + slabs - 1) / slabs;
+    const int64_t wide = (8 * sm_count() + slabs - 1) / slabs;
     const unsigned joins = (unsigned)(plan.chunks < wide ? plan.chunks : wide);
     return launch_next(vec ? join_kernel<true> : join_kernel<false>, dim3(joins, (unsigned)slabs), kThreads, 0, st, u);
 }
