@@ -47,7 +47,7 @@ __device__ __forceinline__ float finished(const Embedding& a, float x, uint32_t 
     return bits < a.drop.below ? 0.0f : SLOPES ? mul_bwd(x, a.keep.s, g, a.keep.off) : a.keep.one(x);
 }
 
-// A thread takes four neighbouring elements of the output, which is what a block of the counter has bits for; here of any row length.
+// A thread takes four neighbouring elements of the output, which is what a block of the counter has bits for; here of any row length and number.
 template <bool SLOPES>
 __global__ void __launch_bounds__(kThreads) embed_kernel(const Embedding a, const float* g, float* out) {
     const int64_t e = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 4, n = a.count * a.dim;
@@ -119,6 +119,51 @@ __global__ void __launch_bounds__(kThreads) embed_quads_kernel(const Embedding a
         }
         reinterpret_cast<float4*>(out)[q] = y;
     }
+}
+
+// Rows of any length of at least four and at any address, fewer than 2^31 elements: quads of the output, most of which lie within a row.
+template <bool SLOPES>
+__global__ void __launch_bounds__(kThreads) embed_odd_kernel(const Embedding a, const float* g, float* out, uint32_t n, Divide by_row, Divide by_pos) {
+    const uint32_t q = blockIdx.x * kThreads + threadIdx.x, e = q * 4;
+    if (e >= n) return;
+    const uint2 key = a.drops ? key_of(a.drop) : make_uint2(0u, 0u);
+    const uint32_t i = by_row(e), c = e - i * by_row.d;
+    const auto at = [&](uint32_t row, uint32_t column, int64_t token) {
+        float x = quiet_nan();
+        if ((uint64_t)token < (uint64_t)a.vocab) x = __ldg(a.table + token * a.table_row + column);
+        return x;
+    };
+    const auto place = [&](uint32_t row, uint32_t column) { return a.pos ? __ldg(a.pos + (int64_t)(row - by_pos(row) * by_pos.d) * a.pos_row + column) : 0.0f; };
+    const int64_t token = token_at(a.tokens, i);
+    float x[4], p[4], d[4];
+    int64_t next = -1;
+    if (c + 3 >= by_row.d && i + 1 < (uint32_t)a.count) next = token_at(a.tokens, i + 1);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const bool behind = c + k >= by_row.d;
+        const uint32_t row = i + behind, column = c + k - (behind ? by_row.d : 0u);
+        x[k] = p[k] = d[k] = 0.0f;
+        if (e + k >= n) continue;
+        x[k] = at(row, column, behind ? next : token);
+        p[k] = place(row, column);
+        if (SLOPES) d[k] = __ldg(g + e + k);
+    }
+    float4 y = make_float4(x[0], x[1], x[2], x[3]);
+    if (a.scaled) y = a.scale.of(y);
+    if (a.pos) y = make_float4(fadd(y.x, p[0]), fadd(y.y, p[1]), fadd(y.z, p[2]), fadd(y.w, p[3]));
+    if (a.drops) {
+        const uint4 w = philox(q, key);
+        if (!SLOPES) y = a.keep.of(y);
+        const auto last = [&](float v, uint32_t bits, float dv) { return bits < a.drop.below ? 0.0f : SLOPES ? mul_bwd(v, a.keep.s, dv, a.keep.off) : v; };
+        y = make_float4(last(y.x, w.x, d[0]), last(y.y, w.y, d[1]), last(y.z, w.z, d[2]), last(y.w, w.w, d[3]));
+    }
+    const float v[4] = {y.x, y.y, y.z, y.w};
+    if (aligned16(out) && e + 4 <= n)
+        reinterpret_cast<float4*>(out)[q] = y;
+    else
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (e + k < n) out[e + k] = v[k];
 }
 
 // ---- the order of the tokens ------------------------------------------------------------------------------------
@@ -391,31 +436,30 @@ __device__ __forceinline__ Entry entry_at(const Entry* sorted, uint32_t i) {
     return {e.x, e.y};
 }
 
-// The columns of a lane: four neighbours (VEC), or every 32nd.
-template <bool VEC>
-__device__ __forceinline__ int column(int slab, int lane, int k) { return slab * kColumns + (VEC ? lane * 4 + k : lane + 32 * k); }
+// A lane has four neighbouring columns.  VEC: rows of whole quads at aligned addresses.
+__device__ __forceinline__ int column(int slab, int lane) { return slab * kColumns + lane * 4; }
 
 template <bool VEC>
 __device__ __forceinline__ void load_columns(const float* row, int slab, int lane, int dim, float (&v)[4]) {
+    const int c = column(slab, lane);
     if (VEC) {
-        const int c = column<true>(slab, lane, 0);
         const float4 x = c < dim ? __ldg(reinterpret_cast<const float4*>(row + c)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
     } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = column<false>(slab, lane, k) < dim ? __ldg(row + column<false>(slab, lane, k)) : 0.0f;
+        for (int k = 0; k < 4; ++k) v[k] = c + k < dim ? __ldg(row + c + k) : 0.0f;
     }
 }
 
 template <bool VEC>
 __device__ __forceinline__ void store_columns(float* row, int slab, int lane, int dim, const float (&v)[4]) {
+    const int c = column(slab, lane);
     if (VEC) {
-        const int c = column<true>(slab, lane, 0);
         if (c < dim) *reinterpret_cast<float4*>(row + c) = make_float4(v[0], v[1], v[2], v[3]);
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-            if (column<false>(slab, lane, k) < dim) row[column<false>(slab, lane, k)] = v[k];
+            if (c + k < dim) row[c + k] = v[k];
     }
 }
 
@@ -463,13 +507,13 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const Sums a) {
             }
             float4 x = make_float4(v[j][0], v[j][1], v[j][2], v[j][3]);
             if (a.drops) {
-                const uint64_t e = (uint64_t)place * a.dim;
-                uint4 w;
-                if (VEC)
-                    w = philox((e + column<true>(slab, lane, 0)) >> 2, key);
-                else
-                    w = make_uint4(philox_word(e + column<false>(slab, lane, 0), key), philox_word(e + column<false>(slab, lane, 1), key),
-                                   philox_word(e + column<false>(slab, lane, 2), key), philox_word(e + column<false>(slab, lane, 3), key));
+                const uint64_t e = (uint64_t)place * a.dim + column(slab, lane);
+                uint4 w = philox(e >> 2, key);
+                if (!VEC && a.dim % 4) {              // (the four may lie in two blocks)
+                    const uint4 next = philox((e >> 2) + 1, key);
+                    if (e & 1) w = make_uint4(w.y, w.z, w.w, next.x);
+                    if (e & 2) w = e & 1 ? make_uint4(w.z, w.w, next.y, next.z) : make_uint4(w.z, w.w, next.x, next.y);
+                }
                 x = a.keep.of(x);
                 x = make_float4(w.x < a.drop.below ? 0.0f : x.x, w.y < a.drop.below ? 0.0f : x.y, w.z < a.drop.below ? 0.0f : x.z, w.w < a.drop.below ? 0.0f : x.w);
             }
@@ -508,7 +552,7 @@ __device__ __forceinline__ void add_parts(const Sums& a, uint32_t chunk, uint32_
             if (part >= to) continue;
             const float* row = a.parts + ((int64_t)(chunk + part) * 2 + (part == 0)) * a.dim;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[j][k] = column<VEC>(slab, lane, k) < a.dim ? __ldcg(row + column<VEC>(slab, lane, k)) : 0.0f;
+            for (int k = 0; k < 4; ++k) v[j][k] = column(slab, lane) + k < a.dim ? __ldcg(row + column(slab, lane) + k) : 0.0f;
         }
 #pragma unroll
         for (int j = 0; j < kAhead; ++j)
@@ -543,7 +587,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Sums a) {
         float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         add_parts<VEC>(a, chunk, from, to, slab, lane, sum);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) stage[warp][VEC ? lane * 4 + k : lane + 32 * k] = sum[k];
+        for (int k = 0; k < 4; ++k) stage[warp][lane * 4 + k] = sum[k];
         __syncthreads();
         if (threadIdx.x < kColumns && slab * kColumns + threadIdx.x < a.dim) {
             float s = stage[0][threadIdx.x];
@@ -696,6 +740,12 @@ int pamk_embedding(const int64_t* tokens, const float* table, const float* posit
         const uint32_t quads = (uint32_t)(n / 4), ctas = (quads + kThreads * kQuads - 1) / (kThreads * kQuads);
         (dy ? embed_quads_kernel<true> : embed_quads_kernel<false>)<<<ctas, kThreads, 0, st>>>(a, dy, out, quads, Divide((uint32_t)(dim / 4)),
                                                                                               Divide(positions ? (uint32_t)positions_count : 1u));
+        return check_launch();
+    }
+    if (dim >= 4 && n < ((int64_t)1 << 31) - 4) {
+        const uint32_t ctas = (uint32_t)((n + 4 * kThreads - 1) / (4 * kThreads));
+        (dy ? embed_odd_kernel<true> : embed_odd_kernel<false>)<<<ctas, kThreads, 0, st>>>(a, dy, out, (uint32_t)n, Divide((uint32_t)dim),
+                                                                                          Divide(positions ? (uint32_t)positions_count : 1u));
         return check_launch();
     }
     const int64_t ctas = (n + 4 * kThreads - 1) / (4 * kThreads);

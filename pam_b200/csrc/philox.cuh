@@ -44,13 +44,6 @@ __device__ __forceinline__ uint4 philox(uint64_t block, uint2 key) {
     }
     return make_uint4(a, b, c, d);
 }
-
-// The word of one element.
-__device__ __forceinline__ uint32_t philox_word(uint64_t element, uint2 key) {
-    const uint4 w = philox(element >> 2, key);
-    const uint32_t low = element & 1 ? w.y : w.x, high = element & 1 ? w.w : w.z;
-    return element & 2 ? high : low;
-}
 #endif
 
 }  // namespace pamk
