@@ -16,7 +16,8 @@ every swappable layer created the way the forks create it — from configuration
   models/transformer/transformer_decoder.py:149-173, 455-463): projections and feed-forward layers
   from the linear factory, LayerNorms from the norm factory, query scaling, attention products,
   softmax and the embedding scale through the operator dictionary, decoder input and output
-  embeddings tied so that the vocabulary projection is a layer of the linear factory too, and the
+  embeddings tied so that the vocabulary projection is a layer of the linear factory too, dropout after
+  the embedding and the sublayers (transformer_layer.py:270-360, modules/fairseq_dropout.py), and the
   label-smoothed loss of criterions/label_smoothed_cross_entropy.py:36-54 through the loss
   operator dictionary.
 
@@ -31,7 +32,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from . import decoding, factories, fused
+from . import decoding, factories, fused, pam_ops
 from .pam_opt import _pam_binding
 from .steps import DeitConfig, TransformerConfig, sinusoidal_positions
 
@@ -195,6 +196,23 @@ def _plain(bound, t):
     return bound is not None and bound.get("offset") in (None, 1.0) and t.is_cuda and t.dtype == torch.float32
 
 
+def _scaling(ops, t):
+    """The settings of the dictionary's PAM product, where the operators that are made of it (`pam_ops.embedding`, `pam_ops.dropout`) stand for it on this tensor; else None."""
+    bound = _pam_binding(ops, ("mul",))
+    if bound is None or not (t.is_cuda and t.dtype == torch.float32) or not fused._uniform(bound.get("approx_bwd", False)):
+        return None
+    return bound
+
+
+def _dropped(ops, x, p, seed, residual=None):
+    """Dropout of x, added to `residual`: with the dictionary's product where that is PAM's, else the ordinary one."""
+    bound = _scaling(ops, x)
+    if bound is not None:
+        return pam_ops.dropout(x, p, seed, residual, **bound)
+    x = F.dropout(x, p)
+    return x if residual is None else residual + x
+
+
 def _beyond(lengths, slots):
     """-inf at the positions from each length on, 0 before: [count, 1, slots]."""
     beyond = torch.arange(slots, device=lengths.device) >= lengths[:, None]
@@ -203,9 +221,11 @@ def _beyond(lengths, slots):
 
 class TransformerLayer(nn.Module):
     """Post-norm encoder layer, or decoder layer when `cross` is set (transformer_layer.py)."""
+    dropout, op_dict = 0.0, None          # (of a model that was saved before it had them)
 
-    def __init__(self, cfg, cross, linear_factory, norm_layer, op_dict):
+    def __init__(self, cfg, cross, linear_factory, norm_layer, op_dict, dropout=0.0):
         super().__init__()
+        self.dropout, self.op_dict = dropout, op_dict
         self.self_attn = MultiheadAttention(cfg.dim, cfg.heads, linear_factory, op_dict)
         self.self_attn_layer_norm = norm_layer(cfg.dim)
         if cross:
@@ -216,11 +236,14 @@ class TransformerLayer(nn.Module):
         self.final_layer_norm = norm_layer(cfg.dim)
         self.cross = cross
 
-    def forward(self, x, memory=None, self_mask=None):
-        x = self.self_attn_layer_norm(x + self.self_attn(x, x, self_mask))
+    def forward(self, x, memory=None, self_mask=None, seeds=None, drops=True):
+        add = lambda a, b: a + b
+        if drops and self.training and self.dropout:
+            add = lambda a, b: _dropped(self.op_dict, b, self.dropout, next(seeds) if seeds is not None else None, a)
+        x = self.self_attn_layer_norm(add(x, self.self_attn(x, x, self_mask)))
         if self.cross:
-            x = self.encoder_attn_layer_norm(x + self.encoder_attn(x, memory))
-        return self.final_layer_norm(x + self.fc2(torch.relu(self.fc1(x))))
+            x = self.encoder_attn_layer_norm(add(x, self.encoder_attn(x, memory)))
+        return self.final_layer_norm(add(x, self.fc2(torch.relu(self.fc1(x)))))
 
     def step(self, x, own, position, shared, shared_lengths):
         """The decoder layer on one new token of each row, [groups, rows, dim]: its key and value go to `position` of the row's own
@@ -264,12 +287,14 @@ def _kept(module, name, length, device, make, cut):
 
 
 class _Stack(nn.Module):
-    def __init__(self, cfg, layers, cross, linear_factory, norm_layer, op_dict):
+    dropout = 0.0
+
+    def __init__(self, cfg, layers, cross, linear_factory, norm_layer, op_dict, dropout=0.0):
         super().__init__()
-        self.cfg, self.op_dict = cfg, op_dict
+        self.cfg, self.op_dict, self.dropout = cfg, op_dict, dropout
         self.embed_tokens = nn.Embedding(cfg.vocab, cfg.dim, padding_idx=cfg.pad)
         self.embed_scale = math.sqrt(cfg.dim)
-        self.layers = nn.ModuleList([TransformerLayer(cfg, cross, linear_factory, norm_layer, op_dict) for _ in range(layers)])
+        self.layers = nn.ModuleList([TransformerLayer(cfg, cross, linear_factory, norm_layer, op_dict, dropout) for _ in range(layers)])
 
     def _positions(self, length, device):
         """The first rows of the sinusoidal table, which take the host and a copy that waits to make."""
@@ -281,9 +306,18 @@ class _Stack(nn.Module):
         return _kept(self, "future", length, device, lambda n, d: torch.full((n, n), float("-inf"), device=d).triu(1),
                      lambda table, n: table[:n, :n])
 
-    def embed(self, tokens):
-        x = self.op_dict["mul"](self.embed_scale, self.embed_tokens(tokens))
-        return x + self._positions(tokens.shape[1], tokens.device)
+    def embed(self, tokens, positions=None, seed=None, drops=True):
+        """Scaled rows of the table plus `positions` (those of whole sentences, where not given), dropped out in training."""
+        table, p = self.embed_tokens, self.dropout if drops and self.training else 0.0
+        if positions is None:
+            positions = self._positions(tokens.shape[1], tokens.device)
+        bound = _scaling(self.op_dict, table.weight)
+        # (without dropout a training step keeps the chain, and with it the order in which torch adds up the table's gradient)
+        if bound is not None and (p or not torch.is_grad_enabled()) and type(table) is nn.Embedding and table.weight.shape[0] <= 1 << 22 \
+                and not table._forward_hooks and not table._forward_pre_hooks:
+            return pam_ops.embedding(tokens, table.weight, self.embed_scale, positions, table.padding_idx, p=p, seed=seed, **bound)
+        x = self.op_dict["mul"](self.embed_scale, table(tokens)) + positions
+        return _dropped(self.op_dict, x, p, seed) if p else x
 
 
 def _select(ops, logits, scores, count, banned):
@@ -296,6 +330,22 @@ def _select(ops, logits, scores, count, banned):
     return values, at // logits.shape[-1], at % logits.shape[-1]
 
 
+def _draw(ops, logits, uniform, temperature, top_k, top_p, min_p, banned):
+    """A token for every row of logits and its score, as `decoding.sample` gives them."""
+    bound = _pam_binding(ops, ("div", "log_softmax"))
+    if _plain(bound, logits):
+        return decoding.sample(logits, uniform, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, banned=banned)
+    values = ops["log_softmax"](ops["div"](logits, temperature), dim=-1)
+    order = values.masked_fill(banned, float("-inf")).sort(dim=-1, descending=True, stable=True)
+    p = order.values.double().exp()
+    if top_k:
+        p[..., top_k:] = 0.0
+    p = p * (p.cumsum(-1) - p < top_p * p.sum(-1, keepdim=True)) * (p >= min_p * p[..., :1])
+    p = torch.zeros_like(p).scatter(-1, order.indices, p).cumsum(-1)
+    tokens = (p <= uniform.double().unsqueeze(-1) * p[..., -1:]).sum(-1).clamp(max=logits.shape[-1] - 1)
+    return tokens, values.gather(-1, tokens.unsqueeze(-1)).squeeze(-1)
+
+
 def _reorder(states, parents, used):
     if parents.is_cuda:
         return decoding.reorder_states(states, parents, used)
@@ -305,38 +355,107 @@ def _reorder(states, parents, used):
 
 
 class Transformer(nn.Module):
+    """`dropout`: in training, of the embeddings and of what each sublayer adds (the `--dropout` of the reference's fork)."""
+    dropout = 0.0
+
     def __init__(self, cfg=TransformerConfig(), linear_cfg="standard", norm_cfg="layer_norm", functional_cfg="torch",
-                 loss_functional_cfg="torch"):
+                 loss_functional_cfg="torch", dropout=0.0):
         super().__init__()
-        self.cfg = cfg
+        pam_ops._probability(dropout)
+        self.cfg, self.dropout = cfg, dropout
         linear_factory = factories.get_linear_factory(linear_cfg)
         norm_factory = factories.get_norm_factory(norm_cfg)
         norm_layer = lambda dim: norm_factory(dim, eps=cfg.eps)
         op_dict = factories.get_function_dict(functional_cfg)
         self.loss_ops = factories.get_function_dict(loss_functional_cfg)
-        self.encoder = _Stack(cfg, cfg.encoder_layers, False, linear_factory, norm_layer, op_dict)
-        self.decoder = _Stack(cfg, cfg.decoder_layers, True, linear_factory, norm_layer, op_dict)
+        self.encoder = _Stack(cfg, cfg.encoder_layers, False, linear_factory, norm_layer, op_dict, dropout)
+        self.decoder = _Stack(cfg, cfg.decoder_layers, True, linear_factory, norm_layer, op_dict, dropout)
         # the decoder's input and output embeddings are shared: the output projection is a layer of the
         # linear factory whose weight is the embedding table (transformer_decoder.py:455-463)
         self.decoder.output_projection = linear_factory(cfg.dim, cfg.vocab, bias=False)
         self.decoder.output_projection.weight = self.decoder.embed_tokens.weight
 
-    def encode(self, src, src_lengths=None):
+    def _seeds(self, device):
+        """The seeds of a training step's masks, drawn at once: of the embeddings, and of what the sublayers add."""
+        if not (self.training and self.dropout) or device.type != "cuda":
+            return None
+        count = 2 + 2 * len(self.encoder.layers) + 3 * len(self.decoder.layers)
+        return iter(torch.randint(-2 ** 63, 2 ** 63 - 1, (count,), device=device).unbind())
+
+    def encode(self, src, src_lengths=None, seeds=None, drops=True):
         """The encoder's output.  `src_lengths` (int64 [sentences]): the tokens behind a sentence's length are padding, which no other position
         attends to."""
         mask = None if src_lengths is None else _beyond(src_lengths, src.shape[1]).repeat_interleave(self.cfg.heads, 0)
-        x = self.encoder.embed(src)
+        if seeds is None and drops:
+            seeds = self._seeds(src.device)
+        x = self.encoder.embed(src, seed=next(seeds) if seeds is not None else None, drops=drops)
         for layer in self.encoder.layers:
-            x = layer(x, self_mask=mask)
+            x = layer(x, self_mask=mask, seeds=seeds, drops=drops)
         return x
 
     def forward(self, src, prev_out):
-        x = self.encode(src)
+        seeds = self._seeds(src.device)
+        x = self.encode(src, seeds=seeds)
         future = self.decoder._future(prev_out.shape[1], src.device)
-        y = self.decoder.embed(prev_out)
+        y = self.decoder.embed(prev_out, seed=next(seeds) if seeds is not None else None)
         for layer in self.decoder.layers:
-            y = layer(y, x, future)
+            y = layer(y, x, future, seeds)
         return self.decoder.output_projection(y)
+
+    def _start(self, src, src_lengths, rows, max_len, eos):
+        """What generation begins with: the source's keys and values in every layer, caches for `rows` rows of each sentence, and which tokens may
+        not be chosen early, in between and at last."""
+        cfg, device = self.cfg, src.device
+        if eos == cfg.pad or not 0 <= eos < cfg.vocab or cfg.vocab < 3:
+            raise ValueError(f"end of sentence {eos} with padding {cfg.pad} in a vocabulary of {cfg.vocab}")
+        if src_lengths is not None and not bool(((src_lengths >= 1) & (src_lengths <= src.shape[1])).all()):
+            raise ValueError(f"lengths must be from 1 to {src.shape[1]}")
+        memory = self.encode(src, src_lengths, drops=False)
+        shared = [layer.encoder_attn.cache(memory) for layer in self.decoder.layers]
+        G, H = src.shape[0], cfg.heads
+        own = [tuple(torch.empty(G, rows, max_len, H, cfg.dim // H, dtype=memory.dtype, device=device) for _ in range(2)) for _ in self.decoder.layers]
+        banned = torch.zeros(3, cfg.vocab, dtype=torch.bool, device=device)
+        banned[:, cfg.pad] = True
+        banned[0, eos] = True
+        banned[2] = True
+        banned[2, eos] = False
+        return shared, own, banned
+
+    def _step(self, last, place, position, own, shared, src_lengths):
+        """The logits of the tokens behind `last` [sentences, rows], which stand at `position`."""
+        x = self.decoder.embed(last, place, drops=False)
+        for layer, mine, ours in zip(self.decoder.layers, own, shared):
+            x = layer.step(x, mine, position, ours, src_lengths)
+        return self.decoder.output_projection(x)
+
+    @torch.no_grad()
+    def sample(self, src, samples=5, max_len=200, *, src_lengths=None, min_len=1, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, generator=None, eos=2):
+        """`samples` translations of each sentence, drawn token by token (the fork's --sampling, fairseq/search.py:568-700) with the settings of
+        `decoding.sample` and random numbers of `generator` (of the source's device; None: the default one).
+
+        src, src_lengths, max_len, min_len and eos as for `generate`.  Returns (tokens [sentences, samples, n], scores [sentences, samples]): a score is the sum of its
+        tokens' log-probabilities; tokens behind the end are padding."""
+        cfg, ops, device = self.cfg, self.decoder.op_dict, src.device
+        if not 1 <= min_len <= max_len or samples < 1:
+            raise ValueError("sample needs 1 <= min_len <= max_len and at least one sample")
+        shared, own, banned = self._start(src, src_lengths, samples, max_len, eos)
+        positions = self.decoder._positions(max_len, device)
+        shape = (src.shape[0], samples)
+        tokens = torch.full((*shape, max_len), cfg.pad, device=device)
+        last = torch.full(shape, eos, device=device)
+        scores = torch.zeros(shape, device=device)
+        going = torch.ones(shape, dtype=torch.bool, device=device)
+        for t in range(max_len):
+            logits = self._step(last, positions[t], t, own, shared, src_lengths)
+            uniform = torch.rand(shape, generator=generator, device=device)
+            drawn, gained = _draw(ops, logits, uniform, temperature, top_k, top_p, min_p, banned[2 if t == max_len - 1 else 0 if t + 1 < min_len else 1])
+            last = torch.where(going, drawn, cfg.pad)
+            scores = torch.where(going, scores + gained, scores)
+            tokens[:, :, t] = last
+            going = going & (last != eos)
+            if t == max_len - 1 or not bool(going.any()):
+                break
+        return tokens[:, :, :t + 1], scores
 
     @torch.no_grad()
     def generate(self, src, beam=5, max_len=200, *, src_lengths=None, min_len=1, length_penalty=1.0, eos=2):
@@ -353,14 +472,8 @@ class Transformer(nn.Module):
         cfg, ops, device = self.cfg, self.decoder.op_dict, src.device
         if not 1 <= min_len <= max_len or beam < 1 or 2 * beam > decoding.MAX_SELECTED:
             raise ValueError(f"generate needs 1 <= min_len <= max_len and up to {decoding.MAX_SELECTED // 2} beams")
-        if eos == cfg.pad or not 0 <= eos < cfg.vocab or cfg.vocab < 3:
-            raise ValueError(f"end of sentence {eos} with padding {cfg.pad} in a vocabulary of {cfg.vocab}")
-        if src_lengths is not None and not bool(((src_lengths >= 1) & (src_lengths <= src.shape[1])).all()):
-            raise ValueError(f"lengths must be from 1 to {src.shape[1]}")
-        memory = self.encode(src, src_lengths)
-        shared = [layer.encoder_attn.cache(memory) for layer in self.decoder.layers]
-        G, H = src.shape[0], cfg.heads
-        own = [tuple(torch.empty(G, beam, max_len, H, cfg.dim // H, dtype=memory.dtype, device=device) for _ in range(2)) for _ in self.decoder.layers]
+        shared, own, banned = self._start(src, src_lengths, beam, max_len, eos)
+        G = src.shape[0]
         caches = [t for pair in own for t in pair]
         positions = self.decoder._positions(max_len, device)
         tokens = torch.full((G, beam, max_len), cfg.pad, device=device)
@@ -368,19 +481,10 @@ class Transformer(nn.Module):
         scores = torch.full((G, beam), float("-inf"), device=device)
         scores[:, 0] = 0.0
         best, best_tokens = torch.full((G, beam), float("-inf"), device=device), tokens.clone()
-        # what may not be chosen: early, in between and at last
-        banned = torch.zeros(3, cfg.vocab, dtype=torch.bool, device=device)
-        banned[:, cfg.pad] = True
-        banned[0, eos] = True
-        banned[2] = True
-        banned[2, eos] = False
         count = min(2 * beam, beam * cfg.vocab)
         rank = torch.arange(count, device=device)
         for t in range(max_len):
-            x = ops["mul"](self.decoder.embed_scale, self.decoder.embed_tokens(last)) + positions[t]
-            for layer, mine, ours in zip(self.decoder.layers, own, shared):
-                x = layer.step(x, mine, t, ours, src_lengths)
-            logits = self.decoder.output_projection(x)
+            logits = self._step(last, positions[t], t, own, shared, src_lengths)
             found, parents, chosen = _select(ops, logits, scores, count, banned[2 if t == max_len - 1 else 0 if t + 1 < min_len else 1])
             # the ends of sentences among the first `beam` are hypotheses; the best are kept
             ends = chosen == eos
