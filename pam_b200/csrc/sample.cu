@@ -17,7 +17,7 @@
 // A row belongs to a cluster of up to eight CTAs, each of which keeps its part in shared memory: the t of its tokens, then their keys.  A warp has neighbouring
 // tokens, of which a thread has the same four at a time from loading to drawing.  The logits are read once.  What stays is cut off at one token, found as follows:
 //   top-k   each warp's q-th best of its lanes' best tokens, where q of each of w warps are k at least, bounds the k-th best of all; the few tokens as good as the
-//           bound go to a list in the first CTA, which sorts it and draws from it;
+//           bound go to a list in the first CTA, where each counts those before it and their weights, and which draws from them;
 //   top-p   each warp sets aside its tokens that are not too light to matter (most often few), whose weights go into a histogram of as many parts as a CTA has
 //           threads; the few tokens of the part that holds the cut go to the list.  (More than a list holds: the part is divided again.)
 #include <cooperative_groups.h>
@@ -49,19 +49,21 @@ struct Sample {
     float temperature, top_p, min_p;
     int64_t top_k;
     int vocab, part;                                  // a CTA's tokens
+    int vocab_bits;                                   // of the power of two next to the vocabulary from above
     int64_t* tokens;
     float* scores;
 };
 
+constexpr int kListed = 256;
+
 template <int THREADS>
 struct Shared {
-    static constexpr int kWarps = THREADS / 32, kFew = THREADS / 2;
+    static constexpr int kWarps = THREADS / 32, kFew = THREADS;
     union {
-        u64 list[THREADS];                            // as many as there are threads
+        struct { u64 list[kListed], weights[kListed]; };
         struct { uint32_t count[THREADS], low[THREADS], high[THREADS]; };             // of each part: keys, and the sum of their weights' digits by 12 bits
     };
-    uint32_t few[kWarps][kFew];                       // a warp's keys in the range of a search, and their slots
-    uint16_t few_slots[kWarps][kFew];
+    uint16_t few[kWarps][kFew];                       // slots of a warp's keys in the range of a search
     // what the other CTAs of the cluster read
     float all, ok;
     int bad;
@@ -188,32 +190,13 @@ struct Scaling {
     __device__ __noinline__ float any(float x) const { return x <= kMasked ? -INFINITY : mul(div(x, temperature, 0), kLog2e, 0); }
 };
 
-// Sorts the threads' values, the first `size` (a power of two of at least 32) of them, through shared memory where pairs are in different warps.
-__device__ __forceinline__ void sort(u64& own, int size, u64* memory) {
-    const int t = threadIdx.x;
-    for (int run = 2; run <= size; run *= 2)
-        for (int apart = run / 2; apart > 0; apart /= 2) {
-            u64 other;
-            if (apart >= 32) {
-                __syncthreads();
-                memory[t] = own;
-                __syncthreads();
-                other = memory[t ^ apart];
-            } else {
-                other = __shfl_xor_sync(0xffffffffu, own, apart);
-            }
-            const bool up = (t & run) == 0 || run == size, lower = (t & apart) == 0;
-            own = (own < other) == (up == lower) ? own : other;
-        }
-}
-
 // What is asked of a row.
 struct Wanted { float top_p; uint32_t min_p, uniform; };
 
 // A search for the token at which a count or a weight is reached, in the order of (key, number).
 template <int THREADS>
 struct Search {
-    static constexpr int kWarps = THREADS / 32, kListed = THREADS;
+    static constexpr int kWarps = THREADS / 32;
     typedef Shared<THREADS> Sh;
     Sh& sh;
     Team& team;
@@ -225,9 +208,9 @@ struct Search {
     __device__ __forceinline__ uint4 quad(int q) const { return q < last ? reinterpret_cast<const uint4*>(keys)[q] : make_uint4(kOut, kOut, kOut, kOut); }
 
     template <class F>
-    __device__ __forceinline__ void each(F&& f) const {               // f(key, slot) for all; warps stay together
-        for (int q = first + lane; q - lane < last; q += 32) {
-            const uint4 k = quad(q);
+    __device__ __forceinline__ void each(F&& f) const {               // f(key, slot) for all
+        for (int q = first + lane; q < last; q += 32) {
+            const uint4 k = reinterpret_cast<const uint4*>(keys)[q];
             f(k.x, q * 4);
             f(k.y, q * 4 + 1);
             f(k.z, q * 4 + 2);
@@ -235,8 +218,11 @@ struct Search {
         }
     }
     template <class F>
-    __device__ __forceinline__ void each_aside(F&& f) const {
-        for (int i = lane; i - lane < few; i += 32) i < few ? f(sh.few[warp][i], (int)sh.few_slots[warp][i]) : f(kOut, 0);
+    __device__ __forceinline__ void each_aside(F&& f) const {         // f(key, slot) for those set aside
+        for (int i = lane; i < few; i += 32) {
+            const int slot = sh.few[warp][i];
+            f(keys[slot], slot);
+        }
     }
     __device__ __forceinline__ u64 composite(uint32_t key, int slot) const { return (u64)key << kNumberBits | (uint32_t)(begin + slot); }
 
@@ -275,24 +261,30 @@ struct Search {
         return total_of([&](int c, int w) { return team.of(sh, c).staying[turn][w]; }, before);
     }
 
+    // What the lanes before this one have, and (in *all) the warp.
+    __device__ __forceinline__ int before_lane(int mine, int* all) const {
+        int upto = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += v;
+        }
+        *all = __shfl_sync(0xffffffffu, upto, 31);
+        return upto - mine;
+    }
+
     // Sets aside the warp's keys up to `most`, if they are few.
     __device__ void set_aside(uint32_t most) {
-        int found = 0;
-        for (int q = first + lane; q - lane < last; q += 32) {
-            const uint4 k = quad(q);
-            const uint32_t key[4] = {k.x, k.y, k.z, k.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t those = __ballot_sync(0xffffffffu, key[j] <= most);
-                const int place = found + __popc(those & ((1u << lane) - 1u));
-                if (key[j] <= most && place < Sh::kFew) {
-                    sh.few[warp][place] = key[j];
-                    sh.few_slots[warp][place] = (uint16_t)(q * 4 + j);
-                }
-                found += __popc(those);
-            }
+        int mine = 0;
+        each([&](uint32_t key, int) { mine += key <= most; });
+        int place = before_lane(mine, &few);
+        if (few > Sh::kFew) {
+            few = -1;
+            return;
         }
-        few = found <= Sh::kFew ? found : -1;
+        each([&](uint32_t key, int slot) {
+            if (key <= most) sh.few[warp][place++] = (uint16_t)slot;
+        });
         __syncwarp();
     }
 
@@ -356,76 +348,91 @@ struct Search {
     // The tokens with keys from `low` to `high` to the first CTA's list; false where there are too many.  sh.listed is 0 before.  (best: no key of the lane is smaller.)
     __device__ bool gather(uint32_t low, uint32_t high, uint32_t best) {
         Sh& head = team.of(sh, 0);
-        const bool aside = few >= 0;
-        if (aside || __any_sync(0xffffffffu, best <= high)) {
-            int mine = 0;
-            const auto count = [&](uint32_t key, int) { mine += key - low <= high - low; };
-            aside ? each_aside(count) : each(count);
-            const int found = (int)__reduce_add_sync(0xffffffffu, (uint32_t)mine);
-            uint32_t at = 0u;
-            if (found > 0 && lane == 0) at = atomicAdd(&head.listed, (uint32_t)found);
-            at = __shfl_sync(0xffffffffu, at, 0);
+        const bool aside = few >= 0, any = aside || best <= high;
+        int mine = 0;
+        const auto count = [&](uint32_t key, int) { mine += key - low <= high - low; };
+        if (any) aside ? each_aside(count) : each(count);
+        int all;
+        int place = before_lane(mine, &all);
+        if (all > 0) {
+            int at = 0;
+            if (lane == 0) at = (int)atomicAdd(&head.listed, (uint32_t)all);
+            place += __shfl_sync(0xffffffffu, at, 0);
             const auto put = [&](uint32_t key, int slot) {
-                const bool in = key - low <= high - low;
-                const uint32_t those = __ballot_sync(0xffffffffu, in), place = at + __popc(those & ((1u << lane) - 1u));
-                if (in && place < kListed) head.list[place] = composite(key, slot);
-                at += __popc(those);
+                if (key - low > high - low) return;
+                if (place < kListed) head.list[place] = composite(key, slot);
+                ++place;
             };
-            if (found > 0) aside ? each_aside(put) : each(put);
+            if (mine > 0) aside ? each_aside(put) : each(put);
         }
         team.wait();
         return head.listed <= kListed;
     }
 
-    // Sums of weights up to each thread's, which are in order.
-    __device__ u64 upto_of(u64 weight) {
-        const u64 upto_warp = warp_upto(weight);
+    // A token of the list: several neighbouring lanes may have it.
+    struct Listed { u64 own, weight; bool one; };     // one: of these lanes
+    __device__ Listed of_list(int n, int& split) {
+        const int t = threadIdx.x;
+        for (int i = t; i < n; i += THREADS) sh.weights[i] = weight_of((uint32_t)(sh.list[i] >> kNumberBits));
         __syncthreads();
-        if (lane == 31) sh.scan[warp] = upto_warp;
-        __syncthreads();
-        u64 upto = upto_warp;
-        for (int w = 0; w < warp; ++w) upto += sh.scan[w];
-        return upto;
+        split = 1;
+        while (split < 32 && n * split * 2 <= THREADS) split *= 2;
+        const int i = t / split;
+        return {i < n ? sh.list[i] : 0ull, i < n ? sh.weights[i] : 0ull, i < n && t % split == 0};
     }
-    __device__ static int room_for(int n) {
-        int size = 32;
-        while (size < n) size *= 2;
-        return size;
+    // How many tokens of the list a test holds for, and their weights.
+    template <class F>
+    __device__ void count_list(int n, int split, F&& before, uint32_t* count, u64* weight) {
+        uint32_t c = 0u;
+        u64 w = 0ull;
+        if ((int)threadIdx.x / split < n)
+            for (int j = threadIdx.x % split; j < n; j += split)
+                if (before(sh.list[j])) {
+                    ++c;
+                    w += sh.weights[j];
+                }
+        for (int d = split / 2; d > 0; d >>= 1) {
+            c += __shfl_xor_sync(0xffffffffu, c, d);
+            w += __shfl_xor_sync(0xffffffffu, w, d);
+        }
+        *count = c;
+        *weight = w;
     }
 
     // In the first CTA: sets sh.cut to the list's token at which the weight `target` is reached, less_weight before the list (by_count: the target-th, less_count before).
     __device__ void pick(bool by_count, u64 target, uint32_t less_count, u64 less_weight) {
-        const int t = threadIdx.x, n = (int)sh.listed;
-        u64 own = t < n ? sh.list[t] : ~0ull;
-        sort(own, room_for(n), sh.list);
-        const u64 weight = t < n ? weight_of((uint32_t)(own >> kNumberBits)) : 0ull, upto = less_weight + upto_of(weight);
-        if (t < n && (by_count ? less_count + t + 1 == target : upto - weight < target && target <= upto)) sh.cut = own;
+        const int n = (int)sh.listed;
+        int split;
+        const Listed l = of_list(n, split);
+        uint32_t count;
+        u64 before;
+        count_list(n, split, [&](u64 other) { return other < l.own; }, &count, &before);
+        before += less_weight;
+        if (l.one && (by_count ? less_count + count + 1 == target : before < target && target <= before + l.weight)) sh.cut = l.own;
     }
 
     // In the first CTA: draws from the list, which holds the k best tokens and maybe others.  The token's number is then in sh.cut.
     __device__ void draw(int k, const Wanted& wanted, u64 top_weight) {
-        const int t = threadIdx.x, n = (int)sh.listed;
-        u64 own = t < n ? sh.list[t] : ~0ull;
-        sort(own, room_for(n), sh.list);
-        u64 weight = t < k ? weight_of((uint32_t)(own >> kNumberBits)) : 0ull;
-        const u64 upto = upto_of(weight);
-        if (t == k - 1) sh.kept = upto;
+        constexpr u64 kNumbers = (1ull << kNumberBits) - 1;
+        const int n = (int)sh.listed;
+        int split;
+        const Listed l = of_list(n, split);
+        uint32_t count;
+        u64 before;
+        count_list(n, split, [&](u64 other) { return other < l.own; }, &count, &before);
+        if (l.one && (int)count == k - 1) sh.kept = before + l.weight;
         __syncthreads();
         const u64 limit = wanted.top_p < 1.0f ? max(share_up(steps(wanted.top_p, 0xffffffu), sh.kept), 1ull) : ~0ull;
-        if (upto - weight >= limit || weight < share_up(wanted.min_p, top_weight)) weight = 0ull;
-        // in order of their numbers
-        u64 by_number = weight ? (own & ((1u << kNumberBits) - 1u)) << 32 | (uint32_t)t : ~0ull;
+        const bool stays = (int)count < k && before < limit && l.weight >= share_up(wanted.min_p, top_weight);
         __syncthreads();
-        sort(by_number, room_for(k), sh.list);
+        if (l.one && !stays) sh.weights[threadIdx.x / split] = 0ull;
         __syncthreads();
-        sh.list[t] = weight;
-        __syncthreads();
-        weight = by_number != ~0ull ? sh.list[(uint32_t)by_number] : 0ull;
-        const u64 before = upto_of(weight) - weight;
-        if (t == THREADS - 1) sh.kept = before + weight;
-        __syncthreads();
-        const u64 drawn = share(wanted.uniform, sh.kept).whole;
-        if (weight && before <= drawn && drawn < before + weight) sh.cut = by_number >> 32;
+        // those that stay, in order of their numbers
+        u64 total;
+        count_list(n, split, [&](u64) { return true; }, &count, &total);
+        count_list(n, split, [&](u64 other) { return (other & kNumbers) < (l.own & kNumbers); }, &count, &before);
+        const u64 drawn = share(wanted.uniform, total).whole;
+        if (l.one && stays && before <= drawn && drawn < before + l.weight) sh.cut = l.own & kNumbers;
         __syncthreads();
     }
 
@@ -690,8 +697,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
         sh.banned_sums[warp] = banned_sum;
     }
     // of the lanes' best the q-th best, where q of each warp are k at least
-    const int warps = team.ctas * kWarps, q = cut_by_k ? (int)((min(top_k, (int64_t)THREADS) + warps - 1) / warps) : 0;
-    const bool bounded = cut_by_k && top_k <= THREADS / 2 && q <= 32;
+    const int warps = team.ctas * kWarps, q = cut_by_k ? (int)((min(top_k, (int64_t)kListed) + warps - 1) / warps) : 0;
+    const bool bounded = cut_by_k && top_k <= kListed / 2 && q <= 32;
     if (cut_by_k) {
         const uint32_t live = __reduce_add_sync(0xffffffffu, sums.live);
         if (lane == 0) sh.live[warp] = live;
@@ -772,9 +779,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
     }
     if (top_p < 1.0f) {
         const u64 target = max(share_up(steps(top_p, 0xffffffu), total), 1ull);
-        // tokens so light that all of the vocabulary would not make up what is left out: 2^(45 - d) vocab <= total - target
+        // tokens so light that as many as the vocabulary's power of two would not make up what is left out: 2^(45 - d) of them <= total - target
         uint32_t most = kEnd - 1u;
-        const u64 each_less = (total - target) / (u64)a.vocab;
+        const u64 each_less = (total - target) >> a.vocab_bits;
         if (each_less > 0) most = min(most, ((uint32_t)max(45 - (63 - __clzll((long long)each_less)), 1) << 23) - 1u);
         if (cut != ~0ull) most = min(most, (uint32_t)(cut >> kNumberBits));
         cut = search.find(false, target, most);
@@ -888,6 +895,7 @@ int pamk_sample(const float* logits, const float* uniform, const unsigned char* 
     a.min_p = min_p;
     a.top_k = top_k;
     a.vocab = (int)vocab;
+    while (((int64_t)1 << a.vocab_bits) < vocab) ++a.vocab_bits;
     a.part = (int)((vocab + ctas - 1) / ctas + 31) / 32 * 32;
     a.tokens = tokens;
     a.scores = scores;
