@@ -165,7 +165,7 @@ __device__ double log_sum(double shift, double total) {
     const long long bits = __double_as_longlong(total);
     const double fraction = __longlong_as_double((bits & 0xfffffffffffffll) | 0x3ff0000000000000ll) - 1.0;
     const double log2 = shift + ((double)((bits >> 52) - 1023) + fraction), by = (double)kLog2e;
-    if (fabs(log2 / by) < 1e-37) return 0.0;
+    if (log2 == 0.0) return 0.0;                      // (the range rule's only case: any other is 2^-53 at least)
     return __longlong_as_double(__double_as_longlong(log2) - __double_as_longlong(by) + 0x3ff0000000000000ll);
 }
 
@@ -591,10 +591,26 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
 
     // the row's t, and the largest of all and of those that may be drawn
     float top_all = -INFINITY, top_ok = -INFINITY;
+    uint32_t any_out = 0u;
     bool bad = !(temperature > 0.0f && temperature <= i2f(0x7f7fffff));
     constexpr int kAhead = 4;
     const int full_from = phase ? 1 : 0, full_to = max((n + phase) / 4, full_from);    // quads that are all the part's
-    const auto scale = [&](int q, const float4& x) {
+    // A byte of flags for each of a quad's tokens.
+    const auto flags_of = [&](int q) {
+        const int s = q * 4 - phase;
+        if (!banned) return 0u;
+        if (s >= 4 && s + 8 <= n) {                   // (two aligned words hold the four)
+            const uintptr_t at = reinterpret_cast<uintptr_t>(banned + s);
+            const uint32_t* words = reinterpret_cast<const uint32_t*>(at & ~(uintptr_t)3);
+            return __funnelshift_r(__ldg(words), __ldg(words + 1), (uint32_t)(at & 3) * 8u);
+        }
+        uint32_t all = 0u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (s + j >= 0 && s + j < n) all |= (uint32_t)__ldg(banned + s + j) << (8 * j);
+        return all;
+    };
+    const auto scale = [&](int q, const float4& x, uint32_t flag) {
         float4 v;
         if (max(max(scaled.beyond(x.x), scaled.beyond(x.y)), max(scaled.beyond(x.z), scaled.beyond(x.w))) < scaled.span) {
             v = make_float4(scaled.plainly(x.x), scaled.plainly(x.y), scaled.plainly(x.z), scaled.plainly(x.w));
@@ -602,22 +618,21 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
             v = make_float4(scaled.any(x.x), scaled.any(x.y), scaled.any(x.z), scaled.any(x.w));
             bad = bad || v.x != v.x || v.y != v.y || v.z != v.z || v.w != v.w;
         }
-        top_all = fmaxf(top_all, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+        const float most = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
+        top_all = fmaxf(top_all, most);
         if (banned) {
-            const int s = q * 4 - phase;
             uint32_t out = 0u;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (s + j >= 0 && s + j < n && banned[s + j]) out |= 1u << j;
+            if (flag) out = ((flag & 0xffu) != 0) | ((flag & 0xff00u) != 0) << 1 | ((flag & 0xff0000u) != 0) << 2 | ((flag & 0xff000000u) != 0) << 3;
             flags[q] = (unsigned char)out;
-            top_ok = fmaxf(top_ok, fmaxf(fmaxf(out & 1u ? -INFINITY : v.x, out & 2u ? -INFINITY : v.y), fmaxf(out & 4u ? -INFINITY : v.z, out & 8u ? -INFINITY : v.w)));
+            any_out |= out;
+            top_ok = fmaxf(top_ok, !out ? most : fmaxf(fmaxf(out & 1u ? -INFINITY : v.x, out & 2u ? -INFINITY : v.y), fmaxf(out & 4u ? -INFINITY : v.z, out & 8u ? -INFINITY : v.w)));
         }
         reinterpret_cast<float4*>(keys)[q] = v;
     };
     const auto edge = [&](int q) {
         const int s = q * 4 - phase;
         const auto at = [&](int i) { return i >= 0 && i < n ? __ldcs(part + i) : -INFINITY; };
-        scale(q, make_float4(at(s), at(s + 1), at(s + 2), at(s + 3)));
+        scale(q, make_float4(at(s), at(s + 1), at(s + 2), at(s + 3)), flags_of(q));
     };
     {
         int q = first + lane;
@@ -631,8 +646,11 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
             float4 x[kAhead];
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) x[k] = __ldcs(from + q + 32 * k);
+            uint32_t flag[kAhead];
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) scale(q + 32 * k, x[k]);
+            for (int k = 0; k < kAhead; ++k) flag[k] = flags_of(q + 32 * k);
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) scale(q + 32 * k, x[k], flag[k]);
         }
         float4 x[kAhead - 1];
 #pragma unroll
@@ -640,7 +658,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
             if (q + 32 * k < stop) x[k] = __ldcs(from + q + 32 * k);
 #pragma unroll
         for (int k = 0; k < kAhead - 1; ++k)
-            if (q + 32 * k < stop) scale(q + 32 * k, x[k]);
+            if (q + 32 * k < stop) scale(q + 32 * k, x[k], flags_of(q + 32 * k));
         if (full_to >= first && full_to < last && (full_to - first) % 32 == lane) edge(full_to);
     }
     top_all = warp_max(top_all);
@@ -679,9 +697,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
 
     // keys in place of the t, and the sums
     Sums sums;
-    if (!banned) flags = nullptr;
+    const bool bans = banned && __any_sync(0xffffffffu, any_out);      // (one of the warp's tokens)
+    if (!bans) flags = nullptr;
     if (fmaxf(fabsf(shift), fabsf(shift_all)) < 1048576.0f) {
-        if (banned)
+        if (bans)
             cut_by_k ? make_keys<true, true, true>(sums, keys, flags, first + lane, last, shift, shift_all) : make_keys<true, true, false>(sums, keys, flags, first + lane, last, shift, shift_all);
         else
             cut_by_k ? make_keys<true, false, true>(sums, keys, flags, first + lane, last, shift, shift_all) : make_keys<true, false, false>(sums, keys, flags, first + lane, last, shift, shift_all);
@@ -690,7 +709,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
     }
     u64 weight = warp_sum(sums.units.get());
     const double sum = warp_sum(sums.sum + (shift >= -1.0f ? (double)sums.rest * power_of(-shift) : 0.0));     // (|t| < 1 only above)
-    const double banned_sum = banned ? warp_sum(sums.banned) : 0.0;
+    const double banned_sum = bans ? warp_sum(sums.banned) : 0.0;
     if (lane == 0) {
         sh.parts[warp] = weight;
         sh.sums[warp] = sum;
