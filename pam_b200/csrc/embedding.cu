@@ -190,14 +190,20 @@ struct Sort {
 
 // A share of the zeros: part `part` of `parts`, by the CTAs from `first` on.
 __device__ void fill(const Sort& a, int first, int part, int parts) {
-    const int64_t quads = (a.zero_count + 3) / 4, per = (quads + parts - 1) / parts, begin = per * part, end = min(begin + per, quads);
-    const bool aligned = aligned16(a.zeros);
-    for (int64_t q = begin + (int64_t)(blockIdx.x - first) * blockDim.x + threadIdx.x; q < end; q += (int64_t)a.fillers * blockDim.x) {
-        if (aligned && q * 4 + 4 <= a.zero_count)
-            reinterpret_cast<float4*>(a.zeros)[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        else
-            for (int64_t e = q * 4; e < min(q * 4 + 4, a.zero_count); ++e) a.zeros[e] = 0.0f;
+    const int64_t quads = aligned16(a.zeros) ? a.zero_count / 4 : 0, per = (quads + parts - 1) / parts, begin = per * part, end = min(begin + per, quads);
+    const int64_t mine = (int64_t)(blockIdx.x - first) * blockDim.x + threadIdx.x, stride = (int64_t)a.fillers * blockDim.x;
+    const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float4* to = reinterpret_cast<float4*>(a.zeros) + begin + mine;
+    int64_t left = end - begin - mine;
+    for (; left > 3 * stride; left -= 4 * stride, to += 4 * stride) {
+        to[0] = zero;
+        to[stride] = zero;
+        to[2 * stride] = zero;
+        to[3 * stride] = zero;
     }
+    for (; left > 0; left -= stride, to += stride) *to = zero;
+    if (part == parts - 1)                            // (what is no whole quad; all of them at an odd address)
+        for (int64_t e = quads * 4 + mine; e < a.zero_count; e += stride) a.zeros[e] = 0.0f;
 }
 
 __device__ __forceinline__ uint32_t token_of(const Sort& a, int64_t i) {

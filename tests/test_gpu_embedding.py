@@ -189,3 +189,26 @@ def test_module(pam):
     assert not layer.weight.grad[1].any() and bool(layer.weight.grad[3].any())
     layer.eval()
     assert torch.equal(layer(tokens), pam.mul(4.0, torch.nn.functional.embedding(tokens, layer.weight)))
+
+
+@pytest.mark.parametrize("n, vocab, dim", [(3, 5001, 7), (9000, 5001, 7), (20000, 300000, 9), (5, 1, 1), (8193, 3, 2)])
+def test_fills_all_rows(pam, n, vocab, dim):
+    """Rows without a token are zeros, whatever was in their memory, at any address of the gradient."""
+    from pam_b200 import _lib
+    handle = _lib.lib()
+    tokens = torch.randint(0, vocab, (n,)).cuda()
+    dy = torch.randn(n, dim).cuda()
+    ws_bytes = handle.pamk_embedding_bwd_workspace_bytes(n, vocab, dim)
+    ws = torch.full((ws_bytes,), 0xAB, dtype=torch.uint8, device="cuda")
+    want = torch.zeros(vocab, dim, dtype=torch.float64, device="cuda").index_add_(0, tokens, dy.double())
+    for shift in (0, 1):
+        memory = torch.full((vocab * dim + 8,), float("nan"), device="cuda")
+        dw = memory[shift:shift + vocab * dim]
+        _lib.check(handle.pamk_embedding_bwd(tokens.data_ptr(), dy.data_ptr(), None, dw.data_ptr(), n, vocab, dim, dim, -1, 0, 0.0, 0.0, None, 0, 1.0, 1,
+                                             ws.data_ptr(), ws_bytes, torch.cuda.current_stream().cuda_stream), "pamk_embedding_bwd")
+        count = tokens.bincount(minlength=vocab).double()[:, None]
+        size = torch.zeros_like(want).index_add_(0, tokens, dy.double().abs())
+        assert bool(((dw.view(vocab, dim).double() - want).abs() <= count * U * size).all())
+        assert bool(memory[:shift].isnan().all()) and bool(memory[shift + vocab * dim:].isnan().all())
+    assert handle.pamk_embedding_bwd(tokens.data_ptr(), dy.data_ptr(), None, dw.data_ptr(), n, vocab, dim, dim, -1, 0, 0.0, 0.0, None, 0, 1.0, 1, ws.data_ptr(),
+                                     ws_bytes - 1, None) == -4
