@@ -212,3 +212,50 @@ def test_fills_all_rows(pam, n, vocab, dim):
         assert bool(memory[:shift].isnan().all()) and bool(memory[shift + vocab * dim:].isnan().all())
     assert handle.pamk_embedding_bwd(tokens.data_ptr(), dy.data_ptr(), None, dw.data_ptr(), n, vocab, dim, dim, -1, 0, 0.0, 0.0, None, 0, 1.0, 1, ws.data_ptr(),
                                      ws_bytes - 1, None) == -4
+
+
+@pytest.mark.parametrize("scale", [0.0, -3.0, 1e-30, 1e30, 1e-45, 3e38, 1.0])
+@pytest.mark.parametrize("dim", [8, 7])
+def test_scales(pam, scale, dim):
+    """Scales and values at the ends of the range: the products and slopes of pam.mul, to the bit."""
+    tokens = torch.tensor([0, 3, 2, 1, 0]).cuda()
+    some = torch.tensor([0.0, -0.0, 1e-40, -3e-38, 2e-20, -1.5, 7e18, -2e37, 1e38, float("inf"), float("nan")])
+    g = torch.Generator().manual_seed(3)
+    weight = some[torch.randint(0, len(some), (4, dim), generator=g)].cuda().requires_grad_()
+    dy = some[torch.randint(0, 8, (5, dim), generator=g)].cuda()
+    for approx in (True, False):
+        out = pam.embedding(tokens, weight, scale, approx_bwd=approx)
+        rows = torch.nn.functional.embedding(tokens, weight).detach().requires_grad_()
+        want = pam.mul(scale, rows, approx_bwd=approx)
+        assert_bits_equal(out, want)
+        (d,), (terms,) = torch.autograd.grad(out, weight, dy), torch.autograd.grad(want, rows, dy)
+        for v in (1, 2, 3):                                   # (one term each)
+            assert_bits_equal(d[v] + 0.0, terms[tokens == v][0] + 0.0)
+
+
+def test_millions_of_tokens(pam):
+    """More tokens than 512 tiles of 4096: tiles of several."""
+    n, vocab = 2_200_003, 5001
+    tokens, weight, _, g = data((n,), vocab, 2, None, seed=9)
+    w = weight.cuda().requires_grad_()
+    (d,) = torch.autograd.grad(pam.embedding(tokens.cuda(), w, 1.5, padding_idx=3, approx_bwd=True), w, g.cuda())
+    want, bound, _ = define.embedded_grad(g, tokens, weight, 1.5, None, 3, 0.0, 0, True)
+    assert bool(((d.double().cpu() - want).abs() <= bound).all())
+
+
+def test_residual_and_input_are_one_tensor(pam):
+    x = torch.randn(300, device="cuda").requires_grad_()
+    y = pam.dropout(x, 0.4, 8, x, approx_bwd=True)
+    (d,) = torch.autograd.grad(y, x, torch.ones_like(x))
+    kept = pam.dropout(torch.ones(300, device="cuda"), 0.4, 8)
+    assert torch.equal(d, kept + 1.0)
+
+
+def test_expanded_positions(pam):
+    tokens = torch.randint(0, 20, (3, 6)).cuda()
+    w, row = torch.randn(20, 16).cuda().requires_grad_(), torch.randn(16).cuda().requires_grad_()
+    a = pam.embedding(tokens, w, 2.0, row.expand(6, 16), approx_bwd=True)
+    b = pam.embedding(tokens, w, 2.0, row, approx_bwd=True)
+    assert torch.equal(a, b)
+    ga, gb = (torch.autograd.grad(y, row, torch.ones_like(y))[0] for y in (a, b))
+    assert torch.equal(ga, gb)                                # (sums of 18 ones)

@@ -170,3 +170,43 @@ def test_captured(sample):
         graph.replay()
         want = sample(x, u, top_k=40, top_p=0.9)
         assert torch.equal(tokens, want[0]) and torch.equal(scores, want[1])
+
+
+@pytest.mark.parametrize("temperature", [2.0 ** -126, 1e-30, 1e-6, 1e-3, 0.37, 100.0, 1e6, 1e30, 2.0 ** 127])
+def test_temperatures(sample, temperature):
+    x, u = data(5, 800, seed=21)
+    for settings in (dict(), dict(top_k=7), dict(top_p=0.8)):
+        check(sample, x, u, temperature=temperature, **settings)
+
+
+@pytest.mark.parametrize("rows, vocab", [(5, 1003), (3, 4097), (2, 30001), (2, 50002)])
+def test_flags_at_odd_addresses(sample, rows, vocab):
+    x, u = data(rows, vocab, seed=vocab)
+    g = torch.Generator().manual_seed(1)
+    for share in (0.0005, 0.3):
+        banned = torch.rand(rows, vocab, generator=g) < share
+        for settings in (dict(), dict(top_k=20, top_p=0.9), dict(top_p=0.7)):
+            check(sample, x, u, banned=banned, **settings)
+            check(sample, x, u, banned=banned[0], **settings)
+
+
+def test_values_that_the_range_rule_cuts_off(sample):
+    """Zeros and denormals, and quads in which one value is far from the others."""
+    x, u = data(6, 600, seed=31)
+    x[0] = 0.0
+    x[1, ::3] = 0.0
+    x[2, ::5] = 1e-40
+    x[3, ::7] = -0.0
+    x[4] *= 1e-37
+    x[5, ::4] = -INF
+    for settings in SETTINGS:
+        check(sample, x, u, **settings)
+
+
+def test_large_k(sample):
+    """Cuts that no list holds."""
+    for rows, vocab in ((2, 5000), (1, 60000)):
+        x, u = data(rows, vocab, seed=rows)
+        for k in (127, 128, 129, 256, 257, 600, 4000):
+            check(sample, x, u, top_k=k)
+            check(sample, x, u, top_k=k, top_p=0.8, min_p=1e-4)
