@@ -78,35 +78,42 @@ struct Divide {
     __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (__umulhi(n, m) + n) >> s; }
 };
 
-// Rows of whole quads at aligned addresses, fewer than 2^31 quads.  A thread has a few, as far apart as a CTA is wide, with all of its loads on their way before the
-// first product; HBM-bound where the table is small, by the 4 bytes per element that are written.
+// Rows of whole quads at aligned addresses, fewer than 2^31 quads.  A thread has a few, with all of its loads on their way before the first product: as far apart as
+// a CTA is wide, or (SENTENCES) those of as many sentences at one position, which they read once.  What bounds it where the table lies in the L2 is the L2: 2^20 tokens of 128
+// columns with a table of positions, 9.4 TB/s of table, positions and output, 172 us with quads of neighbours.
 constexpr int kQuads = 4;
-template <bool SLOPES>
+template <bool SLOPES, bool SENTENCES>
 __global__ void __launch_bounds__(kThreads) embed_quads_kernel(const Embedding a, const float* g, float* out, uint32_t quads, Divide by_row, Divide by_pos) {
-    const uint32_t first = blockIdx.x * (kThreads * kQuads) + threadIdx.x;
+    const uint32_t sentence = SENTENCES ? (uint32_t)a.pos_count * by_row.d : 0u, at = blockIdx.x * (SENTENCES ? kThreads : kThreads * kQuads) + threadIdx.x;
+    const uint32_t first = SENTENCES ? at + blockIdx.y * kQuads * sentence : at, step = SENTENCES ? sentence : kThreads;
     const uint2 key = a.drops ? key_of(a.drop) : make_uint2(0u, 0u);
+    if (SENTENCES && at >= sentence) return;
     uint32_t row[kQuads];
     int64_t token[kQuads];
     float4 x[kQuads], p[kQuads], d[kQuads];
+    if (SENTENCES) row[0] = by_row(first);
 #pragma unroll
     for (int k = 0; k < kQuads; ++k) {
-        const uint32_t q = first + k * kThreads;
-        row[k] = by_row(q);
+        const uint32_t q = first + k * step;
+        row[k] = SENTENCES ? row[0] + k * (uint32_t)a.pos_count : by_row(q);
         token[k] = q < quads ? token_at(a.tokens, row[k]) : -1;
     }
+    if (SENTENCES) p[0] = __ldg(reinterpret_cast<const float4*>(a.pos + (int64_t)by_row(at) * a.pos_row + (at - by_row(at) * by_row.d) * 4));
 #pragma unroll
     for (int k = 0; k < kQuads; ++k) {
-        const uint32_t q = first + k * kThreads, c = (q - row[k] * by_row.d) * 4;
+        const uint32_t q = first + k * step, c = (SENTENCES ? first - row[0] * by_row.d : q - row[k] * by_row.d) * 4;
         x[k] = make_float4(quiet_nan(), quiet_nan(), quiet_nan(), quiet_nan());
-        p[k] = d[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        d[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if ((uint64_t)token[k] < (uint64_t)a.vocab) x[k] = __ldg(reinterpret_cast<const float4*>(a.table + token[k] * a.table_row + c));
-        if (q >= quads) continue;
-        if (a.pos) p[k] = __ldg(reinterpret_cast<const float4*>(a.pos + (int64_t)(row[k] - by_pos(row[k]) * by_pos.d) * a.pos_row + c));
-        if (SLOPES) d[k] = __ldg(reinterpret_cast<const float4*>(g) + q);
+        if (SENTENCES)
+            p[k] = p[0];
+        else
+            p[k] = a.pos && q < quads ? __ldg(reinterpret_cast<const float4*>(a.pos + (int64_t)(row[k] - by_pos(row[k]) * by_pos.d) * a.pos_row + c)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (SLOPES && q < quads) d[k] = __ldg(reinterpret_cast<const float4*>(g) + q);
     }
 #pragma unroll
     for (int k = 0; k < kQuads; ++k) {
-        const uint32_t q = first + k * kThreads;
+        const uint32_t q = first + k * step;
         if (q >= quads) return;
         float4 y = a.scaled ? a.scale.of(x[k]) : x[k];
         if (a.pos) y = make_float4(fadd(y.x, p[k].x), fadd(y.y, p[k].y), fadd(y.z, p[k].z), fadd(y.w, p[k].w));
@@ -659,7 +666,7 @@ Plan planned(int64_t count, int64_t vocab, int64_t dim) {
         p.tile = (int)((each + kTile - 1) / kTile * kTile);
         p.tiles = (int)((count + p.tile - 1) / p.tile);
     }
-    p.chunk = count > (1 << 18) ? 32 : 16;
+    p.chunk = count > 32768 ? 32 : 16;
     p.chunks = (count + p.chunk - 1) / p.chunk;
     size_t at = 0;
     const auto take = [&](size_t bytes) {
@@ -743,9 +750,18 @@ int pamk_embedding(const int64_t* tokens, const float* table, const float* posit
     const int64_t n = count * dim;
     const auto st = (cudaStream_t)stream;
     if (dim % 4 == 0 && n < ((int64_t)1 << 33) && aligned16(table) && table_row % 4 == 0 && aligned16(positions) && positions_row % 4 == 0 && aligned16(dy) && aligned16(out)) {
-        const uint32_t quads = (uint32_t)(n / 4), ctas = (quads + kThreads * kQuads - 1) / (kThreads * kQuads);
-        (dy ? embed_quads_kernel<true> : embed_quads_kernel<false>)<<<ctas, kThreads, 0, st>>>(a, dy, out, quads, Divide((uint32_t)(dim / 4)),
-                                                                                              Divide(positions ? (uint32_t)positions_count : 1u));
+        const uint32_t quads = (uint32_t)(n / 4);
+        const Divide by_row((uint32_t)(dim / 4)), by_pos(positions ? (uint32_t)positions_count : 1u);
+        // (of sentences at one position: two at least, and positions enough for a wave of CTAs or so)
+        const int64_t sentence = positions_count * (dim / 4), sentences = positions && positions_count > 1 ? count / positions_count : 1;
+        const int64_t groups = (sentences + kQuads - 1) / kQuads;
+        if (sentences >= 2 && groups <= 65535 && sentence >= kThreads) {
+            const dim3 grid((unsigned)((sentence + kThreads - 1) / kThreads), (unsigned)groups);
+            (dy ? embed_quads_kernel<true, true> : embed_quads_kernel<false, true>)<<<grid, kThreads, 0, st>>>(a, dy, out, quads, by_row, by_pos);
+        } else {
+            const uint32_t ctas = (quads + kThreads * kQuads - 1) / (kThreads * kQuads);
+            (dy ? embed_quads_kernel<true, false> : embed_quads_kernel<false, false>)<<<ctas, kThreads, 0, st>>>(a, dy, out, quads, by_row, by_pos);
+        }
         return check_launch();
     }
     if (dim >= 4 && n < ((int64_t)1 << 31) - 4) {
