@@ -381,7 +381,7 @@ int pamk_sample(const float* logits, const float* uniform, const unsigned char* 
 
 /* ---- embedding and dropout -----------------------------------------------------------------------------
  * No counterpart as kernels in the reference, whose fairseq fork looks tokens up, scales, adds positions and drops out one operator after another
- * (fairseq/models/transformer/transformer_encoder.py:177-196, fairseq/modules/fairseq_dropout.py).
+ * (fairseq/models/transformer/transformer_encoder.py, fairseq/modules/fairseq_dropout.py).
  *
  * The mask of a dropout: element i (of the contiguous output) has the 32 bits of word i mod 4 of the Philox4x32-10 block with counter i / 4 under the 64-bit key
  * *seed_at (on the device; NULL: `seed`), and stays where they are at least p 2^32, to the nearest whole number; s is the fp32 number next to 1 / (1 - p).

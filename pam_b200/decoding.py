@@ -1,10 +1,10 @@
-"""Text generation on the GPU: attention over a key/value cache, the selection step of beam search, and the reordering of
-the states that belong to the beams.
+"""Text generation on the GPU: attention over a key/value cache, the selection step of beam search, the reordering of
+the states that belong to the beams, and sampling.
 
 The reference's fairseq fork generates through the operators of its training graph: the whole chain of projections,
 products and softmax per step (fairseq/modules/multihead_attention.py:618-783), log-probabilities sorted over beams
-and vocabulary (fairseq/search.py:103-147), states gathered by beam (fairseq/sequence_generator.py:380-388).  Here each of
-the three is one call in the same PAM arithmetic, fp32 throughout.  None has a backward pass, and none takes an `offset`:
+and vocabulary (fairseq/search.py:103-147) or drawn by sorted probabilities, states gathered by beam (fairseq/sequence_generator.py:380-388).  Here each of
+the four is one call in the same PAM arithmetic, fp32 throughout.  None has a backward pass, and none takes an `offset`:
 with one, the PAM softmax depends on the maximum of the whole tensor.
 """
 import ctypes

@@ -430,7 +430,7 @@ class Transformer(nn.Module):
 
     @torch.no_grad()
     def sample(self, src, samples=5, max_len=200, *, src_lengths=None, min_len=1, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, generator=None, eos=2):
-        """`samples` translations of each sentence, drawn token by token (the fork's --sampling, fairseq/search.py:568-700) with the settings of
+        """`samples` translations of each sentence, drawn token by token (the fork's --sampling, fairseq/search.py) with the settings of
         `decoding.sample` and random numbers of `generator` (of the source's device; None: the default one).
 
         src, src_lengths, max_len, min_len and eos as for `generate`.  Returns (tokens [sentences, samples, n], scores [sentences, samples]): a score is the sum of its
