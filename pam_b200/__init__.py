@@ -2,7 +2,7 @@
 
 A drop-in for the ``pam`` package of epfml/pam: the same functions (``mul div exp exp2 log log2
 pow matmul bmm linear conv2d conv2d_group mean softmax logsumexp log_softmax layer_norm
-cross_entropy``), modules (``Linear Conv2d LayerNorm``) and submodules (``pam_ops native pam_opt
+cross_entropy``; beyond the reference ``dropout embedding``), modules (``Linear Conv2d LayerNorm``, ``Dropout Embedding``) and submodules (``pam_ops native pam_opt
 pam_experimental cuda_bindings utils``), computed by hand-written sm_100a kernels behind the C ABI
 of ``include/pam_b200.h``.  ``pam_b200.factories`` mirrors ``shared/modules/factories.py`` and
 ``pam_b200.optim.Adam`` the PAM Adam of the reference's fairseq fork.

@@ -2,8 +2,9 @@
 //     y_i = r_i + (kept_i ? pam(x_i, s) : 0)       s = fp32(1 / (1 - p))
 //     dx_i = kept_i ? pam(g_i, s) : 0              (approximate gradients: the forward pass on g)
 //     dx_i = kept_i ? g_i slope(x_i, s) : 0        (exact gradients)
-// A dropped element gives zero whatever it holds.  HBM-bound (8 to 12 bytes per element): a thread takes quads of neighbouring elements, which is
-// what a block of the counter has bits for.
+// A dropped element gives zero whatever it holds.  HBM-bound (8 to 12 bytes per element), if closely: a thread takes quads of neighbouring elements, which is
+// what a block of the counter has bits for, and a block is some 70 instructions.  2^26 elements: 87 us (0.94 of the copy rate, issue 75 %), with a residual 118 (1.04); with one quad
+// per thread 122 and 135, with four 87 and 119.
 #include "common.cuh"
 #include "pam_scalar.cuh"
 #include "philox.cuh"
