@@ -388,18 +388,20 @@ class Transformer(nn.Module):
         mask = None if src_lengths is None else _beyond(src_lengths, src.shape[1]).repeat_interleave(self.cfg.heads, 0)
         if seeds is None and drops:
             seeds = self._seeds(src.device)
+        how = dict(seeds=seeds, drops=drops) if self.dropout else {}      # (layers of another kind need not know of dropout that there is none of)
         x = self.encoder.embed(src, seed=next(seeds) if seeds is not None else None, drops=drops)
         for layer in self.encoder.layers:
-            x = layer(x, self_mask=mask, seeds=seeds, drops=drops)
+            x = layer(x, self_mask=mask, **how)
         return x
 
     def forward(self, src, prev_out):
         seeds = self._seeds(src.device)
-        x = self.encode(src, seeds=seeds)
+        how = dict(seeds=seeds) if self.dropout else {}
+        x = self.encode(src, **how)
         future = self.decoder._future(prev_out.shape[1], src.device)
         y = self.decoder.embed(prev_out, seed=next(seeds) if seeds is not None else None)
         for layer in self.decoder.layers:
-            y = layer(y, x, future, seeds)
+            y = layer(y, x, future, **how)
         return self.decoder.output_projection(y)
 
     def _start(self, src, src_lengths, rows, max_len, eos):
@@ -410,7 +412,7 @@ class Transformer(nn.Module):
             raise ValueError(f"end of sentence {eos} with padding {cfg.pad} in a vocabulary of {cfg.vocab}")
         if src_lengths is not None and not bool(((src_lengths >= 1) & (src_lengths <= src.shape[1])).all()):
             raise ValueError(f"lengths must be from 1 to {src.shape[1]}")
-        memory = self.encode(src, src_lengths, drops=False)
+        memory = self.encode(src, src_lengths, **(dict(drops=False) if self.dropout else {}))
         shared = [layer.encoder_attn.cache(memory) for layer in self.decoder.layers]
         G, H = src.shape[0], cfg.heads
         own = [tuple(torch.empty(G, rows, max_len, H, cfg.dim // H, dtype=memory.dtype, device=device) for _ in range(2)) for _ in self.decoder.layers]
@@ -431,16 +433,20 @@ class Transformer(nn.Module):
     @torch.no_grad()
     def sample(self, src, samples=5, max_len=200, *, src_lengths=None, min_len=1, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, generator=None, eos=2):
         """`samples` translations of each sentence, drawn token by token (the fork's --sampling, fairseq/search.py) with the settings of
-        `decoding.sample` and random numbers of `generator` (of the source's device; None: the default one).
+        `decoding.sample`, one number each, and random numbers of `generator` (of the source's device; None: the default one).
 
         src, src_lengths, max_len, min_len and eos as for `generate`.  Returns (tokens [sentences, samples, n], scores [sentences, samples]): a score is the sum of its
         tokens' log-probabilities; tokens behind the end are padding."""
         cfg, ops, device = self.cfg, self.decoder.op_dict, src.device
         if not 1 <= min_len <= max_len or samples < 1:
             raise ValueError("sample needs 1 <= min_len <= max_len and at least one sample")
+        shape = (src.shape[0], samples)
+        for name, value, low, high in (("temperature", temperature, 2.0 ** -126, 2.0 ** 127), ("top_k", top_k, 0, 2 ** 62), ("top_p", top_p, 2.0 ** -24, 1.0), ("min_p", min_p, 0.0, 1.0)):
+            if isinstance(value, torch.Tensor):
+                raise TypeError(f"{name} must be a number")
+            decoding._setting(name, value, shape, low, high, whole=name == "top_k")
         shared, own, banned = self._start(src, src_lengths, samples, max_len, eos)
         positions = self.decoder._positions(max_len, device)
-        shape = (src.shape[0], samples)
         tokens = torch.full((*shape, max_len), cfg.pad, device=device)
         last = torch.full(shape, eos, device=device)
         scores = torch.zeros(shape, device=device)

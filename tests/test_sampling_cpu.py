@@ -34,9 +34,12 @@ def test_best_token_each_time():
 def test_refusals():
     net = cases.model({}, "cpu")
     src = torch.full((1, 3), 4)
-    for kw in (dict(samples=0), dict(max_len=0), dict(min_len=5, max_len=4), dict(eos=1), dict(eos=40), dict(src_lengths=torch.tensor([4]))):
+    for kw in (dict(samples=0), dict(max_len=0), dict(min_len=5, max_len=4), dict(eos=1), dict(eos=40), dict(src_lengths=torch.tensor([4])), dict(temperature=0.0), dict(top_k=-1),
+               dict(top_k=1.5), dict(top_p=0.0), dict(top_p=1.1), dict(min_p=-0.1), dict(min_p=True)):
         with pytest.raises(ValueError):
             net.sample(src, **kw)
+    with pytest.raises(TypeError):
+        net.sample(src, temperature=torch.ones(1, 5))
 
 
 def test_dropout_in_training_alone():
