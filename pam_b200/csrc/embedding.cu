@@ -412,10 +412,13 @@ __global__ void __launch_bounds__(kTileThreads) scatter_kernel(const Sort a) {
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < kRounds; ++r) {
-            if (digit[r] == kNone) continue;
-            const uint32_t to = start[digit[r]] + counts[warp * bins + digit[r]] + rank[r];
-            (HIGH ? a.sorted : a.by_low)[to] = {token[r], place[r]};
-            if (!HIGH) atomicAdd(a.counts_high + ((int64_t)(to / (uint32_t)a.tile) << a.high_bits) + (token[r] >> a.low_bits), 1u);
+            const bool is = digit[r] != kNone;
+            const uint32_t to = is ? start[digit[r]] + counts[warp * bins + digit[r]] + rank[r] : 0u;
+            if (is) (HIGH ? a.sorted : a.by_low)[to] = {token[r], place[r]};
+            if (HIGH) continue;
+            // the high digits of the next pass's tiles: one addition for all of the warp's that are alike
+            const uint32_t count = is ? (to / (uint32_t)a.tile << a.high_bits) + (token[r] >> a.low_bits) : kNone, alike = __match_any_sync(0xffffffffu, count);
+            if (is && lane == __ffs(alike) - 1) atomicAdd(a.counts_high + count, __popc(alike));
         }
         __syncthreads();
         for (int b = t; b < bins; b += kTileThreads) start[b] += totals[b];
@@ -557,9 +560,9 @@ __global__ void __launch_bounds__(kThreads, 4) sum_kernel(const Sums a) {
 }
 
 // A token's parts from..to - 1: the end of the chunk that it starts in, the beginnings of those that it goes on in.
-template <bool VEC>
+template <bool VEC, int kAhead>
 __device__ __forceinline__ void add_parts(const Sums& a, uint32_t chunk, uint32_t from, uint32_t to, int slab, int lane, float (&sum)[4]) {
-    constexpr int kAhead = 8;
+    const int c = column(slab, lane);
     for (uint32_t first = from; first < to; first += kAhead) {
         float v[kAhead][4];
 #pragma unroll
@@ -567,8 +570,13 @@ __device__ __forceinline__ void add_parts(const Sums& a, uint32_t chunk, uint32_
             const uint32_t part = first + j;
             if (part >= to) continue;
             const float* row = a.parts + ((int64_t)(chunk + part) * 2 + (part == 0)) * a.dim;
+            if (VEC) {
+                const float4 x = c < a.dim ? __ldcg(reinterpret_cast<const float4*>(row + c)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                v[j][0] = x.x, v[j][1] = x.y, v[j][2] = x.z, v[j][3] = x.w;
+            } else {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[j][k] = column(slab, lane) + k < a.dim ? __ldcg(row + column(slab, lane) + k) : 0.0f;
+                for (int k = 0; k < 4; ++k) v[j][k] = c + k < a.dim ? __ldcg(row + c + k) : 0.0f;
+            }
         }
 #pragma unroll
         for (int j = 0; j < kAhead; ++j)
@@ -578,13 +586,16 @@ __device__ __forceinline__ void add_parts(const Sums& a, uint32_t chunk, uint32_
     }
 }
 
-// How many parts the token has that starts in this chunk.
+// How many parts the token has that starts in this chunk: a warp looks at the next 32 chunks, then at 32 places of what is left, and so on.
 __device__ __forceinline__ uint32_t parts_of(const Sums& a, uint32_t chunk, uint32_t live, int lane, uint32_t* token) {
     *token = entry_at(a.sorted, (chunk + 1) * (uint32_t)a.chunk).token;
-    for (uint32_t more = 1;; more += 32) {
-        const uint64_t at = (uint64_t)(chunk + 1 + more + lane) * a.chunk;
+    uint32_t last = chunk + 1, end = a.chunks, step = 1;              // chunks that begin with the token, and with another or behind the last one
+    for (;; step = (end - last + 31) / 32) {
+        const uint64_t at = (last + (uint64_t)step * (lane + 1)) * a.chunk;
         const uint32_t other = __ballot_sync(0xffffffffu, at >= live || entry_at(a.sorted, (uint32_t)at).token != *token);
-        if (other) return more + __ffs(other);
+        if (other) end = min(end, last + step * __ffs(other));
+        last += step * (other ? __ffs(other) - 1 : 32);
+        if (last + 1 >= end) return end - chunk;
     }
 }
 
@@ -601,7 +612,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Sums a) {
         const uint32_t chunk = __ldcg(a.list + a.chunks - 1 - i), count = parts_of(a, chunk, live, lane, &token);
         const uint32_t each = (count + kWarps - 1) / kWarps, from = min(warp * each, count), to = min(from + each, count);
         float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        add_parts<VEC>(a, chunk, from, to, slab, lane, sum);
+        add_parts<VEC, VEC ? 16 : 8>(a, chunk, from, to, slab, lane, sum);
 #pragma unroll
         for (int k = 0; k < 4; ++k) stage[warp][lane * 4 + k] = sum[k];
         __syncthreads();
@@ -615,7 +626,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Sums a) {
     for (uint32_t i = blockIdx.x * kWarps + warp; i < some; i += gridDim.x * kWarps) {
         const uint32_t chunk = __ldcg(a.list + i), count = parts_of(a, chunk, live, lane, &token);
         float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        add_parts<VEC>(a, chunk, 0u, count, slab, lane, sum);
+        add_parts<VEC, 8>(a, chunk, 0u, count, slab, lane, sum);
         store_columns<VEC>(a.dw + (int64_t)token * a.dim, slab, lane, a.dim, sum);
     }
 }

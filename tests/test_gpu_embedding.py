@@ -233,6 +233,19 @@ def test_scales(pam, scale, dim):
             assert_bits_equal(d[v] + 0.0, terms[tokens == v][0] + 0.0)
 
 
+@pytest.mark.parametrize("runs", [(5000,), (1, 16 * 33, 16 * 34 - 1, 16 * 34 + 1, 17, 16, 15, 2000), (32 * 24, 32 * 25 - 1, 32 * 33 + 5, 40000, 1, 32 * 34, 32 * 1057 + 31, 32 * 66, 3), (5, 1100000, 7, 99)])
+@pytest.mark.parametrize("dim", [4, 5, 132])
+def test_lengths_of_runs(pam, runs, dim):
+    """Sums of whole numbers below 2^24, which are exact in any order."""
+    order = torch.randperm(sum(runs), generator=torch.Generator().manual_seed(dim))
+    tokens = torch.arange(len(runs)).repeat_interleave(torch.tensor(runs))[order]
+    g = torch.randint(-3, 4, (len(tokens), dim), generator=torch.Generator().manual_seed(2)).float()
+    w = torch.zeros(len(runs) + 2, dim, device="cuda", requires_grad=True)
+    (d,) = torch.autograd.grad(pam.embedding(tokens.cuda(), w), w, g.cuda())
+    want = torch.zeros(len(runs) + 2, dim, dtype=torch.float64).index_add_(0, tokens, g.double())
+    assert torch.equal(d.double().cpu(), want)
+
+
 def test_millions_of_tokens(pam):
     """More tokens than 512 tiles of 4096: tiles of several."""
     n, vocab = 2_200_003, 5001
