@@ -5,7 +5,7 @@
 // A token outside the table reads nothing: its row is NaN, and it has no gradient.
 //
 // The gradient is a sort and a segmented sum, so that every row of g is read once, wherever its token occurs, and no atomics decide on an order:
-//   sort   the places of the tokens in the order (token, place).  Up to 8192 tokens each counts those before it, which all SMs share (4096 tokens: 17 million comparisons);
+//   sort   the places of the tokens in the order (token, place).  Up to 4096 tokens each counts those before it, which all SMs share (4096 tokens: 17 million comparisons);
 //          more are cut into tiles and moved by two digits of at most 11 bits, each pass stable.  The other CTAs of these launches fill the gradient with zeros
 //          meanwhile.  (One CTA that moves up to 8192 tokens by digits in its shared memory: 14 us for 4096.)
 //   sums   a warp adds the rows of 16 neighbours in that order (32 where there are many), 128 columns of them, and writes the tokens that lie within;
@@ -175,10 +175,12 @@ __global__ void __launch_bounds__(kThreads) embed_odd_kernel(const Embedding a, 
 
 // ---- the order of the tokens ------------------------------------------------------------------------------------
 
-// Tokens that count each other (10000 words of 512 columns, backward: 2048 tokens 21 us, 29 by digits; 4096 28 and 38; 8192 44 and 43); a CTA's, one of a lane.
-constexpr int kMostCounted = 8192, kRanked = 32;
-constexpr int kTileThreads = 512, kTileWarps = kTileThreads / 32, kRounds = 8, kTile = kTileThreads * kRounds;
-constexpr int kMostTiles = 512;           // each reads the counts of all
+// Tokens that count each other (10000 words of 512 columns, dropout, backward: 2048 tokens 23 us, 29 by digits; 4096 29 and 30; 8192 49 and 35); a CTA's, one of a lane.
+constexpr int kMostCounted = 4096, kRanked = 32;
+// (Tiles of 1024: what a warp does one after the other, ranks by __match_any_sync of many different digits above all, takes 0.5 us for 32 tokens.  65536 tokens of 512 columns backward:
+// 86 us with tiles of 4096, 78 of 2048, 72.)
+constexpr int kTileThreads = 512, kTileWarps = kTileThreads / 32, kRounds = 2, kTile = kTileThreads * kRounds;
+constexpr int kMostTiles = 296;           // each reads the counts of all (2^19 tokens of 4000000 words backward: 512 of them 320 us, 296 173; 2^22 of 200000 788 and 807)
 constexpr uint32_t kNone = 0xffffffffu;
 
 struct Entry { uint32_t token, place; };
@@ -291,11 +293,13 @@ __global__ void __launch_bounds__(kThreads) rank_kernel(const Sort a, int ranker
         return;
     }
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, count = (int)a.count, padded = (count + 3) / 4 * 4;
-    uint32_t mine = 0u;
-#pragma unroll 8
-    for (int i = t; i < padded; i += kThreads) {
-        tokens[i] = token_of(a, i);
-        mine += tokens[i] != kNone;
+    uint32_t mine = 0u, loaded[kMostCounted / kThreads];
+#pragma unroll
+    for (int k = 0; k < kMostCounted / kThreads; ++k) loaded[k] = token_of(a, t + k * kThreads);
+#pragma unroll
+    for (int k = 0; k < kMostCounted / kThreads; ++k) {
+        if (t + k * kThreads < padded) tokens[t + k * kThreads] = loaded[k];
+        mine += loaded[k] != kNone;
     }
     mine = __reduce_add_sync(0xffffffffu, mine);
     if (lane == 0) live[warp] = mine;
@@ -347,9 +351,13 @@ __global__ void __launch_bounds__(kTileThreads) count_kernel(const Sort a) {
     if (blockIdx.x == 0 && threadIdx.x < 3) a.totals[threadIdx.x] = 0u;
     __syncthreads();
     const int64_t begin = (int64_t)blockIdx.x * a.tile;
-    for (int i = threadIdx.x; i < a.tile; i += kTileThreads) {
-        const uint32_t token = token_of(a, begin + i);
-        if (token != kNone) atomicAdd(&counts[token & (bins - 1)], 1u);
+    for (int i = threadIdx.x; i < a.tile; i += kTile) {
+        uint32_t token[kRounds];
+#pragma unroll
+        for (int r = 0; r < kRounds; ++r) token[r] = token_of(a, begin + i + r * kTileThreads);
+#pragma unroll
+        for (int r = 0; r < kRounds; ++r)
+            if (token[r] != kNone) atomicAdd(&counts[token[r] & (bins - 1)], 1u);
     }
     __syncthreads();
     for (int b = threadIdx.x; b < bins; b += kTileThreads) a.counts_low[(int64_t)blockIdx.x * bins + b] = counts[b];
@@ -372,38 +380,55 @@ __global__ void __launch_bounds__(kTileThreads) scatter_kernel(const Sort a) {
     uint32_t* start = reinterpret_cast<uint32_t*>(memory);                            // where the tile's next element of each digit goes
     uint32_t* totals = start + bins;
     uint16_t* counts = reinterpret_cast<uint16_t*>(totals + bins);
+    for (int b = t; b < bins; b += kTileThreads) start[b] = totals[b] = 0u;
+    __syncthreads();
     after_previous();
-    const uint32_t* all = HIGH ? a.counts_high : a.counts_low;
-    for (int b = t; b < bins; b += kTileThreads) {
-        uint32_t before = 0u, sum = 0u;
-        for (int k = 0; k < a.tiles; ++k) {
-            if (k == (int)blockIdx.x) before = sum;
-            sum += __ldcg(all + (int64_t)k * bins + b);
-        }
-        start[b] = sum;
-        totals[b] = before;
-    }
-    const uint32_t live = sums_before(start, bins, warp_sums);
-    for (int b = t; b < bins; b += kTileThreads) start[b] += totals[b];
-    if (!HIGH && blockIdx.x == 0 && t == 0) a.totals[0] = live;
-    const int64_t tile_begin = (int64_t)blockIdx.x * a.tile, tile_end = min(tile_begin + a.tile, HIGH ? (int64_t)live : a.count);
+    const int64_t tile_begin = (int64_t)blockIdx.x * a.tile;
     uint32_t token[kRounds], place[kRounds], digit[kRounds], rank[kRounds];
-    for (int64_t begin = tile_begin; begin < tile_end; begin += kTile) {
-        for (int i = t; i < bins * kTileWarps / 2; i += kTileThreads) reinterpret_cast<uint32_t*>(counts)[i] = 0u;
+    const auto load = [&](int64_t begin) {            // (of the second pass also what lies behind the last one: it is not looked at)
 #pragma unroll
         for (int r = 0; r < kRounds; ++r) {
-            token[r] = digit[r] = kNone;
             const int64_t i = begin + (warp * kRounds + r) * 32 + lane;
-            if (i >= tile_end) continue;
             if (HIGH) {
-                const uint2 e = __ldcg(reinterpret_cast<const uint2*>(a.by_low) + i);
+                const uint2 e = i < a.count ? __ldcg(reinterpret_cast<const uint2*>(a.by_low) + i) : make_uint2(kNone, 0u);
                 token[r] = e.x;
                 place[r] = e.y;
             } else {
                 token[r] = token_of(a, i);
                 place[r] = (uint32_t)i;
             }
-            if (token[r] != kNone) digit[r] = HIGH ? token[r] >> a.low_bits : token[r] & (bins - 1);
+        }
+    };
+    load(tile_begin);
+    {
+        // a thread adds four neighbouring digits of every so-many-th tile
+        const uint4* all = reinterpret_cast<const uint4*>(HIGH ? a.counts_high : a.counts_low);
+        const int quad_bits = bits - 2, quad = t & ((1 << quad_bits) - 1), groups = kTileThreads >> quad_bits;
+        uint4 sum = make_uint4(0u, 0u, 0u, 0u), before = sum;
+#pragma unroll 8
+        for (int k = t >> quad_bits; k < a.tiles; k += groups) {
+            const uint4 v = __ldcg(all + ((int64_t)k << quad_bits) + quad);
+            sum = make_uint4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
+            if (k < (int)blockIdx.x) before = make_uint4(before.x + v.x, before.y + v.y, before.z + v.z, before.w + v.w);
+        }
+        const uint32_t s[4] = {sum.x, sum.y, sum.z, sum.w}, p[4] = {before.x, before.y, before.z, before.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (s[k]) atomicAdd(&start[quad * 4 + k], s[k]);
+            if (p[k]) atomicAdd(&totals[quad * 4 + k], p[k]);
+        }
+    }
+    const uint32_t live = sums_before(start, bins, warp_sums);
+    for (int b = t; b < bins; b += kTileThreads) start[b] += totals[b];
+    if (!HIGH && blockIdx.x == 0 && t == 0) a.totals[0] = live;
+    const int64_t tile_end = min(tile_begin + a.tile, HIGH ? (int64_t)live : a.count);
+    for (int64_t begin = tile_begin; begin < tile_end; begin += kTile) {
+        if (begin != tile_begin) load(begin);
+        for (int i = t; i < bins * kTileWarps / 2; i += kTileThreads) reinterpret_cast<uint32_t*>(counts)[i] = 0u;
+#pragma unroll
+        for (int r = 0; r < kRounds; ++r) {
+            const bool is = begin + (warp * kRounds + r) * 32 + lane < tile_end && token[r] != kNone;
+            digit[r] = !is ? kNone : HIGH ? token[r] >> a.low_bits : token[r] & (bins - 1);
         }
         __syncthreads();
         rank_in_warp<kRounds>(counts + warp * bins, digit, rank, kRounds);
@@ -412,13 +437,10 @@ __global__ void __launch_bounds__(kTileThreads) scatter_kernel(const Sort a) {
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < kRounds; ++r) {
-            const bool is = digit[r] != kNone;
-            const uint32_t to = is ? start[digit[r]] + counts[warp * bins + digit[r]] + rank[r] : 0u;
-            if (is) (HIGH ? a.sorted : a.by_low)[to] = {token[r], place[r]};
-            if (HIGH) continue;
-            // the high digits of the next pass's tiles: one addition for all of the warp's that are alike
-            const uint32_t count = is ? (to / (uint32_t)a.tile << a.high_bits) + (token[r] >> a.low_bits) : kNone, alike = __match_any_sync(0xffffffffu, count);
-            if (is && lane == __ffs(alike) - 1) atomicAdd(a.counts_high + count, __popc(alike));
+            if (digit[r] == kNone) continue;
+            const uint32_t to = start[digit[r]] + counts[warp * bins + digit[r]] + rank[r];
+            (HIGH ? a.sorted : a.by_low)[to] = {token[r], place[r]};
+            if (!HIGH) atomicAdd(a.counts_high + ((int64_t)(to / (uint32_t)a.tile) << a.high_bits) + (token[r] >> a.low_bits), 1u);
         }
         __syncthreads();
         for (int b = t; b < bins; b += kTileThreads) start[b] += totals[b];
@@ -600,7 +622,7 @@ __device__ __forceinline__ uint32_t parts_of(const Sums& a, uint32_t chunk, uint
 }
 
 template <bool VEC>
-__global__ void __launch_bounds__(kThreads) join_kernel(const Sums a) {
+__global__ void __launch_bounds__(kThreads, 2) join_kernel(const Sums a) {
     constexpr int kWarps = kThreads / 32;
     __shared__ float stage[kWarps][kColumns];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, slab = blockIdx.y;
@@ -671,7 +693,7 @@ struct Plan {
 
 Plan planned(int64_t count, int64_t vocab, int64_t dim) {
     Plan p{};
-    int bits = 2;
+    int bits = 4;                         // (digits of two at least, whose counts are read by four)
     while (((int64_t)1 << bits) < vocab) ++bits;
     p.low_bits = (bits + 1) / 2;
     p.high_bits = bits - p.low_bits;
@@ -854,7 +876,7 @@ int pamk_embedding_bwd(const int64_t* tokens, const float* dy, const float* tabl
     const bool vec = dim % 4 == 0 && aligned16(dy) && aligned16(dtable) && (!slopes || (aligned16(table) && table_row % 4 == 0));
     const auto sums = vec ? (slopes ? sum_kernel<true, true> : sum_kernel<true, false>) : (slopes ? sum_kernel<false, true> : sum_kernel<false, false>);
     if (const int status = launch_next(sums, dim3((unsigned)ctas), kThreads, 0, st, u)) return status;
-    const int64_t wide = (8 * sm_count() + slabs - 1) / slabs;
+    const int64_t wide = (2 * sm_count() + slabs - 1) / slabs;
     const unsigned joins = (unsigned)(plan.chunks < wide ? plan.chunks : wide);
     return launch_next(vec ? join_kernel<true> : join_kernel<false>, dim3(joins, (unsigned)slabs), kThreads, 0, st, u);
 }

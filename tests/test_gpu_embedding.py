@@ -247,7 +247,7 @@ def test_lengths_of_runs(pam, runs, dim):
 
 
 def test_millions_of_tokens(pam):
-    """More tokens than 512 tiles of 4096: tiles of several."""
+    """More tokens than there are tiles at their smallest: a tile is walked over in several steps."""
     n, vocab = 2_200_003, 5001
     tokens, weight, _, g = data((n,), vocab, 2, None, seed=9)
     w = weight.cuda().requires_grad_()
