@@ -468,7 +468,7 @@ struct Sums {
     Dropping drop;
 };
 
-constexpr uint32_t kMany = 24;            // chunks of a token that a warp adds alone (its loads wait three times; of 8192 tokens there are 512)
+constexpr uint32_t kMany = 12;            // chunks of a token that a warp adds alone (its loads wait twice; 2^18 tokens of 4 columns backward: 48 chunks 73.4 us, 24 71.3, 12 69.9)
 
 __device__ __forceinline__ Entry entry_at(const Entry* sorted, uint32_t i) {
     const uint2 e = __ldcg(reinterpret_cast<const uint2*>(sorted) + i);
@@ -503,7 +503,7 @@ __device__ __forceinline__ void store_columns(float* row, int slab, int lane, in
 }
 
 // Bound by instructions with dropout (194 for each quad of a row, 70 of them its random bits): 64 x 1024 rows of 512 columns in 70 us, by the trips to memory without.  Four CTAs per
-// SM with four rows on their way each, not three with eight: 64 x 1024 tokens backward 122 -> 118 us, without dropout 90 -> 85.
+// SM with four rows on their way each, not three with eight: 4 us less with dropout and without, of 103 and 71 for all of the backward pass.
 template <bool VEC, bool SLOPES>
 __global__ void __launch_bounds__(kThreads, 4) sum_kernel(const Sums a) {
     constexpr int kAhead = 4;             // rows on their way
@@ -702,7 +702,7 @@ Plan planned(int64_t count, int64_t vocab, int64_t dim) {
         p.tile = (int)((each + kTile - 1) / kTile * kTile);
         p.tiles = (int)((count + p.tile - 1) / p.tile);
     }
-    p.chunk = count > 32768 ? 32 : 16;    // (2^20 tokens of 128 columns backward: 16 rows 370 us, 32 279; 4096 of 512: 28.2 and 28.8)
+    p.chunk = count > 32768 ? 32 : 16;    // (2^20 tokens of 128 columns backward: 16 rows 261 us, 32 221; 4096 of 512: 28.3 and 34.9)
     p.chunks = (count + p.chunk - 1) / p.chunk;
     size_t at = 0;
     const auto take = [&](size_t bytes) {
