@@ -237,13 +237,14 @@ class TransformerLayer(nn.Module):
         self.cross = cross
 
     def forward(self, x, memory=None, self_mask=None, seeds=None, drops=True):
-        add = lambda a, b: a + b
+        """`seeds`: one for each sublayer (None: the masks draw theirs), so that the layer has the same masks when it runs again in a backward pass."""
+        add = lambda a, b, sublayer: a + b
         if drops and self.training and self.dropout:
-            add = lambda a, b: _dropped(self.op_dict, b, self.dropout, next(seeds) if seeds is not None else None, a)
-        x = self.self_attn_layer_norm(add(x, self.self_attn(x, x, self_mask)))
+            add = lambda a, b, sublayer: _dropped(self.op_dict, b, self.dropout, seeds[sublayer] if seeds is not None else None, a)
+        x = self.self_attn_layer_norm(add(x, self.self_attn(x, x, self_mask), 0))
         if self.cross:
-            x = self.encoder_attn_layer_norm(add(x, self.encoder_attn(x, memory)))
-        return self.final_layer_norm(add(x, self.fc2(torch.relu(self.fc1(x)))))
+            x = self.encoder_attn_layer_norm(add(x, self.encoder_attn(x, memory), 1))
+        return self.final_layer_norm(add(x, self.fc2(torch.relu(self.fc1(x))), -1))
 
     def step(self, x, own, position, shared, shared_lengths):
         """The decoder layer on one new token of each row, [groups, rows, dim]: its key and value go to `position` of the row's own
@@ -354,6 +355,11 @@ def _reorder(states, parents, used):
         t[:, :, :used] = t[group, parents, :used]
 
 
+def _handed_out(seeds, stack, layers):
+    """The seed of a stack's embedding and those of each layer, from what `Transformer._seeds` gives."""
+    return (None, [None] * len(layers)) if seeds is None else seeds[stack]
+
+
 class Transformer(nn.Module):
     """`dropout`: in training, of the embeddings and of what each sublayer adds (the `--dropout` of the reference's fork)."""
     dropout = 0.0
@@ -376,11 +382,13 @@ class Transformer(nn.Module):
         self.decoder.output_projection.weight = self.decoder.embed_tokens.weight
 
     def _seeds(self, device):
-        """The seeds of a training step's masks, drawn at once: of the embeddings, and of what the sublayers add."""
+        """The seeds of a training step's masks, drawn at once: for the encoder and the decoder those of the embedding and of the sublayers of each layer."""
         if not (self.training and self.dropout) or device.type != "cuda":
             return None
         count = 2 + 2 * len(self.encoder.layers) + 3 * len(self.decoder.layers)
-        return iter(torch.randint(-2 ** 63, 2 ** 63 - 1, (count,), device=device).unbind())
+        seeds = iter(torch.randint(-2 ** 63, 2 ** 63 - 1, (count,), device=device).unbind())
+        return tuple((next(seeds), [tuple(next(seeds) for _ in range(sublayers)) for _ in stack.layers])
+                     for stack, sublayers in ((self.encoder, 2), (self.decoder, 3)))
 
     def encode(self, src, src_lengths=None, seeds=None, drops=True):
         """The encoder's output.  `src_lengths` (int64 [sentences]): the tokens behind a sentence's length are padding, which no other position
@@ -388,20 +396,20 @@ class Transformer(nn.Module):
         mask = None if src_lengths is None else _beyond(src_lengths, src.shape[1]).repeat_interleave(self.cfg.heads, 0)
         if seeds is None and drops:
             seeds = self._seeds(src.device)
-        how = dict(seeds=seeds, drops=drops) if self.dropout else {}      # (layers of another kind need not know of dropout that there is none of)
-        x = self.encoder.embed(src, seed=next(seeds) if seeds is not None else None, drops=drops)
-        for layer in self.encoder.layers:
-            x = layer(x, self_mask=mask, **how)
+        first, each = _handed_out(seeds, 0, self.encoder.layers)
+        x = self.encoder.embed(src, seed=first, drops=drops)
+        for layer, own in zip(self.encoder.layers, each):
+            x = layer(x, self_mask=mask, **(dict(seeds=own, drops=drops) if self.dropout else {}))      # (layers of another kind need not know of dropout that there is none of)
         return x
 
     def forward(self, src, prev_out):
         seeds = self._seeds(src.device)
-        how = dict(seeds=seeds) if self.dropout else {}
-        x = self.encode(src, **how)
+        x = self.encode(src, **(dict(seeds=seeds) if self.dropout else {}))
         future = self.decoder._future(prev_out.shape[1], src.device)
-        y = self.decoder.embed(prev_out, seed=next(seeds) if seeds is not None else None)
-        for layer in self.decoder.layers:
-            y = layer(y, x, future, **how)
+        first, each = _handed_out(seeds, 1, self.decoder.layers)
+        y = self.decoder.embed(prev_out, seed=first)
+        for layer, own in zip(self.decoder.layers, each):
+            y = layer(y, x, future, **(dict(seeds=own) if self.dropout else {}))
         return self.decoder.output_projection(y)
 
     def _start(self, src, src_lengths, rows, max_len, eos):
