@@ -344,7 +344,8 @@ def _draw(ops, logits, uniform, temperature, top_k, top_p, min_p, banned):
     p = p * (p.cumsum(-1) - p < top_p * p.sum(-1, keepdim=True)) * (p >= min_p * p[..., :1])
     p = torch.zeros_like(p).scatter(-1, order.indices, p).cumsum(-1)
     tokens = (p <= uniform.double().unsqueeze(-1) * p[..., -1:]).sum(-1).clamp(max=logits.shape[-1] - 1)
-    return tokens, values.gather(-1, tokens.unsqueeze(-1)).squeeze(-1)
+    scores, none = values.gather(-1, tokens.unsqueeze(-1)).squeeze(-1), ~(p[..., -1] > 0)             # (NaN among them)
+    return tokens.masked_fill(none, -1), scores.masked_fill(none, float("-inf"))
 
 
 def _reorder(states, parents, used):
@@ -444,7 +445,8 @@ class Transformer(nn.Module):
         `decoding.sample`, one number each, and random numbers of `generator` (of the source's device; None: the default one).
 
         src, src_lengths, max_len, min_len and eos as for `generate`.  Returns (tokens [sentences, samples, n], scores [sentences, samples]): a score is the sum of its
-        tokens' log-probabilities; tokens behind the end are padding."""
+        tokens' log-probabilities; tokens behind the end are padding.  A sample whose logits leave no token to draw (a NaN, values beyond the range of the arithmetic) ends
+        there without one, with score -inf."""
         cfg, ops, device = self.cfg, self.decoder.op_dict, src.device
         if not 1 <= min_len <= max_len or samples < 1:
             raise ValueError("sample needs 1 <= min_len <= max_len and at least one sample")
@@ -463,10 +465,10 @@ class Transformer(nn.Module):
             logits = self._step(last, positions[t], t, own, shared, src_lengths)
             uniform = torch.rand(shape, generator=generator, device=device)
             drawn, gained = _draw(ops, logits, uniform, temperature, top_k, top_p, min_p, banned[2 if t == max_len - 1 else 0 if t + 1 < min_len else 1])
-            last = torch.where(going, drawn, cfg.pad)
+            last = torch.where(going & (drawn >= 0), drawn, cfg.pad)
             scores = torch.where(going, scores + gained, scores)
             tokens[:, :, t] = last
-            going = going & (last != eos)
+            going = going & (drawn >= 0) & (last != eos)
             if t == max_len - 1 or not bool(going.any()):
                 break
         return tokens[:, :, :t + 1], scores
