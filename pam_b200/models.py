@@ -197,7 +197,7 @@ def _plain(bound, t):
 
 
 def _scaling(ops, t):
-    """The settings of the dictionary's PAM product, where the operators that are made of it (`pam_ops.embedding`, `pam_ops.dropout`) stand for it on this tensor; else None."""
+    """The settings of the dictionary's PAM product, where `pam_ops.embedding`, which is made of it, stands for it on this tensor; else None."""
     bound = _pam_binding(ops, ("mul",))
     if bound is None or not (t.is_cuda and t.dtype == torch.float32) or not fused._uniform(bound.get("approx_bwd", False)):
         return None
@@ -205,10 +205,11 @@ def _scaling(ops, t):
 
 
 def _dropped(ops, x, p, seed, residual=None):
-    """Dropout of x, added to `residual`: with the dictionary's product where that is PAM's, else the ordinary one."""
-    bound = _scaling(ops, x)
+    """Dropout of x, added to `residual`: with the dictionary's product where that is PAM's (x is its first operand, and taken as fp32 as that does), else the ordinary one."""
+    bound = _pam_binding(ops, ("mul",))
     if bound is not None:
-        return pam_ops.dropout(x, p, seed, residual, **bound)
+        bound["approx_bwd"] = fused._flag(bound.get("approx_bwd", False))
+        return pam_ops.dropout(x.float(), p, seed, None if residual is None else residual.float(), **bound)
     x = F.dropout(x, p)
     return x if residual is None else residual + x
 

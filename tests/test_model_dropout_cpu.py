@@ -57,3 +57,35 @@ def test_each_mask_has_a_seed_of_its_own(net, monkeypatch):
     net(torch.full((2, 5), 7), torch.full((2, 4), 9))
     # the embeddings, two sublayers of an encoder layer and three of a decoder layer
     assert len(seeds) == len(set(seeds)) == 2 + 2 * 2 + 3 * 2
+
+
+@pytest.mark.parametrize("flags, first", [((True, False), True), ((False, True), False), (True, True), ((False, False), False)], ids=str)
+def test_a_pam_dictionary_has_a_pam_dropout(monkeypatch, flags, first):
+    """Whatever its gradient mode and the tensors' type: never the ordinary product."""
+    from pam_b200 import factories, models, pam_ops
+    name = lambda v: str(v).lower()
+    mode = name(flags) if isinstance(flags, bool) else "[" + ", ".join(map(name, flags)) + "]"
+    ops = factories.get_function_dict('{"type": "pam", "dkwargs": {"approx_bwd": %s}}' % mode)
+    assert models._pam_binding(ops, ("mul",)) is not None
+    calls = []
+    monkeypatch.setattr(pam_ops, "dropout", lambda x, p, seed, residual, **kw: calls.append((x, p, seed, residual, kw)) or x)
+    monkeypatch.setattr(models.F, "dropout", lambda *a, **kw: pytest.fail("an ordinary dropout"))
+    x, r = torch.randn(3, 4), torch.randn(3, 4)
+    models._dropped(ops, x, 0.3, 5, r)
+    models._dropped(ops, x.bfloat16(), 0.3, None)
+    for (got, p, seed, residual, kw), want in zip(calls, ((x, 5, r), (x.bfloat16().float(), None, None))):
+        assert got.dtype == torch.float32 and torch.equal(got, want[0]) and (p, seed) == (0.3, want[1]) and residual is want[2]
+        assert _flag(kw["approx_bwd"]) is first and kw.get("offset") in (None, 1.0)
+
+
+def _flag(approx_bwd):
+    return approx_bwd if isinstance(approx_bwd, bool) else (set(approx_bwd).pop() if len(set(approx_bwd)) == 1 else None)
+
+
+def test_other_dictionaries_have_the_ordinary_one():
+    from pam_b200 import models
+    x, r = torch.randn(3, 4), torch.randn(3, 4)
+    torch.manual_seed(1)
+    got = models._dropped(dict(mul=torch.mul), x, 0.3, None, r)
+    torch.manual_seed(1)
+    assert torch.equal(got, r + torch.nn.functional.dropout(x, 0.3))
