@@ -288,6 +288,15 @@ def _kept(module, name, length, device, make, cut):
     return view
 
 
+_HOOKS = ("forward_hooks", "forward_pre_hooks", "backward_hooks", "backward_pre_hooks")
+
+
+def _looks_up_alone(table):
+    """Whether a call of the table is the lookup of rows and nothing else: no settings that change the table or its gradient, no hooks of its own or of all modules."""
+    return type(table) is nn.Embedding and table.max_norm is None and not (table.sparse or table.scale_grad_by_freq or "forward" in table.__dict__) \
+        and not any(getattr(table, "_" + name) or getattr(nn.modules.module, "_global_" + name) for name in _HOOKS)
+
+
 class _Stack(nn.Module):
     dropout = 0.0
 
@@ -315,8 +324,7 @@ class _Stack(nn.Module):
             positions = self._positions(tokens.shape[1], tokens.device)
         bound = _scaling(self.op_dict, table.weight)
         # (without dropout a training step keeps the chain, and with it the order in which torch adds up the table's gradient)
-        if bound is not None and (p or not torch.is_grad_enabled()) and type(table) is nn.Embedding and table.weight.shape[0] <= 1 << 22 \
-                and not table._forward_hooks and not table._forward_pre_hooks:
+        if bound is not None and (p or not torch.is_grad_enabled()) and _looks_up_alone(table) and table.weight.shape[0] <= 1 << 22:
             return pam_ops.embedding(tokens, table.weight, self.embed_scale, positions, table.padding_idx, p=p, seed=seed, **bound)
         x = self.op_dict["mul"](self.embed_scale, table(tokens)) + positions
         return _dropped(self.op_dict, x, p, seed) if p else x
