@@ -581,15 +581,18 @@ __global__ void __launch_bounds__(kThreads, 4) sum_kernel(const Sums a) {
     next_may_start();
 }
 
-// A token's parts from..to - 1: the end of the chunk that it starts in, the beginnings of those that it goes on in.
+// A token's parts from..to - 1: the end of the chunk that it starts in, the beginnings of those that it goes on in.  Those that are on their way together are added pair by pair in
+// 32 bits, these sums in 64: there may be 2^26 parts, and the error does not grow with them.  (2^20 rows of one token, 128 columns, backward: 735 us, with every part in 64 bits 833; 4096 of
+// 512 28.7, in 32 bits alone 28.1.)
 template <bool VEC, int kAhead>
-__device__ __forceinline__ void add_parts(const Sums& a, uint32_t chunk, uint32_t from, uint32_t to, int slab, int lane, float (&sum)[4]) {
+__device__ __forceinline__ void add_parts(const Sums& a, uint32_t chunk, uint32_t from, uint32_t to, int slab, int lane, double (&sum)[4]) {
     const int c = column(slab, lane);
     for (uint32_t first = from; first < to; first += kAhead) {
         float v[kAhead][4];
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             const uint32_t part = first + j;
+            v[j][0] = v[j][1] = v[j][2] = v[j][3] = 0.0f;
             if (part >= to) continue;
             const float* row = a.parts + ((int64_t)(chunk + part) * 2 + (part == 0)) * a.dim;
             if (VEC) {
@@ -601,10 +604,13 @@ __device__ __forceinline__ void add_parts(const Sums& a, uint32_t chunk, uint32_
             }
         }
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j)
-            if (first + j < to)
+        for (int apart = 1; apart < kAhead; apart *= 2)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) sum[k] = fadd(sum[k], v[j][k]);
+            for (int j = 0; j < kAhead; j += 2 * apart)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[j][k] = fadd(v[j][k], v[j + apart][k]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum[k] += v[0][k];
     }
 }
 
@@ -624,7 +630,7 @@ __device__ __forceinline__ uint32_t parts_of(const Sums& a, uint32_t chunk, uint
 template <bool VEC>
 __global__ void __launch_bounds__(kThreads, 2) join_kernel(const Sums a) {
     constexpr int kWarps = kThreads / 32;
-    __shared__ float stage[kWarps][kColumns];
+    __shared__ double stage[kWarps][kColumns];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, slab = blockIdx.y;
     after_previous();
     const uint32_t live = __ldcg(a.totals), some = __ldcg(a.totals + 1), many = __ldcg(a.totals + 2);
@@ -633,23 +639,24 @@ __global__ void __launch_bounds__(kThreads, 2) join_kernel(const Sums a) {
         // a warp has neighbouring parts
         const uint32_t chunk = __ldcg(a.list + a.chunks - 1 - i), count = parts_of(a, chunk, live, lane, &token);
         const uint32_t each = (count + kWarps - 1) / kWarps, from = min(warp * each, count), to = min(from + each, count);
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        double sum[4] = {0.0, 0.0, 0.0, 0.0};
         add_parts<VEC, VEC ? 16 : 8>(a, chunk, from, to, slab, lane, sum);
 #pragma unroll
         for (int k = 0; k < 4; ++k) stage[warp][lane * 4 + k] = sum[k];
         __syncthreads();
         if (threadIdx.x < kColumns && slab * kColumns + threadIdx.x < a.dim) {
-            float s = stage[0][threadIdx.x];
-            for (int w = 1; w < kWarps; ++w) s = fadd(s, stage[w][threadIdx.x]);
-            a.dw[(int64_t)token * a.dim + slab * kColumns + threadIdx.x] = s;
+            double s = stage[0][threadIdx.x];
+            for (int w = 1; w < kWarps; ++w) s += stage[w][threadIdx.x];
+            a.dw[(int64_t)token * a.dim + slab * kColumns + threadIdx.x] = (float)s;
         }
         __syncthreads();
     }
     for (uint32_t i = blockIdx.x * kWarps + warp; i < some; i += gridDim.x * kWarps) {
         const uint32_t chunk = __ldcg(a.list + i), count = parts_of(a, chunk, live, lane, &token);
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        double sum[4] = {0.0, 0.0, 0.0, 0.0};
         add_parts<VEC, 8>(a, chunk, 0u, count, slab, lane, sum);
-        store_columns<VEC>(a.dw + (int64_t)token * a.dim, slab, lane, a.dim, sum);
+        const float rounded[4] = {(float)sum[0], (float)sum[1], (float)sum[2], (float)sum[3]};
+        store_columns<VEC>(a.dw + (int64_t)token * a.dim, slab, lane, a.dim, rounded);
     }
 }
 
