@@ -371,7 +371,10 @@ def _handed_out(seeds, stack, layers):
 
 
 class Transformer(nn.Module):
-    """`dropout`: in training, of the embeddings and of what each sublayer adds (the `--dropout` of the reference's fork)."""
+    """`dropout`: in training, of the embeddings and of what each sublayer adds (the `--dropout` of the reference's fork).
+
+    Tokens outside the vocabulary: `generate` and `sample` refuse them.  Other passes give NaN where the PAM lookup runs (without gradients, and with dropout), which the PAM softmax, whose
+    shift is the whole tensor's, spreads over the batch; they end as torch's lookup does where that runs."""
     dropout = 0.0
 
     def __init__(self, cfg=TransformerConfig(), linear_cfg="standard", norm_cfg="layer_norm", functional_cfg="torch",
@@ -428,6 +431,8 @@ class Transformer(nn.Module):
         cfg, device = self.cfg, src.device
         if eos == cfg.pad or not 0 <= eos < cfg.vocab or cfg.vocab < 3:
             raise ValueError(f"end of sentence {eos} with padding {cfg.pad} in a vocabulary of {cfg.vocab}")
+        if not bool(((src >= 0) & (src < cfg.vocab)).all()):                  # (the lookup would give NaN, which the selection of tokens passes over)
+            raise ValueError(f"source tokens outside the vocabulary of {cfg.vocab}")
         if src_lengths is not None and not bool(((src_lengths >= 1) & (src_lengths <= src.shape[1])).all()):
             raise ValueError(f"lengths must be from 1 to {src.shape[1]}")
         memory = self.encode(src, src_lengths, **(dict(drops=False) if self.dropout else {}))
