@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(kThreads) embed_odd_kernel(const Embedding a, 
     if (e >= n) return;
     const uint2 key = a.drops ? key_of(a.drop) : make_uint2(0u, 0u);
     const uint32_t i = by_row(e), c = e - i * by_row.d;
-    const auto at = [&](uint32_t row, uint32_t column, int64_t token) {
+    const auto at = [&](uint32_t column, int64_t token) {
         float x = quiet_nan();
         if ((uint64_t)token < (uint64_t)a.vocab) x = __ldg(a.table + token * a.table_row + column);
         return x;
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(kThreads) embed_odd_kernel(const Embedding a, 
         const uint32_t row = i + behind, column = c + k - (behind ? by_row.d : 0u);
         x[k] = p[k] = d[k] = 0.0f;
         if (e + k >= n) continue;
-        x[k] = at(row, column, behind ? next : token);
+        x[k] = at(column, behind ? next : token);
         p[k] = place(row, column);
         if (SLOPES) d[k] = __ldg(g + e + k);
     }
@@ -224,11 +224,10 @@ __device__ __forceinline__ uint32_t token_of(const Sort& a, int64_t i) {
 
 // How many of the warp's earlier elements have the same digit (kNone: no element), which its counts are left with.
 template <int ROUNDS>
-__device__ __forceinline__ void rank_in_warp(uint16_t* counts, const uint32_t (&digit)[ROUNDS], uint32_t (&rank)[ROUNDS], int rounds) {
+__device__ __forceinline__ void rank_in_warp(uint16_t* counts, const uint32_t (&digit)[ROUNDS], uint32_t (&rank)[ROUNDS]) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) {
-        if (r >= rounds) break;
         const bool is = digit[r] != kNone;
         const uint32_t peers = __match_any_sync(0xffffffffu, digit[r]);
         const uint32_t before = is ? counts[digit[r]] : 0u;
@@ -431,7 +430,7 @@ __global__ void __launch_bounds__(kTileThreads) scatter_kernel(const Sort a) {
             digit[r] = !is ? kNone : HIGH ? token[r] >> a.low_bits : token[r] & (bins - 1);
         }
         __syncthreads();
-        rank_in_warp<kRounds>(counts + warp * bins, digit, rank, kRounds);
+        rank_in_warp<kRounds>(counts + warp * bins, digit, rank);
         __syncthreads();
         sums_over_warps(counts, totals, bins, kTileWarps);
         __syncthreads();
