@@ -397,7 +397,7 @@ int pamk_dropout_bwd(const float* x, const float* dy, float* dx, int64_t n, doub
  * its slope at the sum, 0 where dropped.
  * pamk_embedding_bwd: dtable[v] = sum over the i with tokens[i] = v, v != padding, of pam(drop'(dy[i]), scale), [vocab, dim] contiguous; with approx_bwd 0 of
  * dy[i] slope(table[v], scale), and then p must be 0 (pamk_embedding gives the dropout's gradient).  Rows without a token get zeros.  The terms of a row are added
- * in an order that follows from the tokens alone.  padding: -1 for none.
+ * in an order that follows from the tokens alone, 32 of them at most one after the other in 32 bits.  padding: -1 for none.
  * count < 2^31, vocab <= 2^22.  `workspace`: pamk_embedding_bwd_workspace_bytes(...) bytes, 256-byte aligned; NULL where that is 0. */
 int pamk_embedding(const int64_t* tokens, const float* table, const float* positions, const float* dy, float* out, int64_t count, int64_t vocab, int64_t dim,
                    int64_t table_row, int64_t positions_row, int64_t positions_count, int has_scale, float scale, double p, const int64_t* seed_at, int64_t seed,
